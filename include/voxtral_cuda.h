@@ -188,6 +188,16 @@ int vox_cuda_decoder_full_step(vox_cuda_dec_state *s, const float *embed,
  * alt_ids[0] = best and returns the number of ids written (1..n_alt). */
 int vox_cuda_decoder_fill_alts(vox_cuda_dec_state *s, int n_alt, float cutoff, int *alt_ids);
 
+/* Confidence of a token under the last step's logits: its natural log
+ * probability, the distribution's entropy (nats), and the n_top (0..32) most
+ * likely ids with their log probabilities, best first, ties to the lowest id.
+ * logprob, entropy: host, one value each; top_ids, top_logprob: host [n_top].
+ * Returns n_top.  The device form for rows of logits is
+ * vox_cuda_token_logprobs_dev.  Additive: the reference keeps no
+ * probabilities beyond the ratio that stream_fill_alts cuts off at. */
+int vox_cuda_decoder_token_logprobs(vox_cuda_dec_state *s, int token, int n_top, float *logprob,
+                                    float *entropy, int *top_ids, float *top_logprob);
+
 /* Prefill seq_len rows (host x [seq_len, 3072]) at the current position
  * (voxtral_decoder.c:233-373; vox_metal_decoder_prefill_step,
  * voxtral_metal.h:254).  rope_freqs: host [seq_len][64][2] or NULL. */
@@ -517,6 +527,128 @@ int vox_cuda_attention_decode_noalloc(const float *q, const float *k_ring, const
  * the device (vox_apply_rope, voxtral_kernels.c:502-526). */
 int vox_cuda_rope_dev(float *x, int n_heads, int head_dim, int pos, const float *rope_freqs,
                       void *stream);
+
+/* ------------------------------------------------------------------------
+ * Row operators over a cache slab: rotary append, attention with a sliding
+ * window and sinks, attention of a tree of drafted tokens, commit of the
+ * accepted path, fork of a stream.  For callers that compose their own step
+ * over several streams, transcribe without an end, or draft tokens.  No
+ * counterpart in the reference, whose cache is one stream's.
+ *
+ * They are enqueued on `stream` (NULL: the library's stream; the legacy
+ * default stream is (void *)1, cudaStreamLegacy) without a host wait, keep no
+ * workspace and allocate nothing: calls on different streams do not disturb
+ * each other, and a call may be captured into a CUDA graph and replayed (the
+ * positions, row ranges and trees are read on the device).  They run on the
+ * calling thread's device (vox_cuda_set_device), whichever device is current;
+ * all pointers belong to it.  Results do not depend on timing.
+ * ------------------------------------------------------------------------ */
+
+#define VOX_CUDA_F32  0
+#define VOX_CUDA_BF16 1
+#define VOX_CUDA_F16  2
+
+#define VOX_CUDA_TREE_MAX 256   /* rows of one stream's tree at most */
+#define VOX_CUDA_TOP_MAX  32    /* alternatives of one row at most */
+
+/* A slab of K and V: element (layer, stream, slot, head, dim) lies at
+ * layer * layer_stride + stream * stream_stride + slot * slot_stride +
+ * head * head_stride + dim.  A stride of 0 is the contiguous one for
+ * [layer][stream][slot][head][dim]; others are multiples of 16 bytes, and k
+ * and v are 16-byte aligned.  Positions j < n_sink of a stream stay in slot j
+ * for good (its sinks); later ones live in slot
+ * n_sink + (j - n_sink) mod (cap - n_sink), so the newest cap - n_sink of
+ * them are held.  Positions are at most 2^30. */
+typedef struct {
+    void *k, *v;                 /* device */
+    int dtype;                   /* VOX_CUDA_F32, _BF16 or _F16 */
+    int n_layers, n_streams, cap;
+    int n_kv_heads, head_dim;    /* head_dim 64 or 128 */
+    int n_sink;
+    long long layer_stride, stream_stride, slot_stride, head_stride;   /* elements */
+} vox_cuda_kv_cache;
+
+/* The rows of a call: stream s's are row_start[s] .. row_start[s + 1] - 1 of
+ * the row buffers and are stored at positions pos[s] + i, i = 0, 1, ...
+ * row_start NULL: one row for each stream.  A stream with no rows, or with a
+ * negative pos, sits out; its rows and rows behind the last stream's are left
+ * as they were.  max_rows bounds a stream's rows (rows beyond it are left
+ * out) and must fit the ring.  parent (trees): for each row the index of its
+ * parent among its stream's rows, an earlier one, or -1 for a root; row i
+ * then stands at the logical position pos[s] + depth(i), a root at pos[s]. */
+typedef struct {
+    const int *pos;              /* device [n_streams] */
+    const int *row_start;        /* device [n_streams + 1], or NULL */
+    const int *parent;           /* device [n_rows], or NULL */
+    int n_rows;                  /* rows of the row buffers */
+    int max_rows;                /* rows of one stream at most */
+} vox_cuda_rows;
+
+/* The KV ring of a decoder state as a slab of one stream (fp32, no sinks):
+ * stream 0's position is the state's.  Valid until the state is freed; order
+ * calls on other streams against the state's own steps. */
+int vox_cuda_dec_state_kv_cache(vox_cuda_dec_state *s, vox_cuda_kv_cache *cache);
+
+/* One pass over rows of fused q|k|v projections: q and k heads are normalised
+ * (RMS over head_dim, times q_norm / k_norm, fp32 [head_dim]; NULL: not) and
+ * rotated in interleaved pairs at their logical position (frequencies
+ * theta^(-2d / head_dim), as vox_compute_rope_freqs; theta 0: not); q goes to
+ * q_out [n_rows][n_heads][head_dim] of the cache's type, k and v to the rows'
+ * cache slots.  qkv: [n_rows] rows of n_heads + 2 * n_kv_heads heads,
+ * qkv_stride elements apart (0: contiguous), fp32 or of the cache's type.
+ * Several layers of a step call it once each. */
+int vox_cuda_rope_append_dev(const vox_cuda_kv_cache *cache, int layer, const vox_cuda_rows *rows, const void *qkv,
+                             int qkv_type, int n_heads, long long qkv_stride, const float *q_norm,
+                             const float *k_norm, float eps, float theta, void *q_out, void *stream);
+
+/* Attention of rows whose keys are in the cache already: row i, at position
+ * p = pos + i, sees the positions j <= p that the cache holds and that are
+ * among the n_sink first or the `window` last (j > p - window; window 0: no
+ * limit).  q, out: [n_rows][n_heads][head_dim] of the cache's type (out may
+ * be q); lse: fp32 [n_rows][n_heads] log of the sum of e^score (natural), or
+ * NULL.  n_heads: a multiple of n_kv_heads, at most 64 times as many; scale 0:
+ * 1 / sqrt(head_dim).  What a masked key holds, NaN included, does not
+ * matter; a row all of whose scores are -inf gets zeros and lse -inf. */
+int vox_cuda_attention_window_dev(const vox_cuda_kv_cache *cache, int layer, const vox_cuda_rows *rows,
+                                  const void *q, int n_heads, int window, float scale, void *out, float *lse,
+                                  void *stream);
+
+/* The same for a tree of drafted rows (rows->parent): row i, at the logical
+ * position p = pos + depth(i), sees the positions j < pos as above and, of the
+ * drafted rows, its ancestors and itself, by their logical positions. */
+int vox_cuda_attention_tree_dev(const vox_cuda_kv_cache *cache, int layer, const vox_cuda_rows *rows,
+                                const void *q, int n_heads, int window, float scale, void *out, float *lse,
+                                void *stream);
+
+/* Keep the accepted path of each stream's tree: in every layer the rows at
+ * pos[s] + path[s][k] move to pos[s] + k for k < n_accept[s].  path: device
+ * [n_streams][path_stride], indices of the stream's drafted rows, ascending;
+ * a path ends before an entry that does not ascend (or is beyond 255).
+ * n_accept: device [n_streams], at most max_accept (<= 256).  new_pos: device
+ * [n_streams] = pos + the rows kept, or NULL; not pos itself.  A stream with
+ * a negative pos sits out. */
+int vox_cuda_kv_commit_dev(const vox_cuda_kv_cache *cache, const int *pos, const int *path, int path_stride,
+                           const int *n_accept, int max_accept, int *new_pos, void *stream);
+
+/* Copy what stream src[i] holds - the slots that pos[src[i]] positions use -
+ * to stream dst[i], in every layer, for i < n (n <= 64; src, dst: host).  No
+ * stream is written twice, or both read and written.  pos: device
+ * [n_streams], the streams' lengths; the caller copies the position. */
+int vox_cuda_kv_fork_dev(const vox_cuda_kv_cache *cache, const int *src, const int *dst, int n, const int *pos,
+                         void *stream);
+
+/* Natural log probability of a given token, entropy (nats) and the n_top
+ * (0..32) most likely ids of each row of logits [n_rows][vocab], row_stride
+ * elements apart (0: vocab), fp32, bf16 or fp16.  tokens: device [n_rows] with
+ * logprob: device [n_rows] (both or neither; an id outside [0, vocab) gives
+ * NaN); entropy: device [n_rows] or NULL; top_ids, top_logprob: device
+ * [n_rows][n_top], best first, ties to the lowest id (top_logprob may be
+ * NULL).  A logit of -inf has probability 0; a row with a NaN or +inf, or
+ * without a finite logit, gives NaN, and NaN logits are no alternatives
+ * (places left over get id -1).  Enqueued on `stream` as the row operators. */
+int vox_cuda_token_logprobs_dev(const void *logits, int type, int n_rows, int vocab, long long row_stride,
+                                const int *tokens, int n_top, float *logprob, float *entropy, int *top_ids,
+                                float *top_logprob, void *stream);
 
 /* Diagnostics: runs a kernel whose bounded wait (the mbarrier wait with a
  * %globaltimer deadline that every tensor-core kernel uses) can never

@@ -155,6 +155,85 @@ cudaError_t launch_attn_decode(int M, const AttnParams &p, cudaStream_t st, bool
 cudaError_t launch_fill_alts(const float *logits, int vocab, const int *best, int n_alt,
                              float cutoff, int *out_ids, cudaStream_t st);
 
+// ---- row operators over a cache slab (vc_rt_ops.cu and its kernels) ----
+enum ElemType : int { ELEM_F32 = 0, ELEM_BF16 = 1, ELEM_F16 = 2 };
+constexpr int kMaxPosition = 1 << 30;   // the largest position of a row operator's stream
+constexpr int kTreeMax = 256;           // nodes of one stream's tree at most
+constexpr int kMaxGroup = 64;           // query heads per KV head at most
+constexpr int kForkMax = 64;            // (source, destination) pairs of one fork
+constexpr int kTopMax = 32;             // alternatives of one row at most
+
+struct CacheView {            // vox_cuda_kv_cache, checked
+    char *k, *v;              // layer 0, stream 0, slot 0, head 0
+    long long layer_stride, stream_stride, slot_stride, head_stride;   // elements
+    int dtype;                // ElemType
+    int n_layers, n_streams, cap, n_kv_heads, head_dim;
+    int n_sink, ring;         // ring = cap - n_sink
+};
+struct RowsView {             // vox_cuda_rows, checked
+    const int *pos, *start, *parent;
+    int n_rows, max_rows;
+};
+
+struct RowsAttnParams {
+    CacheView c;
+    RowsView r;
+    long long layer_off;      // elements from layer 0 to the call's layer
+    const void *q;            // [n_rows][n_heads][head_dim], the cache's type
+    void *out;                // the same shape and type
+    float *lse;               // [n_rows][n_heads] or NULL
+    int n_heads, group;       // group = n_heads / n_kv_heads
+    int window;               // 0: everything that the ring holds
+    float scale_log2;         // scale * log2(e)
+    int shares;               // key shares of a row tile (set by the launch)
+};
+cudaError_t launch_attn_rows(const RowsAttnParams &p, int sms, cudaStream_t st);
+
+struct AppendParams {
+    CacheView c;
+    RowsView r;
+    long long layer_off;
+    const void *qkv;          // [n_rows] rows of (n_heads + 2 n_kv_heads) heads
+    int src_type;             // ElemType of qkv
+    long long ld;             // elements between its rows
+    int n_heads;
+    const float *q_norm, *k_norm;   // [head_dim] or NULL
+    float eps;
+    int rotate;               // 0: q and k keep their angles
+    double log2_theta;
+    void *q_out;              // [n_rows][n_heads][head_dim], the cache's type
+};
+cudaError_t launch_rope_append(const AppendParams &p, cudaStream_t st);
+
+struct CommitParams {
+    CacheView c;
+    const int *pos, *path, *n_accept;
+    int path_ld, max_accept;
+    int *new_pos;
+};
+cudaError_t launch_kv_commit(const CommitParams &p, cudaStream_t st);
+
+struct ForkParams {
+    CacheView c;
+    const int *pos;
+    int n;
+    unsigned short src[kForkMax], dst[kForkMax];
+};
+cudaError_t launch_kv_fork(const ForkParams &p, int sms, cudaStream_t st);
+
+struct LogprobParams {
+    const void *logits;
+    int dtype;                // ElemType
+    int n_rows, vocab;
+    long long ld;             // elements between rows
+    const int *tokens;        // [n_rows] or NULL
+    int n_top;
+    float *logprob, *entropy; // [n_rows] or NULL
+    int *top_ids;             // [n_rows][n_top]
+    float *top_logprob;       // [n_rows][n_top] or NULL
+};
+cudaError_t launch_token_logprobs(const LogprobParams &p, int sms, cudaStream_t st);
+
 // ---- tcgen05 tensor-core GEMM (vc_gemm_tc.cu) ----
 enum TcEpi : int {
     TC_STORE = 0,     // out = acc (+ bias) (GELU if act == 1); fp32, or bf16 when out_bf16

@@ -1183,6 +1183,72 @@ extern "C" int vox_cuda_decoder_fill_alts(vox_cuda_dec_state *s, int n_alt, floa
     return n;
 }
 
+extern "C" int vox_cuda_decoder_token_logprobs(vox_cuda_dec_state *s, int token, int n_top, float *logprob,
+                                               float *entropy, int *top_ids, float *top_logprob) {
+    if (!s || n_top < 0 || n_top > kTopMax || n_top > s->dec->vocab || (n_top > 0 && (!top_ids || !top_logprob)) ||
+        token < 0 || token >= s->dec->vocab || !logprob || !entropy) {
+        set_error("decoder_token_logprobs: bad arguments");
+        return VOX_CUDA_ERR_ARG;
+    }
+    if (!s->have_logits) {
+        set_error("decoder_token_logprobs: no decode step since the last reset");
+        return VOX_CUDA_ERR_ARG;
+    }
+    DevCtx *c = ctx_for(s->dec->device);
+    if (!c) return VOX_CUDA_ERR_UNAVAILABLE;
+    cudaSetDevice(s->dec->device);
+    std::lock_guard<std::mutex> lk(c->mu);   // one user of the result buffer at a time
+    constexpr int kWords = 4 + 2 * kTopMax;  // token, logprob, entropy, -; top log probabilities; top ids
+    if (!c->lp_buf) {
+        if (cudaMalloc(&c->lp_buf, kWords * 4) != cudaSuccess) {
+            set_error("decoder_token_logprobs: allocation failed");
+            return VOX_CUDA_ERR_OOM;
+        }
+        c->bytes += kWords * 4;
+    }
+    VC_TRY(cudaMemcpyAsync(c->lp_buf, &token, sizeof(int), cudaMemcpyHostToDevice, c->stream));
+    LogprobParams p = {};
+    p.logits = s->work->logits;
+    p.dtype = ELEM_F32;
+    p.n_rows = 1;
+    p.vocab = s->dec->vocab;
+    p.ld = p.vocab;
+    p.tokens = reinterpret_cast<const int *>(c->lp_buf);
+    p.n_top = n_top;
+    p.logprob = c->lp_buf + 1;
+    p.entropy = c->lp_buf + 2;
+    p.top_logprob = c->lp_buf + 4;
+    p.top_ids = reinterpret_cast<int *>(c->lp_buf + 4 + kTopMax);
+    VC_TRY(launch_token_logprobs(p, c->sms, c->stream));
+    float h[kWords];
+    VC_TRY(cudaMemcpyAsync(h, c->lp_buf, sizeof(h), cudaMemcpyDeviceToHost, c->stream));
+    VC_TRY(cudaStreamSynchronize(c->stream));
+    *logprob = h[1];
+    *entropy = h[2];
+    if (n_top > 0) {
+        memcpy(top_logprob, h + 4, sizeof(float) * n_top);
+        memcpy(top_ids, h + 4 + kTopMax, sizeof(int) * n_top);
+    }
+    return n_top;
+}
+
+extern "C" int vox_cuda_dec_state_kv_cache(vox_cuda_dec_state *s, vox_cuda_kv_cache *cache) {
+    if (!s || !cache) {
+        set_error("dec_state_kv_cache: bad arguments");
+        return VOX_CUDA_ERR_ARG;
+    }
+    memset(cache, 0, sizeof(*cache));
+    cache->k = s->k_ring;
+    cache->v = s->v_ring;
+    cache->dtype = VOX_CUDA_F32;
+    cache->n_layers = s->dec->n_layers;
+    cache->n_streams = 1;
+    cache->cap = s->cap;
+    cache->n_kv_heads = kDecKvHeads;
+    cache->head_dim = kHeadDim;
+    return VOX_CUDA_OK;
+}
+
 extern "C" int vox_cuda_decoder_prefill_step(vox_cuda_dec_state *s, const float *x, int seq_len,
                                              const float *rope_freqs) {
     if (!s || !x || seq_len <= 0) {

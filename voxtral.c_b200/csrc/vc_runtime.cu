@@ -145,6 +145,7 @@ extern "C" int vox_cuda_init(void) {
         return 0;
     }
     c->device = dev;
+    c->sms = prop.multiProcessorCount;
     c->ready = true;
     t_device = dev;
     return 1;
@@ -172,6 +173,7 @@ static void release_scratch(DevCtx *c) {
     cudaFree(c->attn_part_ml);
     cudaFree(c->attn_counters);
     cudaFree(c->rope_tab);
+    cudaFree(c->lp_buf);
     cudaFree(c->lin_xfrag);
     cudaFree(c->lin_err);
     if (c->lin_done) cudaEventDestroy(c->lin_done);
@@ -184,7 +186,7 @@ static void release_scratch(DevCtx *c) {
     c->sx = c->sy = c->sb = nullptr;
     c->sx_n = c->sy_n = c->sb_n = 0;
     c->attn_slot = nullptr;
-    c->attn_part_o = c->attn_part_ml = c->rope_tab = nullptr;
+    c->attn_part_o = c->attn_part_ml = c->rope_tab = c->lp_buf = nullptr;
     c->attn_counters = nullptr;
 }
 

@@ -39,6 +39,7 @@ constexpr int kMaxDevices = 16;
 struct DevCtx {
     int device = -1;
     bool ready = false;
+    int sms = 148;                  // multiprocessors
     cudaStream_t stream = nullptr;
     std::mutex mu;                  // guards the cache and the scratch below
     size_t bytes = 0;               // device bytes held by the library
@@ -66,6 +67,7 @@ struct DevCtx {
     float *attn_part_o = nullptr, *attn_part_ml = nullptr, *rope_tab = nullptr;
     unsigned *attn_counters = nullptr;
     cudaEvent_t attn_done = nullptr;   // orders the attention scratch across caller streams
+    float *lp_buf = nullptr;           // results of vox_cuda_decoder_token_logprobs
 };
 
 int current_device();

@@ -151,6 +151,11 @@ __device__ __forceinline__ float2 ld_dsmem_f2(uint32_t addr_cluster) {
     asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr_cluster) : "memory");
     return v;
 }
+__device__ __forceinline__ float ld_dsmem_f1(uint32_t addr_cluster) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr_cluster) : "memory");
+    return v;
+}
 // shared::cluster address of the variable at shared::cta address `addr` in CTA `rank`
 __device__ __forceinline__ uint32_t mapa_shared(uint32_t addr, uint32_t rank) {
     uint32_t r;

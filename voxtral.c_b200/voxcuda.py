@@ -63,6 +63,36 @@ class _EncW(C.Structure):
                 ("adapter0", C.c_void_p), ("adapter1", C.c_void_p), ("layers", _EncLayerW * 32)]
 
 
+TYPES = {"fp32": 0, "bf16": 1, "fp16": 2}   # VOX_CUDA_F32, _BF16, _F16
+STREAM_LEGACY = 1                           # cudaStreamLegacy: the default stream as a handle
+TREE_MAX, TOP_MAX = 256, 32
+
+
+class KvCache(C.Structure):
+    """A slab of K and V (vox_cuda_kv_cache); k and v are device addresses,
+    dtype a name of TYPES, strides in elements (0: contiguous)."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("dtype", C.c_int), ("n_layers", C.c_int), ("n_streams", C.c_int),
+                ("cap", C.c_int), ("n_kv_heads", C.c_int), ("head_dim", C.c_int), ("n_sink", C.c_int),
+                ("layer_stride", C.c_longlong), ("stream_stride", C.c_longlong), ("slot_stride", C.c_longlong),
+                ("head_stride", C.c_longlong)]
+
+    def __init__(self, k=None, v=None, dtype="fp32", n_layers=1, n_streams=1, cap=0, n_kv_heads=8, head_dim=128, n_sink=0,
+                 layer_stride=0, stream_stride=0, slot_stride=0, head_stride=0):
+        super().__init__(k, v, TYPES[dtype], n_layers, n_streams, cap, n_kv_heads, head_dim, n_sink, layer_stride,
+                         stream_stride, slot_stride, head_stride)
+
+
+class Rows(C.Structure):
+    """The rows of a call (vox_cuda_rows): device addresses of the streams'
+    positions, their row ranges (None: one row each) and the rows' parents
+    (None: no tree)."""
+    _fields_ = [("pos", C.c_void_p), ("row_start", C.c_void_p), ("parent", C.c_void_p), ("n_rows", C.c_int),
+                ("max_rows", C.c_int)]
+
+    def __init__(self, pos, row_start=None, parent=None, n_rows=0, max_rows=1):
+        super().__init__(pos, row_start, parent, n_rows, max_rows)
+
+
 _lib = None
 
 
@@ -149,6 +179,20 @@ def lib():
                                                C.c_int, C.c_void_p, C.c_void_p], C.c_int),
         "vox_cuda_rope_dev": ([C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_void_p, C.c_void_p],
                               C.c_int),
+        "vox_cuda_decoder_token_logprobs": ([C.c_void_p, C.c_int, C.c_int, _fp, _fp, _ip, _fp], C.c_int),
+        "vox_cuda_dec_state_kv_cache": ([C.c_void_p, C.POINTER(KvCache)], C.c_int),
+        "vox_cuda_rope_append_dev": ([C.POINTER(KvCache), C.c_int, C.POINTER(Rows), C.c_void_p, C.c_int, C.c_int,
+                                      C.c_longlong, C.c_void_p, C.c_void_p, C.c_float, C.c_float, C.c_void_p,
+                                      C.c_void_p], C.c_int),
+        "vox_cuda_attention_window_dev": ([C.POINTER(KvCache), C.c_int, C.POINTER(Rows), C.c_void_p, C.c_int, C.c_int,
+                                           C.c_float, C.c_void_p, C.c_void_p, C.c_void_p], C.c_int),
+        "vox_cuda_attention_tree_dev": ([C.POINTER(KvCache), C.c_int, C.POINTER(Rows), C.c_void_p, C.c_int, C.c_int,
+                                         C.c_float, C.c_void_p, C.c_void_p, C.c_void_p], C.c_int),
+        "vox_cuda_kv_commit_dev": ([C.POINTER(KvCache), C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, C.c_int,
+                                    C.c_void_p, C.c_void_p], C.c_int),
+        "vox_cuda_kv_fork_dev": ([C.POINTER(KvCache), _ip, _ip, C.c_int, C.c_void_p, C.c_void_p], C.c_int),
+        "vox_cuda_token_logprobs_dev": ([C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_longlong, C.c_void_p, C.c_int,
+                                         C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p], C.c_int),
         "vox_cuda_fill_normal_bf16_dev": ([C.c_void_p, C.c_size_t, C.c_uint64, C.c_float,
                                            C.c_void_p], C.c_int),
     }
@@ -277,6 +321,21 @@ class DecState:
                   "fill_alts")
         return ids[:n].tolist()
 
+    def token_logprobs(self, token, n_top=0):
+        """(log probability, entropy, top ids, their log probabilities) of the
+        last step's logits."""
+        one = np.empty(2, np.float32)
+        ids, lp = np.empty(TOP_MAX, np.int32), np.empty(TOP_MAX, np.float32)
+        n = check(lib().vox_cuda_decoder_token_logprobs(self.h, token, n_top, _f(one[:1]), _f(one[1:]),
+                                                        ids.ctypes.data_as(_ip), _f(lp)), "token_logprobs")
+        return float(one[0]), float(one[1]), ids[:n], lp[:n]
+
+    def kv_cache(self):
+        """The state's KV ring as a slab of one stream, for the row operators."""
+        c = KvCache()
+        check(lib().vox_cuda_dec_state_kv_cache(self.h, C.byref(c)), "dec_state_kv_cache")
+        return c
+
     def load_kv(self, layer, first_pos, k_rows, v_rows):
         k_rows = np.ascontiguousarray(k_rows, np.float32)
         v_rows = np.ascontiguousarray(v_rows, np.float32)
@@ -327,6 +386,45 @@ def attention_decode_dev(q, k_ring, v_ring, kv_cap, pos, out, stream=None):
     """Stand-alone decode attention on device addresses."""
     check(lib().vox_cuda_attention_decode_dev(q, k_ring, v_ring, kv_cap, pos, out, stream),
           "attention_decode_dev")
+
+
+def rope_append_dev(cache, layer, rows, qkv, qkv_type, n_heads, qkv_stride, q_norm, k_norm, eps, theta, q_out, stream=None):
+    """Norm (optional), rotation and cache write of fused q|k|v rows."""
+    check(lib().vox_cuda_rope_append_dev(cache, layer, rows, qkv, TYPES[qkv_type], n_heads, qkv_stride, q_norm, k_norm, eps,
+                                         theta, q_out, stream), "rope_append_dev")
+
+
+def attention_window_dev(cache, layer, rows, q, n_heads, window, scale, out, lse=None, stream=None):
+    """Attention of rows over the cache, with a sliding window and its sinks."""
+    check(lib().vox_cuda_attention_window_dev(cache, layer, rows, q, n_heads, window, scale, out, lse, stream),
+          "attention_window_dev")
+
+
+def attention_tree_dev(cache, layer, rows, q, n_heads, window, scale, out, lse=None, stream=None):
+    """Attention of trees of drafted rows over the cache."""
+    check(lib().vox_cuda_attention_tree_dev(cache, layer, rows, q, n_heads, window, scale, out, lse, stream),
+          "attention_tree_dev")
+
+
+def kv_commit_dev(cache, pos, path, path_stride, n_accept, max_accept, new_pos=None, stream=None):
+    """Move each stream's accepted path to consecutive positions."""
+    check(lib().vox_cuda_kv_commit_dev(cache, pos, path, path_stride, n_accept, max_accept, new_pos, stream),
+          "kv_commit_dev")
+
+
+def kv_fork_dev(cache, src, dst, pos, stream=None):
+    """Copy what streams src hold to streams dst (lists of stream indices)."""
+    if len(src) != len(dst):
+        raise ValueError("kv_fork_dev: as many sources as destinations")
+    arr = C.c_int * len(src)
+    check(lib().vox_cuda_kv_fork_dev(cache, arr(*src), arr(*dst), len(src), pos, stream), "kv_fork_dev")
+
+
+def token_logprobs_dev(logits, dtype, n_rows, vocab, row_stride, tokens, n_top, logprob, entropy, top_ids, top_logprob,
+                       stream=None):
+    """Log probabilities of given tokens, entropy and top alternatives."""
+    check(lib().vox_cuda_token_logprobs_dev(logits, TYPES[dtype], n_rows, vocab, row_stride, tokens, n_top, logprob, entropy,
+                                            top_ids, top_logprob, stream), "token_logprobs_dev")
 
 
 def prefill_batch(states, rows, rope=None):
