@@ -186,8 +186,11 @@ struct RowsAttnParams {
     int window;               // 0: everything that the ring holds
     float scale_log2;         // scale * log2(e)
     int shares;               // key shares of a row tile (set by the launch)
+    unsigned *err;            // raised when a bounded wait expires (mapped host memory)
 };
 cudaError_t launch_attn_rows(const RowsAttnParams &p, int sms, cudaStream_t st);
+// the tensor-core kernel of the 16-bit types (vc_attn_rows_tc.cu)
+cudaError_t launch_attn_rows_tc(const RowsAttnParams &p, int sms, cudaStream_t st);
 
 struct AppendParams {
     CacheView c;

@@ -145,6 +145,13 @@ int check_heads(const char *who, int n_heads, const CacheView &c) {
     return VOX_CUDA_ERR_ARG;
 }
 
+// A wait that ran out in an earlier call's kernel is reported once.
+int check_waits(const char *who, DevCtx *c) {
+    if (!__atomic_exchange_n(c->op_err, 0u, __ATOMIC_RELAXED)) return VOX_CUDA_OK;
+    set_error("%s: a device-side wait of an earlier call timed out (its results are void)", who);
+    return VOX_CUDA_ERR_CUDA;
+}
+
 int launched(const char *who, cudaError_t e) {
     if (e == cudaSuccess) return VOX_CUDA_OK;
     set_error("%s: %s", who, cudaGetErrorString(e));
@@ -175,6 +182,8 @@ int attention(const char *who, bool tree, const vox_cuda_kv_cache *cache, int la
     if (!c) return VOX_CUDA_ERR_UNAVAILABLE;
     DeviceGuard guard(c->device);
     if (!guard.ok()) return launched(who, cudaGetLastError());
+    if ((rc = check_waits(who, c))) return rc;
+    p.err = c->op_err;
     p.layer_off = (long long)layer * p.c.layer_stride;
     p.q = q;
     p.out = out;

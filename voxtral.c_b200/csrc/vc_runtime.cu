@@ -144,6 +144,12 @@ extern "C" int vox_cuda_init(void) {
         set_error("vox_cuda_init: stream creation failed");
         return 0;
     }
+    if (cudaHostAlloc((void **)&c->op_err, sizeof(unsigned), cudaHostAllocMapped | cudaHostAllocPortable) != cudaSuccess) {
+        cudaStreamDestroy(c->stream);
+        set_error("vox_cuda_init: allocation failed");
+        return 0;
+    }
+    *c->op_err = 0;
     c->device = dev;
     c->sms = prop.multiProcessorCount;
     c->ready = true;
@@ -212,6 +218,8 @@ extern "C" void vox_cuda_shutdown(void) {
         release_scratch(c);
         cudaStreamDestroy(c->stream);
         c->stream = nullptr;
+        cudaFreeHost(c->op_err);
+        c->op_err = nullptr;
         c->bytes = 0;
         c->ready = false;
     }

@@ -67,6 +67,7 @@ struct DevCtx {
     float *attn_part_o = nullptr, *attn_part_ml = nullptr, *rope_tab = nullptr;
     unsigned *attn_counters = nullptr;
     cudaEvent_t attn_done = nullptr;   // orders the attention scratch across caller streams
+    unsigned *op_err = nullptr;        // mapped host word: a row operator's bounded wait ran out
     float *lp_buf = nullptr;           // results of vox_cuda_decoder_token_logprobs
 };
 
