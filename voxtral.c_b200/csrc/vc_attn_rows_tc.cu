@@ -7,11 +7,11 @@
 //   warps 0-3, 4-7   softmax of tile 0 and 1, thread = packed row: the block's
 //                    maximum over S (TMEM), then P = 2^(s - m), rounded to
 //                    the cache's type, over S in TMEM
-//   warps 8-11       loads: Q once, then K and V blocks by 16-byte cp.async
-//                    into the 128-byte-swizzled operand layout, two blocks
-//                    deep, each row from its own slot (ring wrap, sinks and
-//                    any stride need no descriptor; rows past the end are
-//                    zeros)
+//   warps 8-11       loads: Q once, then two warps K and two V blocks by
+//                    16-byte cp.async into the 128-byte-swizzled operand
+//                    layout, two blocks deep, each row from its own slot
+//                    (ring wrap, sinks and any stride need no descriptor;
+//                    rows past the end are zeros)
 //   warp 12          one thread issues the MMAs, M 128:
 //                    S_t = Q_t K^T (N 128, K HD) and O_t += P_t V (N HD,
 //                    K 128; A from TMEM, V an MN-major operand)
@@ -46,7 +46,7 @@ namespace {
 
 constexpr int kAtKeys = 128;            // keys per block
 constexpr int kAtRows = 128;            // packed rows per tile = TMEM lanes
-constexpr int kAtLoaders = 128;         // loading threads
+constexpr int kAtLoaders = 64;          // threads that load K, and as many that load V
 constexpr int kAtThreads = 13 * 32;
 constexpr uint64_t kAtWaitNs = 2000000000ull;
 constexpr float kAtRescale = 8.0f;      // log2 of the largest P before the maximum moves
@@ -163,7 +163,7 @@ __global__ void __launch_bounds__(kAtThreads, 1) attn_rows_tc_kernel(const RowsA
     auto whole = [&](int b) { return b * kAtKeys >= core_s && (b + 1) * kAtKeys <= core_e; };
 
     if (threadIdx.x == 0) {
-        mbar_init(&sh.q_full, kAtLoaders);
+        mbar_init(&sh.q_full, 2 * kAtLoaders);
         for (int i = 0; i < 2; i++) {
             mbar_init(&sh.k_full[i], kAtLoaders);
             mbar_init(&sh.v_full[i], kAtLoaders);
@@ -191,8 +191,9 @@ __global__ void __launch_bounds__(kAtThreads, 1) attn_rows_tc_kernel(const RowsA
     constexpr uint32_t kOCol = NT * kAtKeys;   // S tiles first, then O tiles
 
     if (warp >= 8 && warp < 12) {
-        // ---- loads ----
-        const int tid = threadIdx.x - 256;
+        // ---- loads: warps 8, 9 K, warps 10, 11 V, all of them Q ----
+        const int tid = threadIdx.x & (kAtLoaders - 1);
+        const bool is_v = warp >= 10;
         constexpr int kCh = HD / 8;                   // 16-byte chunks per row
         constexpr int kRowsAtOnce = kAtLoaders / kCh;
         const int ch = tid % kCh, jr = tid / kCh;
@@ -201,8 +202,8 @@ __global__ void __launch_bounds__(kAtThreads, 1) attn_rows_tc_kernel(const RowsA
         for (int t = 0; t < tiles; t++) {
             const uint32_t dst = smem_u32(sh.q[t]);
 #pragma unroll
-            for (int it = 0; it < kAtRows / kRowsAtOnce; it++) {
-                const int r = it * kRowsAtOnce + jr, m = m0 + t * kAtRows + r;
+            for (int it = 0; it < kAtRows / 2 / kRowsAtOnce; it++) {
+                const int r = (2 * it + is_v) * kRowsAtOnce + jr, m = m0 + t * kAtRows + r;
                 const T *src = static_cast<const T *>(p.q);
                 if (m < M) src += ((long long)(s.r0 + m / p.group) * p.n_heads + head0 + m % p.group) * HD + ch * 8;
                 cp_async16(dst + at(r), src, m < M);
@@ -210,20 +211,14 @@ __global__ void __launch_bounds__(kAtThreads, 1) attn_rows_tc_kernel(const RowsA
         }
         cp_async_commit();
         const long long base = p.layer_off + (long long)stream * p.c.stream_stride + (long long)kvh * p.c.head_stride;
-        const char *kb = p.c.k + base * 2 + ch * 16, *vb = p.c.v + base * 2 + ch * 16;
+        const char *src = (is_v ? p.c.v : p.c.k) + base * 2 + ch * 16;
         const long long slot_bytes = p.c.slot_stride * 2;
         const int lo_slot = cache_slot(p.c, kr.lo);
-        // groups: 2b for K of block b, 2b + 1 for V; buffers g % 2 of K / V
-        auto buffer = [&](int g) { return sh.kv[(g & 1) * 2 + ((g >> 1) & 1)]; };
-        auto publish = [&](int g) {
-            if (g < 0) {   // Q
-                fence_async_smem();
-                mbar_arrive(&sh.q_full);
-                return;
-            }
-            const int b = g >> 1;
-            if ((g & 1) && !whole(b0 + b)) {
-                unsigned char *v = buffer(g);
+        unsigned char *const bufs = sh.kv[is_v ? 2 : 0];
+        uint64_t *const full = is_v ? sh.v_full : sh.k_full, *const empty = is_v ? sh.v_empty : sh.k_empty;
+        auto publish = [&](int b) {   // block b (of this share) has landed
+            if (is_v && !whole(b0 + b)) {
+                unsigned char *v = bufs + (b & 1) * Sm::kTile;
                 bool found = false;
 #pragma unroll 4
                 for (int it = 0; it < kAtKeys / kRowsAtOnce; it++) {
@@ -238,46 +233,46 @@ __global__ void __launch_bounds__(kAtThreads, 1) attn_rows_tc_kernel(const RowsA
                 if (found) atomicExch(&sh.bad, 1);
             }
             fence_async_smem();
-            mbar_arrive((g & 1) ? &sh.v_full[b & 1] : &sh.k_full[b & 1]);
+            if (b == 0) mbar_arrive(&sh.q_full);   // Q was ahead of it
+            mbar_arrive(&full[b & 1]);
         };
-        int told = -1;   // groups before this one are published (-1: Q is next)
-        for (int g = 0; g < 2 * nb; g++) {
-            const int b = g >> 1;
-            if (b >= 2) {
-                uint64_t *empty = (g & 1) ? &sh.v_empty[b & 1] : &sh.k_empty[b & 1];
-                const uint32_t parity = ((b >> 1) + 1) & 1u;
-                if (!mbar_try_wait(empty, parity)) {
-                    // the consumer may be waiting for a group that has landed: publish all before waiting
-                    cp_async_wait<0>();
-                    while (told < g) publish(told++);
-                    if (!mbar_wait(empty, parity, deadline)) {
-                        ok = false;
-                        break;
-                    }
-                }
+        for (int b = 0; b < nb; b++) {
+            if (b >= 2 && !mbar_wait(&empty[b & 1], ((b >> 1) + 1) & 1u, deadline)) {
+                ok = false;
+                break;
             }
-            const uint32_t dst = smem_u32(buffer(g));
-            const char *src = (g & 1) ? vb : kb;
+            const uint32_t dst = smem_u32(bufs + (b & 1) * Sm::kTile);
             const int idx0 = (b0 + b) * kAtKeys;
-#pragma unroll
-            for (int it = 0; it < kAtKeys / kRowsAtOnce; it++) {
-                const int r = it * kRowsAtOnce + jr, idx = idx0 + r;
-                int slot = idx;
-                if (idx >= kr.ns) {
-                    slot = lo_slot + (idx - kr.ns);
-                    if (slot >= p.c.cap) slot -= p.c.ring;
+            int slot0 = lo_slot + (idx0 - kr.ns);   // of index idx0, past the sinks
+            if (slot0 >= p.c.cap) slot0 -= p.c.ring;
+            if (idx0 >= kr.ns && idx0 + kAtKeys <= total && slot0 + kAtKeys <= p.c.cap) {
+                const char *a = src + (slot0 + jr) * slot_bytes;   // 128 slots in a row
+                const long long step = kRowsAtOnce * slot_bytes;
+#pragma unroll 8
+                for (int it = 0; it < kAtKeys / kRowsAtOnce; it++) {
+                    cp_async16(dst + at(it * kRowsAtOnce + jr), a, true);
+                    a += step;
                 }
-                cp_async16(dst + at(r), src + (idx < total ? slot * slot_bytes : 0), idx < total);
+            } else {
+#pragma unroll 4
+                for (int it = 0; it < kAtKeys / kRowsAtOnce; it++) {
+                    const int r = it * kRowsAtOnce + jr, idx = idx0 + r;
+                    int slot = idx;
+                    if (idx >= kr.ns) {
+                        slot = lo_slot + (idx - kr.ns);
+                        if (slot >= p.c.cap) slot -= p.c.ring;
+                    }
+                    cp_async16(dst + at(r), src + (idx < total ? slot * slot_bytes : 0), idx < total);
+                }
             }
             cp_async_commit();
-            if (g - 3 >= told) {
-                cp_async_wait<3>();   // Q and the groups up to g - 3 have landed
-                while (told <= g - 3) publish(told++);
+            if (b >= 1) {
+                cp_async_wait<1>();
+                publish(b - 1);
             }
         }
         cp_async_wait<0>();
-        if (ok)
-            while (told < 2 * nb) publish(told++);
+        if (ok && nb > 0) publish(nb - 1);
     } else if (warp == 12) {
         // ---- MMAs ----
         if (lane == 0 && nb > 0) {
