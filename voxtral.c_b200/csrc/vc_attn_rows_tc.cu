@@ -4,28 +4,26 @@
 // A CTA takes NT (1 or 2) tiles of 128 packed query rows (m = row * group +
 // head, TMEM lane = packed row) of one (stream, KV head) and a share of the
 // 128-key blocks that they see; the shares of a tile pair are a cluster.
-//   warps 0-3, 4-7   softmax of tile 0 and 1, thread = packed row: the block's
-//                    maximum over S (TMEM), then P = 2^(s - m), rounded to
-//                    the cache's type, over S in TMEM
-//   warps 8-11       loads: Q once, then two warps K and two V blocks by
-//                    16-byte cp.async into the 128-byte-swizzled operand
-//                    layout, two blocks deep, each row from its own slot
-//                    (ring wrap, sinks and any stride need no descriptor;
-//                    rows past the end are zeros)
-//   warp 12          one thread issues the MMAs, M 128:
-//                    S_t = Q_t K^T (N 128, K HD) and O_t += P_t V (N HD,
-//                    K 128; A from TMEM, V an MN-major operand)
-// Per block and tile 2 x 128 x 128 x HD multiply-adds meet 128 x 128
-// exponentials: at HD 128 the tensor pipe and the exponential unit are both
-// full at the same time, so two tiles alternate - one's softmax runs under the
-// other's MMAs - and share each K and V block.
+//   warps 0-3, 4-7   softmax of tile 0 and 1, thread = packed row, 64 keys a
+//                    step: P = 2^(s - m) of S (TMEM), rounded to the cache's
+//                    type, over the S columns it came from
+//   warps 8, 9, 11   loads: Q once; K (warp 8) and V blocks two deep, by TMA
+//                    where a block's slots follow one another, by 16-byte
+//                    cp.async into the same swizzled layout where they do not
+//                    (ring wrap, sinks, the last block: zeros past the end)
+//   warp 10          issues the MMAs, M 128: S_t = Q_t K^T (N 128, K HD) and,
+//                    by halves, O_t += P_t V (N HD, K 64; A from TMEM, V an
+//                    MN-major operand)
+// S_t(b + 1) overwrites P_t(b), so it is issued behind the MMAs that read it.
+// Two tiles alternate - one's softmax runs under the other's MMAs - and share
+// each K and V block.  (S in two column ranges of 64, so that S(n + 1) runs
+// under the softmax of S(n), was slower: an MMA of N 64 takes as long as one of
+// N 128, reading its A tile.)
 //
-// S_t(b + 1) overwrites P_t(b), so it is issued behind O_t += P_t(b) V(b); its
-// completion therefore also says that O_t may be rescaled.  The running
-// maximum moves only when a block exceeds it by more than 2^8 (P <= 256 in
-// either type), and only then O is rescaled.  Rounding P to 16 bits is one
-// half step of the type per weight, as the output's own rounding; the sums l
-// take the unrounded weights.
+// The running maximum moves only when a step exceeds it by more than 2^8
+// (P <= 256 in either type), and only then O is rescaled.  Rounding P to 16
+// bits is one half step of the type per weight, as the output's own rounding;
+// the sums l take the unrounded weights.
 //
 // Zero times a masked key's NaN or infinity would be NaN: in blocks that some
 // row does not see whole, the loading threads look for non-finite V values,
@@ -45,9 +43,9 @@ using namespace tc;
 namespace {
 
 constexpr int kAtKeys = 128;            // keys per block
+constexpr int kAtHalf = 64;             // keys per softmax step: half a block
 constexpr int kAtRows = 128;            // packed rows per tile = TMEM lanes
-constexpr int kAtLoaders = 64;          // threads that load K, and as many that load V
-constexpr int kAtThreads = 13 * 32;
+constexpr int kAtThreads = 12 * 32;      // three warps per SM quarter: 168 registers
 constexpr uint64_t kAtWaitNs = 2000000000ull;
 constexpr float kAtRescale = 8.0f;      // log2 of the largest P before the maximum moves
 constexpr int kAtOneCta = 120 * 1024;   // more than half an SM's shared memory: one CTA per SM
@@ -60,7 +58,7 @@ struct AtSmem {
     uint32_t anc[NT * kAtRows][kTreeMax / 32];
     float mx[NT * kAtRows], sum[NT * kAtRows];
     short parent[kTreeMax];
-    uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[NT], p_full[NT], o_done;
+    uint64_t q_full, v_land[2], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[NT], p_full[NT][2], o_half[NT], o_done;
     uint32_t tmem;
     int bad;      // a masked block holds non-finite V values
 };
@@ -79,25 +77,71 @@ __device__ __forceinline__ uint64_t at_desc_mn(const void *p) {
            (2ull << 61);
 }
 
-// D[tmem] (+)= A[tmem] . B[smem]: A holds two 16-bit values per column.
-__device__ __forceinline__ void tc_mma_f16_ta(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
-                                              uint32_t accumulate) {
+// A bounded wait of a whole warp: the same answer in every lane.
+__device__ __forceinline__ bool warp_wait(uint64_t *bar, uint32_t parity, uint64_t deadline) {
+    return __all_sync(0xffffffffu, mbar_wait(bar, parity, deadline));
+}
+
+// The MMA warp's instructions: all 32 lanes reach them and `lead` is set in
+// one, so that the warp never diverges and its operands stay in uniform
+// registers (issued from a branch of one lane each MMA took ~75 cycles).
+// D[tmem] (+)= A[smem] . B[smem]
+__device__ __forceinline__ void warp_mma(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                         uint32_t accumulate, uint32_t lead) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
-        "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(lead)
+        : "memory");
+}
+// D[tmem] (+)= A[tmem] . B[smem]: A holds two 16-bit values per column
+__device__ __forceinline__ void warp_mma_ta(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
+                                            uint32_t accumulate, uint32_t lead) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(lead)
+        : "memory");
+}
+__device__ __forceinline__ void warp_commit(uint64_t *bar, uint32_t lead) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar)),
+        "r"(lead)
         : "memory");
 }
 
-// 16 columns of this thread's TMEM lane
-__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16]) {
+// Columns of this thread's TMEM lane: a store is complete after tmem_wait_st,
+// a load after tmem_ld_wait, which names the values so that no use moves ahead
+// of it.
+__device__ __forceinline__ void tmem_st32_async(uint32_t taddr, const uint32_t *v) {
     asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(
-            taddr),
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+        "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+        "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
         "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
-        "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+        "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]),
+        "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]),
+        "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
         : "memory");
+}
+__device__ __forceinline__ void tmem_ld16_async(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_ld_wait(uint32_t (&r)[16]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]),
+                   "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+                 :
+                 : "memory");
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
@@ -125,6 +169,102 @@ struct RowKeys {
     }
 };
 
+// Two fp32 values per register pair: one issue slot for two results.
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void unpair(uint64_t p, float &a, float &b) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ float fmax_nan(float a, float b) {   // NaN if either is
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+
+// 2^x of two values on the FMA pipe: x = n + f, n the nearest whole number
+// (left in the low bits by adding 1.5 * 2^23), 2^f by its minimax polynomial
+// of degree 4 on [-1/2, 1/2] (Remez: relative error 2.6e-6, of either sign),
+// n added to the exponent.  Below -126 the result stays near 2^-126.
+__device__ __forceinline__ void exp2_poly2(float &a, float &b) {
+    const uint64_t x = pair(fmax_nan(a, -126.f), fmax_nan(b, -126.f));
+    const uint64_t t = add2(x, pair(12582912.f, 12582912.f));
+    const uint64_t f = fma2(add2(t, pair(-12582912.f, -12582912.f)), pair(-1.f, -1.f), x);
+    uint64_t r = fma2(f, pair(0.00957010201463f, 0.00957010201463f), pair(0.0559178603063f, 0.0559178603063f));
+    r = fma2(f, r, pair(0.24024744825f, 0.24024744825f));
+    r = fma2(f, r, pair(0.693121814743f, 0.693121814743f));
+    r = fma2(f, r, pair(0.999999261447f, 0.999999261447f));
+    float ta, tb;
+    unpair(t, ta, tb);
+    unpair(r, a, b);
+    a = __int_as_float(__float_as_int(a) + (__float_as_int(ta) << 23));
+    b = __int_as_float(__float_as_int(b) + (__float_as_int(tb) << 23));
+}
+
+// Half a block of a row: w = 2^(s sl2 - base) as pairs of T, ls their sum
+// before rounding; the largest s sl2 - base as the result (NaN if one is).
+// The next 16 scores are on their way from TMEM while 16 are worked on.  The
+// exponential unit takes 8 cycles per warp, so in blocks without a mask
+// kAtPoly of 8 pairs go through the FMA pipe instead.
+constexpr int kAtPoly = 3;
+template <typename T, bool MASKED>
+__device__ __forceinline__ float weigh_half(uint32_t ts, float sl2, float base, const RowKeys &keys, int c0,
+                                            const uint32_t *anc, uint32_t (&w)[kAtHalf / 2], float &ls) {
+    float mx[2] = {-INFINITY, -INFINITY};
+    uint64_t rs[2] = {0, 0};
+    const uint64_t sl = pair(sl2, sl2), nb = pair(-base, -base);
+    uint32_t ra[16], rb[16], vis = 0xffffffffu;
+    tmem_ld16_async(ts, ra);
+#pragma unroll
+    for (int c = 0; c < kAtHalf; c += 16) {
+        uint32_t(&cur)[16] = (c & 16) ? rb : ra;
+        tmem_ld_wait(cur);
+        if (c + 16 < kAtHalf) tmem_ld16_async(ts + c + 16, (c & 16) ? ra : rb);
+        if (MASKED) vis = (c & 16) ? vis >> 16 : keys.bits(c0 + c, anc);
+#pragma unroll
+        for (int j = 0; j < 16; j += 2) {
+            float xa, xb;
+            unpair(fma2(pair(__uint_as_float(cur[j]), __uint_as_float(cur[j + 1])), sl, nb), xa, xb);
+            if (MASKED) {
+                xa = (vis >> j) & 1u ? xa : -INFINITY;
+                xb = (vis >> (j + 1)) & 1u ? xb : -INFINITY;
+            }
+            mx[0] = fmax_nan(mx[0], xa);
+            mx[1] = fmax_nan(mx[1], xb);
+            if (!MASKED && (j >> 1) % 8 < kAtPoly) {
+                exp2_poly2(xa, xb);
+            } else {
+                xa = exp2_approx(xa);
+                xb = exp2_approx(xb);
+            }
+            rs[(j >> 1) & 1] = add2(rs[(j >> 1) & 1], pair(xa, xb));
+            w[(c + j) >> 1] = pack2<T>(xa, xb);
+        }
+    }
+    float a, b;
+    unpair(add2(rs[0], rs[1]), a, b);
+    ls = a + b;
+    return fmax_nan(mx[0], mx[1]);
+}
+template <typename T>
+__device__ __forceinline__ float weigh(uint32_t ts, float sl2, float base, bool full, const RowKeys &keys, int c0,
+                                       const uint32_t *anc, uint32_t (&w)[kAtHalf / 2], float &ls) {
+    return full ? weigh_half<T, false>(ts, sl2, base, keys, c0, anc, w, ls)
+                : weigh_half<T, true>(ts, sl2, base, keys, c0, anc, w, ls);
+}
+
 template <typename T>
 __device__ __forceinline__ uint32_t nonfinite2(uint32_t u) {   // 0xffff in each half that is inf or NaN
     constexpr uint32_t e = std::is_same<T, __nv_bfloat16>::value ? 0x7f807f80u : 0x7c007c00u;
@@ -132,7 +272,9 @@ __device__ __forceinline__ uint32_t nonfinite2(uint32_t u) {   // 0xffff in each
 }
 
 template <typename T, int HD, int NT>
-__global__ void __launch_bounds__(kAtThreads, 1) attn_rows_tc_kernel(const RowsAttnParams p) {
+__global__ void __launch_bounds__(kAtThreads, 1) attn_rows_tc_kernel(const __grid_constant__ CUtensorMap tm_k,
+                                                                   const __grid_constant__ CUtensorMap tm_v,
+                                                                   const RowsAttnParams p) {
     using Sm = AtSmem<HD, NT>;
     constexpr int kSub = HD / 64;            // 64-dim sub-tiles of a tile
     constexpr uint32_t kTmemCols = NT == 2 ? 512 : 256;
@@ -163,23 +305,29 @@ __global__ void __launch_bounds__(kAtThreads, 1) attn_rows_tc_kernel(const RowsA
     auto whole = [&](int b) { return b * kAtKeys >= core_s && (b + 1) * kAtKeys <= core_e; };
 
     if (threadIdx.x == 0) {
-        mbar_init(&sh.q_full, 2 * kAtLoaders);
+        mbar_init(&sh.q_full, 96);
         for (int i = 0; i < 2; i++) {
-            mbar_init(&sh.k_full[i], kAtLoaders);
-            mbar_init(&sh.v_full[i], kAtLoaders);
+            mbar_init(&sh.v_land[i], 1);
+            mbar_init(&sh.k_full[i], 1);
+            mbar_init(&sh.v_full[i], 2);   // one arrival per V warp
             mbar_init(&sh.k_empty[i], 1);
             mbar_init(&sh.v_empty[i], 1);
         }
         for (int t = 0; t < NT; t++) {
             mbar_init(&sh.s_full[t], 1);
+            mbar_init(&sh.o_half[t], 1);
             // one arrival per warp with rows
-            mbar_init(&sh.p_full[t], max(1, min(4, (M - m0 - t * kAtRows + 31) / 32)));
+            const int warps = max(1, min(4, (M - m0 - t * kAtRows + 31) / 32));
+            mbar_init(&sh.p_full[t][0], warps);
+            mbar_init(&sh.p_full[t][1], warps);
         }
         mbar_init(&sh.o_done, 1);
         sh.bad = 0;
+        prefetch_tensormap(&tm_k);
+        prefetch_tensormap(&tm_v);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 12) {
+    if (warp == 10) {
         tmem_alloc(&sh.tmem, kTmemCols);
         tmem_relinquish();
     }
@@ -190,40 +338,47 @@ __global__ void __launch_bounds__(kAtThreads, 1) attn_rows_tc_kernel(const RowsA
     const uint32_t tmem = sh.tmem;
     constexpr uint32_t kOCol = NT * kAtKeys;   // S tiles first, then O tiles
 
-    if (warp >= 8 && warp < 12) {
-        // ---- loads: warps 8, 9 K, warps 10, 11 V, all of them Q ----
-        const int tid = threadIdx.x & (kAtLoaders - 1);
-        const bool is_v = warp >= 10;
+    if (warp == 8 || warp == 9 || warp == 11) {
+        // ---- loads: warp 8 K, warps 9 and 11 V, all of them Q ----
         constexpr int kCh = HD / 8;                   // 16-byte chunks per row
-        constexpr int kRowsAtOnce = kAtLoaders / kCh;
-        const int ch = tid % kCh, jr = tid / kCh;
+        const bool is_v = warp != 8;
         // chunk ch of row r: sub-tile ch / 8, swizzled by the row
-        auto at = [&](int r) { return (ch >> 3) * 16384 + r * 128 + (((ch & 7) ^ (r & 7)) << 4); };
-        for (int t = 0; t < tiles; t++) {
-            const uint32_t dst = smem_u32(sh.q[t]);
-#pragma unroll
-            for (int it = 0; it < kAtRows / 2 / kRowsAtOnce; it++) {
-                const int r = (2 * it + is_v) * kRowsAtOnce + jr, m = m0 + t * kAtRows + r;
-                const T *src = static_cast<const T *>(p.q);
-                if (m < M) src += ((long long)(s.r0 + m / p.group) * p.n_heads + head0 + m % p.group) * HD + ch * 8;
-                cp_async16(dst + at(r), src, m < M);
-            }
+        auto at = [&](int r, int ch) { return (ch >> 3) * 16384 + r * 128 + (((ch & 7) ^ (r & 7)) << 4); };
+        for (int e = (warp == 11 ? 64 : (warp - 8) * 32) + lane; e < tiles * kAtRows * kCh; e += 96) {
+            const int r = e / kCh, ch = e % kCh, m = m0 + r;
+            const T *src = static_cast<const T *>(p.q);
+            if (m < M) src += ((long long)(s.r0 + m / p.group) * p.n_heads + head0 + m % p.group) * HD + ch * 8;
+            cp_async16(smem_u32(sh.q[r / kAtRows]) + at(r % kAtRows, ch), src, m < M);
         }
         cp_async_commit();
         const long long base = p.layer_off + (long long)stream * p.c.stream_stride + (long long)kvh * p.c.head_stride;
-        const char *src = (is_v ? p.c.v : p.c.k) + base * 2 + ch * 16;
+        const char *src = (is_v ? p.c.v : p.c.k) + base * 2;
         const long long slot_bytes = p.c.slot_stride * 2;
         const int lo_slot = cache_slot(p.c, kr.lo);
         unsigned char *const bufs = sh.kv[is_v ? 2 : 0];
         uint64_t *const full = is_v ? sh.v_full : sh.k_full, *const empty = is_v ? sh.v_empty : sh.k_empty;
-        auto publish = [&](int b) {   // block b (of this share) has landed
-            if (is_v && !whole(b0 + b)) {
-                unsigned char *v = bufs + (b & 1) * Sm::kTile;
+        // this warp's chunks of a block that it copies or looks through itself
+        const int first = is_v ? (warp == 11 ? 32 : 0) + lane : lane, step = is_v ? 64 : 32;
+        enum { kNone, kLook, kCopied };
+        int pending = kNone, pending_b = 0;
+        uint32_t land = 0;   // bit i: the phase that v_land[i] completes next
+        auto settle = [&]() {   // publish the pending block once it has landed
+            if (pending == kNone) return;
+            if (pending == kLook) {
+                const int i = pending_b & 1;
+                if (!mbar_wait(&sh.v_land[i], (land >> i) & 1u, deadline)) ok = false;
+                land ^= 1u << i;
+            } else {
+                cp_async_wait<0>();
+            }
+            if (is_v && !whole(b0 + pending_b)) {
+                unsigned char *v = bufs + (pending_b & 1) * Sm::kTile;
                 bool found = false;
-#pragma unroll 4
-                for (int it = 0; it < kAtKeys / kRowsAtOnce; it++) {
-                    uint4 *c = reinterpret_cast<uint4 *>(v + at(it * kRowsAtOnce + jr));
-                    uint4 u = *c;
+                // after TMA any thread may look at any chunk; after copies, at its own
+#pragma unroll 8
+                for (int e = first; e < kAtKeys * kCh; e += step) {
+                    uint4 *c = reinterpret_cast<uint4 *>(v + at(e / kCh, e % kCh));
+                    const uint4 u = *c;
                     const uint4 n = make_uint4(nonfinite2<T>(u.x), nonfinite2<T>(u.y), nonfinite2<T>(u.z), nonfinite2<T>(u.w));
                     if (n.x | n.y | n.z | n.w) {
                         *c = make_uint4(u.x & ~n.x, u.y & ~n.y, u.z & ~n.z, u.w & ~n.w);
@@ -233,49 +388,61 @@ __global__ void __launch_bounds__(kAtThreads, 1) attn_rows_tc_kernel(const RowsA
                 if (found) atomicExch(&sh.bad, 1);
             }
             fence_async_smem();
-            if (b == 0) mbar_arrive(&sh.q_full);   // Q was ahead of it
-            mbar_arrive(&full[b & 1]);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&full[pending_b & 1]);
+            pending = kNone;
         };
         for (int b = 0; b < nb; b++) {
-            if (b >= 2 && !mbar_wait(&empty[b & 1], ((b >> 1) + 1) & 1u, deadline)) {
+            if (b >= 2 && !__all_sync(0xffffffffu, mbar_wait(&empty[b & 1], ((b >> 1) + 1) & 1u, deadline))) {
                 ok = false;
                 break;
             }
-            const uint32_t dst = smem_u32(bufs + (b & 1) * Sm::kTile);
+            unsigned char *buf = bufs + (b & 1) * Sm::kTile;
             const int idx0 = (b0 + b) * kAtKeys;
             int slot0 = lo_slot + (idx0 - kr.ns);   // of index idx0, past the sinks
             if (slot0 >= p.c.cap) slot0 -= p.c.ring;
-            if (idx0 >= kr.ns && idx0 + kAtKeys <= total && slot0 + kAtKeys <= p.c.cap) {
-                const char *a = src + (slot0 + jr) * slot_bytes;   // 128 slots in a row
-                const long long step = kRowsAtOnce * slot_bytes;
-#pragma unroll 8
-                for (int it = 0; it < kAtKeys / kRowsAtOnce; it++) {
-                    cp_async16(dst + at(it * kRowsAtOnce + jr), a, true);
-                    a += step;
+            const bool look = is_v && !whole(b0 + b);
+            if (p.maps && idx0 >= kr.ns && idx0 + kAtKeys <= total && slot0 + kAtKeys <= p.c.cap) {   // 128 slots in a row
+                uint64_t *bar = look ? &sh.v_land[b & 1] : &full[b & 1];
+                if (warp != 11 && lane == 0) {
+                    mbar_expect_tx(bar, Sm::kTile);
+#pragma unroll
+                    for (int h = 0; h < kSub; h++)
+                        tma_load_4d(buf + h * 16384, is_v ? &tm_v : &tm_k, h * 64, kvh, slot0, stream, bar);
+                } else if (warp == 11 && lane == 0 && !look) {
+                    mbar_arrive(bar);
                 }
+                settle();
+                if (look) pending = kLook;
             } else {
+                const uint32_t dst = smem_u32(buf);
 #pragma unroll 4
-                for (int it = 0; it < kAtKeys / kRowsAtOnce; it++) {
-                    const int r = it * kRowsAtOnce + jr, idx = idx0 + r;
+                for (int e = first; e < kAtKeys * kCh; e += step) {
+                    const int r = e / kCh, ch = e % kCh, idx = idx0 + r;
                     int slot = idx;
                     if (idx >= kr.ns) {
                         slot = lo_slot + (idx - kr.ns);
                         if (slot >= p.c.cap) slot -= p.c.ring;
                     }
-                    cp_async16(dst + at(r), src + (idx < total ? slot * slot_bytes : 0), idx < total);
+                    cp_async16(dst + at(r, ch), src + (idx < total ? slot * slot_bytes + ch * 16 : 0), idx < total);
                 }
+                cp_async_commit();
+                settle();
+                pending = kCopied;
             }
-            cp_async_commit();
-            if (b >= 1) {
-                cp_async_wait<1>();
-                publish(b - 1);
+            pending_b = b;
+            if (b == 0) {   // Q
+                cp_async_wait<0>();
+                fence_async_smem();
+                mbar_arrive(&sh.q_full);
             }
         }
+        settle();
         cp_async_wait<0>();
-        if (ok && nb > 0) publish(nb - 1);
-    } else if (warp == 12) {
+    } else if (warp == 10) {
         // ---- MMAs ----
-        if (lane == 0 && nb > 0) {
+        if (nb > 0) {
+            const uint32_t lead = lane == 0, tm = __shfl_sync(0xffffffffu, tmem, 0);
             constexpr uint32_t id_s = at_idesc<T>(kAtKeys, false), id_o = at_idesc<T>(HD, true);
             auto issue_s = [&](int t, int b) {
                 const uint64_t a0 = smem_desc_sw128(sh.q[t]), k0 = smem_desc_sw128(sh.kv[b & 1]);
@@ -283,39 +450,45 @@ __global__ void __launch_bounds__(kAtThreads, 1) attn_rows_tc_kernel(const RowsA
                 for (int h = 0; h < kSub; h++)
 #pragma unroll
                     for (int k = 0; k < 4; k++)   // 16 dims: +32 bytes
-                        tc_mma_f16(tmem + t * kAtKeys, a0 + h * 1024 + 2 * k, k0 + h * 1024 + 2 * k, id_s,
-                                   (h | k) != 0 ? 1u : 0u);
-                tc_commit(&sh.s_full[t]);
+                        warp_mma(tm + t * kAtKeys, a0 + h * 1024 + 2 * k, k0 + h * 1024 + 2 * k, id_s,
+                                 (h | k) != 0 ? 1u : 0u, lead);
+                warp_commit(&sh.s_full[t], lead);
             };
-            ok = mbar_wait(&sh.q_full, 0u, deadline) && mbar_wait(&sh.k_full[0], 0u, deadline);
+            ok = warp_wait(&sh.q_full, 0u, deadline) && warp_wait(&sh.k_full[0], 0u, deadline);
             if (ok) {
                 tc_fence_after();
                 for (int t = 0; t < tiles; t++) issue_s(t, 0);
-                tc_commit(&sh.k_empty[0]);
+                warp_commit(&sh.k_empty[0], lead);
             }
             for (int b = 0; b < nb && ok; b++) {
+                ok = warp_wait(&sh.v_full[b & 1], (b >> 1) & 1u, deadline);
                 for (int t = 0; t < tiles && ok; t++) {
-                    ok = mbar_wait(&sh.p_full[t], b & 1u, deadline) &&
-                         (t > 0 || mbar_wait(&sh.v_full[b & 1], (b >> 1) & 1u, deadline));
-                    if (!ok) break;
-                    tc_fence_after();
+                    const uint64_t v0 = at_desc_mn(sh.kv[2 + (b & 1)]);
 #pragma unroll
-                    for (int k = 0; k < kAtKeys / 16; k++)   // 16 keys: 8 columns of P, 2048 bytes of V
-                        tc_mma_f16_ta(tmem + kOCol + t * HD, tmem + t * kAtKeys + 8 * k,
-                                      at_desc_mn(sh.kv[2 + (b & 1)] + k * 2048), id_o, (b | k) != 0 ? 1u : 0u);
-                    if (t == tiles - 1) tc_commit(&sh.v_empty[b & 1]);
+                    for (int h = 0; h < 2; h++) {
+                        if (ok) ok = warp_wait(&sh.p_full[t][h], b & 1u, deadline);
+                        if (!ok) break;
+                        tc_fence_after();
+#pragma unroll
+                        for (int k = 0; k < kAtHalf / 16; k++)   // 16 keys: 8 columns of P, 2048 bytes of V
+                            warp_mma_ta(tm + kOCol + t * HD, tm + t * kAtKeys + h * kAtHalf + 8 * k,
+                                        v0 + (h * 8192 + k * 2048) / 16, id_o, (b | h | k) != 0 ? 1u : 0u, lead);
+                        if (h == 0) warp_commit(&sh.o_half[t], lead);
+                    }
+                    if (!ok) break;
+                    if (t == tiles - 1) warp_commit(&sh.v_empty[b & 1], lead);
                     if (b + 1 < nb) {
                         if (t == 0) {
-                            ok = mbar_wait(&sh.k_full[(b + 1) & 1], ((b + 1) >> 1) & 1u, deadline);
+                            ok = warp_wait(&sh.k_full[(b + 1) & 1], ((b + 1) >> 1) & 1u, deadline);
                             if (!ok) break;
                             tc_fence_after();
                         }
-                        issue_s(t, b + 1);
-                        if (t == tiles - 1) tc_commit(&sh.k_empty[(b + 1) & 1]);
+                        issue_s(t, b + 1);   // over P(b), behind the MMAs that read it
+                        if (t == tiles - 1) warp_commit(&sh.k_empty[(b + 1) & 1], lead);
                     }
                 }
             }
-            tc_commit(&sh.o_done);
+            warp_commit(&sh.o_done, lead);
         }
     } else {
         // ---- softmax: thread = packed row ----
@@ -341,82 +514,60 @@ __global__ void __launch_bounds__(kAtThreads, 1) attn_rows_tc_kernel(const RowsA
             keys.e2 = kr.ns + min(max(0, up - kr.lo + 1), kr.nm);
             keys.node = s.pos < kr.ns ? s.pos : kr.ns + s.pos - kr.lo;
             const uint32_t tl = tmem + ((uint32_t)(32 * q) << 16);
-            const uint32_t ts = tl + t * kAtKeys, to = tl + kOCol + t * HD;
+            const uint32_t to = tl + kOCol + t * HD;
             const float sl2 = p.scale_log2;
-            const bool neg = sl2 < 0.f;
-            const float hidden = neg ? INFINITY : -INFINITY;   // a masked key's score
             float mr = -INFINITY, l = 0.f;
             float sv[32];
             for (int b = 0; b < nb; b++) {
                 if (!__all_sync(0xffffffffu, mbar_wait(&sh.s_full[t], b & 1u, deadline))) ok = false;
                 tc_fence_after();
-                const int c0 = (b0 + b) * kAtKeys;
                 const bool full = whole(b0 + b);
-                float mx[4] = {hidden, hidden, hidden, hidden};
-#pragma unroll
-                for (int c = 0; c < kAtKeys; c += 32) {
-                    tmem_ld32(ts + c, sv);
-                    if (!full) {
-                        const uint32_t vis = keys.bits(c0 + c, anc);
-#pragma unroll
-                        for (int j = 0; j < 32; j++) sv[j] = (vis >> j) & 1u ? sv[j] : hidden;
+#pragma unroll 1
+                for (int h = 0; h < 2; h++) {
+                    const uint32_t ts = tl + t * kAtKeys + h * kAtHalf;
+                    const int c0 = (b0 + b) * kAtKeys + h * kAtHalf;
+                    // P against the maximum so far; a row whose keys exceed it
+                    // by more than 2^8 takes theirs, and the warp goes over
+                    // them again (S is intact until P is stored)
+                    uint32_t w[kAtHalf / 2];
+                    float base = mr == -INFINITY ? 0.f : mr, factor = 1.f, ls = 0.f;
+                    float over = weigh<T>(ts, sl2, base, full, keys, c0, anc, w, ls);   // the largest less base
+                    const bool move = mr == -INFINITY ? over > -INFINITY : over > kAtRescale;
+                    const bool moved = __any_sync(0xffffffffu, move);
+                    if (moved) {
+                        if (move) {
+                            const float mn = base + over;
+                            factor = mr == -INFINITY ? 0.f : exp2_approx(mr - mn);
+                            mr = base = mn;
+                            l *= factor;
+                        }
+                        over = weigh<T>(ts, sl2, base, full, keys, c0, anc, w, ls);
                     }
-                    if (neg) {
+                    if (mr > -INFINITY) l += ls;
+                    if (over != over) l = over;   // a NaN score: the row is NaN
+                    tmem_st32_async(ts, w);       // over S
+                    if (moved && b + h > 0) {
+                        // O holds the weights before these: S(b) is behind the
+                        // last block's MMAs, the second half waits for the first's
+                        if (h == 1 && !__all_sync(0xffffffffu, mbar_wait(&sh.o_half[t], b & 1u, deadline))) ok = false;
+                        tc_fence_after();
 #pragma unroll
-                        for (int j = 0; j < 32; j++) mx[j & 3] = fminf(mx[j & 3], sv[j]);
-                    } else {
+                        for (int c = 0; c < HD; c += 32) {
+                            tmem_ld32(to + c, sv);
 #pragma unroll
-                        for (int j = 0; j < 32; j++) mx[j & 3] = fmaxf(mx[j & 3], sv[j]);
+                            for (int j = 0; j < 32; j++) sv[j] *= factor;
+                            tmem_st32(to + c, sv);
+                        }
                     }
+                    tmem_wait_st();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&sh.p_full[t][h]);
                 }
-                const float mb = sl2 * (neg ? fminf(fminf(mx[0], mx[1]), fminf(mx[2], mx[3]))
-                                            : fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])));
-                const bool move = mb > mr + kAtRescale;
-                float factor = 1.f;
-                if (move) {
-                    factor = mr == -INFINITY ? 0.f : exp2_approx(mr - mb);
-                    mr = mb;
-                    l *= factor;
-                }
-                const float base = mr == -INFINITY ? 0.f : mr;
-                float rs[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int c = 0; c < kAtKeys; c += 32) {
-                    tmem_ld32(ts + c, sv);
-                    if (!full) {
-                        const uint32_t vis = keys.bits(c0 + c, anc);
-#pragma unroll
-                        for (int j = 0; j < 32; j++) sv[j] = (vis >> j) & 1u ? sv[j] : hidden;
-                    }
-                    uint32_t h[16];
-#pragma unroll
-                    for (int j = 0; j < 32; j += 2) {
-                        const float ea = exp2_approx(fmaf(sv[j], sl2, -base));
-                        const float eb = exp2_approx(fmaf(sv[j + 1], sl2, -base));
-                        rs[(j >> 1) & 3] += ea + eb;
-                        h[j >> 1] = pack2<T>(ea, eb);
-                    }
-                    tmem_st16(ts + c / 2, h);   // over S columns that were read already
-                }
-                l += (rs[0] + rs[1]) + (rs[2] + rs[3]);
-                // O_t += P_t(b - 1) V(b - 1) is complete (S_t(b) was behind it)
-                if (b > 0 && __any_sync(0xffffffffu, move)) {
-#pragma unroll
-                    for (int c = 0; c < HD; c += 32) {
-                        tmem_ld32(to + c, sv);
-#pragma unroll
-                        for (int j = 0; j < 32; j++) sv[j] *= factor;
-                        tmem_st32(to + c, sv);
-                    }
-                }
-                tmem_wait_st();
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&sh.p_full[t]);
             }
             if (nb > 0 && !__all_sync(0xffffffffu, mbar_wait(&sh.o_done, 0u, deadline))) ok = false;
             tc_fence_after();
-            const float il = l == 0.f ? 0.f : 1.0f / l;   // no weight at all: zeros
+            const float il = l == 0.f ? 0.f : 1.0f / l;   // no weight at all: zeros (O is tiny, not NaN)
             const bool bad = *(volatile int *)&sh.bad != 0;
             const long long row = (long long)(s.r0 + i) * p.n_heads + head0 + min(m, M - 1) % p.group;
 #pragma unroll
@@ -480,7 +631,7 @@ __global__ void __launch_bounds__(kAtThreads, 1) attn_rows_tc_kernel(const RowsA
     // for a peer that may itself wait for TMEM
     tc_fence_before();
     __syncthreads();
-    if (warp == 12) {
+    if (warp == 10) {
         tc_fence_after();
         tmem_dealloc(tmem, kTmemCols);
     }
@@ -513,6 +664,38 @@ __global__ void __launch_bounds__(kAtThreads, 1) attn_rows_tc_kernel(const RowsA
         }
         cluster_sync_all();   // no CTA leaves while a peer still reads its share
     }
+}
+
+typedef CUresult (*EncodeTiledFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
+                                  const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
+                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiledFn encode_fn() {
+    static const EncodeTiledFn fn = [] {
+        void *q = nullptr;
+        cudaDriverEntryPointQueryResult r;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &q, cudaEnableDefault, &r) != cudaSuccess ||
+            r != cudaDriverEntryPointSuccess)
+            q = nullptr;
+        return (EncodeTiledFn)q;
+    }();
+    return fn;
+}
+
+// One layer's K or V as [stream][slot][head][dim], boxes of 128 slots x 64 dims
+// of one head, 128-byte swizzle.
+bool cache_map(CUtensorMap *m, char *base, const CacheView &c) {
+    EncodeTiledFn fn = encode_fn();
+    const long long most = 1ll << 40;   // bytes of a stride
+    if (!fn || c.cap < kAtKeys || c.head_stride * 2 >= most || c.slot_stride * 2 >= most || c.stream_stride * 2 >= most)
+        return false;
+    const cuuint64_t dims[4] = {(cuuint64_t)c.head_dim, (cuuint64_t)c.n_kv_heads, (cuuint64_t)c.cap, (cuuint64_t)c.n_streams};
+    const cuuint64_t strides[3] = {(cuuint64_t)c.head_stride * 2, (cuuint64_t)c.slot_stride * 2,
+                                   (cuuint64_t)c.stream_stride * 2};
+    const cuuint32_t box[4] = {64, 1, kAtKeys, 1}, estr[4] = {1, 1, 1, 1};
+    return fn(m, c.dtype == ELEM_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, base, dims,
+              strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 template <typename T, int HD, int NT>
@@ -550,7 +733,9 @@ cudaError_t launch_tiles(RowsAttnParams p, int sms, cudaStream_t st) {
     a[0].val.clusterDim.z = 1;
     cfg.attrs = a;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kernel, p);
+    CUtensorMap mk = {}, mv = {};
+    p.maps = cache_map(&mk, p.c.k + p.layer_off * 2, p.c) && cache_map(&mv, p.c.v + p.layer_off * 2, p.c);
+    return cudaLaunchKernelEx(&cfg, kernel, mk, mv, p);
 }
 
 template <typename T>

@@ -187,6 +187,7 @@ struct RowsAttnParams {
     float scale_log2;         // scale * log2(e)
     int shares;               // key shares of a row tile (set by the launch)
     unsigned *err;            // raised when a bounded wait expires (mapped host memory)
+    int maps;                 // tensor maps of K and V came with the launch (set by it)
 };
 cudaError_t launch_attn_rows(const RowsAttnParams &p, int sms, cudaStream_t st);
 // the tensor-core kernel of the 16-bit types (vc_attn_rows_tc.cu)
