@@ -629,6 +629,7 @@ cudaError_t launch_typed(const RowsAttnParams &p, int sms, cudaStream_t st) {
                               pp, st);
     };
     static std::atomic<uint64_t> d4{0}, d8{0}, d32{0};
+    if constexpr (sizeof(T) == 2) return launch_attn_rows_tc(p, sms, st);
     if (M <= 4) return go(attn_rows_few_kernel<T, HD, 4>, sizeof(ArFewSmem<T, HD, 4>), 4, d4);
     if (M <= 8) return go(attn_rows_few_kernel<T, HD, 8>, sizeof(ArFewSmem<T, HD, 8>), 8, d8);
     if constexpr (sizeof(T) == 2) return launch_attn_rows_tc(p, sms, st);

@@ -3,22 +3,20 @@
 //
 // A CTA takes NT (1 or 2) tiles of 128 packed query rows (m = row * group +
 // head, TMEM lane = packed row) of one (stream, KV head) and a share of the
-// 128-key blocks that they see; the shares of a tile pair are a cluster.
-//   warps 0-3, 4-7   softmax of tile 0 and 1, thread = packed row, 64 keys a
-//                    step: P = 2^(s - m) of S (TMEM), rounded to the cache's
-//                    type, over the S columns it came from
-//   warps 8, 9, 11   loads: Q once; K (warp 8) and V blocks two deep, by TMA
-//                    where a block's slots follow one another, by 16-byte
-//                    cp.async into the same swizzled layout where they do not
-//                    (ring wrap, sinks, the last block: zeros past the end)
-//   warp 10          issues the MMAs, M 128: S_t = Q_t K^T (N 128, K HD) and,
-//                    by halves, O_t += P_t V (N HD, K 64; A from TMEM, V an
+// blocks of 64 or 128 keys that they see; the shares are a cluster.
+//   4 warps per tile softmax, thread = packed row, 64 keys a step: P = 2^(s - m)
+//                    of S (TMEM), rounded to the cache's type, over the S
+//                    columns it came from; before that they load their rows of Q
+//   3 warps          loads: K (one warp) and V blocks two deep, by TMA where a
+//                    block's slots follow one another, by 16-byte cp.async into
+//                    the same swizzled layout where they do not (ring wrap,
+//                    sinks, the last block: zeros past the end)
+//   1 warp           issues the MMAs, M 128: S_t = Q_t K^T (K HD) and, by
+//                    steps of 64 keys, O_t += P_t V (N HD; A from TMEM, V an
 //                    MN-major operand)
-// S_t(b + 1) overwrites P_t(b), so it is issued behind the MMAs that read it.
-// Two tiles alternate - one's softmax runs under the other's MMAs - and share
-// each K and V block.  (S in two column ranges of 64, so that S(n + 1) runs
-// under the softmax of S(n), was slower: an MMA of N 64 takes as long as one of
-// N 128, reading its A tile.)
+// Two tiles: S_t(b + 1) overwrites P_t(b), so it is issued behind the MMAs that
+// read it; the tiles alternate - one's softmax runs under the other's MMAs -
+// and share each K and V block.
 //
 // The running maximum moves only when a step exceeds it by more than 2^8
 // (P <= 256 in either type), and only then O is rescaled.  Rounding P to 16
@@ -35,6 +33,7 @@
 #include <algorithm>
 #include <atomic>
 #include <type_traits>
+#include <math.h>
 
 namespace vc {
 
@@ -42,23 +41,41 @@ using namespace tc;
 
 namespace {
 
-constexpr int kAtKeys = 128;            // keys per block
-constexpr int kAtHalf = 64;             // keys per softmax step: half a block
-constexpr int kAtRows = 128;            // packed rows per tile = TMEM lanes
-constexpr int kAtThreads = 12 * 32;      // three warps per SM quarter: 168 registers
+constexpr int kAtHalf = 64;             // keys per softmax step
+constexpr int kAtRows = 128;            // packed rows per MMA tile = TMEM lanes
+// Three shapes: NT tiles of RT rows that exist (the MMA's other rows are
+// whatever lies behind Q in shared memory; nobody reads their lanes).
+//   <2, 128>  bound by the tensor and exponential units: 128-key blocks (an MMA
+//             of N 64 takes as long as one of N 128, reading its A tile), one
+//             CTA per SM
+//   <1, 128>  64-key blocks with two S ranges, so that S(b + 1) is ready when
+//             the softmax is done with S(b); two CTAs per SM
+//   <1, 32>   a token's or a few tokens' heads, bound by HBM: Q is small, 96 KB
+//             of keys in flight per CTA, two CTAs per SM
+constexpr int at_keys(int nt) { return nt == 1 ? 64 : 128; }
+constexpr int at_stages(int hd, int nt, int rt) { return nt == 2 ? 2 : (rt == 32 ? 3 : 2) * (128 / hd); }
+// RT / 32 softmax warps per tile, a K and two V loaders, an MMA warp
+constexpr int at_threads(int nt, int rt) { return (nt * rt / 32 + 4) * 32; }
 constexpr uint64_t kAtWaitNs = 2000000000ull;
 constexpr float kAtRescale = 8.0f;      // log2 of the largest P before the maximum moves
 constexpr int kAtOneCta = 120 * 1024;   // more than half an SM's shared memory: one CTA per SM
+constexpr int kAtFixed = 4;             // block times of a CTA's start and merge
 
-template <int HD, int NT>
+template <int HD, int NT, int RT>
 struct AtSmem {
-    static constexpr int kTile = 128 * HD * 2;   // bytes of a Q, K or V tile: HD / 64 sub-tiles of [128][128 bytes]
-    unsigned char kv[4][kTile];                  // K stages 0, 1, V stages 0, 1; at the end O [NT * 128][HD] fp32
-    unsigned char q[NT][kTile];
-    uint32_t anc[NT * kAtRows][kTreeMax / 32];
-    float mx[NT * kAtRows], sum[NT * kAtRows];
+    static constexpr int kKeys = at_keys(NT), kStages = at_stages(HD, NT, RT);
+    // Q, K and V tiles are HD / 64 sub-tiles of [rows or keys][128 bytes]
+    static constexpr int kTile = kKeys * HD * 2, kSubTile = kKeys * 128, kQTile = RT * HD * 2, kQSub = RT * 128;
+    static constexpr int kO = NT * RT * HD * 4;   // bytes of O in fp32, over K and V at the end
+    unsigned char q[NT][kQTile];
+    union {
+        unsigned char kv[2][kStages][kTile];      // K, V
+        unsigned char o[kO];
+    };
+    uint32_t anc[NT * RT][kTreeMax / 32];
+    float mx[NT * RT], sum[NT * RT];
     short parent[kTreeMax];
-    uint64_t q_full, v_land[2], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[NT], p_full[NT][2], o_half[NT], o_done;
+    uint64_t q_full, v_land[kStages], k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages], s_full[2], p_full[NT][2], o_part[NT], o_done;   // s_full: by tile, or (one tile) by S range
     uint32_t tmem;
     int bad;      // a masked block holds non-finite V values
 };
@@ -69,11 +86,11 @@ __host__ __device__ constexpr uint32_t at_idesc(int N, bool b_mn) {
            (b_mn ? (1u << 16) : 0u) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(kAtRows >> 4) << 24);
 }
 
-// MN-major operand, 128-byte swizzle: 64-element atoms along N 16384 bytes
-// apart (a sub-tile of 128 keys), 8-key groups 1024 bytes apart.
-__device__ __forceinline__ uint64_t at_desc_mn(const void *p) {
+// MN-major operand, 128-byte swizzle: 64-element atoms along N `atom` bytes
+// apart (a sub-tile), 8-key groups 1024 bytes apart.
+__device__ __forceinline__ uint64_t at_desc_mn(const void *p, int atom) {
     const uint64_t addr = smem_u32(p);
-    return ((addr >> 4) & 0x3FFFull) | ((uint64_t)(16384 >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) |
+    return ((addr >> 4) & 0x3FFFull) | ((uint64_t)(atom >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) |
            (2ull << 61);
 }
 
@@ -271,27 +288,32 @@ __device__ __forceinline__ uint32_t nonfinite2(uint32_t u) {   // 0xffff in each
     return __vcmpeq2(u & e, e);
 }
 
-template <typename T, int HD, int NT>
-__global__ void __launch_bounds__(kAtThreads, 1) attn_rows_tc_kernel(const __grid_constant__ CUtensorMap tm_k,
+template <typename T, int HD, int NT, int RT>
+__global__ void __launch_bounds__(at_threads(NT, RT), NT == 1 ? 2 : 1) attn_rows_tc_kernel(const __grid_constant__ CUtensorMap tm_k,
                                                                    const __grid_constant__ CUtensorMap tm_v,
                                                                    const RowsAttnParams p) {
-    using Sm = AtSmem<HD, NT>;
+    using Sm = AtSmem<HD, NT, RT>;
     constexpr int kSub = HD / 64;            // 64-dim sub-tiles of a tile
+    constexpr int kSoft = RT / 32;           // softmax warps of a tile
+    constexpr int kThreads = at_threads(NT, RT), kWarpK = kSoft * NT, kWarpV2 = kWarpK + 2, kWarpMma = kWarpK + 3;
+    constexpr int kStages = Sm::kStages;
+    constexpr int kKeys = Sm::kKeys, kSteps = kKeys / kAtHalf;
+    constexpr bool kTwoS = NT == 1;          // two S ranges
     constexpr uint32_t kTmemCols = NT == 2 ? 512 : 256;
     extern __shared__ __align__(1024) unsigned char at_smem_raw[];
     Sm &sh = *reinterpret_cast<Sm *>(at_smem_raw);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int z = blockIdx.x % p.shares, Z = p.shares;
-    const int m0 = blockIdx.x / p.shares * (NT * kAtRows), kvh = blockIdx.y, stream = blockIdx.z;
+    const int m0 = blockIdx.x / p.shares * (NT * RT), kvh = blockIdx.y, stream = blockIdx.z;
     const RowSpan s = row_span(p.r, stream);
     const int M = s.n * p.group;
     if (m0 >= M) return;   // the whole cluster leaves
     const bool tree = p.r.parent != nullptr;
-    const int i0 = m0 / p.group, i1 = (min(m0 + NT * kAtRows, M) - 1) / p.group + 1;
+    const int i0 = m0 / p.group, i1 = (min(m0 + NT * RT, M) - 1) / p.group + 1;
     const KeyRange kr = key_range(p.c, s, i0, i1, p.window, tree);
-    const int total = kr.total(), blocks = (total + kAtKeys - 1) / kAtKeys;
+    const int total = kr.total(), blocks = (total + kKeys - 1) / kKeys;
     const int b0 = (int)((long long)z * blocks / Z), nb = (int)((long long)(z + 1) * blocks / Z) - b0;
-    const int tiles = M - m0 > kAtRows ? NT : 1;   // tiles with rows
+    const int tiles = M - m0 > RT ? NT : 1;   // tiles with rows
     const int head0 = kvh * p.group;
     const uint64_t deadline = globaltimer() + kAtWaitNs;
     bool ok = true;
@@ -302,11 +324,11 @@ __global__ void __launch_bounds__(kAtThreads, 1) attn_rows_tc_kernel(const __gri
     int core_s = kr.ns + (p.window > 0 ? max(0, min(s.pos + i1 - p.window - kr.lo, kr.nm)) : 0), core_e = kr.ns + max(0, min(up_min - kr.lo + 1, kr.nm));
     if (up_min < kr.ns - 1) core_e = 0;
     else if (core_s == kr.ns) core_s = 0;
-    auto whole = [&](int b) { return b * kAtKeys >= core_s && (b + 1) * kAtKeys <= core_e; };
+    auto whole = [&](int b) { return b * kKeys >= core_s && (b + 1) * kKeys <= core_e; };
 
     if (threadIdx.x == 0) {
-        mbar_init(&sh.q_full, 96);
-        for (int i = 0; i < 2; i++) {
+        mbar_init(&sh.q_full, min(NT * kSoft, (M - m0 + 31) / 32));   // the warps with rows
+        for (int i = 0; i < kStages; i++) {
             mbar_init(&sh.v_land[i], 1);
             mbar_init(&sh.k_full[i], 1);
             mbar_init(&sh.v_full[i], 2);   // one arrival per V warp
@@ -314,69 +336,63 @@ __global__ void __launch_bounds__(kAtThreads, 1) attn_rows_tc_kernel(const __gri
             mbar_init(&sh.v_empty[i], 1);
         }
         for (int t = 0; t < NT; t++) {
-            mbar_init(&sh.s_full[t], 1);
-            mbar_init(&sh.o_half[t], 1);
+            mbar_init(&sh.o_part[t], 1);
             // one arrival per warp with rows
-            const int warps = max(1, min(4, (M - m0 - t * kAtRows + 31) / 32));
+            const int warps = max(1, min(kSoft, (M - m0 - t * RT + 31) / 32));
             mbar_init(&sh.p_full[t][0], warps);
             mbar_init(&sh.p_full[t][1], warps);
         }
+        mbar_init(&sh.s_full[0], 1);
+        mbar_init(&sh.s_full[1], 1);
         mbar_init(&sh.o_done, 1);
         sh.bad = 0;
         prefetch_tensormap(&tm_k);
         prefetch_tensormap(&tm_v);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 10) {
+    if (warp == kWarpMma) {
         tmem_alloc(&sh.tmem, kTmemCols);
         tmem_relinquish();
     }
-    if (tree) load_parents(sh.parent, p.r, s, threadIdx.x, kAtThreads);
+    if (tree) load_parents(sh.parent, p.r, s, threadIdx.x, kThreads);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = sh.tmem;
-    constexpr uint32_t kOCol = NT * kAtKeys;   // S tiles first, then O tiles
+    constexpr uint32_t kOCol = kTwoS ? 2 * kKeys : NT * kKeys;   // S ranges first, then O tiles
 
-    if (warp == 8 || warp == 9 || warp == 11) {
-        // ---- loads: warp 8 K, warps 9 and 11 V, all of them Q ----
+    if (warp >= kWarpK && warp <= kWarpV2) {
+        // ---- loads: one warp K, two V ----
         constexpr int kCh = HD / 8;                   // 16-byte chunks per row
-        const bool is_v = warp != 8;
+        const bool is_v = warp != kWarpK;
         // chunk ch of row r: sub-tile ch / 8, swizzled by the row
-        auto at = [&](int r, int ch) { return (ch >> 3) * 16384 + r * 128 + (((ch & 7) ^ (r & 7)) << 4); };
-        for (int e = (warp == 11 ? 64 : (warp - 8) * 32) + lane; e < tiles * kAtRows * kCh; e += 96) {
-            const int r = e / kCh, ch = e % kCh, m = m0 + r;
-            const T *src = static_cast<const T *>(p.q);
-            if (m < M) src += ((long long)(s.r0 + m / p.group) * p.n_heads + head0 + m % p.group) * HD + ch * 8;
-            cp_async16(smem_u32(sh.q[r / kAtRows]) + at(r % kAtRows, ch), src, m < M);
-        }
-        cp_async_commit();
+        auto at = [&](int r, int ch) { return (ch >> 3) * Sm::kSubTile + r * 128 + (((ch & 7) ^ (r & 7)) << 4); };
         const long long base = p.layer_off + (long long)stream * p.c.stream_stride + (long long)kvh * p.c.head_stride;
         const char *src = (is_v ? p.c.v : p.c.k) + base * 2;
         const long long slot_bytes = p.c.slot_stride * 2;
         const int lo_slot = cache_slot(p.c, kr.lo);
-        unsigned char *const bufs = sh.kv[is_v ? 2 : 0];
+        unsigned char(*const bufs)[Sm::kTile] = sh.kv[is_v];
         uint64_t *const full = is_v ? sh.v_full : sh.k_full, *const empty = is_v ? sh.v_empty : sh.k_empty;
         // this warp's chunks of a block that it copies or looks through itself
-        const int first = is_v ? (warp == 11 ? 32 : 0) + lane : lane, step = is_v ? 64 : 32;
+        const int first = (warp == kWarpV2 ? 32 : 0) + lane, step = is_v ? 64 : 32;
         enum { kNone, kLook, kCopied };
         int pending = kNone, pending_b = 0;
         uint32_t land = 0;   // bit i: the phase that v_land[i] completes next
         auto settle = [&]() {   // publish the pending block once it has landed
             if (pending == kNone) return;
             if (pending == kLook) {
-                const int i = pending_b & 1;
+                const int i = pending_b % kStages;
                 if (!mbar_wait(&sh.v_land[i], (land >> i) & 1u, deadline)) ok = false;
                 land ^= 1u << i;
             } else {
                 cp_async_wait<0>();
             }
             if (is_v && !whole(b0 + pending_b)) {
-                unsigned char *v = bufs + (pending_b & 1) * Sm::kTile;
+                unsigned char *v = bufs[pending_b % kStages];
                 bool found = false;
                 // after TMA any thread may look at any chunk; after copies, at its own
 #pragma unroll 8
-                for (int e = first; e < kAtKeys * kCh; e += step) {
+                for (int e = first; e < kKeys * kCh; e += step) {
                     uint4 *c = reinterpret_cast<uint4 *>(v + at(e / kCh, e % kCh));
                     const uint4 u = *c;
                     const uint4 n = make_uint4(nonfinite2<T>(u.x), nonfinite2<T>(u.y), nonfinite2<T>(u.z), nonfinite2<T>(u.w));
@@ -389,27 +405,28 @@ __global__ void __launch_bounds__(kAtThreads, 1) attn_rows_tc_kernel(const __gri
             }
             fence_async_smem();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&full[pending_b & 1]);
+            if (lane == 0) mbar_arrive(&full[pending_b % kStages]);
             pending = kNone;
         };
         for (int b = 0; b < nb; b++) {
-            if (b >= 2 && !__all_sync(0xffffffffu, mbar_wait(&empty[b & 1], ((b >> 1) + 1) & 1u, deadline))) {
+            if (b >= kStages &&
+                !__all_sync(0xffffffffu, mbar_wait(&empty[b % kStages], (b / kStages + 1) & 1u, deadline))) {
                 ok = false;
                 break;
             }
-            unsigned char *buf = bufs + (b & 1) * Sm::kTile;
-            const int idx0 = (b0 + b) * kAtKeys;
+            unsigned char *buf = bufs[b % kStages];
+            const int idx0 = (b0 + b) * kKeys;
             int slot0 = lo_slot + (idx0 - kr.ns);   // of index idx0, past the sinks
             if (slot0 >= p.c.cap) slot0 -= p.c.ring;
             const bool look = is_v && !whole(b0 + b);
-            if (p.maps && idx0 >= kr.ns && idx0 + kAtKeys <= total && slot0 + kAtKeys <= p.c.cap) {   // 128 slots in a row
-                uint64_t *bar = look ? &sh.v_land[b & 1] : &full[b & 1];
-                if (warp != 11 && lane == 0) {
+            if (p.maps && idx0 >= kr.ns && idx0 + kKeys <= total && slot0 + kKeys <= p.c.cap) {   // slots in a row
+                uint64_t *bar = look ? &sh.v_land[b % kStages] : &full[b % kStages];
+                if (warp != kWarpV2 && lane == 0) {
                     mbar_expect_tx(bar, Sm::kTile);
 #pragma unroll
                     for (int h = 0; h < kSub; h++)
-                        tma_load_4d(buf + h * 16384, is_v ? &tm_v : &tm_k, h * 64, kvh, slot0, stream, bar);
-                } else if (warp == 11 && lane == 0 && !look) {
+                        tma_load_4d(buf + h * Sm::kSubTile, is_v ? &tm_v : &tm_k, h * 64, kvh, slot0, stream, bar);
+                } else if (warp == kWarpV2 && lane == 0 && !look) {
                     mbar_arrive(bar);
                 }
                 settle();
@@ -417,7 +434,7 @@ __global__ void __launch_bounds__(kAtThreads, 1) attn_rows_tc_kernel(const __gri
             } else {
                 const uint32_t dst = smem_u32(buf);
 #pragma unroll 4
-                for (int e = first; e < kAtKeys * kCh; e += step) {
+                for (int e = first; e < kKeys * kCh; e += step) {
                     const int r = e / kCh, ch = e % kCh, idx = idx0 + r;
                     int slot = idx;
                     if (idx >= kr.ns) {
@@ -431,28 +448,32 @@ __global__ void __launch_bounds__(kAtThreads, 1) attn_rows_tc_kernel(const __gri
                 pending = kCopied;
             }
             pending_b = b;
-            if (b == 0) {   // Q
-                cp_async_wait<0>();
-                fence_async_smem();
-                mbar_arrive(&sh.q_full);
-            }
         }
         settle();
-        cp_async_wait<0>();
-    } else if (warp == 10) {
+    } else if (warp == kWarpMma) {
         // ---- MMAs ----
         if (nb > 0) {
             const uint32_t lead = lane == 0, tm = __shfl_sync(0xffffffffu, tmem, 0);
-            constexpr uint32_t id_s = at_idesc<T>(kAtKeys, false), id_o = at_idesc<T>(HD, true);
-            auto issue_s = [&](int t, int b) {
-                const uint64_t a0 = smem_desc_sw128(sh.q[t]), k0 = smem_desc_sw128(sh.kv[b & 1]);
+            constexpr uint32_t id_s = at_idesc<T>(kKeys, false), id_o = at_idesc<T>(HD, true);
+            auto issue_s = [&](int t, int b) {   // S range t of two tiles, b % 2 of one
+                const uint64_t a0 = smem_desc_sw128(sh.q[t]), k0 = smem_desc_sw128(sh.kv[0][b % kStages]);
+                const int r = kTwoS ? b & 1 : t;
 #pragma unroll
                 for (int h = 0; h < kSub; h++)
 #pragma unroll
                     for (int k = 0; k < 4; k++)   // 16 dims: +32 bytes
-                        warp_mma(tm + t * kAtKeys, a0 + h * 1024 + 2 * k, k0 + h * 1024 + 2 * k, id_s,
-                                 (h | k) != 0 ? 1u : 0u, lead);
-                warp_commit(&sh.s_full[t], lead);
+                        warp_mma(tm + r * kKeys, a0 + h * (Sm::kQSub / 16) + 2 * k, k0 + h * (Sm::kSubTile / 16) + 2 * k,
+                                 id_s, (h | k) != 0 ? 1u : 0u, lead);
+                warp_commit(&sh.s_full[r], lead);
+            };
+            auto issue_o = [&](int t, int b, int h) {   // 64 keys of O += P V
+                const uint64_t v0 = at_desc_mn(sh.kv[1][b % kStages], Sm::kSubTile);
+                const int r = kTwoS ? b & 1 : t;
+#pragma unroll
+                for (int k = 0; k < kAtHalf / 16; k++)   // 16 keys: 8 columns of P, 2048 bytes of V
+                    warp_mma_ta(tm + kOCol + t * HD, tm + r * kKeys + h * kAtHalf + 8 * k, v0 + (h * 8192 + k * 2048) / 16,
+                                id_o, (b | h | k) != 0 ? 1u : 0u, lead);
+                if (kTwoS || h == 0) warp_commit(&sh.o_part[t], lead);
             };
             ok = warp_wait(&sh.q_full, 0u, deadline) && warp_wait(&sh.k_full[0], 0u, deadline);
             if (ok) {
@@ -461,30 +482,41 @@ __global__ void __launch_bounds__(kAtThreads, 1) attn_rows_tc_kernel(const __gri
                 warp_commit(&sh.k_empty[0], lead);
             }
             for (int b = 0; b < nb && ok; b++) {
-                ok = warp_wait(&sh.v_full[b & 1], (b >> 1) & 1u, deadline);
-                for (int t = 0; t < tiles && ok; t++) {
-                    const uint64_t v0 = at_desc_mn(sh.kv[2 + (b & 1)]);
-#pragma unroll
-                    for (int h = 0; h < 2; h++) {
-                        if (ok) ok = warp_wait(&sh.p_full[t][h], b & 1u, deadline);
+                if constexpr (kTwoS) {
+                    if (b + 1 < nb) {   // over P(b - 1), behind the MMAs that read it
+                        ok = warp_wait(&sh.k_full[(b + 1) % kStages], ((b + 1) / kStages) & 1u, deadline);
                         if (!ok) break;
                         tc_fence_after();
-#pragma unroll
-                        for (int k = 0; k < kAtHalf / 16; k++)   // 16 keys: 8 columns of P, 2048 bytes of V
-                            warp_mma_ta(tm + kOCol + t * HD, tm + t * kAtKeys + h * kAtHalf + 8 * k,
-                                        v0 + (h * 8192 + k * 2048) / 16, id_o, (b | h | k) != 0 ? 1u : 0u, lead);
-                        if (h == 0) warp_commit(&sh.o_half[t], lead);
+                        issue_s(0, b + 1);
+                        warp_commit(&sh.k_empty[(b + 1) % kStages], lead);
                     }
+                    ok = warp_wait(&sh.v_full[b % kStages], (b / kStages) & 1u, deadline) &&
+                         warp_wait(&sh.p_full[0][b & 1], (b >> 1) & 1u, deadline);
                     if (!ok) break;
-                    if (t == tiles - 1) warp_commit(&sh.v_empty[b & 1], lead);
-                    if (b + 1 < nb) {
-                        if (t == 0) {
-                            ok = warp_wait(&sh.k_full[(b + 1) & 1], ((b + 1) >> 1) & 1u, deadline);
+                    tc_fence_after();
+                    issue_o(0, b, 0);
+                    warp_commit(&sh.v_empty[b % kStages], lead);
+                } else {
+                    ok = warp_wait(&sh.v_full[b % kStages], (b / kStages) & 1u, deadline);
+                    for (int t = 0; t < tiles && ok; t++) {
+#pragma unroll
+                        for (int h = 0; h < kSteps; h++) {
+                            if (ok) ok = warp_wait(&sh.p_full[t][h], b & 1u, deadline);
                             if (!ok) break;
                             tc_fence_after();
+                            issue_o(t, b, h);
                         }
-                        issue_s(t, b + 1);   // over P(b), behind the MMAs that read it
-                        if (t == tiles - 1) warp_commit(&sh.k_empty[(b + 1) & 1], lead);
+                        if (!ok) break;
+                        if (t == tiles - 1) warp_commit(&sh.v_empty[b % kStages], lead);
+                        if (b + 1 < nb) {
+                            if (t == 0) {
+                                ok = warp_wait(&sh.k_full[(b + 1) % kStages], ((b + 1) / kStages) & 1u, deadline);
+                                if (!ok) break;
+                                tc_fence_after();
+                            }
+                            issue_s(t, b + 1);   // over P(b), behind the MMAs that read it
+                            if (t == tiles - 1) warp_commit(&sh.k_empty[(b + 1) % kStages], lead);
+                        }
                     }
                 }
             }
@@ -492,10 +524,24 @@ __global__ void __launch_bounds__(kAtThreads, 1) attn_rows_tc_kernel(const __gri
         }
     } else {
         // ---- softmax: thread = packed row ----
-        const int t = warp >> 2, q = warp & 3, ml = t * kAtRows + 32 * q + lane, m = m0 + ml;
-        const bool here = t < NT && m0 + t * kAtRows + 32 * q < M;   // the warp has rows
+        const int t = warp / kSoft, q = warp % kSoft, ml = t * RT + 32 * q + lane, m = m0 + ml;
+        const bool here = m0 + t * RT + 32 * q < M;   // the warp has rows
         if (here) {
             const int i = min(m, M - 1) / p.group;
+            {   // the warp's 32 rows of Q: HD / 8 lanes a row, zeros past M
+                constexpr int kCh = HD / 8, kAtOnce = 32 / kCh;
+                const int ch = lane % kCh;
+                const uint32_t dst = smem_u32(sh.q[t]) + (ch >> 3) * Sm::kQSub;
+                const long long row = (long long)(s.r0 + i) * p.n_heads + head0 + min(m, M - 1) % p.group;
+#pragma unroll 8
+                for (int it = 0; it < 32 / kAtOnce; it++) {
+                    const int r = it * kAtOnce + lane / kCh, rt = 32 * q + r;
+                    const long long from = __shfl_sync(0xffffffffu, row, r);
+                    cp_async16(dst + rt * 128 + (((ch & 7) ^ (rt & 7)) << 4),
+                               static_cast<const T *>(p.q) + from * HD + ch * 8, m0 + t * RT + rt < M);
+                }
+                cp_async_commit();
+            }
             int pl = s.pos + i;
             const uint32_t *anc = nullptr;
             if (tree) {
@@ -518,14 +564,19 @@ __global__ void __launch_bounds__(kAtThreads, 1) attn_rows_tc_kernel(const __gri
             const float sl2 = p.scale_log2;
             float mr = -INFINITY, l = 0.f;
             float sv[32];
+            cp_async_wait<0>();
+            fence_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh.q_full);
             for (int b = 0; b < nb; b++) {
-                if (!__all_sync(0xffffffffu, mbar_wait(&sh.s_full[t], b & 1u, deadline))) ok = false;
+                const int r = kTwoS ? b & 1 : t;   // the S range
+                if (!__all_sync(0xffffffffu, mbar_wait(&sh.s_full[r], (kTwoS ? b >> 1 : b) & 1u, deadline))) ok = false;
                 tc_fence_after();
                 const bool full = whole(b0 + b);
 #pragma unroll 1
-                for (int h = 0; h < 2; h++) {
-                    const uint32_t ts = tl + t * kAtKeys + h * kAtHalf;
-                    const int c0 = (b0 + b) * kAtKeys + h * kAtHalf;
+                for (int h = 0; h < kSteps; h++) {
+                    const uint32_t ts = tl + r * kKeys + h * kAtHalf;
+                    const int c0 = (b0 + b) * kKeys + h * kAtHalf;
                     // P against the maximum so far; a row whose keys exceed it
                     // by more than 2^8 takes theirs, and the warp goes over
                     // them again (S is intact until P is stored)
@@ -547,9 +598,13 @@ __global__ void __launch_bounds__(kAtThreads, 1) attn_rows_tc_kernel(const __gri
                     if (over != over) l = over;   // a NaN score: the row is NaN
                     tmem_st32_async(ts, w);       // over S
                     if (moved && b + h > 0) {
-                        // O holds the weights before these: S(b) is behind the
-                        // last block's MMAs, the second half waits for the first's
-                        if (h == 1 && !__all_sync(0xffffffffu, mbar_wait(&sh.o_half[t], b & 1u, deadline))) ok = false;
+                        // O must hold the weights before these.  Two S ranges:
+                        // S(b) is behind the MMAs of block b - 2, those of b - 1
+                        // may be under way; else S(b) is behind block b - 1's,
+                        // and the second step waits for the first's.
+                        if (kTwoS || h == 1)
+                            if (!__all_sync(0xffffffffu, mbar_wait(&sh.o_part[t], (kTwoS ? b - 1 : b) & 1u, deadline)))
+                                ok = false;
                         tc_fence_after();
 #pragma unroll
                         for (int c = 0; c < HD; c += 32) {
@@ -562,7 +617,7 @@ __global__ void __launch_bounds__(kAtThreads, 1) attn_rows_tc_kernel(const __gri
                     tmem_wait_st();
                     tc_fence_before();
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(&sh.p_full[t][h]);
+                    if (lane == 0) mbar_arrive(&sh.p_full[t][kTwoS ? r : h]);
                 }
             }
             if (nb > 0 && !__all_sync(0xffffffffu, mbar_wait(&sh.o_done, 0u, deadline))) ok = false;
@@ -582,8 +637,8 @@ __global__ void __launch_bounds__(kAtThreads, 1) attn_rows_tc_kernel(const __gri
                     const long long base = p.layer_off + (long long)stream * p.c.stream_stride +
                                            (long long)kvh * p.c.head_stride + c;
                     const int lo_slot = cache_slot(p.c, kr.lo);
-                    for (int idx = b0 * kAtKeys; idx < min(total, (b0 + nb) * kAtKeys); idx++) {
-                        if (whole(idx / kAtKeys) || !((keys.bits(idx & ~31, anc) >> (idx & 31)) & 1u)) continue;
+                    for (int idx = b0 * kKeys; idx < min(total, (b0 + nb) * kKeys); idx++) {
+                        if (whole(idx / kKeys) || !((keys.bits(idx & ~31, anc) >> (idx & 31)) & 1u)) continue;
                         int slot = idx;
                         if (idx >= kr.ns) {
                             slot = lo_slot + (idx - kr.ns);
@@ -599,7 +654,7 @@ __global__ void __launch_bounds__(kAtThreads, 1) attn_rows_tc_kernel(const __gri
                 }
                 if (Z > 1) {
                     // this share's sums, 16-byte chunks swizzled by the row
-                    float *o = reinterpret_cast<float *>(sh.kv[0]) + ml * HD;
+                    float *o = reinterpret_cast<float *>(sh.o) + ml * HD;
 #pragma unroll
                     for (int j = 0; j < 32; j += 4)
                         *reinterpret_cast<float4 *>(o + ((((c + j) >> 2) ^ (ml & 7)) << 2)) =
@@ -631,15 +686,15 @@ __global__ void __launch_bounds__(kAtThreads, 1) attn_rows_tc_kernel(const __gri
     // for a peer that may itself wait for TMEM
     tc_fence_before();
     __syncthreads();
-    if (warp == 10) {
+    if (warp == kWarpMma) {
         tc_fence_after();
         tmem_dealloc(tmem, kTmemCols);
     }
     if (Z > 1) {
         cluster_sync_all();
-        const uint32_t o_s = smem_u32(sh.kv[0]), m_s = smem_u32(sh.mx), l_s = smem_u32(sh.sum);
-        const int rows = min(NT * kAtRows, M - m0);
-        for (int e = z * kAtThreads + threadIdx.x; e < rows * (HD / 4); e += Z * kAtThreads) {
+        const uint32_t o_s = smem_u32(sh.o), m_s = smem_u32(sh.mx), l_s = smem_u32(sh.sum);
+        const int rows = min(NT * RT, M - m0);
+        for (int e = z * kThreads + threadIdx.x; e < rows * (HD / 4); e += Z * kThreads) {
             const int ml = e / (HD / 4), d4 = e % (HD / 4), m = m0 + ml;
             float gm = -INFINITY;
             for (int r = 0; r < Z; r++) gm = fmaxf(gm, ld_dsmem_f1(mapa_shared(m_s + 4 * ml, r)));
@@ -682,27 +737,28 @@ EncodeTiledFn encode_fn() {
     return fn;
 }
 
-// One layer's K or V as [stream][slot][head][dim], boxes of 128 slots x 64 dims
-// of one head, 128-byte swizzle.
-bool cache_map(CUtensorMap *m, char *base, const CacheView &c) {
+// One layer's K or V as [stream][slot][head][dim], boxes of `keys` slots x 64
+// dims of one head, 128-byte swizzle.
+bool cache_map(CUtensorMap *m, char *base, const CacheView &c, int keys) {
     EncodeTiledFn fn = encode_fn();
     const long long most = 1ll << 40;   // bytes of a stride
-    if (!fn || c.cap < kAtKeys || c.head_stride * 2 >= most || c.slot_stride * 2 >= most || c.stream_stride * 2 >= most)
+    if (!fn || c.cap < keys || c.head_stride * 2 >= most || c.slot_stride * 2 >= most || c.stream_stride * 2 >= most)
         return false;
     const cuuint64_t dims[4] = {(cuuint64_t)c.head_dim, (cuuint64_t)c.n_kv_heads, (cuuint64_t)c.cap, (cuuint64_t)c.n_streams};
     const cuuint64_t strides[3] = {(cuuint64_t)c.head_stride * 2, (cuuint64_t)c.slot_stride * 2,
                                    (cuuint64_t)c.stream_stride * 2};
-    const cuuint32_t box[4] = {64, 1, kAtKeys, 1}, estr[4] = {1, 1, 1, 1};
+    const cuuint32_t box[4] = {64, 1, (cuuint32_t)keys, 1}, estr[4] = {1, 1, 1, 1};
     return fn(m, c.dtype == ELEM_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, base, dims,
               strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <typename T, int HD, int NT>
+template <typename T, int HD, int NT, int RT>
 cudaError_t launch_tiles(RowsAttnParams p, int sms, cudaStream_t st) {
-    constexpr size_t kSmem = std::max<size_t>(sizeof(AtSmem<HD, NT>), NT == 2 ? kAtOneCta : 0);
-    static_assert(kSmem <= 227 * 1024, "fits an SM");
-    auto kernel = attn_rows_tc_kernel<T, HD, NT>;
+    constexpr int kKeys = at_keys(NT);
+    constexpr size_t kSmem = std::max<size_t>(sizeof(AtSmem<HD, NT, RT>), NT == 2 ? kAtOneCta : 0);
+    static_assert(kSmem <= (NT == 1 ? 113 : 227) * 1024, "two CTAs or one fit an SM");
+    auto kernel = attn_rows_tc_kernel<T, HD, NT, RT>;
     static std::atomic<uint64_t> done{0};
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
@@ -715,15 +771,28 @@ cudaError_t launch_tiles(RowsAttnParams p, int sms, cudaStream_t st) {
         done.fetch_or(bit);
     }
     const long long M = (long long)p.r.max_rows * p.group;
-    const long long tiles = (M + NT * kAtRows - 1) / (NT * kAtRows);
+    const long long tiles = (M + NT * RT - 1) / (NT * RT);
     const long long keys =
         p.window > 0 ? std::min<long long>(p.c.cap, (long long)p.window + p.r.max_rows + p.c.n_sink) : p.c.cap;
-    const long long ctas = tiles * p.c.n_kv_heads * p.c.n_streams;
-    const long long by_sms = std::max<long long>(1, sms / ctas), by_keys = (keys + kAtKeys - 1) / kAtKeys;
-    p.shares = (int)std::max<long long>(1, std::min<long long>(16, std::min(by_sms, by_keys)));
+    const long long ctas = tiles * p.c.n_kv_heads * p.c.n_streams, blocks = (keys + kKeys - 1) / kKeys;
+    // Shares: the least time in units of a block, with kAtFixed for a CTA's
+    // start and merge.  Several waves: each takes a share's blocks.  One wave
+    // that leaves SMs half empty: two CTAs of an SM share its part of the
+    // bandwidth, so a CTA alone there is faster (24 tokens over 4096 keys, 192
+    // CTAs: 69 us in three shares, 57 us in one).
+    const double slots = (double)sms * (NT == 1 ? 2 : 1);
+    double best = 1e30;
+    for (int Z = 1; Z <= 16 && Z <= blocks; Z++) {
+        const double fill = ctas * Z / slots, part = (double)((blocks + Z - 1) / Z);
+        const double t = fill > 1.0 ? ceil(fill) * (part + kAtFixed) : part * std::max(fill, NT == 1 ? 0.5 : 1.0) + kAtFixed;
+        if (t < best) {
+            best = t;
+            p.shares = Z;
+        }
+    }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(p.shares * tiles), p.c.n_kv_heads, p.c.n_streams);
-    cfg.blockDim = dim3(kAtThreads);
+    cfg.blockDim = dim3(at_threads(NT, RT));
     cfg.dynamicSmemBytes = kSmem;
     cfg.stream = st;
     cudaLaunchAttribute a[1];
@@ -734,21 +803,26 @@ cudaError_t launch_tiles(RowsAttnParams p, int sms, cudaStream_t st) {
     cfg.attrs = a;
     cfg.numAttrs = 1;
     CUtensorMap mk = {}, mv = {};
-    p.maps = cache_map(&mk, p.c.k + p.layer_off * 2, p.c) && cache_map(&mv, p.c.v + p.layer_off * 2, p.c);
+    p.maps = cache_map(&mk, p.c.k + p.layer_off * 2, p.c, kKeys) && cache_map(&mv, p.c.v + p.layer_off * 2, p.c, kKeys);
     return cudaLaunchKernelEx(&cfg, kernel, mk, mv, p);
 }
 
-template <typename T>
+template <typename T, int HD>
 cudaError_t launch_typed(const RowsAttnParams &p, int sms, cudaStream_t st) {
-    const bool two = (long long)p.r.max_rows * p.group > kAtRows;
-    if (p.c.head_dim == 64) return two ? launch_tiles<T, 64, 2>(p, sms, st) : launch_tiles<T, 64, 1>(p, sms, st);
-    return two ? launch_tiles<T, 128, 2>(p, sms, st) : launch_tiles<T, 128, 1>(p, sms, st);
+    const long long M = (long long)p.r.max_rows * p.group;
+    if (M <= 32) return launch_tiles<T, HD, 1, 32>(p, sms, st);
+    if (M <= kAtRows) return launch_tiles<T, HD, 1, 128>(p, sms, st);
+    return launch_tiles<T, HD, 2, 128>(p, sms, st);
+}
+template <typename T>
+cudaError_t launch_dim(const RowsAttnParams &p, int sms, cudaStream_t st) {
+    return p.c.head_dim == 64 ? launch_typed<T, 64>(p, sms, st) : launch_typed<T, 128>(p, sms, st);
 }
 
 }  // namespace
 
 cudaError_t launch_attn_rows_tc(const RowsAttnParams &p, int sms, cudaStream_t st) {
-    return p.c.dtype == ELEM_BF16 ? launch_typed<__nv_bfloat16>(p, sms, st) : launch_typed<__half>(p, sms, st);
+    return p.c.dtype == ELEM_BF16 ? launch_dim<__nv_bfloat16>(p, sms, st) : launch_dim<__half>(p, sms, st);
 }
 
 }  // namespace vc
