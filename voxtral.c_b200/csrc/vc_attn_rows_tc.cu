@@ -186,31 +186,6 @@ struct RowKeys {
     }
 };
 
-// Two fp32 values per register pair: one issue slot for two results.
-__device__ __forceinline__ uint64_t pair(float a, float b) {
-    uint64_t r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-    return r;
-}
-__device__ __forceinline__ void unpair(uint64_t p, float &a, float &b) {
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p));
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-    uint64_t r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-    return r;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-    uint64_t r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-__device__ __forceinline__ float fmax_nan(float a, float b) {   // NaN if either is
-    float r;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-    return r;
-}
-
 // 2^x of two values on the FMA pipe: x = n + f, n the nearest whole number
 // (left in the low bits by adding 1.5 * 2^23), 2^f by its minimax polynomial
 // of degree 4 on [-1/2, 1/2] (Remez: relative error 2.6e-6, of either sign),

@@ -4,8 +4,9 @@
 //   log p_t = x_t - m - ln Z          Z = sum_i e^(x_i - m)
 //   H       = ln Z - S / Z            S = sum_i e^(x_i - m) (x_i - m)
 //
-// One pass over a row: each thread keeps a running maximum with Z and S in
-// fp32, rescaled when a batch of its values raises the maximum.  A row with a
+// One pass over a row: each warp keeps a running maximum, its threads Z and S in
+// fp32, rescaled when a batch of values raises the maximum.  Per value about 5
+// instructions, pairs of values where one does for two, and one exponential.  A row with a
 // NaN or +inf, or without a finite logit, has no distribution: NaN.  Bound by HBM
 // for many rows, by latency for one: a row is shared by the CTAs of a cluster
 // when there are fewer rows than SMs.
@@ -13,15 +14,16 @@
 // The alternatives cost no second pass: the threads also leave each batch's
 // maximum in shared memory.  The n_top-th largest of 32 group maxima is a
 // value that at least n_top logits reach, so only batches that reach it -
-// about n_top of them - are looked at again; their values go into a sorted
-// list that a warp holds across its lanes.  Lists order by value, then by the
-// lowest id, and merge by rank.
+// about n_top of them - are looked at again, and their few values that reach it
+// are ranked by counting.  Keys order by value, then by the lowest id; the
+// shares of a row rank their lists against each other's.
 #include "vc_rows.cuh"
 #include "vc_tc.cuh"
 
 #include <algorithm>
 #include <atomic>
-#include <float.h>
+#include <math.h>
+#include <type_traits>
 
 namespace vc {
 
@@ -33,8 +35,10 @@ constexpr int kLpThreads = 256;
 constexpr int kLpWarps = kLpThreads / 32;
 constexpr int kLpLoads = 4;      // 16-byte loads of a thread's batch
 constexpr int kLpSlots = 16;     // batch maxima kept per thread; batch b in slot b % 16
+constexpr int kLpFound = 256;    // candidates kept
+constexpr int kLpShares = 16;    // CTAs of a row at most
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLpFloor = -200.f;   // x - m below this: e^(x - m) is 0 in fp32
+constexpr float kLpFloor = -300.f;   // 2^x below this is 0 in fp32
 
 // A logit and its id as one number: larger is better, ties go to the lower id.
 typedef unsigned long long Key;
@@ -51,19 +55,94 @@ __device__ __forceinline__ int key_id(Key k) { return 0x7fffffff - (int)(uint32_
 
 struct LpSmem {
     float batch_max[kLpSlots][kLpThreads];
-    Key lists[kLpWarps][kTopMax];   // the warps' best, then (list 0) the CTA's
-    Key merged[kTopMax];
+    Key found[kLpFound];            // candidates, in any order
+    Key lists[kLpWarps][kTopMax];   // the warps' best, where `found` overflowed
+    Key merged[kTopMax];            // the CTA's best
     float group_max[32];
     float red[kLpWarps][4];
-    float stat[4];                  // the CTA's (m, top, rest, S)
+    float stat[5];                  // the CTA's (m, top, rest, S) and its largest logit
     float floor;                    // n_top logits of the CTA's share reach this
+    int count;                      // candidates
+};
+struct LpCluster {                  // what the shares of a row show each other
+    Key lists[kLpShares][kTopMax];
+    float stat[kLpShares][5];
+    int rank[kTopMax];
 };
 
-// A thread's vectors of a row: 16-byte vectors from the first aligned
-// element, the unaligned head as vector -1, the rest as the last one.
+// 16 bytes of T as they lie in memory.  The exponentials take values of at
+// least kLowest: e^(x - m) is 0 there, and 0 times a finite distance adds
+// nothing to S.
+template <typename T>
+struct Raw {
+    static constexpr int V = 8;
+    static constexpr bool kBf = std::is_same<T, __nv_bfloat16>::value;
+    static constexpr uint32_t kNone = kBf ? 0xff80ff80u : 0xfc00fc00u;     // -inf
+    static constexpr uint32_t kLowest2 = kBf ? 0xfe96fe96u : 0xfbfffbffu;  // -1e38, or fp16's lowest
+    static __device__ float lowest() { return unpack2<T>(kLowest2).x; }
+    // the largest value, NaN left aside
+    static __device__ __forceinline__ void raise(uint32_t (&m)[2], uint4 u) {
+        m[0] = max2(max2(m[0], u.x), u.z);
+        m[1] = max2(max2(m[1], u.y), u.w);
+    }
+    static __device__ __forceinline__ float largest(const uint32_t (&m)[2]) {
+        const float2 v = unpack2<T>(max2(m[0], m[1]));
+        return fmaxf(v.x, v.y);
+    }
+    static __device__ __forceinline__ float2 pair_of(uint4 u, int i) {   // pair i of 4, raised to kLowest, NaN kept
+        const uint32_t w = i == 0 ? u.x : i == 1 ? u.y : i == 2 ? u.z : u.w;
+        uint32_t r;
+        if (kBf) asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(w), "r"(kLowest2));
+        else asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(w), "r"(kLowest2));
+        return unpack2<T>(r);
+    }
+    static __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
+        uint32_t r;
+        if (kBf) asm("max.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+        else asm("max.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+        return r;
+    }
+    static __device__ void values(uint4 u, float (&f)[V]) {
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const float2 a = unpack2<T>(w[i]);
+            f[2 * i] = a.x;
+            f[2 * i + 1] = a.y;
+        }
+    }
+};
+template <>
+struct Raw<float> {
+    static constexpr int V = 4;
+    static constexpr uint32_t kNone = 0xff800000u;
+    static __device__ float lowest() { return -1e38f; }
+    static __device__ __forceinline__ void raise(uint32_t (&m)[2], uint4 u) {
+        const float a = fmaxf(fmaxf(__uint_as_float(u.x), __uint_as_float(u.y)), __uint_as_float(m[0]));
+        const float b = fmaxf(fmaxf(__uint_as_float(u.z), __uint_as_float(u.w)), __uint_as_float(m[1]));
+        m[0] = __float_as_uint(a);
+        m[1] = __float_as_uint(b);
+    }
+    static __device__ __forceinline__ float largest(const uint32_t (&m)[2]) {
+        return fmaxf(__uint_as_float(m[0]), __uint_as_float(m[1]));
+    }
+    static __device__ __forceinline__ float2 pair_of(uint4 u, int i) {
+        const float a = __uint_as_float(i == 0 ? u.x : u.z), b = __uint_as_float(i == 0 ? u.y : u.w);
+        return make_float2(fmax_nan(a, -1e38f), fmax_nan(b, -1e38f));
+    }
+    static __device__ void values(uint4 u, float (&f)[V]) {
+        f[0] = __uint_as_float(u.x);
+        f[1] = __uint_as_float(u.y);
+        f[2] = __uint_as_float(u.z);
+        f[3] = __uint_as_float(u.w);
+    }
+};
+
+// A row as vectors: 16-byte vectors from the first aligned element, the
+// unaligned head as vector -1, the rest as the last one (`full`).
 template <typename T>
 struct RowView {
-    static constexpr int V = 16 / (int)sizeof(T);
+    static constexpr int V = Raw<T>::V;
     const T *x;
     int head, full, vocab;   // head elements, whole vectors, all elements
     __device__ RowView(const T *row, int n) : x(row), vocab(n) {
@@ -71,40 +150,36 @@ struct RowView {
         head = min(head, n);
         full = (n - head) / V;
     }
-    // vectors -1 .. full; element 0 of vector v
+    // element 0 of vector v and its elements, -1 <= v <= full
     __device__ int first(int v) const { return v < 0 ? 0 : head + v * V; }
     __device__ int count(int v) const { return v < 0 ? head : v < full ? V : vocab - head - full * V; }
-    __device__ void get(int v, float (&f)[V]) const {
-        if (v >= 0 && v < full) {
-            const uint4 u = __ldg(reinterpret_cast<const uint4 *>(x + head) + v);
-            const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-            if constexpr (sizeof(T) == 4) {
+    __device__ __forceinline__ uint4 whole(int v) const { return __ldg(reinterpret_cast<const uint4 *>(x + head) + v); }
+    // vector v, -inf past its end
+    __device__ uint4 any(int v) const {
+        if (v >= 0 && v < full) return whole(v);
+        union {
+            T e[V];
+            uint4 u;
+        } r;
+        const uint32_t none = Raw<T>::kNone;
+        r.u = make_uint4(none, none, none, none);
+        const int n = count(v), b = first(v);
 #pragma unroll
-                for (int i = 0; i < 4; i++) f[i] = __uint_as_float(w[i]);
-            } else {
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const float2 a = unpack2<T>(w[i]);
-                    f[2 * i] = a.x;
-                    f[2 * i + 1] = a.y;
-                }
-            }
-        } else {
-            const int n = count(v), b = first(v);
-#pragma unroll
-            for (int i = 0; i < V; i++) f[i] = i < n ? (float)x[b + i] : -INFINITY;   // adds nothing
-        }
+        for (int i = 0; i < V; i++)
+            if (i < n) r.e[i] = x[b + i];
+        return r.u;
     }
 };
 
-// the larger value, or NaN if either is
-__device__ __forceinline__ float fmax_nan(float a, float b) {
+// the warp's largest value, NaN left aside
+__device__ __forceinline__ float warp_max(float v) {
     float r;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
     return r;
 }
 
-// Adds a second part (m2, ...) of a row to the first.
+// Adds a second part (m2, ...) of a row to the first.  S is kept in log2
+// units: the sum of e^(x - m) (x - m) log2(e).
 __device__ __forceinline__ void fold(float &m, float &top, float &rest, float &mom, float m2, float top2, float rest2,
                                      float mom2) {
     if (m2 == m) {
@@ -114,7 +189,7 @@ __device__ __forceinline__ void fold(float &m, float &top, float &rest, float &m
         return;
     }
     const bool up = m2 > m;   // the second part's maximum is the larger: it keeps its top
-    const float d = fmax_nan(up ? m - m2 : m2 - m, kLpFloor), w = exp2_approx(d * kLog2e);
+    const float d = fmax_nan((up ? m - m2 : m2 - m) * kLog2e, kLpFloor), w = exp2_approx(d);
     const float low = up ? rest + top : rest2 + top2, low_mom = up ? mom : mom2;
     mom = (up ? mom2 : mom) + w * fmaf(low, d, low_mom);
     rest = (up ? rest2 : rest) + w * low;
@@ -143,15 +218,73 @@ __device__ __forceinline__ int better(const Key *list, int n, Key k) {
     return lo;
 }
 
+// fold() over the lanes' parts (NULL: none) of a power of two of lanes.
+__device__ __forceinline__ void fold_lanes(const float *part, int n, float &m, float &top, float &rest, float &mom) {
+    m = part ? part[0] : -INFINITY;
+    top = part ? part[1] : 0.f;
+    rest = part ? part[2] : 0.f;
+    mom = part ? part[3] : 0.f;
+    for (int o = n / 2; o > 0; o >>= 1)
+        fold(m, top, rest, mom, __shfl_xor_sync(0xffffffffu, m, o), __shfl_xor_sync(0xffffffffu, top, o),
+             __shfl_xor_sync(0xffffffffu, rest, o), __shfl_xor_sync(0xffffffffu, mom, o));
+    m = __shfl_sync(0xffffffffu, m, 0);
+    top = __shfl_sync(0xffffffffu, top, 0);
+    rest = __shfl_sync(0xffffffffu, rest, 0);
+    mom = __shfl_sync(0xffffffffu, mom, 0);
+}
+
+// The CTA's K best where more than kLpFound logits reach the floor (equal
+// logits, sorted rows): each warp holds a sorted list across its lanes and
+// goes over its values in the order of their ids, so that equal ones later in
+// the row cost a comparison each.
 template <typename T>
-__global__ void __launch_bounds__(kLpThreads) token_logprobs_kernel(const LogprobParams p, int Z) {
-    using R = RowView<T>;
-    constexpr int V = R::V;
+__device__ __noinline__ void list_rows(LpSmem &sh, const RowView<T> &x, int v0, int v1, int K, float floor) {
+    constexpr int V = Raw<T>::V, kBatch = kLpThreads * kLpLoads;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    Key mine = 0;   // lane i: the warp's i-th best
+    int b = 0;
+    for (int vb = v0; vb < v1; vb += kBatch, b++) {
+        const bool hit = sh.batch_max[b % kLpSlots][threadIdx.x] >= floor;
+        if (!__any_sync(0xffffffffu, hit)) continue;
+        for (int u = 0; u < kLpLoads; u++) {
+            const int v = vb + u * kLpThreads + threadIdx.x;
+            const uint32_t none = Raw<T>::kNone;
+            float f[V];
+            Raw<T>::values(hit && v < v1 ? x.any(v) : make_uint4(none, none, none, none), f);
+            const int id0 = x.first(v), n = hit && v < v1 ? x.count(v) : 0;
+#pragma unroll
+            for (int i = 0; i < V; i++) {
+                bool cand = i < n && f[i] >= floor;
+                if (!__any_sync(0xffffffffu, cand)) continue;
+                const Key k = make_key(f[i], id0 + i);
+                for (;;) {
+                    const Key last = __shfl_sync(0xffffffffu, mine, K - 1);
+                    const unsigned todo = __ballot_sync(0xffffffffu, cand && k > last);
+                    if (!todo) break;
+                    const int from = __ffs(todo) - 1;
+                    list_insert(mine, __shfl_sync(0xffffffffu, k, from), lane);
+                    if (lane == from) cand = false;
+                }
+            }
+        }
+    }
+    sh.lists[warp][lane] = lane < K ? mine : 0;
+    __syncthreads();
+    if (lane < K && mine != 0) {   // the rank of each key among the 8 lists
+        int rank = 0;
+        for (int w = 0; w < kLpWarps; w++) rank += better(sh.lists[w], K, mine);
+        if (rank < K) sh.merged[rank] = mine;
+    }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kLpThreads, 4) token_logprobs_kernel(const LogprobParams p, int Z) {
+    constexpr int V = Raw<T>::V;
     __shared__ LpSmem sh;
-    __shared__ Key all[16 * kTopMax];   // rank 0: the cluster's lists
+    __shared__ LpCluster cl;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int row = blockIdx.x / Z, z = blockIdx.x % Z;
-    const R x(static_cast<const T *>(p.logits) + (long long)row * p.ld, p.vocab);
+    const RowView<T> x(static_cast<const T *>(p.logits) + (long long)row * p.ld, p.vocab);
     // this CTA's vectors, of -1 .. full
     const int nv = x.full + 2;
     const int v0 = (int)((long long)z * nv / Z) - 1, v1 = (int)((long long)(z + 1) * nv / Z) - 1;
@@ -160,52 +293,85 @@ __global__ void __launch_bounds__(kLpThreads) token_logprobs_kernel(const Logpro
     // Z = top + rest: `top` counts the logits equal to m, the others' e^(x - m)
     // add up apart from it, so that a confident row's ln Z and H keep their
     // leading digits (ln Z = log1p(rest)).
-    float m = -FLT_MAX, top = 0.f, rest = 0.f, mom = 0.f, best = -INFINITY;
+    // The maximum is the warp's, so that few batches move it.
+    const float lowest = Raw<T>::lowest();
+    float m = lowest, top = 0.f, rest = 0.f, mom = 0.f, best = -INFINITY;
     for (int s = 0; s < kLpSlots; s++) sh.batch_max[s][threadIdx.x] = -INFINITY;
-    int b = 0;
-    for (int vb = v0; vb < v1; vb += kLpThreads * kLpLoads, b++) {
-        float f[kLpLoads][V];
+    constexpr int kBatch = kLpThreads * kLpLoads;
+    auto load = [&](int vb, uint4 (&u)[kLpLoads]) {
+        const int v = vb + threadIdx.x;
+        if (vb >= 0 && vb + kBatch <= min(v1, x.full)) {
 #pragma unroll
-        for (int u = 0; u < kLpLoads; u++) {
-            const int v = vb + u * kLpThreads + threadIdx.x;
-            if (v < v1) x.get(v, f[u]);
-            else {
+            for (int i = 0; i < kLpLoads; i++) u[i] = x.whole(v + i * kLpThreads);
+        } else {
 #pragma unroll
-                for (int i = 0; i < V; i++) f[u][i] = -INFINITY;
+            for (int i = 0; i < kLpLoads; i++) {
+                const uint32_t none = Raw<T>::kNone;
+                u[i] = v + i * kLpThreads < v1 ? x.any(v + i * kLpThreads) : make_uint4(none, none, none, none);
             }
         }
-        float bm = -INFINITY;
+    };
+    uint4 u[kLpLoads], next[kLpLoads];
+    if (v0 < v1) load(v0, u);
+    int b = 0;
+    for (int vb = v0; vb < v1; vb += kBatch, b++) {
+        if (vb + kBatch < v1) load(vb + kBatch, next);
+        uint32_t mw[2] = {Raw<T>::kNone, Raw<T>::kNone};
 #pragma unroll
-        for (int u = 0; u < kLpLoads; u++)
-#pragma unroll
-            for (int i = 0; i < V; i++) bm = fmaxf(bm, f[u][i]);
+        for (int i = 0; i < kLpLoads; i++) Raw<T>::raise(mw, u[i]);
+        const float bm = Raw<T>::largest(mw);
+        best = fmaxf(best, bm);
         if (K > 0) {
             float &slot = sh.batch_max[b % kLpSlots][threadIdx.x];
             slot = fmaxf(slot, bm);
-            best = fmaxf(best, bm);
         }
-        if (bm > m) {
-            const float d = fmax_nan(m - bm, kLpFloor), w = exp2_approx(d * kLog2e);
+        const float wm = fmaxf(warp_max(bm), lowest);
+        if (wm > m) {
+            const float d = fmax_nan((m - wm) * kLog2e, kLpFloor), w = exp2_approx(d);
             rest += top;
             mom = w * fmaf(rest, d, mom);
             rest *= w;
             top = 0.f;
-            m = bm;
+            m = wm;
         }
-        if (bm == m) {
+        const uint64_t l2 = pair(kLog2e, kLog2e), ml = pair(-m * kLog2e, -m * kLog2e);
+        uint64_t s2[2] = {0, 0}, t2[2] = {0, 0};
+        if (wm < m) {   // (the maximum is in another batch)
 #pragma unroll
-            for (int u = 0; u < kLpLoads; u++)
+            for (int i = 0; i < kLpLoads; i++)
 #pragma unroll
-                for (int i = 0; i < V; i++) top += f[u][i] == m ? 1.f : 0.f;
+                for (int j = 0; j < V / 2; j++) {
+                    const float2 f = Raw<T>::pair_of(u[i], j);
+                    const uint64_t t = fma2(pair(f.x, f.y), l2, ml);
+                    float ta, tb;
+                    unpair(t, ta, tb);
+                    const uint64_t e = pair(exp2_approx(ta), exp2_approx(tb));
+                    s2[j & 1] = add2(s2[j & 1], e);
+                    t2[j & 1] = fma2(e, t, t2[j & 1]);
+                }
+        } else {
+#pragma unroll
+            for (int i = 0; i < kLpLoads; i++)
+#pragma unroll
+                for (int j = 0; j < V / 2; j++) {
+                    const float2 f = Raw<T>::pair_of(u[i], j);
+                    const uint64_t t = fma2(pair(f.x, f.y), l2, ml);
+                    float ta, tb;
+                    unpair(t, ta, tb);
+                    const bool a = f.x == m, c = f.y == m;
+                    top += (a ? 1.f : 0.f) + (c ? 1.f : 0.f);
+                    const uint64_t e = pair(a ? 0.f : exp2_approx(ta), c ? 0.f : exp2_approx(tb));
+                    s2[j & 1] = add2(s2[j & 1], e);
+                    t2[j & 1] = fma2(e, t, t2[j & 1]);
+                }
         }
+        float a, c;
+        unpair(add2(s2[0], s2[1]), a, c);
+        rest += a + c;
+        unpair(add2(t2[0], t2[1]), a, c);
+        mom += a + c;
 #pragma unroll
-        for (int u = 0; u < kLpLoads; u++)
-#pragma unroll
-            for (int i = 0; i < V; i++) {
-                const float d = fmax_nan(f[u][i] - m, kLpFloor), e = exp2_approx(d * kLog2e);
-                if (!(d == 0.f)) rest += e;
-                mom = fmaf(e, d, mom);
-            }
+        for (int i = 0; i < kLpLoads; i++) u[i] = next[i];
     }
 
     // the CTA's (m, top, rest, S)
@@ -219,130 +385,163 @@ __global__ void __launch_bounds__(kLpThreads) token_logprobs_kernel(const Logpro
         sh.red[warp][2] = rest;
         sh.red[warp][3] = mom;
     }
-    if (K > 0) {
+    {
         float g = best;
 #pragma unroll
         for (int o = 4; o > 0; o >>= 1) g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, o));
         if ((lane & 7) == 0) sh.group_max[warp * 4 + lane / 8] = g;
     }
+    if (threadIdx.x < kTopMax) sh.merged[threadIdx.x] = 0;
+    if (threadIdx.x == 0) sh.count = 0;
     __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int w = 1; w < kLpWarps; w++)
-            fold(m, top, rest, mom, sh.red[w][0], sh.red[w][1], sh.red[w][2], sh.red[w][3]);
-        sh.stat[0] = m;
-        sh.stat[1] = top;
-        sh.stat[2] = rest;
-        sh.stat[3] = mom;
+    if (warp == 0) {
+        fold_lanes(lane < kLpWarps ? sh.red[lane] : nullptr, kLpWarps, m, top, rest, mom);
+        const float g = warp_max(sh.group_max[lane]);
+        if (lane == 0) {
+            sh.stat[0] = m;
+            sh.stat[1] = top;
+            sh.stat[2] = rest;
+            sh.stat[3] = mom;
+            sh.stat[4] = g;
+        }
     }
     if (K > 0) {
         if (warp == 1) {   // the K-th largest group maximum: K - 1 others are at least as large
             const float g = sh.group_max[lane];
             int rank = 0;
+#pragma unroll
             for (int o = 0; o < 32; o++) {
-                const float h = __shfl_sync(0xffffffffu, g, o);
+                const float h = sh.group_max[o];
                 rank += h > g || (h == g && o < lane);
             }
             if (rank == K - 1) sh.floor = g;
         }
         __syncthreads();
         const float floor = sh.floor;
-        Key mine = 0;   // lane i: the warp's i-th best
         for (int s = 0; s < kLpSlots; s++) {
-            bool hit = sh.batch_max[s][threadIdx.x] >= floor;
-            if (!__any_sync(0xffffffffu, hit)) continue;
-            for (int vb = v0 + s * kLpThreads * kLpLoads; vb < v1; vb += kLpSlots * kLpThreads * kLpLoads) {
-                float f[kLpLoads][V];
+            if (!(sh.batch_max[s][threadIdx.x] >= floor)) continue;
+            for (int vb = v0 + s * kBatch; vb < v1; vb += kLpSlots * kBatch) {
+                uint4 c[kLpLoads];
+                load(vb, c);
 #pragma unroll
-                for (int u = 0; u < kLpLoads; u++) {
-                    const int v = vb + u * kLpThreads + threadIdx.x;
-                    if (hit && v < v1) x.get(v, f[u]);
-                    else {
+                for (int i = 0; i < kLpLoads; i++) {
+                    const int v = vb + i * kLpThreads + threadIdx.x;
+                    const int id0 = x.first(v), n = v < v1 ? x.count(v) : 0;
+                    float f[V];
+                    Raw<T>::values(c[i], f);
 #pragma unroll
-                        for (int i = 0; i < V; i++) f[u][i] = -INFINITY;
-                    }
-                }
-#pragma unroll
-                for (int u = 0; u < kLpLoads; u++) {
-                    const int v = vb + u * kLpThreads + threadIdx.x;
-                    const int id0 = x.first(v), n = hit && v < v1 ? x.count(v) : 0;
-#pragma unroll
-                    for (int i = 0; i < V; i++) {
-                        bool cand = i < n && f[u][i] >= floor;
-                        if (!__any_sync(0xffffffffu, cand)) continue;
-                        const Key k = make_key(f[u][i], id0 + i);
-                        for (;;) {
-                            const Key last = __shfl_sync(0xffffffffu, mine, K - 1);
-                            const unsigned todo = __ballot_sync(0xffffffffu, cand && k > last);
-                            if (!todo) break;
-                            const int from = __ffs(todo) - 1;
-                            list_insert(mine, __shfl_sync(0xffffffffu, k, from), lane);
-                            if (lane == from) cand = false;
+                    for (int j = 0; j < V; j++)
+                        if (f[j] >= floor && j < n) {
+                            const int at = atomicAdd(&sh.count, 1);
+                            if (at < kLpFound) sh.found[at] = make_key(f[j], id0 + j);
                         }
-                    }
                 }
             }
         }
-        sh.lists[warp][lane] = lane < K ? mine : 0;
         __syncthreads();
-        if (threadIdx.x < kTopMax) sh.merged[threadIdx.x] = 0;
-        __syncthreads();
-        if (lane < K && mine != 0) {   // the rank of each key among the 8 lists
-            int rank = 0;
-            for (int w = 0; w < kLpWarps; w++) rank += better(sh.lists[w], K, mine);
-            if (rank < K) sh.merged[rank] = mine;
-        }
-    }
-    if (Z > 1) cluster_sync_all();
-    else __syncthreads();
-
-    if (z == 0) {
-        // the cluster's (m, top, rest, S), in every thread
-        float gm = sh.stat[0], gn = sh.stat[1], gr = sh.stat[2], gt = sh.stat[3];
-        for (int r = 1; r < Z; r++) {
-            const uint32_t a = mapa_shared(smem_u32(sh.stat), r);
-            fold(gm, gn, gr, gt, ld_dsmem_f1(a), ld_dsmem_f1(a + 4), ld_dsmem_f1(a + 8), ld_dsmem_f1(a + 12));
-        }
-        const float lz = gn == 1.f ? log1pf(gr) : logf(gn + gr);
-        if (threadIdx.x == 0) {
-            if (p.logprob) {
-                const int tok = p.tokens ? __ldg(p.tokens + row) : -1;
-                // a row without a finite logit has no distribution: NaN
-                p.logprob[row] = tok >= 0 && tok < p.vocab ? ((float)x.x[tok] - gm) - lz : NAN;
-            }
-            if (p.entropy) p.entropy[row] = lz - gt / (gn + gr);
-        }
-        if (K > 0) {
-            const Key *lists = sh.merged;
-            if (Z > 1) {
-                for (int e = threadIdx.x; e < Z * kTopMax; e += kLpThreads) {
-                    const uint32_t a = mapa_shared(smem_u32(sh.merged + e % kTopMax), e / kTopMax);
-                    const float2 v = ld_dsmem_f2(a);
-                    all[e] = ((Key)__float_as_uint(v.y) << 32) | __float_as_uint(v.x);
-                }
-                __syncthreads();
-                lists = all;
-            }
-            if (threadIdx.x < K) {   // NaN logits are no alternatives: places that nothing fills
-                int found = 0;
-                for (int r = 0; r < Z; r++) found += better(lists + r * kTopMax, K, 0);
-                if (threadIdx.x >= found) {
-                    p.top_ids[(long long)row * K + threadIdx.x] = -1;
-                    if (p.top_logprob) p.top_logprob[(long long)row * K + threadIdx.x] = NAN;
-                }
-            }
-            for (int e = threadIdx.x; e < Z * kTopMax; e += kLpThreads) {
-                const Key k = lists[e];
-                if (k == 0) continue;
+        const int found = sh.count;
+        if (found <= kLpFound) {
+            if (threadIdx.x < found) {
+                const Key k = sh.found[threadIdx.x];
                 int rank = 0;
-                for (int r = 0; r < Z; r++) rank += better(lists + r * kTopMax, K, k);
-                if (rank < K) {
-                    p.top_ids[(long long)row * K + rank] = key_id(k);
-                    if (p.top_logprob) p.top_logprob[(long long)row * K + rank] = (key_value(k) - gm) - lz;
-                }
+#pragma unroll 8
+                for (int o = 0; o < found; o++) rank += sh.found[o] > k;
+                if (rank < K) sh.merged[rank] = k;
             }
+        } else {
+            list_rows<T>(sh, x, v0, v1, K, floor);
         }
     }
-    if (Z > 1) cluster_sync_all();   // no CTA leaves while rank 0 still reads its share
+    __syncthreads();
+
+    // the row's (m, top, rest, S) and largest logit
+    float gm, gn, gr, gt, gb;
+    if (Z > 1) {
+        cluster_sync_all();
+        if (threadIdx.x < Z * 5)
+            cl.stat[threadIdx.x / 5][threadIdx.x % 5] =
+                ld_dsmem_f1(mapa_shared(smem_u32(sh.stat + threadIdx.x % 5), threadIdx.x / 5));
+        for (int e = threadIdx.x; e < Z * kTopMax && K > 0; e += kLpThreads) {
+            const float2 v = ld_dsmem_f2(mapa_shared(smem_u32(sh.merged + e % kTopMax), e / kTopMax));
+            cl.lists[e / kTopMax][e % kTopMax] = ((Key)__float_as_uint(v.y) << 32) | __float_as_uint(v.x);
+        }
+        if (threadIdx.x < kTopMax) cl.rank[threadIdx.x] = 0;
+        cluster_sync_all();   // (peers may leave now: their shares have been read)
+        fold_lanes(lane < Z ? cl.stat[lane] : nullptr, kLpShares, gm, gn, gr, gt);
+        gb = warp_max(lane < Z ? cl.stat[lane][4] : -INFINITY);
+    } else {
+        gm = sh.stat[0];
+        gn = sh.stat[1];
+        gr = sh.stat[2];
+        gt = sh.stat[3];
+        gb = sh.stat[4];
+    }
+    if (gb <= lowest && gb > -INFINITY) {
+        // every logit is as low as a mask's: the sums above took the vectors'
+        // padding along, so once more, value by value
+        gn = gr = gt = 0.f;
+        for (int i = threadIdx.x; i < p.vocab; i += kLpThreads) {
+            const float d = ((float)x.x[i] - gb) * kLog2e, e = exp2_approx(d);
+            if (d == 0.f) gn += 1.f;
+            else {
+                gr += e;
+                if (e != 0.f) gt = fmaf(e, d, gt);
+            }
+        }
+        gn = warp_sum(gn);
+        gr = warp_sum(gr);
+        gt = warp_sum(gt);
+        __syncthreads();
+        if (lane == 0) {
+            sh.red[warp][0] = gn;
+            sh.red[warp][1] = gr;
+            sh.red[warp][2] = gt;
+        }
+        __syncthreads();
+        gn = gr = gt = 0.f;
+        for (int w = 0; w < kLpWarps; w++) {
+            gn += sh.red[w][0];
+            gr += sh.red[w][1];
+            gt += sh.red[w][2];
+        }
+    }
+    float lz = gn == 1.f ? log1pf(gr) : logf(gn + gr);
+    gt *= 0.69314718055994531f;              // from log2 units
+    if (!(fabsf(gb) < INFINITY)) lz = NAN;   // no finite logit, or an infinite one
+    if (z == 0 && threadIdx.x == 0) {
+        if (p.logprob) {
+            const int tok = __ldg(p.tokens + row);
+            p.logprob[row] = tok >= 0 && tok < p.vocab ? ((float)x.x[tok] - gb) - lz : NAN;
+        }
+        if (p.entropy) p.entropy[row] = lz - gt / (gn + gr);
+    }
+    if (K == 0) return;
+    int *ids = p.top_ids + (long long)row * K;
+    float *lps = p.top_logprob ? p.top_logprob + (long long)row * K : nullptr;
+    auto put = [&](int rank, Key k) {   // NaN logits are no alternatives: key 0 where nothing is left
+        ids[rank] = k ? key_id(k) : -1;
+        if (lps) lps[rank] = k ? (key_value(k) - gb) - lz : NAN;
+    };
+    if (Z == 1) {
+        if (threadIdx.x < K) put(threadIdx.x, sh.merged[threadIdx.x]);
+        return;
+    }
+    // each share ranks its own list among all: a thread per (key, list)
+    for (int e = threadIdx.x; e < Z * kTopMax; e += kLpThreads) {
+        const Key k = cl.lists[z][e % kTopMax];
+        if (k) atomicAdd(&cl.rank[e % kTopMax], better(cl.lists[e / kTopMax], K, k));
+    }
+    __syncthreads();
+    if (threadIdx.x < K) {
+        const Key k = cl.lists[z][threadIdx.x];
+        if (k && cl.rank[threadIdx.x] < K) put(cl.rank[threadIdx.x], k);
+    }
+    if (z == 0 && threadIdx.x < 32) {   // places that nothing fills
+        int found = lane < Z ? better(cl.lists[lane], K, 0) : 0;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) found += __shfl_xor_sync(0xffffffffu, found, o);
+        if (lane < K && lane >= found) put(lane, 0);
+    }
 }
 
 template <typename T>
