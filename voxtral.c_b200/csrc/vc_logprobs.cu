@@ -31,11 +31,13 @@ using namespace tc;
 
 namespace {
 
-constexpr int kLpThreads = 256;
-constexpr int kLpWarps = kLpThreads / 32;
+// Threads of a CTA: 256 where a row is shared by CTAs and latency counts, 128
+// where every CTA has a row: twice as many rows are under way on an SM, and one
+// row's end hides under the others.
+constexpr int kLpFew = 256, kLpMany = 128;
 constexpr int kLpLoads = 4;      // 16-byte loads of a thread's batch
-constexpr int kLpSlots = 16;     // batch maxima kept per thread; batch b in slot b % 16
-constexpr int kLpFound = 256;    // candidates kept
+constexpr int kLpKept = 4096;    // batch maxima kept: NTH threads x 4096 / NTH slots, batch b in slot b % slots
+constexpr int kLpFound = 256;    // candidates, and batches with some, kept
 constexpr int kLpShares = 16;    // CTAs of a row at most
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLpFloor = -300.f;   // 2^x below this is 0 in fp32
@@ -53,15 +55,18 @@ __device__ __forceinline__ float key_value(Key k) {
 }
 __device__ __forceinline__ int key_id(Key k) { return 0x7fffffff - (int)(uint32_t)k; }
 
+template <int NTH>
 struct LpSmem {
-    float batch_max[kLpSlots][kLpThreads];
+    static constexpr int kWarps = NTH / 32, kSlots = kLpKept / NTH;
+    float batch_max[kSlots][NTH];
     Key found[kLpFound];            // candidates, in any order
-    Key lists[kLpWarps][kTopMax];   // the warps' best, where `found` overflowed
+    Key lists[kWarps][kTopMax];   // the warps' best, where `found` overflowed
     Key merged[kTopMax];            // the CTA's best
     float group_max[32];
-    float red[kLpWarps][4];
+    float red[kWarps][4];
     float stat[5];                  // the CTA's (m, top, rest, S) and its largest logit
     float floor;                    // n_top logits of the CTA's share reach this
+    int hit[kLpFound], hits;        // batches with candidates: batch * NTH + thread
     int count;                      // candidates
 };
 struct LpCluster {                  // what the shares of a row show each other
@@ -237,17 +242,17 @@ __device__ __forceinline__ void fold_lanes(const float *part, int n, float &m, f
 // logits, sorted rows): each warp holds a sorted list across its lanes and
 // goes over its values in the order of their ids, so that equal ones later in
 // the row cost a comparison each.
-template <typename T>
-__device__ __noinline__ void list_rows(LpSmem &sh, const RowView<T> &x, int v0, int v1, int K, float floor) {
-    constexpr int V = Raw<T>::V, kBatch = kLpThreads * kLpLoads;
+template <typename T, int NTH>
+__device__ __noinline__ void list_rows(LpSmem<NTH> &sh, const RowView<T> &x, int v0, int v1, int K, float floor) {
+    constexpr int V = Raw<T>::V, kBatch = NTH * kLpLoads;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     Key mine = 0;   // lane i: the warp's i-th best
     int b = 0;
     for (int vb = v0; vb < v1; vb += kBatch, b++) {
-        const bool hit = sh.batch_max[b % kLpSlots][threadIdx.x] >= floor;
+        const bool hit = sh.batch_max[b % LpSmem<NTH>::kSlots][threadIdx.x] >= floor;
         if (!__any_sync(0xffffffffu, hit)) continue;
         for (int u = 0; u < kLpLoads; u++) {
-            const int v = vb + u * kLpThreads + threadIdx.x;
+            const int v = vb + u * NTH + threadIdx.x;
             const uint32_t none = Raw<T>::kNone;
             float f[V];
             Raw<T>::values(hit && v < v1 ? x.any(v) : make_uint4(none, none, none, none), f);
@@ -272,15 +277,15 @@ __device__ __noinline__ void list_rows(LpSmem &sh, const RowView<T> &x, int v0, 
     __syncthreads();
     if (lane < K && mine != 0) {   // the rank of each key among the 8 lists
         int rank = 0;
-        for (int w = 0; w < kLpWarps; w++) rank += better(sh.lists[w], K, mine);
+        for (int w = 0; w < (NTH / 32); w++) rank += better(sh.lists[w], K, mine);
         if (rank < K) sh.merged[rank] = mine;
     }
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kLpThreads, 4) token_logprobs_kernel(const LogprobParams p, int Z) {
+template <typename T, int NTH>
+__global__ void __launch_bounds__(NTH, 1024 / NTH) token_logprobs_kernel(const LogprobParams p, int Z) {
     constexpr int V = Raw<T>::V;
-    __shared__ LpSmem sh;
+    __shared__ LpSmem<NTH> sh;
     __shared__ LpCluster cl;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int row = blockIdx.x / Z, z = blockIdx.x % Z;
@@ -296,35 +301,30 @@ __global__ void __launch_bounds__(kLpThreads, 4) token_logprobs_kernel(const Log
     // The maximum is the warp's, so that few batches move it.
     const float lowest = Raw<T>::lowest();
     float m = lowest, top = 0.f, rest = 0.f, mom = 0.f, best = -INFINITY;
-    for (int s = 0; s < kLpSlots; s++) sh.batch_max[s][threadIdx.x] = -INFINITY;
-    constexpr int kBatch = kLpThreads * kLpLoads;
+    constexpr int kSlots = LpSmem<NTH>::kSlots;
+    for (int s = 0; s < kSlots; s++) sh.batch_max[s][threadIdx.x] = -INFINITY;
+    constexpr int kBatch = NTH * kLpLoads;
     auto load = [&](int vb, uint4 (&u)[kLpLoads]) {
         const int v = vb + threadIdx.x;
         if (vb >= 0 && vb + kBatch <= min(v1, x.full)) {
 #pragma unroll
-            for (int i = 0; i < kLpLoads; i++) u[i] = x.whole(v + i * kLpThreads);
+            for (int i = 0; i < kLpLoads; i++) u[i] = x.whole(v + i * NTH);
         } else {
 #pragma unroll
             for (int i = 0; i < kLpLoads; i++) {
                 const uint32_t none = Raw<T>::kNone;
-                u[i] = v + i * kLpThreads < v1 ? x.any(v + i * kLpThreads) : make_uint4(none, none, none, none);
+                u[i] = v + i * NTH < v1 ? x.any(v + i * NTH) : make_uint4(none, none, none, none);
             }
         }
     };
-    uint4 u[kLpLoads], next[kLpLoads];
-    if (v0 < v1) load(v0, u);
-    int b = 0;
-    for (int vb = v0; vb < v1; vb += kBatch, b++) {
-        if (vb + kBatch < v1) load(vb + kBatch, next);
+    auto take = [&](const uint4 (&u)[kLpLoads], int b) {   // batch b
         uint32_t mw[2] = {Raw<T>::kNone, Raw<T>::kNone};
 #pragma unroll
         for (int i = 0; i < kLpLoads; i++) Raw<T>::raise(mw, u[i]);
         const float bm = Raw<T>::largest(mw);
         best = fmaxf(best, bm);
-        if (K > 0) {
-            float &slot = sh.batch_max[b % kLpSlots][threadIdx.x];
-            slot = fmaxf(slot, bm);
-        }
+        if (b < kSlots) sh.batch_max[b][threadIdx.x] = bm;
+        else sh.batch_max[b % kSlots][threadIdx.x] = fmaxf(sh.batch_max[b % kSlots][threadIdx.x], bm);
         const float wm = fmaxf(warp_max(bm), lowest);
         if (wm > m) {
             const float d = fmax_nan((m - wm) * kLog2e, kLpFloor), w = exp2_approx(d);
@@ -370,8 +370,11 @@ __global__ void __launch_bounds__(kLpThreads, 4) token_logprobs_kernel(const Log
         rest += a + c;
         unpair(add2(t2[0], t2[1]), a, c);
         mom += a + c;
-#pragma unroll
-        for (int i = 0; i < kLpLoads; i++) u[i] = next[i];
+    };
+    for (int vb = v0, b = 0; vb < v1; vb += kBatch, b++) {
+        uint4 u[kLpLoads];
+        load(vb, u);
+        take(u, b);
     }
 
     // the CTA's (m, top, rest, S)
@@ -388,14 +391,14 @@ __global__ void __launch_bounds__(kLpThreads, 4) token_logprobs_kernel(const Log
     {
         float g = best;
 #pragma unroll
-        for (int o = 4; o > 0; o >>= 1) g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, o));
-        if ((lane & 7) == 0) sh.group_max[warp * 4 + lane / 8] = g;
+        for (int o = NTH / 64; o > 0; o >>= 1) g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, o));
+        if (lane % (NTH / 32) == 0) sh.group_max[threadIdx.x / (NTH / 32)] = g;   // 32 groups of threads
     }
     if (threadIdx.x < kTopMax) sh.merged[threadIdx.x] = 0;
-    if (threadIdx.x == 0) sh.count = 0;
+    if (threadIdx.x == 0) sh.count = sh.hits = 0;
     __syncthreads();
     if (warp == 0) {
-        fold_lanes(lane < kLpWarps ? sh.red[lane] : nullptr, kLpWarps, m, top, rest, mom);
+        fold_lanes(lane < (NTH / 32) ? sh.red[lane] : nullptr, (NTH / 32), m, top, rest, mom);
         const float g = warp_max(sh.group_max[lane]);
         if (lane == 0) {
             sh.stat[0] = m;
@@ -418,38 +421,45 @@ __global__ void __launch_bounds__(kLpThreads, 4) token_logprobs_kernel(const Log
         }
         __syncthreads();
         const float floor = sh.floor;
-        for (int s = 0; s < kLpSlots; s++) {
-            if (!(sh.batch_max[s][threadIdx.x] >= floor)) continue;
-            for (int vb = v0 + s * kBatch; vb < v1; vb += kLpSlots * kBatch) {
-                uint4 c[kLpLoads];
-                load(vb, c);
-#pragma unroll
-                for (int i = 0; i < kLpLoads; i++) {
-                    const int v = vb + i * kLpThreads + threadIdx.x;
-                    const int id0 = x.first(v), n = v < v1 ? x.count(v) : 0;
-                    float f[V];
-                    Raw<T>::values(c[i], f);
-#pragma unroll
-                    for (int j = 0; j < V; j++)
-                        if (f[j] >= floor && j < n) {
-                            const int at = atomicAdd(&sh.count, 1);
-                            if (at < kLpFound) sh.found[at] = make_key(f[j], id0 + j);
-                        }
+        // the batches that reach it: 16 * kLpLoads bytes of one thread each
+        const int batches = (v1 - v0 + kBatch - 1) / kBatch;
+        if (best >= floor)
+            for (int s = 0; s < min(kSlots, batches); s++)
+                if (sh.batch_max[s][threadIdx.x] >= floor)
+                    for (int b = s; b < batches; b += kSlots) {
+                        const int at = atomicAdd(&sh.hits, 1);
+                        if (at < kLpFound) sh.hit[at] = b * NTH + threadIdx.x;
+                    }
+        __syncthreads();
+        // a warp per batch, a value per lane
+        constexpr int kValues = V * kLpLoads;
+        const int hits = sh.hits;
+#pragma unroll 4
+        for (int h = warp; h < min(hits, kLpFound); h += NTH / 32) {
+            const int e = sh.hit[h], v = v0 + e / NTH * kBatch + lane / V * NTH + e % NTH;
+            float f = -INFINITY;
+            int id = 0;
+            if (lane < kValues && v < v1 && lane % V < x.count(v)) {
+                id = x.first(v) + lane % V;
+                f = (float)x.x[id];
+                if (f >= floor) {
+                    const int at = atomicAdd(&sh.count, 1);
+                    if (at < kLpFound) sh.found[at] = make_key(f, id);
                 }
             }
         }
         __syncthreads();
         const int found = sh.count;
-        if (found <= kLpFound) {
-            if (threadIdx.x < found) {
-                const Key k = sh.found[threadIdx.x];
+        if (found <= kLpFound && hits <= kLpFound) {
+            for (int f = threadIdx.x; f < found; f += NTH) {
+                const Key k = sh.found[f];
                 int rank = 0;
 #pragma unroll 8
                 for (int o = 0; o < found; o++) rank += sh.found[o] > k;
                 if (rank < K) sh.merged[rank] = k;
             }
         } else {
-            list_rows<T>(sh, x, v0, v1, K, floor);
+            list_rows<T, NTH>(sh, x, v0, v1, K, floor);
         }
     }
     __syncthreads();
@@ -458,10 +468,9 @@ __global__ void __launch_bounds__(kLpThreads, 4) token_logprobs_kernel(const Log
     float gm, gn, gr, gt, gb;
     if (Z > 1) {
         cluster_sync_all();
-        if (threadIdx.x < Z * 5)
-            cl.stat[threadIdx.x / 5][threadIdx.x % 5] =
-                ld_dsmem_f1(mapa_shared(smem_u32(sh.stat + threadIdx.x % 5), threadIdx.x / 5));
-        for (int e = threadIdx.x; e < Z * kTopMax && K > 0; e += kLpThreads) {
+        for (int e = threadIdx.x; e < Z * 5; e += NTH)
+            cl.stat[e / 5][e % 5] = ld_dsmem_f1(mapa_shared(smem_u32(sh.stat + e % 5), e / 5));
+        for (int e = threadIdx.x; e < Z * kTopMax && K > 0; e += NTH) {
             const float2 v = ld_dsmem_f2(mapa_shared(smem_u32(sh.merged + e % kTopMax), e / kTopMax));
             cl.lists[e / kTopMax][e % kTopMax] = ((Key)__float_as_uint(v.y) << 32) | __float_as_uint(v.x);
         }
@@ -480,7 +489,7 @@ __global__ void __launch_bounds__(kLpThreads, 4) token_logprobs_kernel(const Log
         // every logit is as low as a mask's: the sums above took the vectors'
         // padding along, so once more, value by value
         gn = gr = gt = 0.f;
-        for (int i = threadIdx.x; i < p.vocab; i += kLpThreads) {
+        for (int i = threadIdx.x; i < p.vocab; i += NTH) {
             const float d = ((float)x.x[i] - gb) * kLog2e, e = exp2_approx(d);
             if (d == 0.f) gn += 1.f;
             else {
@@ -499,7 +508,7 @@ __global__ void __launch_bounds__(kLpThreads, 4) token_logprobs_kernel(const Log
         }
         __syncthreads();
         gn = gr = gt = 0.f;
-        for (int w = 0; w < kLpWarps; w++) {
+        for (int w = 0; w < (NTH / 32); w++) {
             gn += sh.red[w][0];
             gr += sh.red[w][1];
             gt += sh.red[w][2];
@@ -527,7 +536,7 @@ __global__ void __launch_bounds__(kLpThreads, 4) token_logprobs_kernel(const Log
         return;
     }
     // each share ranks its own list among all: a thread per (key, list)
-    for (int e = threadIdx.x; e < Z * kTopMax; e += kLpThreads) {
+    for (int e = threadIdx.x; e < Z * kTopMax; e += NTH) {
         const Key k = cl.lists[z][e % kTopMax];
         if (k) atomicAdd(&cl.rank[e % kTopMax], better(cl.lists[e / kTopMax], K, k));
     }
@@ -544,21 +553,21 @@ __global__ void __launch_bounds__(kLpThreads, 4) token_logprobs_kernel(const Log
     }
 }
 
-template <typename T>
-cudaError_t launch_typed(const LogprobParams &p, int Z, cudaStream_t st) {
+template <typename T, int NTH>
+cudaError_t launch_threads(const LogprobParams &p, int Z, cudaStream_t st) {
     static std::atomic<uint64_t> done{0};
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
     const uint64_t bit = 1ull << (dev & 63);
     if (!(done.load() & bit)) {
-        e = cudaFuncSetAttribute(token_logprobs_kernel<T>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+        e = cudaFuncSetAttribute(token_logprobs_kernel<T, NTH>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
         if (e != cudaSuccess) return e;
         done.fetch_or(bit);
     }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(p.n_rows * Z));
-    cfg.blockDim = dim3(kLpThreads);
+    cfg.blockDim = dim3(NTH);
     cfg.stream = st;
     cudaLaunchAttribute a[1];
     a[0].id = cudaLaunchAttributeClusterDimension;
@@ -567,7 +576,12 @@ cudaError_t launch_typed(const LogprobParams &p, int Z, cudaStream_t st) {
     a[0].val.clusterDim.z = 1;
     cfg.attrs = a;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, token_logprobs_kernel<T>, p, Z);
+    return cudaLaunchKernelEx(&cfg, token_logprobs_kernel<T, NTH>, p, Z);
+}
+
+template <typename T>
+cudaError_t launch_typed(const LogprobParams &p, int Z, int sms, cudaStream_t st) {
+    return p.n_rows <= sms ? launch_threads<T, kLpFew>(p, Z, st) : launch_threads<T, kLpMany>(p, Z, st);
 }
 
 }  // namespace
@@ -576,14 +590,14 @@ cudaError_t launch_token_logprobs(const LogprobParams &p, int sms, cudaStream_t 
     // shares of a row: as many as fill the SMs twice, each with a batch of
     // work for its threads, at most a cluster's 16
     const int elem = p.dtype == ELEM_F32 ? 4 : 2;
-    const long long batch = (long long)kLpThreads * 16 / elem;
+    const long long batch = (long long)kLpFew * 16 / elem;
     const long long by_work = std::max<long long>(1, p.vocab / batch);
     const long long by_sms = std::max<long long>(1, 2ll * sms / p.n_rows);
     const int Z = (int)std::min<long long>(16, std::min(by_work, by_sms));
     switch (p.dtype) {
-        case ELEM_F32: return launch_typed<float>(p, Z, st);
-        case ELEM_BF16: return launch_typed<__nv_bfloat16>(p, Z, st);
-        default: return launch_typed<__half>(p, Z, st);
+        case ELEM_F32: return launch_typed<float>(p, Z, sms, st);
+        case ELEM_BF16: return launch_typed<__nv_bfloat16>(p, Z, sms, st);
+        default: return launch_typed<__half>(p, Z, sms, st);
     }
 }
 
