@@ -1,10 +1,10 @@
 // vc_attn_rows.cu - attention of a call's rows over a cache slab, with a
-// sliding window, sinks that stay visible, and trees of drafted rows: the
-// CUDA-core kernels.
+// sliding window, sinks that stay visible, and trees of drafted rows: the fp32
+// kernels, on the CUDA cores (16-bit slabs: vc_attn_rows_tc.cu).
 //
 // o = sum_j 2^(s_j - m) v_j / l, s = scale * log2(e) * q.k, over the keys that
-// the row sees (vc_rows.cuh), in one pass with a running maximum m and sum l
-// in fp32.  A masked key adds nothing, whatever its K and V hold.
+// the row sees (vc_rows.cuh), in one pass with a running maximum m and sum l.
+// A masked key adds nothing, whatever its K and V hold.
 //
 // A CTA takes a tile of RB query rows of one (stream, KV head) - row i and
 // query head g of the group are packed as m = i * group + g, so a KV head's
@@ -12,6 +12,7 @@
 // tile sees.  The shares of a tile are the CTAs of one cluster; they merge
 // through distributed shared memory, in rank order, so there is no workspace,
 // no ticket and no second launch, and a result does not depend on timing.
+#include "vc_cluster.h"
 #include "vc_rows.cuh"
 #include "vc_tc.cuh"
 
@@ -24,17 +25,16 @@ using namespace tc;
 
 namespace {
 
-constexpr int kArThreads = 128;       // 4 warps
-constexpr int kArTileBytes = 16384;   // K (and V) bytes of a key tile
+constexpr int kArThreads = 128;       // many rows: 4 warps
+constexpr int kArTileBytes = 16384;   // K (and V) bytes of their key tile
 
-template <typename T, int HD>
+template <int HD>
 struct ArShape {
-    static constexpr int kChunk = 16 / (int)sizeof(T);                   // elements per 16 bytes
-    static constexpr int kChunks = HD / kChunk;                          // 16-byte chunks per key
-    static constexpr int kKeys = kArTileBytes / (HD * (int)sizeof(T));   // keys per tile
-    static constexpr int kPerLane = kKeys / 32;                          // keys per lane
-    static constexpr int kLanesPerKey = HD / 4;                          // P.V: 4 dims per lane
-    static constexpr int kKeysAtOnce = 32 / kLanesPerKey;                // P.V: keys per warp step
+    static constexpr int kChunks = HD / 4;                    // 16-byte chunks per key
+    static constexpr int kKeys = kArTileBytes / (HD * 4);     // keys per tile
+    static constexpr int kPerLane = kKeys / 32;               // keys per lane
+    static constexpr int kLanesPerKey = HD / 4;               // P.V: 4 dims per lane
+    static constexpr int kKeysAtOnce = 32 / kLanesPerKey;     // P.V: keys per warp step
 };
 
 // What a tile's rows see, and where they are (shared memory).
@@ -74,31 +74,30 @@ __device__ __forceinline__ bool row_sees(const ArRows<RB> &rows, int m, int j, i
     return tree && ((rows.anc[m][a >> 5] >> (a & 31)) & 1u);
 }
 
-// The tile's query rows, scaled, into shared memory as fp32 (zeros past M).
-template <typename T, int HD, int RB>
-__device__ __forceinline__ void load_queries(float *q, const RowsAttnParams &p, const RowSpan &s, int head0, int m0, int M) {
+// The tile's query rows, scaled, into shared memory: `row` floats apart, and 4
+// floats more between the `parts` of a row; zeros past M.
+template <int HD, int RB>
+__device__ __forceinline__ void load_queries(float *q, int row, int parts, const RowsAttnParams &p, const RowSpan &s,
+                                             int head0, int m0, int M) {
     for (int e = threadIdx.x; e < RB * HD / 4; e += blockDim.x) {
         const int m = e / (HD / 4), d = e % (HD / 4) * 4;
         float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
         if (m0 + m < M) {
             const int i = (m0 + m) / p.group, g = (m0 + m) % p.group;
-            v = load4<T>(static_cast<const T *>(p.q) + ((long long)(s.r0 + i) * p.n_heads + head0 + g) * HD + d);
-            v.x *= p.scale_log2;
-            v.y *= p.scale_log2;
-            v.z *= p.scale_log2;
-            v.w *= p.scale_log2;
+            v = load4<float>(static_cast<const float *>(p.q) + ((long long)(s.r0 + i) * p.n_heads + head0 + g) * HD + d);
+            v = make_float4(v.x * p.scale_log2, v.y * p.scale_log2, v.z * p.scale_log2, v.w * p.scale_log2);
         }
-        *reinterpret_cast<float4 *>(q + m * HD + d) = v;
+        *reinterpret_cast<float4 *>(q + m * row + d + d / (HD / parts) * 4) = v;
     }
 }
 
 // Asynchronous copy of key tile t's K and V rows; rows past `end` become
 // zeros.  K rows are chunk-swizzled (chunk c of key j at c ^ (j & 7)), so that
 // 32 lanes reading chunk c of 32 keys do not conflict.
-template <typename T, int HD>
+template <int HD>
 __device__ __forceinline__ void load_tile(unsigned char *dst, const char *kb, const char *vb, long long slot_bytes,
                                           const KeyRange &kr, int lo_slot, const CacheView &c, int idx0, int end) {
-    using S = ArShape<T, HD>;
+    using S = ArShape<HD>;
     const uint32_t k_s = smem_u32(dst), v_s = k_s + kArTileBytes;
 #pragma unroll
     for (int it = 0; it < kArTileBytes / 16 / kArThreads; it++) {
@@ -112,101 +111,129 @@ __device__ __forceinline__ void load_tile(unsigned char *dst, const char *kb, co
         }
         const bool ok = idx < end;
         const long long off = ok ? slot * slot_bytes + ch * 16 : 0;
-        cp_async16(k_s + j * (HD * (int)sizeof(T)) + ((ch ^ (j & 7)) << 4), kb + off, ok);
-        cp_async16(v_s + j * (HD * (int)sizeof(T)) + (ch << 4), vb + off, ok);
+        cp_async16(k_s + j * (HD * 4) + ((ch ^ (j & 7)) << 4), kb + off, ok);
+        cp_async16(v_s + j * (HD * 4) + (ch << 4), vb + off, ok);
     }
 }
 
-// One 16-byte chunk of a key row in shared memory as fp32.
-template <typename T>
-struct Chunk {
-    float f[8];
-    __device__ __forceinline__ explicit Chunk(const unsigned char *p) {
-        const uint4 u = *reinterpret_cast<const uint4 *>(p);
-        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const float2 a = unpack2<T>(w[i]);
-            f[2 * i] = a.x;
-            f[2 * i + 1] = a.y;
-        }
-    }
-};
-template <>
-struct Chunk<float> {
-    float f[4];
-    __device__ __forceinline__ explicit Chunk(const unsigned char *p) {
-        const float4 a = *reinterpret_cast<const float4 *>(p);
-        f[0] = a.x;
-        f[1] = a.y;
-        f[2] = a.z;
-        f[3] = a.w;
-    }
+__device__ __forceinline__ void bulk_load(void *dst, const void *src, uint32_t bytes, uint64_t *bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                     smem_u32(dst)),
+                 "l"(src), "r"(bytes), "r"(smem_u32(bar))
+                 : "memory");
+}
+
+// The shares of a tile merge by pushing: rank z owns a Z-th of the tile's sums
+// (groups of 4 dims), every CTA writes its part of them, and its rows' maxima
+// and sums, into the owners' shared memory, and after one cluster barrier each
+// owner finds all parts in its own.
+template <int HD, int RB>
+struct ArMerge {
+    static constexpr int kGroups = RB * HD / 4;
+    float4 part[kGroups + kMaxCluster];       // [rank][group of this owner]
+    float2 ml[kMaxCluster][RB];               // the ranks' maxima and sums
 };
 
-// Merges the cluster's shares of a tile and writes the rows.  Every CTA has
-// put its rows' unnormalised sums o [RB][HD], maxima and sums into its own
-// shared memory; rank z takes every Z-th group of 4 dims.
-template <typename T, int HD, int RB>
-__device__ __forceinline__ void merge_store(const float *o, const float *mx, const float *sum, const RowsAttnParams &p,
-                                            const RowSpan &s, int head0, int m0, int M, int z, int Z) {
+// Called once by every thread before merge_store, early: the peers have started.
+__device__ __forceinline__ void peers_arrive(int Z) {
+    if (Z > 1) asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");
+}
+__device__ __forceinline__ void peers_wait(int Z) {
+    if (Z > 1) asm volatile("barrier.cluster.wait;" ::: "memory");
+}
+
+// sum(r, d): this CTA's unnormalised sums of row r, dims d .. d + 3; ml(r): its
+// maximum and sum.
+template <int HD, int RB, int NTH, typename Sum, typename Ml>
+__device__ __forceinline__ void merge_store(ArMerge<HD, RB> &mg, Sum sum, Ml ml, const RowsAttnParams &p, const RowSpan &s,
+                                            int head0, int m0, int M, int z, int Z) {
+    constexpr int N = ArMerge<HD, RB>::kGroups;
+    const int per = (N + Z - 1) / Z;
+    peers_wait(Z);
+    for (int e = threadIdx.x; e < N; e += NTH) {
+        const int owner = e / per, at = z * per + e - owner * per;
+        const float4 v = sum(e / (HD / 4), e % (HD / 4) * 4);
+        asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(mapa_shared(smem_u32(mg.part + at), owner)),
+                     "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w)
+                     : "memory");
+    }
+    for (int e = threadIdx.x; e < RB * Z; e += NTH) {
+        const float2 v = ml(e % RB);
+        asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(mapa_shared(smem_u32(&mg.ml[z][e % RB]), e / RB)),
+                     "f"(v.x), "f"(v.y)
+                     : "memory");
+    }
     if (Z > 1) cluster_sync_all();
     else __syncthreads();
-    const uint32_t o_s = smem_u32(o), m_s = smem_u32(mx), l_s = smem_u32(sum);
-    for (int e = threadIdx.x + z * kArThreads; e < RB * HD / 4; e += Z * kArThreads) {
+    for (int e = z * per + threadIdx.x; e < min(N, (z + 1) * per); e += NTH) {
         const int m = e / (HD / 4), d = e % (HD / 4) * 4;
         if (m0 + m >= M) continue;
         float gm = -INFINITY;
-        for (int r = 0; r < Z; r++) gm = fmaxf(gm, ld_dsmem_f1(mapa_shared(m_s + 4 * m, r)));
+#pragma unroll 4
+        for (int r = 0; r < Z; r++) gm = fmaxf(gm, mg.ml[r][m].x);
         float gl = 0.f;
         float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
         for (int r = 0; r < Z; r++) {
-            const float mr = ld_dsmem_f1(mapa_shared(m_s + 4 * m, r));
-            const float w = mr == -INFINITY ? 0.f : exp2_approx(mr - gm);
-            const float l = ld_dsmem_f1(mapa_shared(l_s + 4 * m, r));
-            const float4 v = ld_dsmem_f4(mapa_shared(o_s + 4 * (m * HD + d), r));
-            if (mr == -INFINITY && l == 0.f) continue;   // this share saw no key of the row
-            gl = fmaf(w, l, gl);
-            a.x = fmaf(w, v.x, a.x);
-            a.y = fmaf(w, v.y, a.y);
-            a.z = fmaf(w, v.z, a.z);
-            a.w = fmaf(w, v.w, a.w);
+            const float2 w = mg.ml[r][m];
+            const float4 v = mg.part[r * per + e - z * per];
+            if (w.x == -INFINITY && w.y == 0.f) continue;   // this share saw no key of the row
+            const float f = w.x == -INFINITY ? 0.f : exp2_approx(w.x - gm);
+            gl = fmaf(f, w.y, gl);
+            a = make_float4(fmaf(f, v.x, a.x), fmaf(f, v.y, a.y), fmaf(f, v.z, a.z), fmaf(f, v.w, a.w));
         }
         const float il = gl == 0.f ? 0.f : 1.0f / gl;   // no key at all: zeros
         const long long row = (long long)(s.r0 + (m0 + m) / p.group) * p.n_heads + head0 + (m0 + m) % p.group;
-        store4<T>(static_cast<T *>(p.out) + row * HD + d, make_float4(a.x * il, a.y * il, a.z * il, a.w * il));
+        store4<float>(static_cast<float *>(p.out) + row * HD + d, make_float4(a.x * il, a.y * il, a.z * il, a.w * il));
         if (p.lse && d == 0) p.lse[row] = gl == 0.f ? -INFINITY : (gm + log2f(gl)) * 0.69314718055994531f;
     }
-    if (Z > 1) cluster_sync_all();   // no CTA leaves while a peer still reads its share
 }
 
 // ---------------------------------------------------------------------------
-// Few rows: RB (4 or 8) packed rows, one token of one KV head's group.
+// Few rows: RB (4 or 8) packed rows.
 //
-// Bound by HBM: a tile is 32 KB of keys and 2 * RB flops per byte.  The four
-// warps split a key's dims for the scores (each lane one key or more, so that
-// a K chunk is read from shared memory once for all RB rows) and the tile's
-// keys for P.V (each lane 4 dims); three tiles are in flight per CTA.
+// Bound by HBM at long contexts: 2 * RB flops per byte.  A warp works on tiles
+// of its own - 4 KB of K and as much of V, two under way - so nothing but its
+// own copies holds it up: a bulk copy per key row, one per lane at most, into
+// rows that are 16 bytes longer than a key for K (lanes then read one chunk of
+// different keys without conflicts).  Scores: 2 or 4 lanes share a key's dims,
+// against RB broadcast rows; the running maximum moves only when a score
+// exceeds it by more than 2^8, so most tiles need no shuffles across keys.
+// P.V: a lane has 4 dims of every row.
 // ---------------------------------------------------------------------------
 
-template <typename T, int HD, int RB>
-struct ArFewSmem {
-    static constexpr int kKeys = ArShape<T, HD>::kKeys;
-    static constexpr int kStages = 3;
-    unsigned char kv[kStages][2 * kArTileBytes];
-    float q[RB * HD];
-    float part[4][RB][kKeys];     // the warps' partial scores
-    float p[kKeys][RB];           // 2^(s - m), or -1 for a masked key
-    float alpha[RB];              // the rows' rescale factors of this tile
-    float mx[RB], sum[RB];
-    int masked[4];                // a warp's rows have a masked key in this tile
+constexpr int kAfWarps = 12;
+constexpr int kAfThreads = kAfWarps * 32;
+constexpr int kAfTile = 4096;              // K bytes of a warp's tile
+constexpr float kAfRescale = 8.0f;         // log2 of the largest weight before the maximum moves
+constexpr uint64_t kAfWaitNs = 2000000000ull;
+constexpr int kArFixed = 3;                // rounds' worth of a CTA's start and merge
+
+template <int HD, int RB>
+struct AfSmem {
+    static constexpr int kKeys = kAfTile / (HD * 4);       // keys of a tile: 8 or 16
+    static constexpr int kRow = HD * 4 + 16;               // a K row in shared memory
+    static constexpr int kParts = 32 / kKeys;              // lanes that share a key: 4 or 2
+    static constexpr int kQRow = HD + 4 * (kParts - 1);    // a query row: its parts on different banks
+    struct Tile {
+        unsigned char k[kKeys * kRow];
+        unsigned char v[kAfTile];
+    };
+    union {
+        Tile tile[kAfWarps][2];
+        float sums[kAfWarps][RB][HD];       // the warps' at the end
+    };
+    float q[RB * kQRow];
+    float p[kAfWarps][kKeys][RB];           // 2^(s - m), or -1 for a masked key
+    float wm[kAfWarps][RB], wl[kAfWarps][RB];
+    ArMerge<HD, RB> merge;
     ArRows<RB> rows;
+    uint64_t full[kAfWarps][2];
 };
 
-template <typename T, int HD, int RB>
-__global__ void __launch_bounds__(kArThreads) attn_rows_few_kernel(const RowsAttnParams p) {
-    using S = ArShape<T, HD>;
-    using Sm = ArFewSmem<T, HD, RB>;
+template <int HD, int RB>
+__global__ void __launch_bounds__(kAfThreads) attn_rows_few_kernel(const RowsAttnParams p) {
+    using Sm = AfSmem<HD, RB>;
     extern __shared__ __align__(128) unsigned char smem_raw[];
     Sm &sh = *reinterpret_cast<Sm *>(smem_raw);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -219,169 +246,208 @@ __global__ void __launch_bounds__(kArThreads) attn_rows_few_kernel(const RowsAtt
     const int i0 = m0 / p.group, i1 = (min(m0 + RB, M) - 1) / p.group + 1;
     const KeyRange kr = key_range(p.c, s, i0, i1, p.window, tree);
     const int lo_slot = cache_slot(p.c, kr.lo);
-    const int total = kr.total(), tiles = (total + S::kKeys - 1) / S::kKeys;
-    const int t0 = (int)((long long)z * tiles / Z), t1 = (int)((long long)(z + 1) * tiles / Z);
+    const int total = kr.total(), tiles = (total + Sm::kKeys - 1) / Sm::kKeys;
+    // the warp's tiles: every (Z * kAfWarps)-th
+    const int t0 = z + warp * Z, step = Z * kAfWarps;
     const long long base = p.layer_off + (long long)stream * p.c.stream_stride + (long long)kvh * p.c.head_stride;
-    const char *kb = p.c.k + base * (long long)sizeof(T), *vb = p.c.v + base * (long long)sizeof(T);
-    const long long slot_bytes = p.c.slot_stride * (long long)sizeof(T);
+    const char *kb = p.c.k + base * 4, *vb = p.c.v + base * 4;
+    const long long slot_bytes = p.c.slot_stride * 4;
     const int head0 = kvh * p.group;
+    const uint64_t deadline = globaltimer() + kAfWaitNs;
+    bool ok = true;
 
-#pragma unroll
-    for (int i = 0; i < Sm::kStages - 1; i++) {
-        if (t0 + i < t1)
-            load_tile<T, HD>(sh.kv[i], kb, vb, slot_bytes, kr, lo_slot, p.c, (t0 + i) * S::kKeys, total);
-        cp_async_commit();
+    if (lane == 0) {
+        mbar_init(&sh.full[warp][0], 1);
+        mbar_init(&sh.full[warp][1], 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    load_queries<T, HD, RB>(sh.q, p, s, head0, m0, M);
+    __syncwarp();
+    auto fetch = [&](int t, int buf) {
+        const int idx0 = t * Sm::kKeys, n = min(Sm::kKeys, total - idx0);
+        typename Sm::Tile &tl = sh.tile[warp][buf];
+        uint64_t *bar = &sh.full[warp][buf];
+        if (lane == 0) mbar_expect_tx(bar, 2 * n * HD * 4);
+        __syncwarp();
+#pragma unroll
+        for (int e = lane; e < 2 * Sm::kKeys; e += 32) {
+            const int j = e % Sm::kKeys, idx = idx0 + j;
+            if (j >= n) continue;
+            int slot = idx;
+            if (idx >= kr.ns) {
+                slot = lo_slot + (idx - kr.ns);
+                if (slot >= p.c.cap) slot -= p.c.ring;
+            }
+            if (e < Sm::kKeys) bulk_load(tl.k + j * Sm::kRow, kb + slot * slot_bytes, HD * 4, bar);
+            else bulk_load(tl.v + j * (HD * 4), vb + slot * slot_bytes, HD * 4, bar);
+        }
+    };
+    peers_arrive(Z);
+    if (t0 < tiles) fetch(t0, 0);
+    if (t0 + step < tiles) fetch(t0 + step, 1);
+
+    load_queries<HD, RB>(sh.q, Sm::kQRow, Sm::kParts, p, s, head0, m0, M);
     setup_rows<RB>(sh.rows, p, s, m0, M);
+    __syncthreads();
 
-    constexpr int kRowsPerWarp = RB / 4;
-    float m_run[kRowsPerWarp], l_run[kRowsPerWarp];
-#pragma unroll
-    for (int r = 0; r < kRowsPerWarp; r++) {
-        m_run[r] = -INFINITY;
-        l_run[r] = 0.f;
-    }
+    constexpr int kLanesPerKey = HD / 4, kAtOnce = 32 / kLanesPerKey;   // P.V
+    const int j = lane % Sm::kKeys, part = lane / Sm::kKeys;            // scores
+    const int sub = lane / kLanesPerKey, d4 = lane % kLanesPerKey * 4;
+    float mr[RB], l[RB];   // l: this lane's keys only
     float4 o[RB];
 #pragma unroll
-    for (int r = 0; r < RB; r++) o[r] = make_float4(0.f, 0.f, 0.f, 0.f);
-
-    for (int t = t0; t < t1; t++) {
-        const int st = (t - t0) % Sm::kStages;
-        cp_async_wait<Sm::kStages - 2>();
-        __syncthreads();   // tile t is in; every warp is done with tile t - 1
-        if (t + Sm::kStages - 1 < t1)
-            load_tile<T, HD>(sh.kv[(t - t0 + Sm::kStages - 1) % Sm::kStages], kb, vb, slot_bytes, kr, lo_slot, p.c,
-                             (t + Sm::kStages - 1) * S::kKeys, total);
-        cp_async_commit();
-
-        // scores of this warp's quarter of the dims
-        float acc[RB][S::kPerLane];
-#pragma unroll
-        for (int r = 0; r < RB; r++)
-#pragma unroll
-            for (int x = 0; x < S::kPerLane; x++) acc[r][x] = 0.f;
-#pragma unroll
-        for (int c = 0; c < S::kChunks / 4; c++) {
-            const int ch = warp * (S::kChunks / 4) + c;
-#pragma unroll
-            for (int x = 0; x < S::kPerLane; x++) {
-                const int j = lane + 32 * x;
-                const Chunk<T> k(sh.kv[st] + j * (HD * (int)sizeof(T)) + ((ch ^ (j & 7)) << 4));
-#pragma unroll
-                for (int r = 0; r < RB; r++)
-#pragma unroll
-                    for (int y = 0; y < S::kChunk; y += 4) {
-                        const float4 qv = *reinterpret_cast<const float4 *>(sh.q + r * HD + ch * S::kChunk + y);
-                        acc[r][x] = fmaf(qv.x, k.f[y], acc[r][x]);
-                        acc[r][x] = fmaf(qv.y, k.f[y + 1], acc[r][x]);
-                        acc[r][x] = fmaf(qv.z, k.f[y + 2], acc[r][x]);
-                        acc[r][x] = fmaf(qv.w, k.f[y + 3], acc[r][x]);
-                    }
-            }
+    for (int r = 0; r < RB; r++) {
+        mr[r] = -INFINITY;
+        l[r] = 0.f;
+        o[r] = make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    int n = 0;
+    for (int t = t0; t < tiles; t += step, n++) {
+        const int buf = n & 1;
+        if (!__all_sync(0xffffffffu, mbar_wait(&sh.full[warp][buf], (n >> 1) & 1u, deadline))) {
+            ok = false;
+            break;
         }
+        const typename Sm::Tile &tl = sh.tile[warp][buf];
+        float acc[RB];
 #pragma unroll
-        for (int r = 0; r < RB; r++)
-#pragma unroll
-            for (int x = 0; x < S::kPerLane; x++) sh.part[warp][r][lane + 32 * x] = acc[r][x];
-        __syncthreads();
-
-        // softmax: warp w takes rows w, w + 4
-        bool any_masked = false;
-#pragma unroll
-        for (int rr = 0; rr < kRowsPerWarp; rr++) {
-            const int r = warp + 4 * rr;
-            float sc[S::kPerLane];
-            bool vis[S::kPerLane];
-            float mt = -INFINITY;
-#pragma unroll
-            for (int x = 0; x < S::kPerLane; x++) {
-                const int j = lane + 32 * x, idx = t * S::kKeys + j;
-                sc[x] = (sh.part[0][r][j] + sh.part[1][r][j]) + (sh.part[2][r][j] + sh.part[3][r][j]);
-                vis[x] = idx < total && row_sees<RB>(sh.rows, r, kr.position(idx), s.pos, p.c.n_sink, tree);
-                any_masked |= !vis[x];
-                if (vis[x]) mt = fmaxf(mt, sc[x]);
-            }
-#pragma unroll
-            for (int d = 16; d > 0; d >>= 1) mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, d));
-            const float mn = fmaxf(m_run[rr], mt);
-            const float b = mn == -INFINITY ? 0.f : mn;
-            const float al = m_run[rr] == -INFINITY ? 0.f : exp2_approx(m_run[rr] - b);
-            float ls = 0.f;
-#pragma unroll
-            for (int x = 0; x < S::kPerLane; x++) {
-                const float pv = exp2_approx(sc[x] - b);
-                if (vis[x]) ls += pv;
-                sh.p[lane + 32 * x][r] = vis[x] ? pv : -1.f;
-            }
-            l_run[rr] = l_run[rr] * al + warp_sum(ls);
-            m_run[rr] = mn;
-            if (lane == 0) sh.alpha[r] = al;
-        }
-        any_masked = __any_sync(0xffffffffu, any_masked);
-        if (lane == 0) sh.masked[warp] = any_masked;
-        __syncthreads();
-
-        // o = o * alpha + P V over this warp's quarter of the keys
-        const unsigned char *vt = sh.kv[st] + kArTileBytes;
-        const int sub = lane / S::kLanesPerKey, d4 = lane % S::kLanesPerKey * 4;
-#pragma unroll
-        for (int r = 0; r < RB; r++) {
-            const float al = sh.alpha[r];
-            o[r].x *= al;
-            o[r].y *= al;
-            o[r].z *= al;
-            o[r].w *= al;
-        }
-        const bool masked = (sh.masked[0] | sh.masked[1] | sh.masked[2] | sh.masked[3]) != 0;
-#pragma unroll 4
-        for (int x = 0; x < S::kKeys / 4 / S::kKeysAtOnce; x++) {
-            const int j = warp * (S::kKeys / 4) + x * S::kKeysAtOnce + sub;
-            const float4 v = load4<T>(reinterpret_cast<const T *>(vt) + j * HD + d4);
-            float pr[RB];
-#pragma unroll
-            for (int r = 0; r < RB; r += 4)
-                *reinterpret_cast<float4 *>(pr + r) = *reinterpret_cast<const float4 *>(&sh.p[j][r]);
+        for (int r = 0; r < RB; r++) acc[r] = 0.f;
+        constexpr int kChunks = HD / 4 / Sm::kParts;
+#pragma unroll 8
+        for (int c = 0; c < kChunks; c++) {
+            const float4 k = *reinterpret_cast<const float4 *>(tl.k + j * Sm::kRow + (part * kChunks + c) * 16);
 #pragma unroll
             for (int r = 0; r < RB; r++) {
-                if (masked && pr[r] < 0.f) continue;
-                o[r].x = fmaf(pr[r], v.x, o[r].x);
-                o[r].y = fmaf(pr[r], v.y, o[r].y);
-                o[r].z = fmaf(pr[r], v.z, o[r].z);
-                o[r].w = fmaf(pr[r], v.w, o[r].w);
+                const float4 q =
+                    *reinterpret_cast<const float4 *>(sh.q + r * Sm::kQRow + part * (HD / Sm::kParts + 4) + c * 4);
+                acc[r] = fmaf(q.x, k.x, acc[r]);
+                acc[r] = fmaf(q.y, k.y, acc[r]);
+                acc[r] = fmaf(q.z, k.z, acc[r]);
+                acc[r] = fmaf(q.w, k.w, acc[r]);
             }
         }
-    }
-    cp_async_wait<0>();
-    __syncthreads();   // the tiles are done with: their memory takes the partial sums
-
-    float *red = reinterpret_cast<float *>(sh.kv[0]);            // [4 warps][RB][HD]
-    float *of = reinterpret_cast<float *>(sh.kv[1]);             // [RB][HD]
-    static_assert(4 * RB * HD * 4 <= 2 * kArTileBytes, "the warps' partial sums fit a stage");
-    {
-        const int sub = lane / S::kLanesPerKey, d4 = lane % S::kLanesPerKey * 4;
+#pragma unroll
+        for (int d = Sm::kKeys; d < 32; d *= 2)
+#pragma unroll
+            for (int r = 0; r < RB; r++) acc[r] += __shfl_xor_sync(0xffffffffu, acc[r], d);
+        const int idx = t * Sm::kKeys + j;
+        uint32_t vis = 0;
+        bool move = false;
+        if (idx < total) {
+            const int at = kr.position(idx);
+#pragma unroll
+            for (int r = 0; r < RB; r++)
+                if (row_sees<RB>(sh.rows, r, at, s.pos, p.c.n_sink, tree)) {
+                    vis |= 1u << r;
+                    move |= mr[r] == -INFINITY ? acc[r] > -INFINITY : acc[r] > mr[r] + kAfRescale;
+                }
+        }
+        if (__any_sync(0xffffffffu, move)) {
+#pragma unroll
+            for (int r = 0; r < RB; r++) {
+                float mt = (vis >> r) & 1u ? acc[r] : -INFINITY;
+#pragma unroll
+                for (int d = 16; d > 0; d >>= 1) mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, d));
+                if (mt > mr[r]) {
+                    const float al = mr[r] == -INFINITY ? 0.f : exp2_approx(mr[r] - mt);
+                    mr[r] = mt;
+                    l[r] *= al;
+                    o[r] = make_float4(o[r].x * al, o[r].y * al, o[r].z * al, o[r].w * al);
+                }
+            }
+        }
 #pragma unroll
         for (int r = 0; r < RB; r++) {
-            float4 v = o[r];
-            if (S::kKeysAtOnce == 2) {
-                v.x += __shfl_xor_sync(0xffffffffu, v.x, 16);
-                v.y += __shfl_xor_sync(0xffffffffu, v.y, 16);
-                v.z += __shfl_xor_sync(0xffffffffu, v.z, 16);
-                v.w += __shfl_xor_sync(0xffffffffu, v.w, 16);
-            }
-            if (sub == 0) *reinterpret_cast<float4 *>(red + (warp * RB + r) * HD + d4) = v;
+            const float w = exp2_approx(acc[r] - (mr[r] == -INFINITY ? 0.f : mr[r]));
+            const bool see = (vis >> r) & 1u;
+            if (see && part == 0) l[r] += w;
+            acc[r] = see ? w : -1.f;
         }
+        const bool masked = __any_sync(0xffffffffu, vis != (1u << RB) - 1u);
+        if (part == 0)
 #pragma unroll
-        for (int rr = 0; rr < kRowsPerWarp; rr++)
-            if (lane == 0) {
-                sh.mx[warp + 4 * rr] = m_run[rr];
-                sh.sum[warp + 4 * rr] = l_run[rr];
+            for (int r = 0; r < RB; r += 4)
+                *reinterpret_cast<float4 *>(&sh.p[warp][j][r]) = make_float4(acc[r], acc[r + 1], acc[r + 2], acc[r + 3]);
+        __syncwarp();
+#pragma unroll 4
+        for (int x = 0; x < Sm::kKeys / kAtOnce; x++) {
+            const int jj = x * kAtOnce + sub;
+            const float4 v = *reinterpret_cast<const float4 *>(tl.v + (jj * HD + d4) * 4);
+            float w[RB];
+#pragma unroll
+            for (int r = 0; r < RB; r += 4)
+                *reinterpret_cast<float4 *>(w + r) = *reinterpret_cast<const float4 *>(&sh.p[warp][jj][r]);
+#pragma unroll
+            for (int r = 0; r < RB; r++) {
+                if (masked && w[r] < 0.f) continue;
+                o[r].x = fmaf(w[r], v.x, o[r].x);
+                o[r].y = fmaf(w[r], v.y, o[r].y);
+                o[r].z = fmaf(w[r], v.z, o[r].z);
+                o[r].w = fmaf(w[r], v.w, o[r].w);
             }
+        }
+        __syncwarp();   // the tile and p are done with
+        if (t + 2 * step < tiles) fetch(t + 2 * step, buf);
+    }
+    if (!ok) {
+        if (lane == 0 && p.err) atomicExch_system(p.err, 1u);
+        const uint64_t grace = globaltimer() + 10000000ull;   // let copies in flight land
+        while (globaltimer() < grace) {
+        }
+    }
+    __syncthreads();   // every tile is done with: the sums take their memory
+#pragma unroll
+    for (int r = 0; r < RB; r++) {
+        float4 v = o[r];
+        if (kAtOnce == 2) {
+            v.x += __shfl_xor_sync(0xffffffffu, v.x, 16);
+            v.y += __shfl_xor_sync(0xffffffffu, v.y, 16);
+            v.z += __shfl_xor_sync(0xffffffffu, v.z, 16);
+            v.w += __shfl_xor_sync(0xffffffffu, v.w, 16);
+        }
+        const float lt = warp_sum(l[r]);
+        if (sub == 0) *reinterpret_cast<float4 *>(&sh.sums[warp][r][d4]) = v;
+        if (lane == 0) {
+            sh.wm[warp][r] = mr[r];
+            sh.wl[warp][r] = lt;
+        }
     }
     __syncthreads();
-    for (int e = threadIdx.x; e < RB * HD; e += kArThreads)
-        of[e] = (red[e] + red[RB * HD + e]) + (red[2 * RB * HD + e] + red[3 * RB * HD + e]);
-    merge_store<T, HD, RB>(of, sh.mx, sh.sum, p, s, head0, m0, M, z, Z);
+    // the CTA's sums, in warp order
+    auto top = [&](int r) {
+        float gm = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < kAfWarps; w++) gm = fmaxf(gm, sh.wm[w][r]);
+        return gm;
+    };
+    auto weight = [&](int w, int r, float gm) {   // of warp w's part; -1: it saw no key of the row
+        const float mw = sh.wm[w][r];
+        return mw == -INFINITY ? (sh.wl[w][r] == 0.f ? -1.f : 0.f) : exp2_approx(mw - gm);
+    };
+    merge_store<HD, RB, kAfThreads>(
+        sh.merge,
+        [&](int r, int d) {
+            const float gm = top(r);
+            float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int w = 0; w < kAfWarps; w++) {
+                const float f = weight(w, r, gm);
+                if (f == -1.f) continue;
+                const float4 v = *reinterpret_cast<const float4 *>(&sh.sums[w][r][d]);
+                a = make_float4(fmaf(f, v.x, a.x), fmaf(f, v.y, a.y), fmaf(f, v.z, a.z), fmaf(f, v.w, a.w));
+            }
+            return a;
+        },
+        [&](int r) {
+            const float gm = top(r);
+            float gl = 0.f;
+#pragma unroll
+            for (int w = 0; w < kAfWarps; w++) {
+                const float f = weight(w, r, gm);
+                if (f != -1.f) gl = fmaf(f, sh.wl[w][r], gl);
+            }
+            return make_float2(gm, gl);
+        },
+        p, s, head0, m0, M, z, Z);
 }
 
 // ---------------------------------------------------------------------------
@@ -397,21 +463,22 @@ __global__ void __launch_bounds__(kArThreads) attn_rows_few_kernel(const RowsAtt
 constexpr int kArManyRows = 32;
 constexpr int kArWarpRows = kArManyRows / 4;
 
-template <typename T, int HD>
+template <int HD>
 struct ArManySmem {
-    static constexpr int kKeys = ArShape<T, HD>::kKeys;
+    static constexpr int kKeys = ArShape<HD>::kKeys;
     static constexpr int kStages = 2;
     unsigned char kv[kStages][2 * kArTileBytes];
     float q[kArManyRows * HD];
     float p[4][kKeys][kArWarpRows];
     float mx[kArManyRows], sum[kArManyRows];
+    ArMerge<HD, kArManyRows> merge;
     ArRows<kArManyRows> rows;
 };
 
-template <typename T, int HD>
+template <int HD>
 __global__ void __launch_bounds__(kArThreads) attn_rows_many_kernel(const RowsAttnParams p) {
-    using S = ArShape<T, HD>;
-    using Sm = ArManySmem<T, HD>;
+    using S = ArShape<HD>;
+    using Sm = ArManySmem<HD>;
     constexpr int RB = kArManyRows, WR = kArWarpRows;
     extern __shared__ __align__(128) unsigned char smem_raw[];
     Sm &sh = *reinterpret_cast<Sm *>(smem_raw);
@@ -428,13 +495,14 @@ __global__ void __launch_bounds__(kArThreads) attn_rows_many_kernel(const RowsAt
     const int total = kr.total(), tiles = (total + S::kKeys - 1) / S::kKeys;
     const int t0 = (int)((long long)z * tiles / Z), t1 = (int)((long long)(z + 1) * tiles / Z);
     const long long base = p.layer_off + (long long)stream * p.c.stream_stride + (long long)kvh * p.c.head_stride;
-    const char *kb = p.c.k + base * (long long)sizeof(T), *vb = p.c.v + base * (long long)sizeof(T);
-    const long long slot_bytes = p.c.slot_stride * (long long)sizeof(T);
+    const char *kb = p.c.k + base * 4, *vb = p.c.v + base * 4;
+    const long long slot_bytes = p.c.slot_stride * 4;
     const int head0 = kvh * p.group;
 
-    if (t0 < t1) load_tile<T, HD>(sh.kv[0], kb, vb, slot_bytes, kr, lo_slot, p.c, t0 * S::kKeys, total);
+    peers_arrive(Z);
+    if (t0 < t1) load_tile<HD>(sh.kv[0], kb, vb, slot_bytes, kr, lo_slot, p.c, t0 * S::kKeys, total);
     cp_async_commit();
-    load_queries<T, HD, RB>(sh.q, p, s, head0, m0, M);
+    load_queries<HD, RB>(sh.q, HD, 1, p, s, head0, m0, M);
     setup_rows<RB>(sh.rows, p, s, m0, M);
 
     float m_run[WR], l_run[WR];   // l: this lane's keys only
@@ -453,7 +521,7 @@ __global__ void __launch_bounds__(kArThreads) attn_rows_many_kernel(const RowsAt
         cp_async_wait<0>();
         __syncthreads();   // tile t is in; every warp is done with tile t - 1
         if (t + 1 < t1)
-            load_tile<T, HD>(sh.kv[st ^ 1], kb, vb, slot_bytes, kr, lo_slot, p.c, (t + 1) * S::kKeys, total);
+            load_tile<HD>(sh.kv[st ^ 1], kb, vb, slot_bytes, kr, lo_slot, p.c, (t + 1) * S::kKeys, total);
         cp_async_commit();
         if (idle) continue;
 
@@ -464,27 +532,23 @@ __global__ void __launch_bounds__(kArThreads) attn_rows_many_kernel(const RowsAt
             for (int x = 0; x < S::kPerLane; x++) acc[r][x] = 0.f;
 #pragma unroll 2
         for (int ch = 0; ch < S::kChunks; ch++) {
-            float k[S::kPerLane][S::kChunk];
+            float4 k[S::kPerLane];
 #pragma unroll
             for (int x = 0; x < S::kPerLane; x++) {
                 const int j = lane + 32 * x;
-                const Chunk<T> c(sh.kv[st] + j * (HD * (int)sizeof(T)) + ((ch ^ (j & 7)) << 4));
-#pragma unroll
-                for (int y = 0; y < S::kChunk; y++) k[x][y] = c.f[y];
+                k[x] = *reinterpret_cast<const float4 *>(sh.kv[st] + j * (HD * 4) + ((ch ^ (j & 7)) << 4));
             }
 #pragma unroll
-            for (int r = 0; r < WR; r++)
+            for (int r = 0; r < WR; r++) {
+                const float4 qv = *reinterpret_cast<const float4 *>(qw + r * HD + ch * 4);
 #pragma unroll
-                for (int y = 0; y < S::kChunk; y += 4) {
-                    const float4 qv = *reinterpret_cast<const float4 *>(qw + r * HD + ch * S::kChunk + y);
-#pragma unroll
-                    for (int x = 0; x < S::kPerLane; x++) {
-                        acc[r][x] = fmaf(qv.x, k[x][y], acc[r][x]);
-                        acc[r][x] = fmaf(qv.y, k[x][y + 1], acc[r][x]);
-                        acc[r][x] = fmaf(qv.z, k[x][y + 2], acc[r][x]);
-                        acc[r][x] = fmaf(qv.w, k[x][y + 3], acc[r][x]);
-                    }
+                for (int x = 0; x < S::kPerLane; x++) {
+                    acc[r][x] = fmaf(qv.x, k[x].x, acc[r][x]);
+                    acc[r][x] = fmaf(qv.y, k[x].y, acc[r][x]);
+                    acc[r][x] = fmaf(qv.z, k[x].z, acc[r][x]);
+                    acc[r][x] = fmaf(qv.w, k[x].w, acc[r][x]);
                 }
+            }
         }
 
         bool any_masked = false;
@@ -533,7 +597,7 @@ __global__ void __launch_bounds__(kArThreads) attn_rows_many_kernel(const RowsAt
 #pragma unroll 4
         for (int x = 0; x < S::kKeys / S::kKeysAtOnce; x++) {
             const int j = x * S::kKeysAtOnce + sub;
-            const float4 v = load4<T>(reinterpret_cast<const T *>(vt) + j * HD + d4);
+            const float4 v = *reinterpret_cast<const float4 *>(vt + (j * HD + d4) * 4);
             float pr[WR];
 #pragma unroll
             for (int r = 0; r < WR; r += 4)
@@ -571,84 +635,57 @@ __global__ void __launch_bounds__(kArThreads) attn_rows_many_kernel(const RowsAt
             sh.sum[warp * WR + r] = l;
         }
     }
-    merge_store<T, HD, RB>(of, sh.mx, sh.sum, p, s, head0, m0, M, z, Z);
+    __syncthreads();
+    merge_store<HD, RB, kArThreads>(
+        sh.merge, [&](int r, int d) { return *reinterpret_cast<const float4 *>(of + r * HD + d); },
+        [&](int r) { return make_float2(sh.mx[r], sh.sum[r]); }, p, s, head0, m0, M, z, Z);
 }
 
-// The shared-memory and cluster-size opt-ins of one kernel, once per device.
-template <typename K>
-cudaError_t prepare_kernel(K kernel, size_t smem, std::atomic<uint64_t> &done) {
-    int dev = 0;
-    cudaError_t e = cudaGetDevice(&dev);
-    if (e != cudaSuccess) return e;
-    const uint64_t bit = 1ull << (dev & 63);
-    if (done.load() & bit) return cudaSuccess;
-    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-    if (e == cudaSuccess) done.fetch_or(bit);
-    return e;
-}
-
-template <typename K>
-cudaError_t launch_cluster(K kernel, dim3 grid, int Z, size_t smem, const RowsAttnParams &p, cudaStream_t st) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = grid;
-    cfg.blockDim = dim3(kArThreads);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = st;
-    cudaLaunchAttribute a[1];
-    a[0].id = cudaLaunchAttributeClusterDimension;
-    a[0].val.clusterDim.x = Z;
-    a[0].val.clusterDim.y = 1;
-    a[0].val.clusterDim.z = 1;
-    cfg.attrs = a;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kernel, p);
-}
-
-// Key shares of a tile: as many as two CTAs per SM hold, at most one per key
-// tile and 16, a cluster's limit.
-int shares(long long ctas, long long keys, int tile, int sms) {
-    const long long by_sms = std::max<long long>(1, 2ll * sms / ctas), by_keys = (keys + tile - 1) / tile;
-    return (int)std::max<long long>(1, std::min<long long>(16, std::min(by_sms, by_keys)));
-}
-
-template <typename T, int HD>
-cudaError_t launch_typed(const RowsAttnParams &p, int sms, cudaStream_t st) {
-    constexpr int kKeys = ArShape<T, HD>::kKeys;
+template <int HD>
+cudaError_t launch_dim(const RowsAttnParams &p, cudaStream_t st) {
     const long long M = (long long)p.r.max_rows * p.group;
     // most keys that one tile can see
     const long long keys =
         p.window > 0 ? std::min<long long>(p.c.cap, (long long)p.window + p.r.max_rows + p.c.n_sink) : p.c.cap;
-    auto go = [&](auto kernel, size_t smem, int rb, std::atomic<uint64_t> &done) {
-        cudaError_t e = prepare_kernel(kernel, smem, done);
+    // rb: packed rows of a tile, round: keys that a CTA takes at once
+    auto go = [&](auto kernel, size_t smem, int threads, int rb, int round, ClusterKernel &ck) {
+        int dev = 0;
+        cudaError_t e = cluster_prepare(ck, kernel, smem, &dev);
         if (e != cudaSuccess) return e;
-        const long long tiles = (M + rb - 1) / rb;
+        const long long tiles = (M + rb - 1) / rb, clusters = tiles * p.c.n_kv_heads * p.c.n_streams;
+        const long long rounds = (keys + round - 1) / round;
+        // Key shares of a tile, each a CTA of its cluster: the fewest rounds
+        // until the last wave of clusters is done, with kArFixed for a CTA's
+        // start and merge.
         RowsAttnParams pp = p;
-        pp.shares = shares(tiles * p.c.n_kv_heads * p.c.n_streams, keys, kKeys, sms);
-        return launch_cluster(kernel, dim3((unsigned)(pp.shares * tiles), p.c.n_kv_heads, p.c.n_streams), pp.shares, smem,
-                              pp, st);
+        pp.shares = 1;
+        long long best = LLONG_MAX;
+        for (int Z = 1; Z <= kMaxCluster && Z <= rounds; Z++) {
+            const int at_once = cluster_active(ck, kernel, dev, threads, smem, Z);
+            if (at_once < 1) continue;
+            const long long t = (clusters + at_once - 1) / at_once * ((rounds + Z - 1) / Z + kArFixed);
+            if (t < best) {
+                best = t;
+                pp.shares = Z;
+            }
+        }
+        cudaLaunchAttribute a;
+        const cudaLaunchConfig_t cfg = cluster_config(dim3((unsigned)(pp.shares * tiles), p.c.n_kv_heads, p.c.n_streams),
+                                                      threads, smem, pp.shares, &a, st);
+        return cudaLaunchKernelEx(&cfg, kernel, pp);
     };
-    static std::atomic<uint64_t> d4{0}, d8{0}, d32{0};
-    if constexpr (sizeof(T) == 2) return launch_attn_rows_tc(p, sms, st);
-    if (M <= 4) return go(attn_rows_few_kernel<T, HD, 4>, sizeof(ArFewSmem<T, HD, 4>), 4, d4);
-    if (M <= 8) return go(attn_rows_few_kernel<T, HD, 8>, sizeof(ArFewSmem<T, HD, 8>), 8, d8);
-    if constexpr (sizeof(T) == 2) return launch_attn_rows_tc(p, sms, st);
-    else return go(attn_rows_many_kernel<T, HD>, sizeof(ArManySmem<T, HD>), kArManyRows, d32);
-}
-
-template <typename T>
-cudaError_t launch_dim(const RowsAttnParams &p, int sms, cudaStream_t st) {
-    return p.c.head_dim == 64 ? launch_typed<T, 64>(p, sms, st) : launch_typed<T, 128>(p, sms, st);
+    static ClusterKernel d4, d8, d32;
+    constexpr int kRound = AfSmem<HD, 4>::kKeys * kAfWarps;
+    if (M <= 4) return go(attn_rows_few_kernel<HD, 4>, sizeof(AfSmem<HD, 4>), kAfThreads, 4, kRound, d4);
+    if (M <= kArManyRows) return go(attn_rows_few_kernel<HD, 8>, sizeof(AfSmem<HD, 8>), kAfThreads, 8, kRound, d8);
+    return go(attn_rows_many_kernel<HD>, sizeof(ArManySmem<HD>), kArThreads, kArManyRows, ArShape<HD>::kKeys, d32);
 }
 
 }  // namespace
 
 cudaError_t launch_attn_rows(const RowsAttnParams &p, int sms, cudaStream_t st) {
-    switch (p.c.dtype) {
-        case ELEM_F32: return launch_dim<float>(p, sms, st);
-        case ELEM_BF16: return launch_dim<__nv_bfloat16>(p, sms, st);
-        default: return launch_dim<__half>(p, sms, st);
-    }
+    if (p.c.dtype != ELEM_F32) return launch_attn_rows_tc(p, sms, st);
+    return p.c.head_dim == 64 ? launch_dim<64>(p, st) : launch_dim<128>(p, st);
 }
 
 }  // namespace vc

@@ -1,0 +1,70 @@
+// vc_cluster.h - launches whose CTAs share a row tile as one cluster along x:
+// per-device opt-ins, how many clusters of each size the device runs at once,
+// and the launch.
+#pragma once
+
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include <atomic>
+
+namespace vc {
+
+constexpr int kMaxCluster = 16;
+
+// One per kernel (a function-local static of its launch).
+struct ClusterKernel {
+    std::atomic<uint64_t> ready{0};                        // devices with the opt-ins set
+    std::atomic<int> active[16][kMaxCluster + 1] = {};     // by device (of 16) and size: clusters at once, 0: not asked yet
+};
+
+inline cudaLaunchConfig_t cluster_config(dim3 grid, int threads, size_t smem, int size, cudaLaunchAttribute *attr,
+                                         cudaStream_t st) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    attr->id = cudaLaunchAttributeClusterDimension;
+    attr->val.clusterDim.x = size;
+    attr->val.clusterDim.y = 1;
+    attr->val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cfg;
+}
+
+// Sets the current device's opt-ins: dynamic shared memory, clusters of 16.
+template <typename K>
+cudaError_t cluster_prepare(ClusterKernel &ck, K kernel, size_t smem, int *dev) {
+    cudaError_t e = cudaGetDevice(dev);
+    if (e != cudaSuccess) return e;
+    const uint64_t bit = 1ull << (*dev & 63);
+    if (ck.ready.load() & bit) return cudaSuccess;
+    if (smem) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e == cudaSuccess) ck.ready.fetch_or(bit);
+    return e;
+}
+
+// Clusters of `size` CTAs that run at once (a cluster lies within one GPC, so
+// this falls off in steps: with one CTA per SM a B200 runs 148, 74, ... 15 of
+// 9, 11 of 10 and 7 of 11 to 16).
+template <typename K>
+int cluster_active(ClusterKernel &ck, K kernel, int dev, int threads, size_t smem, int size) {
+    std::atomic<int> &slot = ck.active[dev & 15][size];
+    int n = slot.load();
+    if (n == 0) {
+        cudaLaunchAttribute a;
+        const cudaLaunchConfig_t cfg = cluster_config(dim3(size), threads, smem, size, &a, nullptr);
+        if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess) {
+            cudaGetLastError();
+            n = 0;
+        }
+        n = n > 0 ? n : -1;
+        slot.store(n);
+    }
+    return n;
+}
+
+}  // namespace vc
