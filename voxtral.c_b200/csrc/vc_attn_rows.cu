@@ -116,13 +116,6 @@ __device__ __forceinline__ void load_tile(unsigned char *dst, const char *kb, co
     }
 }
 
-__device__ __forceinline__ void bulk_load(void *dst, const void *src, uint32_t bytes, uint64_t *bar) {
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
-                     smem_u32(dst)),
-                 "l"(src), "r"(bytes), "r"(smem_u32(bar))
-                 : "memory");
-}
-
 // The shares of a tile merge by pushing: rank z owns a Z-th of the tile's sums
 // (groups of 4 dims), every CTA writes its part of them, and its rows' maxima
 // and sums, into the owners' shared memory, and after one cluster barrier each
@@ -194,19 +187,19 @@ __device__ __forceinline__ void merge_store(ArMerge<HD, RB> &mg, Sum sum, Ml ml,
 //
 // Bound by HBM at long contexts: 2 * RB flops per byte.  A warp works on tiles
 // of its own - 4 KB of K and as much of V, two under way - so nothing but its
-// own copies holds it up: a bulk copy per key row, one per lane at most, into
-// rows that are 16 bytes longer than a key for K (lanes then read one chunk of
-// different keys without conflicts).  Scores: 2 or 4 lanes share a key's dims,
-// against RB broadcast rows; the running maximum moves only when a score
-// exceeds it by more than 2^8, so most tiles need no shuffles across keys.
-// P.V: a lane has 4 dims of every row.
+// own copies holds it up (16 bytes per lane: a bulk copy per row costs the warp
+// a turn per lane, 818 instructions a tile against 500).  A K row is 16 bytes
+// longer than a key, so that lanes read one chunk of different keys without
+// conflicts.  Scores: 2 or 4 lanes share a key's dims, against RB broadcast
+// rows; the running maximum moves only when a score exceeds it by more than
+// 2^8, so most tiles need no shuffles across keys.  P.V: a lane has 4 dims of
+// every row.
 // ---------------------------------------------------------------------------
 
 constexpr int kAfWarps = 12;
 constexpr int kAfThreads = kAfWarps * 32;
 constexpr int kAfTile = 4096;              // K bytes of a warp's tile
 constexpr float kAfRescale = 8.0f;         // log2 of the largest weight before the maximum moves
-constexpr uint64_t kAfWaitNs = 2000000000ull;
 constexpr int kArFixed = 3;                // rounds' worth of a CTA's start and merge
 
 template <int HD, int RB>
@@ -224,11 +217,11 @@ struct AfSmem {
         float sums[kAfWarps][RB][HD];       // the warps' at the end
     };
     float q[RB * kQRow];
-    float p[kAfWarps][kKeys][RB];           // 2^(s - m), or -1 for a masked key
-    float wm[kAfWarps][RB], wl[kAfWarps][RB];
+    float2 p[kAfWarps][kKeys][RB];          // 2^(s - m) twice, or -1 for a masked key
+    float wm[kAfWarps][RB], wl[kAfWarps][RB], wf[kAfWarps][RB];
+    float mx[RB], sum[RB];
     ArMerge<HD, RB> merge;
     ArRows<RB> rows;
-    uint64_t full[kAfWarps][2];
 };
 
 template <int HD, int RB>
@@ -253,37 +246,39 @@ __global__ void __launch_bounds__(kAfThreads) attn_rows_few_kernel(const RowsAtt
     const char *kb = p.c.k + base * 4, *vb = p.c.v + base * 4;
     const long long slot_bytes = p.c.slot_stride * 4;
     const int head0 = kvh * p.group;
-    const uint64_t deadline = globaltimer() + kAfWaitNs;
-    bool ok = true;
-
-    if (lane == 0) {
-        mbar_init(&sh.full[warp][0], 1);
-        mbar_init(&sh.full[warp][1], 1);
-        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    }
-    __syncwarp();
+    // a group of copies even where no tile is left, so that the groups count
+    constexpr int kCh = HD / 4, kRowsAtOnce = 32 / kCh;   // 16-byte chunks of a row
+    const int ch = lane % kCh, jr = lane / kCh;
     auto fetch = [&](int t, int buf) {
-        const int idx0 = t * Sm::kKeys, n = min(Sm::kKeys, total - idx0);
-        typename Sm::Tile &tl = sh.tile[warp][buf];
-        uint64_t *bar = &sh.full[warp][buf];
-        if (lane == 0) mbar_expect_tx(bar, 2 * n * HD * 4);
-        __syncwarp();
+        const int idx0 = t * Sm::kKeys;
+        if (t < tiles) {
+            typename Sm::Tile &tl = sh.tile[warp][buf];
+            const uint32_t kd = smem_u32(tl.k) + jr * Sm::kRow + ch * 16, vd = smem_u32(tl.v) + jr * (HD * 4) + ch * 16;
+            int slot0 = lo_slot + (idx0 - kr.ns);   // of index idx0, past the sinks
+            if (slot0 >= p.c.cap) slot0 -= p.c.ring;
+            const bool run = idx0 >= kr.ns && idx0 + Sm::kKeys <= total && slot0 + Sm::kKeys <= p.c.cap;
+            long long off = (slot0 + jr) * slot_bytes + ch * 16;
 #pragma unroll
-        for (int e = lane; e < 2 * Sm::kKeys; e += 32) {
-            const int j = e % Sm::kKeys, idx = idx0 + j;
-            if (j >= n) continue;
-            int slot = idx;
-            if (idx >= kr.ns) {
-                slot = lo_slot + (idx - kr.ns);
-                if (slot >= p.c.cap) slot -= p.c.ring;
+            for (int it = 0; it < Sm::kKeys / kRowsAtOnce; it++) {
+                const int jj = it * kRowsAtOnce + jr, idx = idx0 + jj;
+                if (!run) {
+                    int slot = idx;
+                    if (idx >= kr.ns) {
+                        slot = lo_slot + (idx - kr.ns);
+                        if (slot >= p.c.cap) slot -= p.c.ring;
+                    }
+                    off = idx < total ? slot * slot_bytes + ch * 16 : 0;
+                }
+                cp_async16(kd + it * kRowsAtOnce * Sm::kRow, kb + off, run || idx < total);
+                cp_async16(vd + it * kRowsAtOnce * (HD * 4), vb + off, run || idx < total);
+                off += kRowsAtOnce * slot_bytes;
             }
-            if (e < Sm::kKeys) bulk_load(tl.k + j * Sm::kRow, kb + slot * slot_bytes, HD * 4, bar);
-            else bulk_load(tl.v + j * (HD * 4), vb + slot * slot_bytes, HD * 4, bar);
         }
+        cp_async_commit();
     };
     peers_arrive(Z);
-    if (t0 < tiles) fetch(t0, 0);
-    if (t0 + step < tiles) fetch(t0 + step, 1);
+    fetch(t0, 0);
+    fetch(t0 + step, 1);
 
     load_queries<HD, RB>(sh.q, Sm::kQRow, Sm::kParts, p, s, head0, m0, M);
     setup_rows<RB>(sh.rows, p, s, m0, M);
@@ -293,111 +288,124 @@ __global__ void __launch_bounds__(kAfThreads) attn_rows_few_kernel(const RowsAtt
     const int j = lane % Sm::kKeys, part = lane / Sm::kKeys;            // scores
     const int sub = lane / kLanesPerKey, d4 = lane % kLanesPerKey * 4;
     float mr[RB], l[RB];   // l: this lane's keys only
-    float4 o[RB];
+    uint64_t o[RB][2];     // pairs of dims
 #pragma unroll
     for (int r = 0; r < RB; r++) {
         mr[r] = -INFINITY;
         l[r] = 0.f;
-        o[r] = make_float4(0.f, 0.f, 0.f, 0.f);
+        o[r][0] = o[r][1] = 0;
     }
+    // keys that every row of the tile sees, in the walk's order
+    const int up_min = tree ? s.pos - 1 : s.pos + i0;
+    int core_s = kr.ns + (p.window > 0 ? max(0, min(s.pos + i1 - p.window - kr.lo, kr.nm)) : 0);
+    int core_e = kr.ns + max(0, min(up_min - kr.lo + 1, kr.nm));
+    if (up_min < kr.ns - 1) core_e = 0;
+    else if (core_s == kr.ns) core_s = 0;
     int n = 0;
     for (int t = t0; t < tiles; t += step, n++) {
         const int buf = n & 1;
-        if (!__all_sync(0xffffffffu, mbar_wait(&sh.full[warp][buf], (n >> 1) & 1u, deadline))) {
-            ok = false;
-            break;
-        }
+        cp_async_wait<1>();
+        __syncwarp();
         const typename Sm::Tile &tl = sh.tile[warp][buf];
-        float acc[RB];
+        uint64_t a2[RB];
 #pragma unroll
-        for (int r = 0; r < RB; r++) acc[r] = 0.f;
+        for (int r = 0; r < RB; r++) a2[r] = 0;
         constexpr int kChunks = HD / 4 / Sm::kParts;
 #pragma unroll 8
         for (int c = 0; c < kChunks; c++) {
-            const float4 k = *reinterpret_cast<const float4 *>(tl.k + j * Sm::kRow + (part * kChunks + c) * 16);
+            const ulonglong2 k = *reinterpret_cast<const ulonglong2 *>(tl.k + j * Sm::kRow + (part * kChunks + c) * 16);
 #pragma unroll
             for (int r = 0; r < RB; r++) {
-                const float4 q =
-                    *reinterpret_cast<const float4 *>(sh.q + r * Sm::kQRow + part * (HD / Sm::kParts + 4) + c * 4);
-                acc[r] = fmaf(q.x, k.x, acc[r]);
-                acc[r] = fmaf(q.y, k.y, acc[r]);
-                acc[r] = fmaf(q.z, k.z, acc[r]);
-                acc[r] = fmaf(q.w, k.w, acc[r]);
+                const ulonglong2 q =
+                    *reinterpret_cast<const ulonglong2 *>(sh.q + r * Sm::kQRow + part * (HD / Sm::kParts + 4) + c * 4);
+                a2[r] = fma2(q.x, k.x, a2[r]);
+                a2[r] = fma2(q.y, k.y, a2[r]);
             }
+        }
+        float acc[RB];
+#pragma unroll
+        for (int r = 0; r < RB; r++) {
+            float x, y;
+            unpair(a2[r], x, y);
+            acc[r] = x + y;
         }
 #pragma unroll
         for (int d = Sm::kKeys; d < 32; d *= 2)
 #pragma unroll
             for (int r = 0; r < RB; r++) acc[r] += __shfl_xor_sync(0xffffffffu, acc[r], d);
         const int idx = t * Sm::kKeys + j;
-        uint32_t vis = 0;
-        bool move = false;
-        if (idx < total) {
+        uint32_t vis = (1u << RB) - 1u;
+        const bool whole = t * Sm::kKeys >= core_s && (t + 1) * Sm::kKeys <= core_e;
+        if (!whole) {
+            vis = 0;
             const int at = kr.position(idx);
+            if (idx < total)
+#pragma unroll
+                for (int r = 0; r < RB; r++)
+                    if (row_sees<RB>(sh.rows, r, at, s.pos, p.c.n_sink, tree)) vis |= 1u << r;
 #pragma unroll
             for (int r = 0; r < RB; r++)
-                if (row_sees<RB>(sh.rows, r, at, s.pos, p.c.n_sink, tree)) {
-                    vis |= 1u << r;
-                    move |= mr[r] == -INFINITY ? acc[r] > -INFINITY : acc[r] > mr[r] + kAfRescale;
-                }
+                if (!((vis >> r) & 1u)) acc[r] = -INFINITY;
         }
+        bool move = false;
+#pragma unroll
+        for (int r = 0; r < RB; r++) move |= mr[r] == -INFINITY ? acc[r] > -INFINITY : acc[r] > mr[r] + kAfRescale;
         if (__any_sync(0xffffffffu, move)) {
 #pragma unroll
             for (int r = 0; r < RB; r++) {
-                float mt = (vis >> r) & 1u ? acc[r] : -INFINITY;
+                float mt = acc[r];
 #pragma unroll
-                for (int d = 16; d > 0; d >>= 1) mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, d));
+                for (int d = Sm::kKeys / 2; d > 0; d >>= 1) mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, d));
                 if (mt > mr[r]) {
                     const float al = mr[r] == -INFINITY ? 0.f : exp2_approx(mr[r] - mt);
                     mr[r] = mt;
                     l[r] *= al;
-                    o[r] = make_float4(o[r].x * al, o[r].y * al, o[r].z * al, o[r].w * al);
+                    o[r][0] = mul2(o[r][0], pair(al, al));
+                    o[r][1] = mul2(o[r][1], pair(al, al));
                 }
             }
         }
 #pragma unroll
         for (int r = 0; r < RB; r++) {
-            const float w = exp2_approx(acc[r] - (mr[r] == -INFINITY ? 0.f : mr[r]));
-            const bool see = (vis >> r) & 1u;
-            if (see && part == 0) l[r] += w;
-            acc[r] = see ? w : -1.f;
+            const float w = exp2_approx(acc[r] - (mr[r] == -INFINITY ? 0.f : mr[r]));   // (0 for a masked key)
+            if (part == 0) l[r] += w;
+            acc[r] = w;
         }
-        const bool masked = __any_sync(0xffffffffu, vis != (1u << RB) - 1u);
         if (part == 0)
 #pragma unroll
-            for (int r = 0; r < RB; r += 4)
-                *reinterpret_cast<float4 *>(&sh.p[warp][j][r]) = make_float4(acc[r], acc[r + 1], acc[r + 2], acc[r + 3]);
+            for (int r = 0; r < RB; r += 2)
+                *reinterpret_cast<float4 *>(&sh.p[warp][j][r]) = make_float4(acc[r], acc[r], acc[r + 1], acc[r + 1]);
         __syncwarp();
-#pragma unroll 4
+        // keys outside the core: a row skips those that it does not see
+        const uint32_t seen = __all_sync(0xffffffffu, vis == (1u << RB) - 1u);
+#pragma unroll
         for (int x = 0; x < Sm::kKeys / kAtOnce; x++) {
             const int jj = x * kAtOnce + sub;
-            const float4 v = *reinterpret_cast<const float4 *>(tl.v + (jj * HD + d4) * 4);
-            float w[RB];
+            const ulonglong2 v = *reinterpret_cast<const ulonglong2 *>(tl.v + (jj * HD + d4) * 4);
+            const uint32_t vj = seen ? 0xffffffffu : __shfl_sync(0xffffffffu, vis, jj);
 #pragma unroll
-            for (int r = 0; r < RB; r += 4)
-                *reinterpret_cast<float4 *>(w + r) = *reinterpret_cast<const float4 *>(&sh.p[warp][jj][r]);
-#pragma unroll
-            for (int r = 0; r < RB; r++) {
-                if (masked && w[r] < 0.f) continue;
-                o[r].x = fmaf(w[r], v.x, o[r].x);
-                o[r].y = fmaf(w[r], v.y, o[r].y);
-                o[r].z = fmaf(w[r], v.z, o[r].z);
-                o[r].w = fmaf(w[r], v.w, o[r].w);
+            for (int r = 0; r < RB; r += 2) {
+                const ulonglong2 w = *reinterpret_cast<const ulonglong2 *>(&sh.p[warp][jj][r]);
+                if (seen || ((vj >> r) & 1u)) {
+                    o[r][0] = fma2(w.x, v.x, o[r][0]);
+                    o[r][1] = fma2(w.x, v.y, o[r][1]);
+                }
+                if (seen || ((vj >> (r + 1)) & 1u)) {
+                    o[r + 1][0] = fma2(w.y, v.x, o[r + 1][0]);
+                    o[r + 1][1] = fma2(w.y, v.y, o[r + 1][1]);
+                }
             }
         }
         __syncwarp();   // the tile and p are done with
-        if (t + 2 * step < tiles) fetch(t + 2 * step, buf);
+        fetch(t + 2 * step, buf);
     }
-    if (!ok) {
-        if (lane == 0 && p.err) atomicExch_system(p.err, 1u);
-        const uint64_t grace = globaltimer() + 10000000ull;   // let copies in flight land
-        while (globaltimer() < grace) {
-        }
-    }
+    cp_async_wait<0>();
     __syncthreads();   // every tile is done with: the sums take their memory
 #pragma unroll
     for (int r = 0; r < RB; r++) {
-        float4 v = o[r];
+        float4 v;
+        unpair(o[r][0], v.x, v.y);
+        unpair(o[r][1], v.z, v.w);
         if (kAtOnce == 2) {
             v.x += __shfl_xor_sync(0xffffffffu, v.x, 16);
             v.y += __shfl_xor_sync(0xffffffffu, v.y, 16);
@@ -412,40 +420,32 @@ __global__ void __launch_bounds__(kAfThreads) attn_rows_few_kernel(const RowsAtt
         }
     }
     __syncthreads();
-    // the CTA's sums, in warp order
-    auto top = [&](int r) {
+    if (threadIdx.x < kAfWarps * RB) {   // the warps' weights; a warp that saw no key of a row has sums of 0
+        const int w = threadIdx.x / RB, r = threadIdx.x % RB;
         float gm = -INFINITY;
 #pragma unroll
-        for (int w = 0; w < kAfWarps; w++) gm = fmaxf(gm, sh.wm[w][r]);
-        return gm;
-    };
-    auto weight = [&](int w, int r, float gm) {   // of warp w's part; -1: it saw no key of the row
-        const float mw = sh.wm[w][r];
-        return mw == -INFINITY ? (sh.wl[w][r] == 0.f ? -1.f : 0.f) : exp2_approx(mw - gm);
-    };
+        for (int x = 0; x < kAfWarps; x++) gm = fmaxf(gm, sh.wm[x][r]);
+        sh.wf[w][r] = sh.wm[w][r] == -INFINITY ? 0.f : exp2_approx(sh.wm[w][r] - gm);
+        if (w == 0) sh.mx[r] = gm;
+    }
+    __syncthreads();
     merge_store<HD, RB, kAfThreads>(
         sh.merge,
-        [&](int r, int d) {
-            const float gm = top(r);
+        [&](int r, int d) {   // in warp order
             float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
             for (int w = 0; w < kAfWarps; w++) {
-                const float f = weight(w, r, gm);
-                if (f == -1.f) continue;
+                const float f = sh.wf[w][r];
                 const float4 v = *reinterpret_cast<const float4 *>(&sh.sums[w][r][d]);
                 a = make_float4(fmaf(f, v.x, a.x), fmaf(f, v.y, a.y), fmaf(f, v.z, a.z), fmaf(f, v.w, a.w));
             }
             return a;
         },
         [&](int r) {
-            const float gm = top(r);
             float gl = 0.f;
 #pragma unroll
-            for (int w = 0; w < kAfWarps; w++) {
-                const float f = weight(w, r, gm);
-                if (f != -1.f) gl = fmaf(f, sh.wl[w][r], gl);
-            }
-            return make_float2(gm, gl);
+            for (int w = 0; w < kAfWarps; w++) gl = fmaf(sh.wf[w][r], sh.wl[w][r], gl);
+            return make_float2(sh.mx[r], gl);
         },
         p, s, head0, m0, M, z, Z);
 }
