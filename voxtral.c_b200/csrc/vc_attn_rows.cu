@@ -18,6 +18,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <type_traits>
 
 namespace vc {
 
@@ -186,47 +187,51 @@ __device__ __forceinline__ void merge_store(ArMerge<HD, RB> &mg, Sum sum, Ml ml,
 // Few rows: RB (4 or 8) packed rows.
 //
 // Bound by HBM at long contexts: 2 * RB flops per byte.  A warp works on tiles
-// of its own - 4 KB of K and as much of V, two under way - so nothing but its
-// own copies holds it up (16 bytes per lane: a bulk copy per row costs the warp
-// a turn per lane, 818 instructions a tile against 500).  A K row is 16 bytes
-// longer than a key, so that lanes read one chunk of different keys without
-// conflicts.  Scores: 2 or 4 lanes share a key's dims, against RB broadcast
-// rows; the running maximum moves only when a score exceeds it by more than
-// 2^8, so most tiles need no shuffles across keys.  P.V: a lane has 4 dims of
-// every row.
+// of its own - 8 KB of K and as much of V - so nothing but its own copies holds
+// it up (16 bytes per lane: a bulk copy per row costs the warp a turn per
+// lane): the next tile's K is on its way from when the scores are done, its V
+// from when P.V is, and the other warps work meanwhile.  A K row is 16
+// bytes longer than a key, so that lanes read one chunk of different keys
+// without conflicts.  Scores: a lane has 32 dims of two keys against RB
+// broadcast rows; the running maximum moves only when a score exceeds it by
+// more than 2^8, so most tiles need no shuffles across keys.  P.V: a lane has 4
+// dims of every row.
 // ---------------------------------------------------------------------------
 
-constexpr int kAfWarps = 12;
-constexpr int kAfThreads = kAfWarps * 32;
-constexpr int kAfTile = 4096;              // K bytes of a warp's tile
+constexpr int af_warps(int hd, int rb) { return hd == 64 && rb == 8 ? 11 : 12; }   // as shared memory allows
+constexpr int kAfTile = 8192;              // K bytes of a warp's tile
 constexpr float kAfRescale = 8.0f;         // log2 of the largest weight before the maximum moves
-constexpr int kArFixed = 3;                // rounds' worth of a CTA's start and merge
+constexpr double kArFixed = 4;             // rounds' worth of a CTA's start and merge
 
 template <int HD, int RB>
 struct AfSmem {
-    static constexpr int kKeys = kAfTile / (HD * 4);       // keys of a tile: 8 or 16
+    static constexpr int kWarps = af_warps(HD, RB), kThreads = kWarps * 32, kRows = RB;
+    static constexpr int kKeys = kAfTile / (HD * 4);       // keys of a tile: 16 or 32
     static constexpr int kRow = HD * 4 + 16;               // a K row in shared memory
-    static constexpr int kParts = 32 / kKeys;              // lanes that share a key: 4 or 2
+    static constexpr int kParts = HD / 32;                 // lanes that share a key: 4 or 2
+    static constexpr int kAtOnce = 32 / kParts;            // keys that the lanes hold at once: half a tile
     static constexpr int kQRow = HD + 4 * (kParts - 1);    // a query row: its parts on different banks
     struct Tile {
         unsigned char k[kKeys * kRow];
         unsigned char v[kAfTile];
     };
     union {
-        Tile tile[kAfWarps][2];
-        float sums[kAfWarps][RB][HD];       // the warps' at the end
+        Tile tile[kWarps];
+        float sums[kWarps][RB][HD];       // the warps' at the end
     };
     float q[RB * kQRow];
-    float2 p[kAfWarps][kKeys][RB];          // 2^(s - m) twice, or -1 for a masked key
-    float wm[kAfWarps][RB], wl[kAfWarps][RB], wf[kAfWarps][RB];
+    float2 p[kWarps][kKeys][RB];          // 2^(s - m) twice
+    float wm[kWarps][RB], wl[kWarps][RB], wf[kWarps][RB];
     float mx[RB], sum[RB];
     ArMerge<HD, RB> merge;
     ArRows<RB> rows;
 };
 
 template <int HD, int RB>
-__global__ void __launch_bounds__(kAfThreads) attn_rows_few_kernel(const RowsAttnParams p) {
+__global__ void __launch_bounds__(AfSmem<HD, RB>::kThreads) attn_rows_few_kernel(const RowsAttnParams p) {
     using Sm = AfSmem<HD, RB>;
+    constexpr int kAfWarps = Sm::kWarps, kAfThreads = Sm::kThreads;
+    static_assert(sizeof(Sm) <= 227 * 1024, "fits an SM");
     extern __shared__ __align__(128) unsigned char smem_raw[];
     Sm &sh = *reinterpret_cast<Sm *>(smem_raw);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -249,43 +254,48 @@ __global__ void __launch_bounds__(kAfThreads) attn_rows_few_kernel(const RowsAtt
     // a group of copies even where no tile is left, so that the groups count
     constexpr int kCh = HD / 4, kRowsAtOnce = 32 / kCh;   // 16-byte chunks of a row
     const int ch = lane % kCh, jr = lane / kCh;
-    auto fetch = [&](int t, int buf) {
+    typename Sm::Tile &tl = sh.tile[warp];
+    auto fetch = [&](int t, bool is_v) {
         const int idx0 = t * Sm::kKeys;
         if (t < tiles) {
-            typename Sm::Tile &tl = sh.tile[warp][buf];
-            const uint32_t kd = smem_u32(tl.k) + jr * Sm::kRow + ch * 16, vd = smem_u32(tl.v) + jr * (HD * 4) + ch * 16;
+            const char *src = is_v ? vb : kb;
+            const int row = is_v ? HD * 4 : Sm::kRow;
+            const uint32_t dst = smem_u32(is_v ? tl.v : tl.k) + jr * row + ch * 16;
             int slot0 = lo_slot + (idx0 - kr.ns);   // of index idx0, past the sinks
             if (slot0 >= p.c.cap) slot0 -= p.c.ring;
             const bool run = idx0 >= kr.ns && idx0 + Sm::kKeys <= total && slot0 + Sm::kKeys <= p.c.cap;
-            long long off = (slot0 + jr) * slot_bytes + ch * 16;
+            constexpr int kIts = Sm::kKeys / kRowsAtOnce;
+            if (run) {
+                const char *a = src + (slot0 + jr) * slot_bytes + ch * 16;
+                const long long step_bytes = kRowsAtOnce * slot_bytes;
 #pragma unroll
-            for (int it = 0; it < Sm::kKeys / kRowsAtOnce; it++) {
-                const int jj = it * kRowsAtOnce + jr, idx = idx0 + jj;
-                if (!run) {
+                for (int it = 0; it < kIts; it++, a += step_bytes) cp_async16(dst + it * kRowsAtOnce * row, a, true);
+            } else {
+#pragma unroll 1
+                for (int it = 0; it < kIts; it++) {
+                    const int idx = idx0 + it * kRowsAtOnce + jr;
                     int slot = idx;
                     if (idx >= kr.ns) {
                         slot = lo_slot + (idx - kr.ns);
                         if (slot >= p.c.cap) slot -= p.c.ring;
                     }
-                    off = idx < total ? slot * slot_bytes + ch * 16 : 0;
+                    const bool ok = idx < total;
+                    cp_async16(dst + it * kRowsAtOnce * row, src + (ok ? slot * slot_bytes + ch * 16 : 0), ok);
                 }
-                cp_async16(kd + it * kRowsAtOnce * Sm::kRow, kb + off, run || idx < total);
-                cp_async16(vd + it * kRowsAtOnce * (HD * 4), vb + off, run || idx < total);
-                off += kRowsAtOnce * slot_bytes;
             }
         }
         cp_async_commit();
     };
     peers_arrive(Z);
-    fetch(t0, 0);
-    fetch(t0 + step, 1);
+    fetch(t0, false);
+    fetch(t0, true);
 
     load_queries<HD, RB>(sh.q, Sm::kQRow, Sm::kParts, p, s, head0, m0, M);
     setup_rows<RB>(sh.rows, p, s, m0, M);
     __syncthreads();
 
-    constexpr int kLanesPerKey = HD / 4, kAtOnce = 32 / kLanesPerKey;   // P.V
-    const int j = lane % Sm::kKeys, part = lane / Sm::kKeys;            // scores
+    constexpr int kLanesPerKey = HD / 4, kPvKeys = 32 / kLanesPerKey;   // P.V
+    const int j = lane % Sm::kAtOnce, part = lane / Sm::kAtOnce;        // scores: keys j and j + kAtOnce
     const int sub = lane / kLanesPerKey, d4 = lane % kLanesPerKey * 4;
     float mr[RB], l[RB];   // l: this lane's keys only
     uint64_t o[RB][2];     // pairs of dims
@@ -301,61 +311,67 @@ __global__ void __launch_bounds__(kAfThreads) attn_rows_few_kernel(const RowsAtt
     int core_e = kr.ns + max(0, min(up_min - kr.lo + 1, kr.nm));
     if (up_min < kr.ns - 1) core_e = 0;
     else if (core_s == kr.ns) core_s = 0;
-    int n = 0;
-    for (int t = t0; t < tiles; t += step, n++) {
-        const int buf = n & 1;
-        cp_async_wait<1>();
+    for (int t = t0; t < tiles; t += step) {
+        cp_async_wait<1>();   // K is in
         __syncwarp();
-        const typename Sm::Tile &tl = sh.tile[warp][buf];
-        uint64_t a2[RB];
+        uint64_t a2[2][RB];
 #pragma unroll
-        for (int r = 0; r < RB; r++) a2[r] = 0;
-        constexpr int kChunks = HD / 4 / Sm::kParts;
-#pragma unroll 8
-        for (int c = 0; c < kChunks; c++) {
-            const ulonglong2 k = *reinterpret_cast<const ulonglong2 *>(tl.k + j * Sm::kRow + (part * kChunks + c) * 16);
+        for (int r = 0; r < RB; r++) a2[0][r] = a2[1][r] = 0;
+#pragma unroll
+        for (int c = 0; c < 8; c++) {
+            const unsigned char *kp = tl.k + j * Sm::kRow + (part * 8 + c) * 16;
+            const ulonglong2 k0 = *reinterpret_cast<const ulonglong2 *>(kp);
+            const ulonglong2 k1 = *reinterpret_cast<const ulonglong2 *>(kp + Sm::kAtOnce * Sm::kRow);
 #pragma unroll
             for (int r = 0; r < RB; r++) {
-                const ulonglong2 q =
-                    *reinterpret_cast<const ulonglong2 *>(sh.q + r * Sm::kQRow + part * (HD / Sm::kParts + 4) + c * 4);
-                a2[r] = fma2(q.x, k.x, a2[r]);
-                a2[r] = fma2(q.y, k.y, a2[r]);
+                const ulonglong2 q = *reinterpret_cast<const ulonglong2 *>(sh.q + r * Sm::kQRow + part * 36 + c * 4);
+                a2[0][r] = fma2(q.x, k0.x, a2[0][r]);
+                a2[1][r] = fma2(q.x, k1.x, a2[1][r]);
+                a2[0][r] = fma2(q.y, k0.y, a2[0][r]);
+                a2[1][r] = fma2(q.y, k1.y, a2[1][r]);
             }
         }
-        float acc[RB];
+        __syncwarp();
+        fetch(t + step, false);
+        float acc[2][RB];
 #pragma unroll
-        for (int r = 0; r < RB; r++) {
-            float x, y;
-            unpair(a2[r], x, y);
-            acc[r] = x + y;
-        }
+        for (int x = 0; x < 2; x++)
 #pragma unroll
-        for (int d = Sm::kKeys; d < 32; d *= 2)
+            for (int r = 0; r < RB; r++) {
+                float a, b;
+                unpair(a2[x][r], a, b);
+                acc[x][r] = a + b;
 #pragma unroll
-            for (int r = 0; r < RB; r++) acc[r] += __shfl_xor_sync(0xffffffffu, acc[r], d);
-        const int idx = t * Sm::kKeys + j;
-        uint32_t vis = (1u << RB) - 1u;
+                for (int d = Sm::kAtOnce; d < 32; d *= 2) acc[x][r] += __shfl_xor_sync(0xffffffffu, acc[x][r], d);
+            }
+        uint32_t vis[2] = {(1u << RB) - 1u, (1u << RB) - 1u};
         const bool whole = t * Sm::kKeys >= core_s && (t + 1) * Sm::kKeys <= core_e;
         if (!whole) {
-            vis = 0;
-            const int at = kr.position(idx);
-            if (idx < total)
+#pragma unroll
+            for (int x = 0; x < 2; x++) {
+                const int idx = t * Sm::kKeys + x * Sm::kAtOnce + j, at = kr.position(idx);
+                vis[x] = 0;
+                if (idx < total)
+#pragma unroll
+                    for (int r = 0; r < RB; r++)
+                        if (row_sees<RB>(sh.rows, r, at, s.pos, p.c.n_sink, tree)) vis[x] |= 1u << r;
 #pragma unroll
                 for (int r = 0; r < RB; r++)
-                    if (row_sees<RB>(sh.rows, r, at, s.pos, p.c.n_sink, tree)) vis |= 1u << r;
-#pragma unroll
-            for (int r = 0; r < RB; r++)
-                if (!((vis >> r) & 1u)) acc[r] = -INFINITY;
+                    if (!((vis[x] >> r) & 1u)) acc[x][r] = -INFINITY;
+            }
         }
         bool move = false;
 #pragma unroll
-        for (int r = 0; r < RB; r++) move |= mr[r] == -INFINITY ? acc[r] > -INFINITY : acc[r] > mr[r] + kAfRescale;
+        for (int r = 0; r < RB; r++) {
+            const float a = fmaxf(acc[0][r], acc[1][r]);
+            move |= mr[r] == -INFINITY ? a > -INFINITY : a > mr[r] + kAfRescale;
+        }
         if (__any_sync(0xffffffffu, move)) {
 #pragma unroll
             for (int r = 0; r < RB; r++) {
-                float mt = acc[r];
+                float mt = fmaxf(acc[0][r], acc[1][r]);
 #pragma unroll
-                for (int d = Sm::kKeys / 2; d > 0; d >>= 1) mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, d));
+                for (int d = Sm::kAtOnce / 2; d > 0; d >>= 1) mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, d));
                 if (mt > mr[r]) {
                     const float al = mr[r] == -INFINITY ? 0.f : exp2_approx(mr[r] - mt);
                     mr[r] = mt;
@@ -367,37 +383,55 @@ __global__ void __launch_bounds__(kAfThreads) attn_rows_few_kernel(const RowsAtt
         }
 #pragma unroll
         for (int r = 0; r < RB; r++) {
-            const float w = exp2_approx(acc[r] - (mr[r] == -INFINITY ? 0.f : mr[r]));   // (0 for a masked key)
-            if (part == 0) l[r] += w;
-            acc[r] = w;
+            const float base = mr[r] == -INFINITY ? 0.f : mr[r];
+            acc[0][r] = exp2_approx(acc[0][r] - base);   // (0 for a masked key)
+            acc[1][r] = exp2_approx(acc[1][r] - base);
+            if (part == 0) l[r] += acc[0][r] + acc[1][r];
         }
-        if (part == 0)
-#pragma unroll
-            for (int r = 0; r < RB; r += 2)
-                *reinterpret_cast<float4 *>(&sh.p[warp][j][r]) = make_float4(acc[r], acc[r], acc[r + 1], acc[r + 1]);
-        __syncwarp();
-        // keys outside the core: a row skips those that it does not see
-        const uint32_t seen = __all_sync(0xffffffffu, vis == (1u << RB) - 1u);
-#pragma unroll
-        for (int x = 0; x < Sm::kKeys / kAtOnce; x++) {
-            const int jj = x * kAtOnce + sub;
-            const ulonglong2 v = *reinterpret_cast<const ulonglong2 *>(tl.v + (jj * HD + d4) * 4);
-            const uint32_t vj = seen ? 0xffffffffu : __shfl_sync(0xffffffffu, vis, jj);
+        if (part < 2)   // one of the lanes of a key stores its first, one its second weights
 #pragma unroll
             for (int r = 0; r < RB; r += 2) {
-                const ulonglong2 w = *reinterpret_cast<const ulonglong2 *>(&sh.p[warp][jj][r]);
-                if (seen || ((vj >> r) & 1u)) {
+                const float a = part ? acc[1][r] : acc[0][r], b = part ? acc[1][r + 1] : acc[0][r + 1];
+                *reinterpret_cast<float4 *>(&sh.p[warp][j + part * Sm::kAtOnce][r]) = make_float4(a, a, b, b);
+            }
+        cp_async_wait<1>();   // V is in
+        __syncwarp();
+        // keys outside the core: a row skips those that it does not see
+        const bool seen = __all_sync(0xffffffffu, (vis[0] & vis[1]) == (1u << RB) - 1u);
+        if (seen) {
+#pragma unroll 8
+            for (int x = 0; x < Sm::kKeys / kPvKeys; x++) {
+                const int jj = x * kPvKeys + sub;
+                const ulonglong2 v = *reinterpret_cast<const ulonglong2 *>(tl.v + (jj * HD + d4) * 4);
+#pragma unroll
+                for (int r = 0; r < RB; r += 2) {
+                    const ulonglong2 w = *reinterpret_cast<const ulonglong2 *>(&sh.p[warp][jj][r]);
                     o[r][0] = fma2(w.x, v.x, o[r][0]);
                     o[r][1] = fma2(w.x, v.y, o[r][1]);
-                }
-                if (seen || ((vj >> (r + 1)) & 1u)) {
                     o[r + 1][0] = fma2(w.y, v.x, o[r + 1][0]);
                     o[r + 1][1] = fma2(w.y, v.y, o[r + 1][1]);
                 }
             }
+        } else {
+#pragma unroll 1
+            for (int x = 0; x < Sm::kKeys / kPvKeys; x++) {
+                const int jj = x * kPvKeys + sub;
+                const ulonglong2 v = *reinterpret_cast<const ulonglong2 *>(tl.v + (jj * HD + d4) * 4);
+                const uint32_t v0 = __shfl_sync(0xffffffffu, vis[0], jj % Sm::kAtOnce);
+                const uint32_t v1 = __shfl_sync(0xffffffffu, vis[1], jj % Sm::kAtOnce);
+                const uint32_t vj = jj < Sm::kAtOnce ? v0 : v1;
+#pragma unroll
+                for (int r = 0; r < RB; r++) {
+                    const uint64_t w = *reinterpret_cast<const uint64_t *>(&sh.p[warp][jj][r]);
+                    if ((vj >> r) & 1u) {
+                        o[r][0] = fma2(w, v.x, o[r][0]);
+                        o[r][1] = fma2(w, v.y, o[r][1]);
+                    }
+                }
+            }
         }
-        __syncwarp();   // the tile and p are done with
-        fetch(t + 2 * step, buf);
+        __syncwarp();
+        fetch(t + step, true);
     }
     cp_async_wait<0>();
     __syncthreads();   // every tile is done with: the sums take their memory
@@ -406,7 +440,7 @@ __global__ void __launch_bounds__(kAfThreads) attn_rows_few_kernel(const RowsAtt
         float4 v;
         unpair(o[r][0], v.x, v.y);
         unpair(o[r][1], v.z, v.w);
-        if (kAtOnce == 2) {
+        if (kPvKeys == 2) {
             v.x += __shfl_xor_sync(0xffffffffu, v.x, 16);
             v.y += __shfl_xor_sync(0xffffffffu, v.y, 16);
             v.z += __shfl_xor_sync(0xffffffffu, v.z, 16);
@@ -653,17 +687,17 @@ cudaError_t launch_dim(const RowsAttnParams &p, cudaStream_t st) {
         cudaError_t e = cluster_prepare(ck, kernel, smem, &dev);
         if (e != cudaSuccess) return e;
         const long long tiles = (M + rb - 1) / rb, clusters = tiles * p.c.n_kv_heads * p.c.n_streams;
-        const long long rounds = (keys + round - 1) / round;
+        const double rounds = (double)keys / round;
         // Key shares of a tile, each a CTA of its cluster: the fewest rounds
         // until the last wave of clusters is done, with kArFixed for a CTA's
         // start and merge.
         RowsAttnParams pp = p;
         pp.shares = 1;
-        long long best = LLONG_MAX;
-        for (int Z = 1; Z <= kMaxCluster && Z <= rounds; Z++) {
+        double best = 1e30;
+        for (int Z = 1; Z <= kMaxCluster && Z < rounds + 1; Z++) {
             const int at_once = cluster_active(ck, kernel, dev, threads, smem, Z);
             if (at_once < 1) continue;
-            const long long t = (clusters + at_once - 1) / at_once * ((rounds + Z - 1) / Z + kArFixed);
+            const double t = (double)((clusters + at_once - 1) / at_once) * (std::max(1.0, rounds / Z) + kArFixed);
             if (t < best) {
                 best = t;
                 pp.shares = Z;
@@ -675,9 +709,12 @@ cudaError_t launch_dim(const RowsAttnParams &p, cudaStream_t st) {
         return cudaLaunchKernelEx(&cfg, kernel, pp);
     };
     static ClusterKernel d4, d8, d32;
-    constexpr int kRound = AfSmem<HD, 4>::kKeys * kAfWarps;
-    if (M <= 4) return go(attn_rows_few_kernel<HD, 4>, sizeof(AfSmem<HD, 4>), kAfThreads, 4, kRound, d4);
-    if (M <= kArManyRows) return go(attn_rows_few_kernel<HD, 8>, sizeof(AfSmem<HD, 8>), kAfThreads, 8, kRound, d8);
+    auto few = [&](auto kernel, auto *sm, ClusterKernel &ck) {
+        using Sm = std::remove_pointer_t<decltype(sm)>;
+        return go(kernel, sizeof(Sm), Sm::kThreads, Sm::kRows, Sm::kKeys * Sm::kWarps, ck);
+    };
+    if (M <= 4) return few(attn_rows_few_kernel<HD, 4>, (AfSmem<HD, 4> *)nullptr, d4);
+    if (M <= kArManyRows) return few(attn_rows_few_kernel<HD, 8>, (AfSmem<HD, 8> *)nullptr, d8);
     return go(attn_rows_many_kernel<HD>, sizeof(ArManySmem<HD>), kArThreads, kArManyRows, ArShape<HD>::kKeys, d32);
 }
 
