@@ -678,16 +678,13 @@ __global__ void __launch_bounds__(kArThreads) attn_rows_many_kernel(const RowsAt
 template <int HD>
 cudaError_t launch_dim(const RowsAttnParams &p, cudaStream_t st) {
     const long long M = (long long)p.r.max_rows * p.group;
-    // most keys that one tile can see
-    const long long keys =
-        p.window > 0 ? std::min<long long>(p.c.cap, (long long)p.window + p.r.max_rows + p.c.n_sink) : p.c.cap;
     // rb: packed rows of a tile, round: keys that a CTA takes at once
     auto go = [&](auto kernel, size_t smem, int threads, int rb, int round, ClusterKernel &ck) {
         int dev = 0;
         cudaError_t e = cluster_prepare(ck, kernel, smem, &dev);
         if (e != cudaSuccess) return e;
         const long long tiles = (M + rb - 1) / rb, clusters = tiles * p.c.n_kv_heads * p.c.n_streams;
-        const double rounds = (double)keys / round;
+        const double rounds = (double)most_keys(p, rb) / round;
         // Key shares of a tile, each a CTA of its cluster: the fewest rounds
         // until the last wave of clusters is done, with kArFixed for a CTA's
         // start and merge.
@@ -720,8 +717,8 @@ cudaError_t launch_dim(const RowsAttnParams &p, cudaStream_t st) {
 
 }  // namespace
 
-cudaError_t launch_attn_rows(const RowsAttnParams &p, int sms, cudaStream_t st) {
-    if (p.c.dtype != ELEM_F32) return launch_attn_rows_tc(p, sms, st);
+cudaError_t launch_attn_rows(const RowsAttnParams &p, cudaStream_t st) {
+    if (p.c.dtype != ELEM_F32) return launch_attn_rows_tc(p, st);
     return p.c.head_dim == 64 ? launch_dim<64>(p, st) : launch_dim<128>(p, st);
 }
 

@@ -27,6 +27,7 @@
 // row does not see whole, the loading threads look for non-finite V values,
 // put zeros in their place and set a flag, and the rows that do see them add
 // them at the end.
+#include "vc_cluster.h"
 #include "vc_rows.cuh"
 #include "vc_tc.cuh"
 
@@ -59,7 +60,8 @@ constexpr int at_threads(int nt, int rt) { return (nt * rt / 32 + 4) * 32; }
 constexpr uint64_t kAtWaitNs = 2000000000ull;
 constexpr float kAtRescale = 8.0f;      // log2 of the largest P before the maximum moves
 constexpr int kAtOneCta = 120 * 1024;   // more than half an SM's shared memory: one CTA per SM
-constexpr int kAtFixed = 4;             // block times of a CTA's start and merge
+constexpr double kAtFixed = 4;          // block times of a CTA's start and merge
+constexpr double kAtAlone = 0.6;        // a block's time on an SM of its own, of that beside another CTA
 
 template <int HD, int NT, int RT>
 struct AtSmem {
@@ -729,75 +731,58 @@ bool cache_map(CUtensorMap *m, char *base, const CacheView &c, int keys) {
 }
 
 template <typename T, int HD, int NT, int RT>
-cudaError_t launch_tiles(RowsAttnParams p, int sms, cudaStream_t st) {
+cudaError_t launch_tiles(RowsAttnParams p, cudaStream_t st) {
     constexpr int kKeys = at_keys(NT);
     constexpr size_t kSmem = std::max<size_t>(sizeof(AtSmem<HD, NT, RT>), NT == 2 ? kAtOneCta : 0);
     static_assert(kSmem <= (NT == 1 ? 113 : 227) * 1024, "two CTAs or one fit an SM");
     auto kernel = attn_rows_tc_kernel<T, HD, NT, RT>;
-    static std::atomic<uint64_t> done{0};
+    static ClusterKernel ck;
     int dev = 0;
-    cudaError_t e = cudaGetDevice(&dev);
+    cudaError_t e = cluster_prepare(ck, kernel, kSmem, &dev);
     if (e != cudaSuccess) return e;
-    const uint64_t bit = 1ull << (dev & 63);
-    if (!(done.load() & bit)) {
-        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem);
-        if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-        if (e != cudaSuccess) return e;
-        done.fetch_or(bit);
-    }
     const long long M = (long long)p.r.max_rows * p.group;
     const long long tiles = (M + NT * RT - 1) / (NT * RT);
-    const long long keys =
-        p.window > 0 ? std::min<long long>(p.c.cap, (long long)p.window + p.r.max_rows + p.c.n_sink) : p.c.cap;
-    const long long ctas = tiles * p.c.n_kv_heads * p.c.n_streams, blocks = (keys + kKeys - 1) / kKeys;
+    const long long clusters = tiles * p.c.n_kv_heads * p.c.n_streams, blocks = (most_keys(p, NT * RT) + kKeys - 1) / kKeys;
     // Shares: the least time in units of a block, with kAtFixed for a CTA's
-    // start and merge.  Several waves: each takes a share's blocks.  One wave
-    // that leaves SMs half empty: two CTAs of an SM share its part of the
-    // bandwidth, so a CTA alone there is faster (24 tokens over 4096 keys, 192
-    // CTAs: 69 us in three shares, 57 us in one).
-    const double slots = (double)sms * (NT == 1 ? 2 : 1);
+    // start and merge.  Several waves of clusters: each takes a share's blocks.
+    // One wave that leaves SMs half empty: a CTA alone on an SM is faster than
+    // one of two.
     double best = 1e30;
-    for (int Z = 1; Z <= 16 && Z <= blocks; Z++) {
-        const double fill = ctas * Z / slots, part = (double)((blocks + Z - 1) / Z);
-        const double t = fill > 1.0 ? ceil(fill) * (part + kAtFixed) : part * std::max(fill, NT == 1 ? 0.5 : 1.0) + kAtFixed;
+    p.shares = 1;
+    for (int Z = 1; Z <= kMaxCluster && Z <= blocks; Z++) {
+        const int at_once = cluster_active(ck, kernel, dev, at_threads(NT, RT), kSmem, Z);
+        if (at_once < 1) continue;
+        const double fill = (double)clusters / at_once, part = (double)blocks / Z;
+        const double t = fill > 1.0 ? ceil(fill) * (part + kAtFixed) : part * std::max(fill, NT == 1 ? kAtAlone : 1.0) + kAtFixed;
         if (t < best) {
             best = t;
             p.shares = Z;
         }
     }
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(p.shares * tiles), p.c.n_kv_heads, p.c.n_streams);
-    cfg.blockDim = dim3(at_threads(NT, RT));
-    cfg.dynamicSmemBytes = kSmem;
-    cfg.stream = st;
-    cudaLaunchAttribute a[1];
-    a[0].id = cudaLaunchAttributeClusterDimension;
-    a[0].val.clusterDim.x = p.shares;
-    a[0].val.clusterDim.y = 1;
-    a[0].val.clusterDim.z = 1;
-    cfg.attrs = a;
-    cfg.numAttrs = 1;
+    cudaLaunchAttribute attr;
+    const cudaLaunchConfig_t cfg = cluster_config(dim3((unsigned)(p.shares * tiles), p.c.n_kv_heads, p.c.n_streams),
+                                                  at_threads(NT, RT), kSmem, p.shares, &attr, st);
     CUtensorMap mk = {}, mv = {};
     p.maps = cache_map(&mk, p.c.k + p.layer_off * 2, p.c, kKeys) && cache_map(&mv, p.c.v + p.layer_off * 2, p.c, kKeys);
     return cudaLaunchKernelEx(&cfg, kernel, mk, mv, p);
 }
 
 template <typename T, int HD>
-cudaError_t launch_typed(const RowsAttnParams &p, int sms, cudaStream_t st) {
+cudaError_t launch_typed(const RowsAttnParams &p, cudaStream_t st) {
     const long long M = (long long)p.r.max_rows * p.group;
-    if (M <= 32) return launch_tiles<T, HD, 1, 32>(p, sms, st);
-    if (M <= kAtRows) return launch_tiles<T, HD, 1, 128>(p, sms, st);
-    return launch_tiles<T, HD, 2, 128>(p, sms, st);
+    if (M <= 32) return launch_tiles<T, HD, 1, 32>(p, st);
+    if (M <= kAtRows) return launch_tiles<T, HD, 1, 128>(p, st);
+    return launch_tiles<T, HD, 2, 128>(p, st);
 }
 template <typename T>
-cudaError_t launch_dim(const RowsAttnParams &p, int sms, cudaStream_t st) {
-    return p.c.head_dim == 64 ? launch_typed<T, 64>(p, sms, st) : launch_typed<T, 128>(p, sms, st);
+cudaError_t launch_dim(const RowsAttnParams &p, cudaStream_t st) {
+    return p.c.head_dim == 64 ? launch_typed<T, 64>(p, st) : launch_typed<T, 128>(p, st);
 }
 
 }  // namespace
 
-cudaError_t launch_attn_rows_tc(const RowsAttnParams &p, int sms, cudaStream_t st) {
-    return p.c.dtype == ELEM_BF16 ? launch_dim<__nv_bfloat16>(p, sms, st) : launch_dim<__half>(p, sms, st);
+cudaError_t launch_attn_rows_tc(const RowsAttnParams &p, cudaStream_t st) {
+    return p.c.dtype == ELEM_BF16 ? launch_dim<__nv_bfloat16>(p, st) : launch_dim<__half>(p, st);
 }
 
 }  // namespace vc

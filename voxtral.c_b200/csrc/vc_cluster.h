@@ -3,9 +3,9 @@
 // and the launch.
 #pragma once
 
-#include <cuda_runtime.h>
-#include <stdint.h>
+#include "vc_internal.h"
 
+#include <algorithm>
 #include <atomic>
 
 namespace vc {
@@ -45,6 +45,13 @@ cudaError_t cluster_prepare(ClusterKernel &ck, K kernel, size_t smem, int *dev) 
     if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     if (e == cudaSuccess) ck.ready.fetch_or(bit);
     return e;
+}
+
+// The most keys that a tile of `packed` rows can see.
+inline long long most_keys(const RowsAttnParams &p, int packed) {
+    if (p.window <= 0) return p.c.cap;
+    const long long rows = p.r.parent ? p.r.max_rows : std::min<long long>(p.r.max_rows, (packed - 1) / p.group + 2);
+    return std::min<long long>(p.c.cap, p.window + rows + p.c.n_sink);
 }
 
 // Clusters of `size` CTAs that run at once (a cluster lies within one GPC, so

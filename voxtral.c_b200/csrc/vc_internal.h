@@ -189,9 +189,9 @@ struct RowsAttnParams {
     unsigned *err;            // raised when a bounded wait expires (mapped host memory)
     int maps;                 // tensor maps of K and V came with the launch (set by it)
 };
-cudaError_t launch_attn_rows(const RowsAttnParams &p, int sms, cudaStream_t st);
+cudaError_t launch_attn_rows(const RowsAttnParams &p, cudaStream_t st);
 // the tensor-core kernel of the 16-bit types (vc_attn_rows_tc.cu)
-cudaError_t launch_attn_rows_tc(const RowsAttnParams &p, int sms, cudaStream_t st);
+cudaError_t launch_attn_rows_tc(const RowsAttnParams &p, cudaStream_t st);
 
 struct AppendParams {
     CacheView c;

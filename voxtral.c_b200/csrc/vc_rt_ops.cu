@@ -192,7 +192,7 @@ int attention(const char *who, bool tree, const vox_cuda_kv_cache *cache, int la
     p.group = n_heads / p.c.n_kv_heads;
     p.window = window;
     p.scale_log2 = (scale == 0.f ? 1.0f / sqrtf((float)p.c.head_dim) : scale) * 1.4426950408889634f;
-    return launched(who, launch_attn_rows(p, c->sms, stream ? (cudaStream_t)stream : c->stream));
+    return launched(who, launch_attn_rows(p, stream ? (cudaStream_t)stream : c->stream));
 }
 
 }  // namespace
