@@ -12,9 +12,9 @@
 // when there are fewer rows than SMs.
 //
 // The alternatives cost no second pass: the threads also leave each batch's
-// maximum in shared memory.  The n_top-th largest of 32 group maxima is a
+// maximum in shared memory.  The n_top-th largest of 64 group maxima is a
 // value that at least n_top logits reach, so only batches that reach it -
-// about n_top of them - are looked at again, and their few values that reach it
+// 1 to 1.5 n_top of them - are looked at again, and their few values that reach it
 // are ranked by counting.  Keys order by value, then by the lowest id; the
 // shares of a row rank their lists against each other's.
 #include "vc_rows.cuh"
@@ -39,6 +39,7 @@ constexpr int kLpLoads = 4;      // 16-byte loads of a thread's batch
 constexpr int kLpKept = 4096;    // batch maxima kept: NTH threads x 4096 / NTH slots, batch b in slot b % slots
 constexpr int kLpFound = 256;    // candidates, and batches with some, kept
 constexpr int kLpShares = 16;    // CTAs of a row at most
+constexpr int kLpGroups = 64;    // groups of threads whose maxima give the floor
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLpFloor = -300.f;   // 2^x below this is 0 in fp32
 
@@ -62,7 +63,7 @@ struct LpSmem {
     Key found[kLpFound];            // candidates, in any order
     Key lists[kWarps][kTopMax];   // the warps' best, where `found` overflowed
     Key merged[kTopMax];            // the CTA's best
-    float group_max[32];
+    float group_max[kLpGroups];
     float red[kWarps][4];
     float stat[5];                  // the CTA's (m, top, rest, S) and its largest logit
     float floor;                    // n_top logits of the CTA's share reach this
@@ -391,15 +392,15 @@ __global__ void __launch_bounds__(NTH, 1024 / NTH) token_logprobs_kernel(const L
     {
         float g = best;
 #pragma unroll
-        for (int o = NTH / 64; o > 0; o >>= 1) g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, o));
-        if (lane % (NTH / 32) == 0) sh.group_max[threadIdx.x / (NTH / 32)] = g;   // 32 groups of threads
+        for (int o = NTH / kLpGroups / 2; o > 0; o >>= 1) g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, o));
+        if (lane % (NTH / kLpGroups) == 0) sh.group_max[threadIdx.x / (NTH / kLpGroups)] = g;
     }
     if (threadIdx.x < kTopMax) sh.merged[threadIdx.x] = 0;
     if (threadIdx.x == 0) sh.count = sh.hits = 0;
     __syncthreads();
     if (warp == 0) {
         fold_lanes(lane < (NTH / 32) ? sh.red[lane] : nullptr, (NTH / 32), m, top, rest, mom);
-        const float g = warp_max(sh.group_max[lane]);
+        const float g = warp_max(fmaxf(sh.group_max[lane], sh.group_max[lane + 32]));
         if (lane == 0) {
             sh.stat[0] = m;
             sh.stat[1] = top;
@@ -409,13 +410,14 @@ __global__ void __launch_bounds__(NTH, 1024 / NTH) token_logprobs_kernel(const L
         }
     }
     if (K > 0) {
-        if (warp == 1) {   // the K-th largest group maximum: K - 1 others are at least as large
-            const float g = sh.group_max[lane];
+        if (warp == 1 || warp == 2) {   // the K-th largest group maximum: K - 1 others are at least as large
+            const int me = lane + 32 * (warp - 1);
+            const float g = sh.group_max[me];
             int rank = 0;
-#pragma unroll
-            for (int o = 0; o < 32; o++) {
+#pragma unroll 16
+            for (int o = 0; o < kLpGroups; o++) {
                 const float h = sh.group_max[o];
-                rank += h > g || (h == g && o < lane);
+                rank += h > g || (h == g && o < me);
             }
             if (rank == K - 1) sh.floor = g;
         }
