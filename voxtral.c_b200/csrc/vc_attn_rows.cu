@@ -26,18 +26,6 @@ using namespace tc;
 
 namespace {
 
-constexpr int kArThreads = 128;       // many rows: 4 warps
-constexpr int kArTileBytes = 16384;   // K (and V) bytes of their key tile
-
-template <int HD>
-struct ArShape {
-    static constexpr int kChunks = HD / 4;                    // 16-byte chunks per key
-    static constexpr int kKeys = kArTileBytes / (HD * 4);     // keys per tile
-    static constexpr int kPerLane = kKeys / 32;               // keys per lane
-    static constexpr int kLanesPerKey = HD / 4;               // P.V: 4 dims per lane
-    static constexpr int kKeysAtOnce = 32 / kLanesPerKey;     // P.V: keys per warp step
-};
-
 // What a tile's rows see, and where they are (shared memory).
 template <int RB>
 struct ArRows {
@@ -92,28 +80,49 @@ __device__ __forceinline__ void load_queries(float *q, int row, int parts, const
     }
 }
 
-// Asynchronous copy of key tile t's K and V rows; rows past `end` become
-// zeros.  K rows are chunk-swizzled (chunk c of key j at c ^ (j & 7)), so that
-// 32 lanes reading chunk c of 32 keys do not conflict.
-template <int HD>
-__device__ __forceinline__ void load_tile(unsigned char *dst, const char *kb, const char *vb, long long slot_bytes,
-                                          const KeyRange &kr, int lo_slot, const CacheView &c, int idx0, int end) {
-    using S = ArShape<HD>;
-    const uint32_t k_s = smem_u32(dst), v_s = k_s + kArTileBytes;
+// o += P V of a warp's tile, whose lanes hold which of the R rows see their two
+// keys (vis); weigh(j, v, rows) adds key j's to some rows.  A masked key's
+// weight is 0, but 0 times a NaN or an infinity is NaN: where a tile has masked
+// keys and the sums come out NaN, they are taken back and such keys skipped.
+template <int HD, int KEYS, int R, typename Weigh>
+__device__ __forceinline__ void add_values(uint64_t (&o)[R][2], const unsigned char *vt, const uint32_t (&vis)[2], int sub,
+                                           int d4, Weigh weigh) {
+    constexpr int kPvKeys = 128 / HD;   // keys that the lanes take at once
+    constexpr uint32_t kAll = (1u << R) - 1u;
+    const bool masked = __any_sync(0xffffffffu, (vis[0] & vis[1]) != kAll);
+    uint64_t before[R][2];
+    if (masked) {
 #pragma unroll
-    for (int it = 0; it < kArTileBytes / 16 / kArThreads; it++) {
-        const int e = threadIdx.x + it * kArThreads;
-        const int j = e / S::kChunks, ch = e % S::kChunks;
-        const int idx = idx0 + j;
-        int slot = idx;
-        if (idx >= kr.ns) {
-            slot = lo_slot + (idx - kr.ns);
-            if (slot >= c.cap) slot -= c.ring;
+        for (int r = 0; r < R; r++) {
+            before[r][0] = o[r][0];
+            before[r][1] = o[r][1];
         }
-        const bool ok = idx < end;
-        const long long off = ok ? slot * slot_bytes + ch * 16 : 0;
-        cp_async16(k_s + j * (HD * 4) + ((ch ^ (j & 7)) << 4), kb + off, ok);
-        cp_async16(v_s + j * (HD * 4) + (ch << 4), vb + off, ok);
+    }
+#pragma unroll 4
+    for (int x = 0; x < KEYS / kPvKeys; x++) {
+        const int j = x * kPvKeys + sub;
+        weigh(j, *reinterpret_cast<const ulonglong2 *>(vt + (j * HD + d4) * 4), kAll);
+    }
+    if (!masked) return;
+    bool nan = false;
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+        float a, b, c, d;
+        unpair(o[r][0], a, b);
+        unpair(o[r][1], c, d);
+        nan |= a != a || b != b || c != c || d != d;
+    }
+    if (!__any_sync(0xffffffffu, nan)) return;
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+        o[r][0] = before[r][0];
+        o[r][1] = before[r][1];
+    }
+#pragma unroll 1
+    for (int x = 0; x < KEYS / kPvKeys; x++) {
+        const int j = x * kPvKeys + sub;
+        const uint32_t v0 = __shfl_sync(0xffffffffu, vis[0], j % (KEYS / 2)), v1 = __shfl_sync(0xffffffffu, vis[1], j % (KEYS / 2));
+        weigh(j, *reinterpret_cast<const ulonglong2 *>(vt + (j * HD + d4) * 4), j < KEYS / 2 ? v0 : v1);
     }
 }
 
@@ -201,6 +210,7 @@ __device__ __forceinline__ void merge_store(ArMerge<HD, RB> &mg, Sum sum, Ml ml,
 constexpr int af_warps(int hd, int rb) { return hd == 64 && rb == 8 ? 11 : 12; }   // as shared memory allows
 constexpr int kAfTile = 8192;              // K bytes of a warp's tile
 constexpr float kAfRescale = 8.0f;         // log2 of the largest weight before the maximum moves
+constexpr int kArFewRows = 32;             // up to here tiles of 8 rows, each with its own pass over the keys
 constexpr double kArFixed = 4;             // rounds' worth of a CTA's start and merge
 
 template <int HD, int RB>
@@ -396,40 +406,21 @@ __global__ void __launch_bounds__(AfSmem<HD, RB>::kThreads) attn_rows_few_kernel
             }
         cp_async_wait<1>();   // V is in
         __syncwarp();
-        // keys outside the core: a row skips those that it does not see
-        const bool seen = __all_sync(0xffffffffu, (vis[0] & vis[1]) == (1u << RB) - 1u);
-        if (seen) {
-#pragma unroll 8
-            for (int x = 0; x < Sm::kKeys / kPvKeys; x++) {
-                const int jj = x * kPvKeys + sub;
-                const ulonglong2 v = *reinterpret_cast<const ulonglong2 *>(tl.v + (jj * HD + d4) * 4);
+        auto weigh = [&](int jj, const ulonglong2 &v, uint32_t vj) {
 #pragma unroll
-                for (int r = 0; r < RB; r += 2) {
-                    const ulonglong2 w = *reinterpret_cast<const ulonglong2 *>(&sh.p[warp][jj][r]);
+            for (int r = 0; r < RB; r += 2) {
+                const ulonglong2 w = *reinterpret_cast<const ulonglong2 *>(&sh.p[warp][jj][r]);
+                if ((vj >> r) & 1u) {
                     o[r][0] = fma2(w.x, v.x, o[r][0]);
                     o[r][1] = fma2(w.x, v.y, o[r][1]);
+                }
+                if ((vj >> (r + 1)) & 1u) {
                     o[r + 1][0] = fma2(w.y, v.x, o[r + 1][0]);
                     o[r + 1][1] = fma2(w.y, v.y, o[r + 1][1]);
                 }
             }
-        } else {
-#pragma unroll 1
-            for (int x = 0; x < Sm::kKeys / kPvKeys; x++) {
-                const int jj = x * kPvKeys + sub;
-                const ulonglong2 v = *reinterpret_cast<const ulonglong2 *>(tl.v + (jj * HD + d4) * 4);
-                const uint32_t v0 = __shfl_sync(0xffffffffu, vis[0], jj % Sm::kAtOnce);
-                const uint32_t v1 = __shfl_sync(0xffffffffu, vis[1], jj % Sm::kAtOnce);
-                const uint32_t vj = jj < Sm::kAtOnce ? v0 : v1;
-#pragma unroll
-                for (int r = 0; r < RB; r++) {
-                    const uint64_t w = *reinterpret_cast<const uint64_t *>(&sh.p[warp][jj][r]);
-                    if ((vj >> r) & 1u) {
-                        o[r][0] = fma2(w, v.x, o[r][0]);
-                        o[r][1] = fma2(w, v.y, o[r][1]);
-                    }
-                }
-            }
-        }
+        };
+        add_values<HD, Sm::kKeys, RB>(o, tl.v, vis, sub, d4, weigh);
         __syncwarp();
         fetch(t + step, true);
     }
@@ -485,37 +476,47 @@ __global__ void __launch_bounds__(AfSmem<HD, RB>::kThreads) attn_rows_few_kernel
 }
 
 // ---------------------------------------------------------------------------
-// Many rows: 32 packed rows, 8 per warp.
+// Many rows: 64 packed rows, 8 per warp.
 //
-// Bound by the fp32 pipes: 4 * HD flops per (packed row, key).  Every warp
-// reads all of a tile's keys for its 8 rows: a lane holds one key or more
-// against 8 rows for the scores and 4 dims of 8 rows for P.V, so that a value
-// read from shared memory meets 8 multiply-adds; the probabilities stay
-// within the warp.
+// Bound by the fp32 pipes: 4 * HD flops per (packed row, key).  The 8 warps
+// share a tile of 64 keys, the next one under way: a lane has two keys against
+// its warp's 8 rows for the scores and 4 dims of the 8 rows for P.V, two
+// multiply-adds an instruction, so that shared memory (a K chunk and 8 query
+// chunks for 32 pairs of multiply-adds) and the FMA pipes are about equally
+// busy; the probabilities stay within the warp.
 // ---------------------------------------------------------------------------
 
-constexpr int kArManyRows = 32;
-constexpr int kArWarpRows = kArManyRows / 4;
+constexpr int kArManyRows = 64;
+constexpr int kArManyWarps = 8;
+constexpr int kArManyThreads = kArManyWarps * 32;
+constexpr int kArWarpRows = kArManyRows / kArManyWarps;
+constexpr int kArManyKeys = 64;
 
 template <int HD>
 struct ArManySmem {
-    static constexpr int kKeys = ArShape<HD>::kKeys;
-    static constexpr int kStages = 2;
-    unsigned char kv[kStages][2 * kArTileBytes];
+    static constexpr int kRow = HD * 4 + 16;   // a K row: lanes read one chunk of different keys without conflicts
+    struct Tile {
+        unsigned char k[kArManyKeys * kRow];
+        unsigned char v[kArManyKeys * HD * 4];
+    };
+    union {
+        Tile tile[2];
+        float sums[kArManyRows][HD];           // at the end
+    };
     float q[kArManyRows * HD];
-    float p[4][kKeys][kArWarpRows];
+    float p[kArManyWarps][kArManyKeys][kArWarpRows];
     float mx[kArManyRows], sum[kArManyRows];
-    ArMerge<HD, kArManyRows> merge;
     ArRows<kArManyRows> rows;
 };
 
 template <int HD>
-__global__ void __launch_bounds__(kArThreads) attn_rows_many_kernel(const RowsAttnParams p) {
-    using S = ArShape<HD>;
+__global__ void __launch_bounds__(kArManyThreads) attn_rows_many_kernel(const RowsAttnParams p) {
     using Sm = ArManySmem<HD>;
-    constexpr int RB = kArManyRows, WR = kArWarpRows;
+    constexpr int RB = kArManyRows, WR = kArWarpRows, kKeys = kArManyKeys;
+    static_assert(sizeof(Sm) + sizeof(ArMerge<HD, RB>) <= 227 * 1024, "fits an SM");
     extern __shared__ __align__(128) unsigned char smem_raw[];
     Sm &sh = *reinterpret_cast<Sm *>(smem_raw);
+    ArMerge<HD, RB> &merge = *reinterpret_cast<ArMerge<HD, RB> *>(smem_raw + sizeof(Sm));
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int z = blockIdx.x % p.shares, Z = p.shares;
     const int m0 = blockIdx.x / p.shares * RB, kvh = blockIdx.y, stream = blockIdx.z;
@@ -526,152 +527,191 @@ __global__ void __launch_bounds__(kArThreads) attn_rows_many_kernel(const RowsAt
     const int i0 = m0 / p.group, i1 = (min(m0 + RB, M) - 1) / p.group + 1;
     const KeyRange kr = key_range(p.c, s, i0, i1, p.window, tree);
     const int lo_slot = cache_slot(p.c, kr.lo);
-    const int total = kr.total(), tiles = (total + S::kKeys - 1) / S::kKeys;
+    const int total = kr.total(), tiles = (total + kKeys - 1) / kKeys;
     const int t0 = (int)((long long)z * tiles / Z), t1 = (int)((long long)(z + 1) * tiles / Z);
     const long long base = p.layer_off + (long long)stream * p.c.stream_stride + (long long)kvh * p.c.head_stride;
     const char *kb = p.c.k + base * 4, *vb = p.c.v + base * 4;
     const long long slot_bytes = p.c.slot_stride * 4;
     const int head0 = kvh * p.group;
 
+    constexpr int kCh = HD / 4, kRowsAtOnce = kArManyThreads / kCh, kIts = kKeys / kRowsAtOnce;
+    const int ch = threadIdx.x % kCh, jr = threadIdx.x / kCh;
+    auto fetch = [&](int t, int buf) {
+        const int idx0 = t * kKeys;
+        const uint32_t kd = smem_u32(sh.tile[buf].k) + jr * Sm::kRow + ch * 16;
+        const uint32_t vd = smem_u32(sh.tile[buf].v) + jr * (HD * 4) + ch * 16;
+        int slot0 = lo_slot + (idx0 - kr.ns);   // of index idx0, past the sinks
+        if (slot0 >= p.c.cap) slot0 -= p.c.ring;
+        if (idx0 >= kr.ns && idx0 + kKeys <= total && slot0 + kKeys <= p.c.cap) {
+            long long off = (slot0 + jr) * slot_bytes + ch * 16;
+#pragma unroll
+            for (int it = 0; it < kIts; it++, off += kRowsAtOnce * slot_bytes) {
+                cp_async16(kd + it * kRowsAtOnce * Sm::kRow, kb + off, true);
+                cp_async16(vd + it * kRowsAtOnce * (HD * 4), vb + off, true);
+            }
+        } else {
+#pragma unroll 1
+            for (int it = 0; it < kIts; it++) {
+                const int idx = idx0 + it * kRowsAtOnce + jr;
+                int slot = idx;
+                if (idx >= kr.ns) {
+                    slot = lo_slot + (idx - kr.ns);
+                    if (slot >= p.c.cap) slot -= p.c.ring;
+                }
+                const bool ok = idx < total;
+                const long long off = ok ? slot * slot_bytes + ch * 16 : 0;
+                cp_async16(kd + it * kRowsAtOnce * Sm::kRow, kb + off, ok);
+                cp_async16(vd + it * kRowsAtOnce * (HD * 4), vb + off, ok);
+            }
+        }
+    };
     peers_arrive(Z);
-    if (t0 < t1) load_tile<HD>(sh.kv[0], kb, vb, slot_bytes, kr, lo_slot, p.c, t0 * S::kKeys, total);
+    if (t0 < t1) fetch(t0, 0);
     cp_async_commit();
     load_queries<HD, RB>(sh.q, HD, 1, p, s, head0, m0, M);
     setup_rows<RB>(sh.rows, p, s, m0, M);
 
-    float m_run[WR], l_run[WR];   // l: this lane's keys only
-    float4 o[WR];
+    const int up_min = tree ? s.pos - 1 : s.pos + i0;
+    int core_s = kr.ns + (p.window > 0 ? max(0, min(s.pos + i1 - p.window - kr.lo, kr.nm)) : 0);
+    int core_e = kr.ns + max(0, min(up_min - kr.lo + 1, kr.nm));
+    if (up_min < kr.ns - 1) core_e = 0;
+    else if (core_s == kr.ns) core_s = 0;
+
+    constexpr int kLanesPerKey = HD / 4, kPvKeys = 32 / kLanesPerKey;
+    const int sub = lane / kLanesPerKey, d4 = lane % kLanesPerKey * 4;
+    float mr[WR], l[WR];   // l: this lane's keys only
+    uint64_t o[WR][2];     // pairs of dims
 #pragma unroll
     for (int r = 0; r < WR; r++) {
-        m_run[r] = -INFINITY;
-        l_run[r] = 0.f;
-        o[r] = make_float4(0.f, 0.f, 0.f, 0.f);
+        mr[r] = -INFINITY;
+        l[r] = 0.f;
+        o[r][0] = o[r][1] = 0;
     }
     const float *qw = sh.q + warp * WR * HD;
     const bool idle = m0 + warp * WR >= M;   // none of the warp's rows exist
 
     for (int t = t0; t < t1; t++) {
-        const int st = (t - t0) % Sm::kStages;
+        const int buf = (t - t0) & 1;
         cp_async_wait<0>();
         __syncthreads();   // tile t is in; every warp is done with tile t - 1
-        if (t + 1 < t1)
-            load_tile<HD>(sh.kv[st ^ 1], kb, vb, slot_bytes, kr, lo_slot, p.c, (t + 1) * S::kKeys, total);
+        if (t + 1 < t1) fetch(t + 1, buf ^ 1);
         cp_async_commit();
         if (idle) continue;
+        const typename Sm::Tile &tl = sh.tile[buf];
 
-        float acc[WR][S::kPerLane];
+        uint64_t a2[2][WR];
 #pragma unroll
-        for (int r = 0; r < WR; r++)
-#pragma unroll
-            for (int x = 0; x < S::kPerLane; x++) acc[r][x] = 0.f;
-#pragma unroll 2
-        for (int ch = 0; ch < S::kChunks; ch++) {
-            float4 k[S::kPerLane];
-#pragma unroll
-            for (int x = 0; x < S::kPerLane; x++) {
-                const int j = lane + 32 * x;
-                k[x] = *reinterpret_cast<const float4 *>(sh.kv[st] + j * (HD * 4) + ((ch ^ (j & 7)) << 4));
-            }
+        for (int r = 0; r < WR; r++) a2[0][r] = a2[1][r] = 0;
+#pragma unroll 4
+        for (int c = 0; c < HD / 4; c++) {
+            const ulonglong2 k0 = *reinterpret_cast<const ulonglong2 *>(tl.k + lane * Sm::kRow + c * 16);
+            const ulonglong2 k1 = *reinterpret_cast<const ulonglong2 *>(tl.k + (lane + 32) * Sm::kRow + c * 16);
 #pragma unroll
             for (int r = 0; r < WR; r++) {
-                const float4 qv = *reinterpret_cast<const float4 *>(qw + r * HD + ch * 4);
+                const ulonglong2 q = *reinterpret_cast<const ulonglong2 *>(qw + r * HD + c * 4);
+                a2[0][r] = fma2(q.x, k0.x, a2[0][r]);
+                a2[1][r] = fma2(q.x, k1.x, a2[1][r]);
+                a2[0][r] = fma2(q.y, k0.y, a2[0][r]);
+                a2[1][r] = fma2(q.y, k1.y, a2[1][r]);
+            }
+        }
+        float acc[2][WR];
 #pragma unroll
-                for (int x = 0; x < S::kPerLane; x++) {
-                    acc[r][x] = fmaf(qv.x, k[x].x, acc[r][x]);
-                    acc[r][x] = fmaf(qv.y, k[x].y, acc[r][x]);
-                    acc[r][x] = fmaf(qv.z, k[x].z, acc[r][x]);
-                    acc[r][x] = fmaf(qv.w, k[x].w, acc[r][x]);
+        for (int x = 0; x < 2; x++)
+#pragma unroll
+            for (int r = 0; r < WR; r++) {
+                float a, b;
+                unpair(a2[x][r], a, b);
+                acc[x][r] = a + b;
+            }
+        uint32_t vis[2] = {(1u << WR) - 1u, (1u << WR) - 1u};
+        if (!(t * kKeys >= core_s && (t + 1) * kKeys <= core_e)) {
+#pragma unroll
+            for (int x = 0; x < 2; x++) {
+                const int idx = t * kKeys + lane + 32 * x, at = kr.position(idx);
+                vis[x] = 0;
+                if (idx < total)
+#pragma unroll
+                    for (int r = 0; r < WR; r++)
+                        if (row_sees<RB>(sh.rows, warp * WR + r, at, s.pos, p.c.n_sink, tree)) vis[x] |= 1u << r;
+#pragma unroll
+                for (int r = 0; r < WR; r++)
+                    if (!((vis[x] >> r) & 1u)) acc[x][r] = -INFINITY;
+            }
+        }
+        bool move = false;
+#pragma unroll
+        for (int r = 0; r < WR; r++) {
+            const float a = fmaxf(acc[0][r], acc[1][r]);
+            move |= mr[r] == -INFINITY ? a > -INFINITY : a > mr[r] + kAfRescale;
+        }
+        if (__any_sync(0xffffffffu, move)) {
+#pragma unroll
+            for (int r = 0; r < WR; r++) {
+                float mt = fmaxf(acc[0][r], acc[1][r]);
+#pragma unroll
+                for (int d = 16; d > 0; d >>= 1) mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, d));
+                if (mt > mr[r]) {
+                    const float al = mr[r] == -INFINITY ? 0.f : exp2_approx(mr[r] - mt);
+                    mr[r] = mt;
+                    l[r] *= al;
+                    o[r][0] = mul2(o[r][0], pair(al, al));
+                    o[r][1] = mul2(o[r][1], pair(al, al));
                 }
             }
         }
-
-        bool any_masked = false;
 #pragma unroll
         for (int r = 0; r < WR; r++) {
-            bool vis[S::kPerLane];
-            float mt = -INFINITY;
-#pragma unroll
-            for (int x = 0; x < S::kPerLane; x++) {
-                const int idx = t * S::kKeys + lane + 32 * x;
-                vis[x] = idx < total &&
-                         row_sees<RB>(sh.rows, warp * WR + r, kr.position(idx), s.pos, p.c.n_sink, tree);
-                any_masked |= !vis[x];
-                if (vis[x]) mt = fmaxf(mt, acc[r][x]);
-            }
-#pragma unroll
-            for (int d = 16; d > 0; d >>= 1) mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, d));
-            const float mn = fmaxf(m_run[r], mt);
-            const float b = mn == -INFINITY ? 0.f : mn;
-            const float al = m_run[r] == -INFINITY ? 0.f : exp2_approx(m_run[r] - b);
-            m_run[r] = mn;
-            float ls = 0.f;
-#pragma unroll
-            for (int x = 0; x < S::kPerLane; x++) {
-                const float pv = exp2_approx(acc[r][x] - b);
-                if (vis[x]) ls += pv;
-                acc[r][x] = vis[x] ? pv : -1.f;
-            }
-            l_run[r] = l_run[r] * al + ls;
-            o[r].x *= al;
-            o[r].y *= al;
-            o[r].z *= al;
-            o[r].w *= al;
+            const float b = mr[r] == -INFINITY ? 0.f : mr[r];
+            acc[0][r] = exp2_approx(acc[0][r] - b);   // (0 for a masked key)
+            acc[1][r] = exp2_approx(acc[1][r] - b);
+            l[r] += acc[0][r] + acc[1][r];
         }
-        any_masked = __any_sync(0xffffffffu, any_masked);
 #pragma unroll
-        for (int x = 0; x < S::kPerLane; x++)
+        for (int x = 0; x < 2; x++)
 #pragma unroll
             for (int r = 0; r < WR; r += 4)
                 *reinterpret_cast<float4 *>(&sh.p[warp][lane + 32 * x][r]) =
-                    make_float4(acc[r][x], acc[r + 1][x], acc[r + 2][x], acc[r + 3][x]);
+                    make_float4(acc[x][r], acc[x][r + 1], acc[x][r + 2], acc[x][r + 3]);
         __syncwarp();
-
-        const unsigned char *vt = sh.kv[st] + kArTileBytes;
-        const int sub = lane / S::kLanesPerKey, d4 = lane % S::kLanesPerKey * 4;
-#pragma unroll 4
-        for (int x = 0; x < S::kKeys / S::kKeysAtOnce; x++) {
-            const int j = x * S::kKeysAtOnce + sub;
-            const float4 v = *reinterpret_cast<const float4 *>(vt + (j * HD + d4) * 4);
-            float pr[WR];
+        auto weigh = [&](int jj, const ulonglong2 &v, uint32_t vj) {
+            float w[WR];
 #pragma unroll
             for (int r = 0; r < WR; r += 4)
-                *reinterpret_cast<float4 *>(pr + r) = *reinterpret_cast<const float4 *>(&sh.p[warp][j][r]);
+                *reinterpret_cast<float4 *>(w + r) = *reinterpret_cast<const float4 *>(&sh.p[warp][jj][r]);
 #pragma unroll
-            for (int r = 0; r < WR; r++) {
-                if (any_masked && pr[r] < 0.f) continue;
-                o[r].x = fmaf(pr[r], v.x, o[r].x);
-                o[r].y = fmaf(pr[r], v.y, o[r].y);
-                o[r].z = fmaf(pr[r], v.z, o[r].z);
-                o[r].w = fmaf(pr[r], v.w, o[r].w);
-            }
-        }
+            for (int r = 0; r < WR; r++)
+                if ((vj >> r) & 1u) {
+                    o[r][0] = fma2(pair(w[r], w[r]), v.x, o[r][0]);
+                    o[r][1] = fma2(pair(w[r], w[r]), v.y, o[r][1]);
+                }
+        };
+        add_values<HD, kKeys, WR>(o, tl.v, vis, sub, d4, weigh);
         __syncwarp();
     }
     cp_async_wait<0>();
     __syncthreads();   // the tiles are done with: their memory takes the sums
-
-    float *of = reinterpret_cast<float *>(sh.kv[0]);   // [RB][HD]
-    static_assert(RB * HD * 4 <= 2 * kArTileBytes, "the sums fit a stage");
-    const int sub = lane / S::kLanesPerKey, d4 = lane % S::kLanesPerKey * 4;
 #pragma unroll
     for (int r = 0; r < WR; r++) {
-        float4 v = o[r];
-        if (S::kKeysAtOnce == 2) {
+        float4 v;
+        unpair(o[r][0], v.x, v.y);
+        unpair(o[r][1], v.z, v.w);
+        if (kPvKeys == 2) {
             v.x += __shfl_xor_sync(0xffffffffu, v.x, 16);
             v.y += __shfl_xor_sync(0xffffffffu, v.y, 16);
             v.z += __shfl_xor_sync(0xffffffffu, v.z, 16);
             v.w += __shfl_xor_sync(0xffffffffu, v.w, 16);
         }
-        const float l = warp_sum(l_run[r]);
-        if (sub == 0) *reinterpret_cast<float4 *>(of + (warp * WR + r) * HD + d4) = v;
+        const float lt = warp_sum(l[r]);
+        if (sub == 0) *reinterpret_cast<float4 *>(&sh.sums[warp * WR + r][d4]) = v;
         if (lane == 0) {
-            sh.mx[warp * WR + r] = m_run[r];
-            sh.sum[warp * WR + r] = l;
+            sh.mx[warp * WR + r] = mr[r];
+            sh.sum[warp * WR + r] = lt;
         }
     }
     __syncthreads();
-    merge_store<HD, RB, kArThreads>(
-        sh.merge, [&](int r, int d) { return *reinterpret_cast<const float4 *>(of + r * HD + d); },
+    merge_store<HD, RB, kArManyThreads>(
+        merge, [&](int r, int d) { return *reinterpret_cast<const float4 *>(&sh.sums[r][d]); },
         [&](int r) { return make_float2(sh.mx[r], sh.sum[r]); }, p, s, head0, m0, M, z, Z);
 }
 
@@ -705,14 +745,15 @@ cudaError_t launch_dim(const RowsAttnParams &p, cudaStream_t st) {
                                                       threads, smem, pp.shares, &a, st);
         return cudaLaunchKernelEx(&cfg, kernel, pp);
     };
-    static ClusterKernel d4, d8, d32;
+    static ClusterKernel d4, d8, d64;
     auto few = [&](auto kernel, auto *sm, ClusterKernel &ck) {
         using Sm = std::remove_pointer_t<decltype(sm)>;
         return go(kernel, sizeof(Sm), Sm::kThreads, Sm::kRows, Sm::kKeys * Sm::kWarps, ck);
     };
     if (M <= 4) return few(attn_rows_few_kernel<HD, 4>, (AfSmem<HD, 4> *)nullptr, d4);
-    if (M <= kArManyRows) return few(attn_rows_few_kernel<HD, 8>, (AfSmem<HD, 8> *)nullptr, d8);
-    return go(attn_rows_many_kernel<HD>, sizeof(ArManySmem<HD>), kArThreads, kArManyRows, ArShape<HD>::kKeys, d32);
+    if (M <= kArFewRows) return few(attn_rows_few_kernel<HD, 8>, (AfSmem<HD, 8> *)nullptr, d8);
+    return go(attn_rows_many_kernel<HD>, sizeof(ArManySmem<HD>) + sizeof(ArMerge<HD, kArManyRows>), kArManyThreads, kArManyRows,
+              kArManyKeys, d64);
 }
 
 }  // namespace
