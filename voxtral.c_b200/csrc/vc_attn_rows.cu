@@ -207,15 +207,17 @@ __device__ __forceinline__ void merge_store(ArMerge<HD, RB> &mg, Sum sum, Ml ml,
 // dims of every row.
 // ---------------------------------------------------------------------------
 
-constexpr int af_warps(int hd, int rb) { return hd == 64 && rb == 8 ? 11 : 12; }   // as shared memory allows
+// Warps of a CTA: one CTA fills an SM's shared memory, or (small) four do, for
+// tiles of few keys.
+constexpr int af_warps(int hd, int rb, bool small) { return small ? (rb == 8 ? 2 : 3) : hd == 64 && rb == 8 ? 11 : 12; }
 constexpr int kAfTile = 8192;              // K bytes of a warp's tile
 constexpr float kAfRescale = 8.0f;         // log2 of the largest weight before the maximum moves
 constexpr int kArFewRows = 32;             // up to here tiles of 8 rows, each with its own pass over the keys
 constexpr double kArFixed = 4;             // rounds' worth of a CTA's start and merge
 
-template <int HD, int RB>
+template <int HD, int RB, bool SMALL>
 struct AfSmem {
-    static constexpr int kWarps = af_warps(HD, RB), kThreads = kWarps * 32, kRows = RB;
+    static constexpr int kWarps = af_warps(HD, RB, SMALL), kThreads = kWarps * 32;
     static constexpr int kKeys = kAfTile / (HD * 4);       // keys of a tile: 16 or 32
     static constexpr int kRow = HD * 4 + 16;               // a K row in shared memory
     static constexpr int kParts = HD / 32;                 // lanes that share a key: 4 or 2
@@ -237,9 +239,9 @@ struct AfSmem {
     ArRows<RB> rows;
 };
 
-template <int HD, int RB>
-__global__ void __launch_bounds__(AfSmem<HD, RB>::kThreads) attn_rows_few_kernel(const RowsAttnParams p) {
-    using Sm = AfSmem<HD, RB>;
+template <int HD, int RB, bool SMALL>
+__global__ void __launch_bounds__(AfSmem<HD, RB, SMALL>::kThreads) attn_rows_few_kernel(const RowsAttnParams p) {
+    using Sm = AfSmem<HD, RB, SMALL>;
     constexpr int kAfWarps = Sm::kWarps, kAfThreads = Sm::kThreads;
     static_assert(sizeof(Sm) <= 227 * 1024, "fits an SM");
     extern __shared__ __align__(128) unsigned char smem_raw[];
@@ -445,6 +447,7 @@ __global__ void __launch_bounds__(AfSmem<HD, RB>::kThreads) attn_rows_few_kernel
         }
     }
     __syncthreads();
+    static_assert(kAfWarps * RB <= kAfThreads, "a thread per (warp, row)");
     if (threadIdx.x < kAfWarps * RB) {   // the warps' weights; a warp that saw no key of a row has sums of 0
         const int w = threadIdx.x / RB, r = threadIdx.x % RB;
         float gm = -INFINITY;
@@ -715,45 +718,72 @@ __global__ void __launch_bounds__(kArManyThreads) attn_rows_many_kernel(const Ro
         [&](int r) { return make_float2(sh.mx[r], sh.sum[r]); }, p, s, head0, m0, M, z, Z);
 }
 
+// How one kernel would run a call: its cluster size and what that costs.
+struct Plan {
+    double cost = 1e30;
+    int shares = 0;
+};
+
+// rb: packed rows of a tile, round: keys that a CTA takes at once.  Key shares
+// of a tile, each a CTA of its cluster: the fewest rounds until the last wave of
+// clusters is done, with kArFixed for a CTA's start and merge.
+template <typename K>
+cudaError_t plan(ClusterKernel &ck, K kernel, size_t smem, int threads, int rb, int round, const RowsAttnParams &p, Plan *out) {
+    int dev = 0;
+    cudaError_t e = cluster_prepare(ck, kernel, smem, &dev);
+    if (e != cudaSuccess) return e;
+    const long long M = (long long)p.r.max_rows * p.group, tiles = (M + rb - 1) / rb;
+    const long long clusters = tiles * p.c.n_kv_heads * p.c.n_streams;
+    const double rounds = (double)most_keys(p, rb) / round;
+    for (int Z = 1; Z <= kMaxCluster && Z < rounds + 1; Z++) {
+        const int at_once = cluster_active(ck, kernel, dev, threads, smem, Z);
+        if (at_once < 1) continue;
+        const double t = (double)((clusters + at_once - 1) / at_once) * (std::max(1.0, rounds / Z) + kArFixed);
+        if (t < out->cost) {
+            out->cost = t;
+            out->shares = Z;
+        }
+    }
+    return out->shares ? cudaSuccess : cudaErrorInvalidConfiguration;
+}
+
+template <typename K>
+cudaError_t launch(K kernel, size_t smem, int threads, int rb, int shares, RowsAttnParams p, cudaStream_t st) {
+    const long long M = (long long)p.r.max_rows * p.group, tiles = (M + rb - 1) / rb;
+    p.shares = shares;
+    cudaLaunchAttribute a;
+    const cudaLaunchConfig_t cfg = cluster_config(dim3((unsigned)(shares * tiles), p.c.n_kv_heads, p.c.n_streams), threads, smem,
+                                                  shares, &a, st);
+    return cudaLaunchKernelEx(&cfg, kernel, p);
+}
+
+template <int HD, int RB>
+cudaError_t launch_few(const RowsAttnParams &p, cudaStream_t st) {
+    using Large = AfSmem<HD, RB, false>;
+    using Small = AfSmem<HD, RB, true>;
+    static ClusterKernel cl, cs;
+    Plan a, b;
+    cudaError_t e = plan(cl, attn_rows_few_kernel<HD, RB, false>, sizeof(Large), Large::kThreads, RB, Large::kKeys * Large::kWarps,
+                         p, &a);
+    if (e == cudaSuccess)
+        e = plan(cs, attn_rows_few_kernel<HD, RB, true>, sizeof(Small), Small::kThreads, RB, Small::kKeys * Small::kWarps, p, &b);
+    if (e != cudaSuccess) return e;
+    return b.cost < a.cost
+               ? launch(attn_rows_few_kernel<HD, RB, true>, sizeof(Small), Small::kThreads, RB, b.shares, p, st)
+               : launch(attn_rows_few_kernel<HD, RB, false>, sizeof(Large), Large::kThreads, RB, a.shares, p, st);
+}
+
 template <int HD>
 cudaError_t launch_dim(const RowsAttnParams &p, cudaStream_t st) {
     const long long M = (long long)p.r.max_rows * p.group;
-    // rb: packed rows of a tile, round: keys that a CTA takes at once
-    auto go = [&](auto kernel, size_t smem, int threads, int rb, int round, ClusterKernel &ck) {
-        int dev = 0;
-        cudaError_t e = cluster_prepare(ck, kernel, smem, &dev);
-        if (e != cudaSuccess) return e;
-        const long long tiles = (M + rb - 1) / rb, clusters = tiles * p.c.n_kv_heads * p.c.n_streams;
-        const double rounds = (double)most_keys(p, rb) / round;
-        // Key shares of a tile, each a CTA of its cluster: the fewest rounds
-        // until the last wave of clusters is done, with kArFixed for a CTA's
-        // start and merge.
-        RowsAttnParams pp = p;
-        pp.shares = 1;
-        double best = 1e30;
-        for (int Z = 1; Z <= kMaxCluster && Z < rounds + 1; Z++) {
-            const int at_once = cluster_active(ck, kernel, dev, threads, smem, Z);
-            if (at_once < 1) continue;
-            const double t = (double)((clusters + at_once - 1) / at_once) * (std::max(1.0, rounds / Z) + kArFixed);
-            if (t < best) {
-                best = t;
-                pp.shares = Z;
-            }
-        }
-        cudaLaunchAttribute a;
-        const cudaLaunchConfig_t cfg = cluster_config(dim3((unsigned)(pp.shares * tiles), p.c.n_kv_heads, p.c.n_streams),
-                                                      threads, smem, pp.shares, &a, st);
-        return cudaLaunchKernelEx(&cfg, kernel, pp);
-    };
-    static ClusterKernel d4, d8, d64;
-    auto few = [&](auto kernel, auto *sm, ClusterKernel &ck) {
-        using Sm = std::remove_pointer_t<decltype(sm)>;
-        return go(kernel, sizeof(Sm), Sm::kThreads, Sm::kRows, Sm::kKeys * Sm::kWarps, ck);
-    };
-    if (M <= 4) return few(attn_rows_few_kernel<HD, 4>, (AfSmem<HD, 4> *)nullptr, d4);
-    if (M <= kArFewRows) return few(attn_rows_few_kernel<HD, 8>, (AfSmem<HD, 8> *)nullptr, d8);
-    return go(attn_rows_many_kernel<HD>, sizeof(ArManySmem<HD>) + sizeof(ArMerge<HD, kArManyRows>), kArManyThreads, kArManyRows,
-              kArManyKeys, d64);
+    if (M <= 4) return launch_few<HD, 4>(p, st);
+    if (M <= kArFewRows) return launch_few<HD, 8>(p, st);
+    constexpr size_t kSmem = sizeof(ArManySmem<HD>) + sizeof(ArMerge<HD, kArManyRows>);
+    static ClusterKernel ck;
+    Plan a;
+    const cudaError_t e = plan(ck, attn_rows_many_kernel<HD>, kSmem, kArManyThreads, kArManyRows, kArManyKeys, p, &a);
+    if (e != cudaSuccess) return e;
+    return launch(attn_rows_many_kernel<HD>, kSmem, kArManyThreads, kArManyRows, a.shares, p, st);
 }
 
 }  // namespace
