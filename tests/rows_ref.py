@@ -121,11 +121,12 @@ class Case:
     def check(self, out, lse, scale=0.0, rounded_p=False):
         """Compares with the definition.  With u = 2^-24 and S the largest sum
         of |q||k| * scale of a row, a score is off by at most (dim + 4) u S
-        (its products and sums, the scaled q), its exponential by as much and
-        the 2 ulp of ex2, so a weight is off by d = (dim + 8) u S + 2^-22
-        relative; an output by 2 d max|v| (numerator and denominator), the
-        sums' N u max|v|, half a step of a 16-bit weight where weights are
-        rounded, and half a step of its own type."""
+        (its products and sums, the scaled q), its exponential by as much, the
+        2 ulp of ex2 and, where weights are rounded to 16 bits, the 2.7e-6 <
+        2^-18 of a polynomial of degree 4 for 2^x.  So a weight is off by
+        d = (dim + 8) u S + 2^-22 (+ 2^-18) relative; an output by 2 d max|v|
+        (numerator and denominator), the sums' N u max|v|, half a step of a
+        16-bit weight, and half a step of its own type."""
         out, lse = out.double().cpu(), lse.double().cpu()
         scale = scale or 1.0 / math.sqrt(self.dim)
         group = self.heads // self.kv_heads
@@ -138,7 +139,7 @@ class Case:
                     k = self.k[self.layer, s, at, h // group].double()
                     v = self.v[self.layer, s, at, h // group].double()
                     o, z, big = attention(self.q[row, h].double(), k, v, keys, scale)
-                    d = (self.dim + 8) * U32 * big + 2.0 ** -22
+                    d = (self.dim + 8) * U32 * big + 2.0 ** -22 + (2.0 ** -18 if rounded_p else 0.0)
                     most = float(v.abs().max()) if keys else 0.0
                     tol = (2 * d + len(keys) * U32 + (u if rounded_p else 0.0)) * most + u * o.abs() + 1e-30
                     err = (out[row, h] - o).abs()

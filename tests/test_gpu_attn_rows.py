@@ -138,6 +138,57 @@ def test_rows_without_weight(dtype, rows):
     assert bool((out == 0).all()) and bool((lse == -math.inf).all())
 
 
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("heads", [(8, 2, 128), (8, 8, 64), (7, 1, 64), (20, 1, 128)])
+@pytest.mark.parametrize("rows,tree", [(1, None), (9, None), (9, 3), (30, None)])
+def test_long_contexts(dtype, heads, rows, tree):
+    # few tiles, many keys: every kernel's shares and their merge
+    go(Case(dtype, *heads, cap=2500, n_sink=3, positions=[7000], counts=[rows], window=2400, seed=20, tree=tree))
+
+
+def test_the_first_call_may_be_captured():
+    """Every operator's first call in a process, inside a capture."""
+    import os
+    import subprocess
+    import sys
+    code = """
+import sys, torch
+sys.path[:0] = ["tests", "voxtral.c_b200"]
+import voxcuda as V
+from rows_ref import Case
+V.init()
+cases = [Case(d, *h, cap=90, n_sink=1, positions=[40, 60], counts=n, window=0, seed=1, tree=t)
+         for d in ("fp32", "bf16") for h in ((8, 2, 64), (8, 2, 128)) for n in ([1, 1], [3, 9], [30, 20], [64, 70]) for t in (None, 3)]
+x = torch.randn(3, 5000, device="cuda")
+tok, lp = torch.zeros(3, dtype=torch.int32, device="cuda"), torch.empty(3, device="cuda")
+outs = [(torch.empty_like(c.dq), torch.empty(c.dq.shape[:2], device="cuda")) for c in cases]
+k = torch.randn(2, 3, 20, 2, 64, device="cuda")
+kv = V.KvCache(k.data_ptr(), k.clone().data_ptr(), "fp32", 2, 3, 20, 2, 64)
+pos, path = torch.full((3,), 5, dtype=torch.int32, device="cuda"), torch.ones(3, 1, dtype=torch.int32, device="cuda")
+qkv, q = torch.randn(3, 8, 64, device="cuda"), torch.empty(3, 4, 64, device="cuda")
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    st = torch.cuda.current_stream().cuda_stream
+    V.token_logprobs_dev(x.data_ptr(), "fp32", 3, 5000, 0, tok.data_ptr(), 0, lp.data_ptr(), None, None, None, st)
+    V.rope_append_dev(kv, 0, V.Rows(pos.data_ptr(), n_rows=3), qkv.data_ptr(), "fp32", 4, 0, None, None, 0.0, 1e4, q.data_ptr(), st)
+    V.kv_commit_dev(kv, pos.data_ptr(), path.data_ptr(), 1, path.data_ptr(), 1, None, st)
+    V.kv_fork_dev(kv, [0], [1], pos.data_ptr(), st)
+    for c, (o, l) in zip(cases, outs):
+        call = V.attention_window_dev if c.dparent is None else V.attention_tree_dev
+        call(c.cache(V), 0, c.rows(V), c.dq.data_ptr(), c.heads, 0, 0.0, o.data_ptr(), l.data_ptr(), st)
+g.replay()
+torch.cuda.synchronize()
+for c, (o, l) in zip(cases, outs):
+    c.check(o, l, rounded_p=c.dtype != "fp32")
+assert abs(float(lp[0]) - float(torch.log_softmax(x[0].double(), 0)[0])) < 1e-4
+print("captured")
+"""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "captured" in r.stdout, r.stderr[-2000:]
+
+
 def test_device_arrays_are_clamped():
     """Row ranges beyond the buffers and parents out of order fault nothing:
     ranges are cut, such parents count as none."""
