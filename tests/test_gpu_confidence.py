@@ -118,6 +118,20 @@ def test_masked_and_lowest_logits(dtype):
     check(x, tok, 20, dtype, run(x, tok, 20, dtype))
 
 
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("n", [4, 300])
+def test_the_largest_logits(dtype, n):
+    x, tok = rows(n, 5003, dtype, seed=5)
+    most = torch.finfo(x.dtype).max
+    x[0, 77] = most                             # distances of 3e38
+    x[1, ::3] = most
+    x[2] = most / 2
+    x[3, 1::2] = torch.finfo(x.dtype).min
+    x[3, ::2] = most
+    tok[3] = 5002
+    check(x, tok, 5, dtype, run(x, tok, 5, dtype))
+
+
 @pytest.mark.parametrize("dtype", ["fp32", "bf16"])
 def test_rows_without_a_distribution(dtype):
     x, tok = rows(6, 9000, dtype, seed=4)

@@ -487,9 +487,10 @@ __global__ void __launch_bounds__(NTH, 1024 / NTH) token_logprobs_kernel(const L
         gt = sh.stat[3];
         gb = sh.stat[4];
     }
-    if (gb <= lowest && gb > -INFINITY) {
-        // every logit is as low as a mask's: the sums above took the vectors'
-        // padding along, so once more, value by value
+    if ((gb <= lowest || gb > 1e38f) && fabsf(gb) < INFINITY) {
+        // every logit is as low as a mask's, and the sums above took the
+        // vectors' padding along; or distances overflow, and 0 times an
+        // infinite one is NaN: once more, value by value
         gn = gr = gt = 0.f;
         for (int i = threadIdx.x; i < p.vocab; i += NTH) {
             const float d = ((float)x.x[i] - gb) * kLog2e, e = exp2_approx(d);
