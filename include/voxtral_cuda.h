@@ -541,7 +541,9 @@ int vox_cuda_rope_dev(float *x, int n_heads, int head_dim, int pos, const float 
  * each other, and a call may be captured into a CUDA graph and replayed (the
  * positions, row ranges and trees are read on the device).  They run on the
  * calling thread's device (vox_cuda_set_device), whichever device is current;
- * all pointers belong to it.  Results do not depend on timing.
+ * all pointers belong to it.  Results do not depend on timing.  The kernels'
+ * waits are bounded: if one runs out, the call's outputs are void, and the
+ * next attention call that is made says so (VOX_CUDA_ERR_CUDA), once.
  * ------------------------------------------------------------------------ */
 
 #define VOX_CUDA_F32  0

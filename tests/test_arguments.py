@@ -86,7 +86,7 @@ def test_what_a_ring_or_a_tree_cannot_hold():
 
 @pytest.mark.parametrize("bad", [
     dict(layer=2), dict(layer=-1), dict(q=None), dict(q=A + 8), dict(out=None), dict(out=A + 8), dict(heads=0), dict(heads=7),
-    dict(heads=130), dict(window=-1), dict(scale=float("nan")), dict(scale=float("inf"))])
+    dict(heads=130), dict(window=-1), dict(scale=float("nan")), dict(scale=float("inf")), dict(scale=3e38)])
 def test_attention_arguments(bad):
     assert attend(**bad) == V.ERR_ARG
     assert attend(r=rows(parent=A), tree=True, **bad) == V.ERR_ARG

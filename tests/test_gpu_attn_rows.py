@@ -146,6 +146,43 @@ def test_long_contexts(dtype, heads, rows, tree):
     go(Case(dtype, *heads, cap=2500, n_sink=3, positions=[7000], counts=[rows], window=2400, seed=20, tree=tree))
 
 
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("rows,tree", [(1, None), (20, None), (20, 3), (100, None)])
+@pytest.mark.parametrize("n_sink", [0, 100])
+def test_the_largest_windows_are_no_limit(dtype, rows, tree, n_sink):
+    import torch
+
+    def run(window):
+        c = Case(dtype, 8, 4, 64, cap=300, n_sink=n_sink, positions=[3, 700], counts=[rows, rows], window=window, seed=21, tree=tree)
+        got = c.run(V)
+        torch.cuda.synchronize()
+        return got
+    want = run(0)
+    for window in (300 - n_sink, 2 ** 31 - 1):
+        for a, b in zip(run(window), want):
+            assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("kinds", [("bf16", "bf16"), ("bf16", "fp32"), ("fp32", "fp16")])
+def test_two_streams_at_once(kinds):
+    """Calls under way on two streams: each as by itself, again and again."""
+    import torch
+    cases = [Case(d, 8, 2, 128, cap=900, n_sink=0, positions=[800] * 4, counts=[n] * 4, window=0, seed=22 + i)
+             for i, (d, n) in enumerate(zip(kinds, (70, 9)))]
+    want = [c.run(V) for c in cases]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    outs = [[(torch.full_like(c.dq, 7.0), torch.full_like(w[1], 7.0)) for _ in range(10)] for c, w in zip(cases, want)]
+    torch.cuda.synchronize()
+    for turn in range(10):
+        for c, st, o in zip(cases, streams, outs):
+            V.attention_window_dev(c.cache(V), 0, c.rows(V), c.dq.data_ptr(), c.heads, 0, 0.0, o[turn][0].data_ptr(),
+                                   o[turn][1].data_ptr(), st.cuda_stream)
+    torch.cuda.synchronize()
+    for o, w in zip(outs, want):
+        for got in o:
+            assert torch.equal(got[0], w[0]) and torch.equal(got[1], w[1])
+
+
 def test_the_first_call_may_be_captured():
     """Every operator's first call in a process, inside a capture."""
     import os

@@ -57,7 +57,7 @@ constexpr int at_keys(int nt) { return nt == 1 ? 64 : 128; }
 constexpr int at_stages(int hd, int nt, int rt) { return nt == 2 ? 2 : (rt == 32 ? 3 : 2) * (128 / hd); }
 // RT / 32 softmax warps per tile, a K and two V loaders, an MMA warp
 constexpr int at_threads(int nt, int rt) { return (nt * rt / 32 + 4) * 32; }
-constexpr uint64_t kAtWaitNs = 2000000000ull;
+constexpr uint64_t kAtWaitNs = 2000000000ull, kAtBlockNs = 10000ull;   // a CTA's waits end after this, per block as well
 constexpr float kAtRescale = 8.0f;      // log2 of the largest P before the maximum moves
 constexpr int kAtOneCta = 120 * 1024;   // more than half an SM's shared memory: one CTA per SM
 constexpr double kAtFixed = 4;          // block times of a CTA's start and merge
@@ -292,7 +292,6 @@ __global__ void __launch_bounds__(at_threads(NT, RT), NT == 1 ? 2 : 1) attn_rows
     const int b0 = (int)((long long)z * blocks / Z), nb = (int)((long long)(z + 1) * blocks / Z) - b0;
     const int tiles = M - m0 > RT ? NT : 1;   // tiles with rows
     const int head0 = kvh * p.group;
-    const uint64_t deadline = globaltimer() + kAtWaitNs;
     bool ok = true;
 
     // keys that every row of the CTA sees, in the walk's order: [core_s, core_e)
@@ -336,6 +335,7 @@ __global__ void __launch_bounds__(at_threads(NT, RT), NT == 1 ? 2 : 1) attn_rows
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = sh.tmem;
+    const uint64_t deadline = globaltimer() + kAtWaitNs + (uint64_t)nb * kAtBlockNs;   // (TMEM may have been another kernel's)
     constexpr uint32_t kOCol = kTwoS ? 2 * kKeys : NT * kKeys;   // S ranges first, then O tiles
 
     if (warp >= kWarpK && warp <= kWarpV2) {

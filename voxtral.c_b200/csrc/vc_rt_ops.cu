@@ -154,6 +154,7 @@ int check_waits(const char *who, DevCtx *c) {
 
 int launched(const char *who, cudaError_t e) {
     if (e == cudaSuccess) return VOX_CUDA_OK;
+    cudaGetLastError();   // reported here, not by whoever asks next
     set_error("%s: %s", who, cudaGetErrorString(e));
     return VOX_CUDA_ERR_CUDA;
 }
@@ -165,7 +166,7 @@ int attention(const char *who, bool tree, const vox_cuda_kv_cache *cache, int la
     if (rc || (rc = check_rows(who, rows, p.c, tree ? 2 : 0, &p.r)) || (rc = check_layer(who, layer, p.c)) ||
         (rc = check_heads(who, n_heads, p.c)))
         return rc;
-    if (window < 0 || !(fabsf(scale) <= 3.0e38f)) {
+    if (window < 0 || !(fabsf(scale) <= 2.0e38f)) {
         set_error("%s: bad window or scale", who);
         return VOX_CUDA_ERR_ARG;
     }
@@ -190,7 +191,7 @@ int attention(const char *who, bool tree, const vox_cuda_kv_cache *cache, int la
     p.lse = lse;
     p.n_heads = n_heads;
     p.group = n_heads / p.c.n_kv_heads;
-    p.window = window;
+    p.window = window < p.c.ring ? window : 0;   // the ring holds no more: no limit (and no sum overflows)
     p.scale_log2 = (scale == 0.f ? 1.0f / sqrtf((float)p.c.head_dim) : scale) * 1.4426950408889634f;
     return launched(who, launch_attn_rows(p, stream ? (cudaStream_t)stream : c->stream));
 }
