@@ -54,7 +54,9 @@ constexpr int kAtRows = 128;            // packed rows per MMA tile = TMEM lanes
 //   <1, 32>   a token's or a few tokens' heads, bound by HBM: Q is small, 96 KB
 //             of keys in flight per CTA, two CTAs per SM
 constexpr int at_keys(int nt) { return nt == 1 ? 64 : 128; }
-constexpr int at_stages(int hd, int nt, int rt) { return nt == 2 ? 2 : (rt == 32 ? 3 : 2) * (128 / hd); }
+constexpr bool at_three(int hd, int nt, int rt) { return hd == 64 && nt == 1 && rt == 128; }
+constexpr int at_stages(int hd, int nt, int rt) { return at_three(hd, nt, rt) ? 3 : nt == 2 ? 2 : (rt == 32 ? 3 : 2) * (128 / hd); }
+constexpr int at_ctas(int hd, int nt, int rt) { return at_three(hd, nt, rt) ? 3 : nt == 1 ? 2 : 1; }
 // RT / 32 softmax warps per tile, a K and two V loaders, an MMA warp
 constexpr int at_threads(int nt, int rt) { return (nt * rt / 32 + 4) * 32; }
 constexpr uint64_t kAtWaitNs = 2000000000ull, kAtBlockNs = 10000ull;   // a CTA's waits end after this, per block as well
@@ -266,7 +268,7 @@ __device__ __forceinline__ uint32_t nonfinite2(uint32_t u) {   // 0xffff in each
 }
 
 template <typename T, int HD, int NT, int RT>
-__global__ void __launch_bounds__(at_threads(NT, RT), NT == 1 ? 2 : 1) attn_rows_tc_kernel(const __grid_constant__ CUtensorMap tm_k,
+__global__ void __launch_bounds__(at_threads(NT, RT), at_ctas(HD, NT, RT)) attn_rows_tc_kernel(const __grid_constant__ CUtensorMap tm_k,
                                                                    const __grid_constant__ CUtensorMap tm_v,
                                                                    const RowsAttnParams p) {
     using Sm = AtSmem<HD, NT, RT>;
@@ -275,8 +277,8 @@ __global__ void __launch_bounds__(at_threads(NT, RT), NT == 1 ? 2 : 1) attn_rows
     constexpr int kThreads = at_threads(NT, RT), kWarpK = kSoft * NT, kWarpV2 = kWarpK + 2, kWarpMma = kWarpK + 3;
     constexpr int kStages = Sm::kStages;
     constexpr int kKeys = Sm::kKeys, kSteps = kKeys / kAtHalf;
-    constexpr bool kTwoS = NT == 1;          // two S ranges
-    constexpr uint32_t kTmemCols = NT == 2 ? 512 : 256;
+    constexpr bool kTwoS = NT == 1 && !at_three(HD, NT, RT);          // two S ranges
+    constexpr uint32_t kTmemCols = at_three(HD, NT, RT) ? 128 : NT == 2 ? 512 : 256;
     extern __shared__ __align__(1024) unsigned char at_smem_raw[];
     Sm &sh = *reinterpret_cast<Sm *>(at_smem_raw);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -559,17 +561,20 @@ __global__ void __launch_bounds__(at_threads(NT, RT), NT == 1 ? 2 : 1) attn_rows
                     // them again (S is intact until P is stored)
                     uint32_t w[kAtHalf / 2];
                     float base = mr == -INFINITY ? 0.f : mr, factor = 1.f, ls = 0.f;
-                    float over = weigh<T>(ts, sl2, base, full, keys, c0, anc, w, ls);   // the largest less base
-                    const bool move = mr == -INFINITY ? over > -INFINITY : over > kAtRescale;
-                    const bool moved = __any_sync(0xffffffffu, move);
-                    if (moved) {
+                    float over;   // the largest less base
+                    bool moved = false;
+#pragma unroll 1
+                    for (;;) {    // (one copy of its code)
+                        over = weigh<T>(ts, sl2, base, full, keys, c0, anc, w, ls);
+                        const bool move = mr == -INFINITY ? over > -INFINITY : over > kAtRescale;
+                        if (moved || !__any_sync(0xffffffffu, move)) break;
+                        moved = true;
                         if (move) {
                             const float mn = base + over;
                             factor = mr == -INFINITY ? 0.f : exp2_approx(mr - mn);
                             mr = base = mn;
                             l *= factor;
                         }
-                        over = weigh<T>(ts, sl2, base, full, keys, c0, anc, w, ls);
                     }
                     if (mr > -INFINITY) l += ls;
                     if (over != over) l = over;   // a NaN score: the row is NaN
@@ -734,7 +739,7 @@ template <typename T, int HD, int NT, int RT>
 cudaError_t launch_tiles(RowsAttnParams p, cudaStream_t st) {
     constexpr int kKeys = at_keys(NT);
     constexpr size_t kSmem = std::max<size_t>(sizeof(AtSmem<HD, NT, RT>), NT == 2 ? kAtOneCta : 0);
-    static_assert(kSmem <= (NT == 1 ? 113 : 227) * 1024, "two CTAs or one fit an SM");
+    static_assert(kSmem <= (228 / at_ctas(HD, NT, RT) - 1) * 1024, "they fit an SM");
     auto kernel = attn_rows_tc_kernel<T, HD, NT, RT>;
     static ClusterKernel ck;
     int dev = 0;
@@ -771,8 +776,8 @@ template <typename T, int HD>
 cudaError_t launch_typed(const RowsAttnParams &p, cudaStream_t st) {
     const long long M = (long long)p.r.max_rows * p.group;
     if (M <= 32) return launch_tiles<T, HD, 1, 32>(p, st);
-    if (M <= kAtRows) return launch_tiles<T, HD, 1, 128>(p, st);
-    return launch_tiles<T, HD, 2, 128>(p, st);
+    if constexpr (HD == 64) return launch_tiles<T, HD, 1, 128>(p, st);
+    else return M <= kAtRows ? launch_tiles<T, HD, 1, 128>(p, st) : launch_tiles<T, HD, 2, 128>(p, st);
 }
 template <typename T>
 cudaError_t launch_dim(const RowsAttnParams &p, cudaStream_t st) {
