@@ -512,17 +512,32 @@ struct ArManySmem {
     ArRows<kArManyRows> rows;
 };
 
-template <int HD>
-__global__ void __launch_bounds__(kArManyThreads) attn_rows_many_kernel(const RowsAttnParams p) {
+constexpr size_t many_smem(int hd, int ctas) {
+    return hd == 64 ? sizeof(ArManySmem<64>) + (ctas == 1 ? sizeof(ArMerge<64, kArManyRows>) : 0)
+                    : sizeof(ArManySmem<128>) + sizeof(ArMerge<128, kArManyRows>);
+}
+// A round of two CTAs on an SM, of one alone: the launch takes them where more
+// tiles than SMs would run in turn (64-dim heads, trees of 61 rows over short
+// contexts, 512 tiles: 94 -> 35 us; 1605 tiles of up to 730 keys 392 -> 360,
+// 468 of 70 65 -> 51; near the rule's edge up to a tenth is lost, 210 tiles of
+// 800 keys 85 -> 96; what fits one wave is faster alone, 14.5 against 16.5 us).
+constexpr double kArTwo = 1.8;
+
+// CTAS: on an SM.  Two fit with heads of 64, in 128 registers each and one
+// share: the merge's memory is then q's and p's, which no peer writes early.
+template <int HD, int CTAS>
+__global__ void __launch_bounds__(kArManyThreads, CTAS) attn_rows_many_kernel(const RowsAttnParams p) {
     using Sm = ArManySmem<HD>;
     constexpr int RB = kArManyRows, WR = kArWarpRows, kKeys = kArManyKeys;
-    static_assert(sizeof(Sm) + sizeof(ArMerge<HD, RB>) <= 227 * 1024, "fits an SM");
+    constexpr bool kOver = CTAS > 1;
+    static_assert(many_smem(HD, CTAS) <= (228 / CTAS - 1) * 1024, "they fit an SM");
     extern __shared__ __align__(128) unsigned char smem_raw[];
     Sm &sh = *reinterpret_cast<Sm *>(smem_raw);
-    ArMerge<HD, RB> &merge = *reinterpret_cast<ArMerge<HD, RB> *>(smem_raw + sizeof(Sm));
+    static_assert(!kOver || sizeof(ArMerge<HD, RB>) <= sizeof(sh.q) + sizeof(sh.p), "it fits there");
+    ArMerge<HD, RB> &merge = *reinterpret_cast<ArMerge<HD, RB> *>(kOver ? reinterpret_cast<unsigned char *>(sh.q) : smem_raw + sizeof(Sm));
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int z = blockIdx.x % p.shares, Z = p.shares;
-    const int m0 = blockIdx.x / p.shares * RB, kvh = blockIdx.y, stream = blockIdx.z;
+    const int Z = kOver ? 1 : p.shares, z = blockIdx.x % Z;
+    const int m0 = blockIdx.x / Z * RB, kvh = blockIdx.y, stream = blockIdx.z;
     const RowSpan s = row_span(p.r, stream);
     const int M = s.n * p.group;
     if (m0 >= M) return;   // the whole cluster leaves
@@ -726,19 +741,21 @@ struct Plan {
 
 // rb: packed rows of a tile, round: keys that a CTA takes at once.  Key shares
 // of a tile, each a CTA of its cluster: the fewest rounds until the last wave of
-// clusters is done, with kArFixed for a CTA's start and merge.
+// clusters is done, with kArFixed for a CTA's start and merge.  each: a round's
+// time, of that of a CTA alone on its SM.
 template <typename K>
-cudaError_t plan(ClusterKernel &ck, K kernel, size_t smem, int threads, int rb, int round, const RowsAttnParams &p, Plan *out) {
+cudaError_t plan(ClusterKernel &ck, K kernel, size_t smem, int threads, int rb, int round, double each, int most_shares,
+                 const RowsAttnParams &p, Plan *out) {
     int dev = 0;
     cudaError_t e = cluster_prepare(ck, kernel, smem, &dev);
     if (e != cudaSuccess) return e;
     const long long M = (long long)p.r.max_rows * p.group, tiles = (M + rb - 1) / rb;
     const long long clusters = tiles * p.c.n_kv_heads * p.c.n_streams;
     const double rounds = (double)most_keys(p, rb) / round;
-    for (int Z = 1; Z <= kMaxCluster && Z < rounds + 1; Z++) {
+    for (int Z = 1; Z <= most_shares && (Z == 1 || Z < rounds + 1); Z++) {
         const int at_once = cluster_active(ck, kernel, dev, threads, smem, Z);
         if (at_once < 1) continue;
-        const double t = (double)((clusters + at_once - 1) / at_once) * (std::max(1.0, rounds / Z) + kArFixed);
+        const double t = (double)((clusters + at_once - 1) / at_once) * (std::max(1.0, rounds / Z) * each + kArFixed);
         if (t < out->cost) {
             out->cost = t;
             out->shares = Z;
@@ -764,9 +781,10 @@ cudaError_t launch_few(const RowsAttnParams &p, cudaStream_t st) {
     static ClusterKernel cl, cs;
     Plan a, b;
     cudaError_t e = plan(cl, attn_rows_few_kernel<HD, RB, false>, sizeof(Large), Large::kThreads, RB, Large::kKeys * Large::kWarps,
-                         p, &a);
+                         1.0, kMaxCluster, p, &a);
     if (e == cudaSuccess)
-        e = plan(cs, attn_rows_few_kernel<HD, RB, true>, sizeof(Small), Small::kThreads, RB, Small::kKeys * Small::kWarps, p, &b);
+        e = plan(cs, attn_rows_few_kernel<HD, RB, true>, sizeof(Small), Small::kThreads, RB, Small::kKeys * Small::kWarps,
+                 1.0, kMaxCluster, p, &b);
     if (e != cudaSuccess) return e;
     return b.cost < a.cost
                ? launch(attn_rows_few_kernel<HD, RB, true>, sizeof(Small), Small::kThreads, RB, b.shares, p, st)
@@ -778,12 +796,20 @@ cudaError_t launch_dim(const RowsAttnParams &p, cudaStream_t st) {
     const long long M = (long long)p.r.max_rows * p.group;
     if (M <= 4) return launch_few<HD, 4>(p, st);
     if (M <= kArFewRows) return launch_few<HD, 8>(p, st);
-    constexpr size_t kSmem = sizeof(ArManySmem<HD>) + sizeof(ArMerge<HD, kArManyRows>);
+    constexpr size_t kSmem = many_smem(HD, 1);
     static ClusterKernel ck;
     Plan a;
-    const cudaError_t e = plan(ck, attn_rows_many_kernel<HD>, kSmem, kArManyThreads, kArManyRows, kArManyKeys, p, &a);
+    cudaError_t e = plan(ck, attn_rows_many_kernel<HD, 1>, kSmem, kArManyThreads, kArManyRows, kArManyKeys, 1.0, kMaxCluster, p, &a);
     if (e != cudaSuccess) return e;
-    return launch(attn_rows_many_kernel<HD>, kSmem, kArManyThreads, kArManyRows, a.shares, p, st);
+    if constexpr (HD == 64) {
+        static ClusterKernel ck2;
+        Plan b;
+        e = plan(ck2, attn_rows_many_kernel<HD, 2>, many_smem(HD, 2), kArManyThreads, kArManyRows, kArManyKeys, kArTwo, 1, p, &b);
+        if (e != cudaSuccess) return e;
+        if (b.cost < a.cost)
+            return launch(attn_rows_many_kernel<HD, 2>, many_smem(HD, 2), kArManyThreads, kArManyRows, 1, p, st);
+    }
+    return launch(attn_rows_many_kernel<HD, 1>, kSmem, kArManyThreads, kArManyRows, a.shares, p, st);
 }
 
 }  // namespace
