@@ -628,7 +628,9 @@ int vox_cuda_attention_tree_dev(const vox_cuda_kv_cache *cache, int layer, const
  * a path ends before an entry that does not ascend (or is beyond 255).
  * n_accept: device [n_streams], at most max_accept (<= 256).  new_pos: device
  * [n_streams] = pos + the rows kept, or NULL; not pos itself.  A stream with
- * a negative pos sits out. */
+ * a negative pos sits out.  Rows that are not kept have taken the slots of the
+ * oldest positions all the same: later rows must not see those, which a window
+ * of at most cap - n_sink - (rows drafted in a round) sees to. */
 int vox_cuda_kv_commit_dev(const vox_cuda_kv_cache *cache, const int *pos, const int *path, int path_stride,
                            const int *n_accept, int max_accept, int *new_pos, void *stream);
 

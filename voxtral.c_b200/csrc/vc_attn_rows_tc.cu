@@ -7,7 +7,7 @@
 //   4 warps per tile softmax, thread = packed row, 64 keys a step: P = 2^(s - m)
 //                    of S (TMEM), rounded to the cache's type, over the S
 //                    columns it came from; before that they load their rows of Q
-//   3 warps          loads: K (one warp) and V blocks two deep, by TMA where a
+//   3 warps          loads: K (one warp) and V blocks two or more deep, by TMA where a
 //                    block's slots follow one another, by 16-byte cp.async into
 //                    the same swizzled layout where they do not (ring wrap,
 //                    sinks, the last block: zeros past the end)
@@ -44,15 +44,23 @@ namespace {
 
 constexpr int kAtHalf = 64;             // keys per softmax step
 constexpr int kAtRows = 128;            // packed rows per MMA tile = TMEM lanes
-// Three shapes: NT tiles of RT rows that exist (the MMA's other rows are
+// Shapes: NT tiles of RT rows that exist (the MMA's other rows are
 // whatever lies behind Q in shared memory; nobody reads their lanes).
-//   <2, 128>  bound by the tensor and exponential units: 128-key blocks (an MMA
-//             of N 64 takes as long as one of N 128, reading its A tile), one
-//             CTA per SM
-//   <1, 128>  64-key blocks with two S ranges, so that S(b + 1) is ready when
-//             the softmax is done with S(b); two CTAs per SM
-//   <1, 32>   a token's or a few tokens' heads, bound by HBM: Q is small, 96 KB
-//             of keys in flight per CTA, two CTAs per SM
+//   <2, 128>  heads of 128, more than 128 rows: bound by the MMAs' reads of
+//             shared memory and the exponentials.  128-key blocks (an MMA of N
+//             64 takes as long as one of N 128, reading its A tile), one CTA
+//             per SM.  2021 rows of 32 heads over 4100 keys, bf16: 195 us, 0.42
+//             of the bf16 rate (two S ranges of 64 keys: 229)
+//   <1, 128>  heads of 128: 64-key blocks with two S ranges, so that S(b + 1)
+//             is ready when the softmax is done with S(b); two CTAs per SM.
+//             Heads of 64, any number of rows (at_three): one S range, 128 TMEM
+//             columns, three CTAs per SM, whose chains S - softmax - P - P.V
+//             fill each other's gaps.  1500 rows of 32 heads, window 750: 52 us
+//             (<2, 128> took 72: 192 CTAs in two waves)
+//   <1, 32>   up to 32 rows, a token's or a few tokens' heads, bound by HBM: Q
+//             is small, 96 KB of keys in flight per CTA, two CTAs per SM.  24
+//             tokens of 32 / 8 heads over 4100 keys: 56 us, 4.8 TB/s, 0.75 of
+//             the copy rate (<1, 128> for them: 68)
 constexpr int at_keys(int nt) { return nt == 1 ? 64 : 128; }
 constexpr bool at_three(int hd, int nt, int rt) { return hd == 64 && nt == 1 && rt == 128; }
 constexpr int at_stages(int hd, int nt, int rt) { return at_three(hd, nt, rt) ? 3 : nt == 2 ? 2 : (rt == 32 ? 3 : 2) * (128 / hd); }
@@ -62,7 +70,7 @@ constexpr int at_threads(int nt, int rt) { return (nt * rt / 32 + 4) * 32; }
 constexpr uint64_t kAtWaitNs = 2000000000ull, kAtBlockNs = 10000ull;   // a CTA's waits end after this, per block as well
 constexpr float kAtRescale = 8.0f;      // log2 of the largest P before the maximum moves
 constexpr int kAtOneCta = 120 * 1024;   // more than half an SM's shared memory: one CTA per SM
-constexpr double kAtFixed = 4;          // block times of a CTA's start and merge
+constexpr double kAtFixed = 4;          // block times of a CTA's start and merge (6 to 8 us)
 constexpr double kAtAlone = 0.6;        // a block's time on an SM of its own, of that beside another CTA
 
 template <int HD, int NT, int RT>
@@ -213,7 +221,8 @@ __device__ __forceinline__ void exp2_poly2(float &a, float &b) {
 // before rounding; the largest s sl2 - base as the result (NaN if one is).
 // The next 16 scores are on their way from TMEM while 16 are worked on.  The
 // exponential unit takes 8 cycles per warp, so in blocks without a mask
-// kAtPoly of 8 pairs go through the FMA pipe instead.
+// kAtPoly of 8 pairs go through the FMA pipe instead (2021 rows over 4100 keys
+// 196 -> 191 us).
 constexpr int kAtPoly = 3;
 template <typename T, bool MASKED>
 __device__ __forceinline__ float weigh_half(uint32_t ts, float sl2, float base, const RowKeys &keys, int c0,

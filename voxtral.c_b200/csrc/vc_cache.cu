@@ -21,7 +21,7 @@ namespace {
 // there), its fraction to sincospi in fp32; the first heads are on their way
 // meanwhile, each later group while the one before is worked on.  A head is
 // HD / 8 lanes with 8 values each, so the shuffles of a norm serve two or four
-// heads.  4 x 1021 rows of 48 heads of 128, fp32 to bf16: 24.9 us, 0.80 of the
+// heads.  4 streams of up to 1021 rows of 48 heads of 128, fp32 to bf16: 24.9 us, 0.80 of the
 // copy rate (lanes of 4 values, no load ahead: 28.7; of 8: 26.6).
 // ---------------------------------------------------------------------------
 
@@ -116,7 +116,8 @@ __global__ void __launch_bounds__(kApThreads) rope_append_kernel(const AppendPar
 // layer.  path[k] >= k and the path ascends, so a thread that moves its 16
 // bytes of every row in the order of k never overwrites a row it still has to
 // read: a batch's targets lie below every later source.  A few MB at most:
-// bound by latency, so a batch of 8 rows is read before it is written.
+// bound by latency, so a batch of 8 rows is read before it is written.  5 rows
+// of 8 streams, 26 layers of 8 heads of 128, fp32 (14 MB moved): 6.1 us.
 // ---------------------------------------------------------------------------
 
 constexpr int kCmThreads = 128;
@@ -163,7 +164,7 @@ __global__ void __launch_bounds__(kCmThreads) kv_commit_kernel(const CommitParam
 // ---------------------------------------------------------------------------
 // Fork: the slots that a stream uses - its first pos, or all of them - copied
 // to another stream, for every layer.  Bound by HBM: 16-byte loads, four in
-// flight per thread.
+// flight per thread.  1.75 GB moved: 290 us, 0.93 of the copy rate.
 // ---------------------------------------------------------------------------
 
 constexpr int kFkThreads = 256;
@@ -202,8 +203,9 @@ template <typename TS, typename TC>
 cudaError_t append_typed(const AppendParams &p, cudaStream_t st) {
     const int hd = p.c.head_dim, at_once = kApThreads / (hd / 8);
     const int steps = (p.n_heads + 2 * p.c.n_kv_heads + at_once - 1) / at_once;
-    // few rows: a block per group of heads; many: a block per row, so that its
-    // cosines and sines serve every head
+    // few rows: a block per group of heads (a step of 8 rows: 5.2 us, launch
+    // bound); from 512 on, which fill the SMs' 8 blocks half, a block per row,
+    // so that its cosines and sines serve every head
     const long long rows = (long long)p.r.max_rows * p.c.n_streams;
     const int split = (int)(rows >= 512 ? 1 : steps);
     const dim3 grid(p.r.max_rows, split, p.c.n_streams);
