@@ -215,7 +215,6 @@ __device__ __forceinline__ void merge_store(ArMerge<HD, RB> &mg, Sum sum, Ml ml,
 constexpr int af_warps(int hd, int rb, bool small) { return small ? (rb == 8 ? 2 : 3) : hd == 64 && rb == 8 ? 11 : 12; }
 constexpr int kAfTile = 8192;              // K bytes of a warp's tile
 constexpr float kAfRescale = 8.0f;         // log2 of the largest weight before the maximum moves
-constexpr int kArFewRows = 32;             // up to here tiles of 8 rows, each with its own pass over the keys
 constexpr double kArFixed = 4;             // rounds' worth of a CTA's start and merge
 
 template <int HD, int RB, bool SMALL>
@@ -778,41 +777,57 @@ cudaError_t launch(K kernel, size_t smem, int threads, int rb, int shares, RowsA
 }
 
 template <int HD, int RB>
-cudaError_t launch_few(const RowsAttnParams &p, cudaStream_t st) {
+cudaError_t plan_few(const RowsAttnParams &p, Plan *large, Plan *small) {
     using Large = AfSmem<HD, RB, false>;
     using Small = AfSmem<HD, RB, true>;
     static ClusterKernel cl, cs;
-    Plan a, b;
-    cudaError_t e = plan(cl, attn_rows_few_kernel<HD, RB, false>, sizeof(Large), Large::kThreads, RB, Large::kKeys * Large::kWarps,
-                         1.0, kMaxCluster, p, &a);
-    if (e == cudaSuccess)
-        e = plan(cs, attn_rows_few_kernel<HD, RB, true>, sizeof(Small), Small::kThreads, RB, Small::kKeys * Small::kWarps,
-                 1.0, kMaxCluster, p, &b);
+    const cudaError_t e = plan(cl, attn_rows_few_kernel<HD, RB, false>, sizeof(Large), Large::kThreads, RB,
+                               Large::kKeys * Large::kWarps, 1.0, kMaxCluster, p, large);
     if (e != cudaSuccess) return e;
-    return b.cost < a.cost
-               ? launch(attn_rows_few_kernel<HD, RB, true>, sizeof(Small), Small::kThreads, RB, b.shares, p, st)
-               : launch(attn_rows_few_kernel<HD, RB, false>, sizeof(Large), Large::kThreads, RB, a.shares, p, st);
+    return plan(cs, attn_rows_few_kernel<HD, RB, true>, sizeof(Small), Small::kThreads, RB, Small::kKeys * Small::kWarps, 1.0,
+                kMaxCluster, p, small);
 }
+template <int HD, int RB>
+cudaError_t launch_few(const Plan &large, const Plan &small, const RowsAttnParams &p, cudaStream_t st) {
+    using Large = AfSmem<HD, RB, false>;
+    using Small = AfSmem<HD, RB, true>;
+    return small.cost < large.cost
+               ? launch(attn_rows_few_kernel<HD, RB, true>, sizeof(Small), Small::kThreads, RB, small.shares, p, st)
+               : launch(attn_rows_few_kernel<HD, RB, false>, sizeof(Large), Large::kThreads, RB, large.shares, p, st);
+}
+
+// Microseconds of a round, heads of 128: of the few-row kernels (HBM and the
+// loads' latency), and of the many-row one with up to 4 of its warps at work -
+// one to a scheduler - and with all 8.  Tiles of 8 rows each take their own pass
+// over the keys but spread over more SMs; measured, few against many (32 / 8
+// heads): one stream, 4096 keys, 40 packed rows 42 / 62 us, 64 rows 54 / 64;
+// 8 streams, 512 keys, 24 rows 37 / 33, 40 rows 55 / 47; 4096 keys, 64 rows
+// 361 / 266.
+constexpr double kArFewRound = 4.2, kArManyRound4 = 4.9, kArManyRound8 = 7.8;
 
 template <int HD>
 cudaError_t launch_dim(const RowsAttnParams &p, cudaStream_t st) {
     const long long M = (long long)p.r.max_rows * p.group;
-    if (M <= 4) return launch_few<HD, 4>(p, st);
-    if (M <= kArFewRows) return launch_few<HD, 8>(p, st);
+    Plan large, small, many, two;
+    cudaError_t e = M <= 4 ? plan_few<HD, 4>(p, &large, &small) : plan_few<HD, 8>(p, &large, &small);
+    if (e != cudaSuccess) return e;
+    if (M <= 4) return launch_few<HD, 4>(large, small, p, st);
     constexpr size_t kSmem = many_smem(HD, 1);
     static ClusterKernel ck;
-    Plan a;
-    cudaError_t e = plan(ck, attn_rows_many_kernel<HD, 1>, kSmem, kArManyThreads, kArManyRows, kArManyKeys, 1.0, kMaxCluster, p, &a);
+    e = plan(ck, attn_rows_many_kernel<HD, 1>, kSmem, kArManyThreads, kArManyRows, kArManyKeys, 1.0, kMaxCluster, p, &many);
     if (e != cudaSuccess) return e;
     if constexpr (HD == 64) {
         static ClusterKernel ck2;
-        Plan b;
-        e = plan(ck2, attn_rows_many_kernel<HD, 2>, many_smem(HD, 2), kArManyThreads, kArManyRows, kArManyKeys, kArTwo, 1, p, &b);
+        e = plan(ck2, attn_rows_many_kernel<HD, 2>, many_smem(HD, 2), kArManyThreads, kArManyRows, kArManyKeys, kArTwo, 1, p, &two);
         if (e != cudaSuccess) return e;
-        if (b.cost < a.cost)
-            return launch(attn_rows_many_kernel<HD, 2>, many_smem(HD, 2), kArManyThreads, kArManyRows, 1, p, st);
     }
-    return launch(attn_rows_many_kernel<HD, 1>, kSmem, kArManyThreads, kArManyRows, a.shares, p, st);
+    const double round = (M <= 4 * kArWarpRows ? kArManyRound4 : kArManyRound8) * HD / 128;
+    if (std::min(large.cost, small.cost) * kArFewRound < std::min(many.cost, two.cost) * round)
+        return launch_few<HD, 8>(large, small, p, st);
+    if constexpr (HD == 64)
+        if (two.cost < many.cost)
+            return launch(attn_rows_many_kernel<HD, 2>, many_smem(HD, 2), kArManyThreads, kArManyRows, 1, p, st);
+    return launch(attn_rows_many_kernel<HD, 1>, kSmem, kArManyThreads, kArManyRows, many.shares, p, st);
 }
 
 }  // namespace

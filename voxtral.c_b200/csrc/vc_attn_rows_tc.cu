@@ -46,7 +46,7 @@ constexpr int kAtHalf = 64;             // keys per softmax step
 constexpr int kAtRows = 128;            // packed rows per MMA tile = TMEM lanes
 // Shapes: NT tiles of RT rows that exist (the MMA's other rows are
 // whatever lies behind Q in shared memory; nobody reads their lanes).
-//   <2, 128>  heads of 128, more than 128 rows: bound by the MMAs' reads of
+//   <2, 128>  heads of 128, many rows over long contexts: bound by the MMAs' reads of
 //             shared memory and the exponentials.  128-key blocks (an MMA of N
 //             64 takes as long as one of N 128, reading its A tile), one CTA
 //             per SM.  2021 rows of 32 heads over 4100 keys, bf16: 195 us, 0.42
@@ -744,15 +744,26 @@ bool cache_map(CUtensorMap *m, char *base, const CacheView &c, int keys) {
               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// A shape's launch: its cluster size and what that costs.
+struct Plan {
+    double cost = 1e30;
+    int shares = 1;
+};
+
+template <int HD, int NT, int RT>
+constexpr size_t at_smem() {
+    return std::max<size_t>(sizeof(AtSmem<HD, NT, RT>), NT == 2 ? kAtOneCta : 0);
+}
+
 template <typename T, int HD, int NT, int RT>
-cudaError_t launch_tiles(RowsAttnParams p, cudaStream_t st) {
+cudaError_t plan_tiles(const RowsAttnParams &p, Plan *out) {
     constexpr int kKeys = at_keys(NT);
-    constexpr size_t kSmem = std::max<size_t>(sizeof(AtSmem<HD, NT, RT>), NT == 2 ? kAtOneCta : 0);
+    constexpr size_t kSmem = at_smem<HD, NT, RT>();
     static_assert(kSmem <= (228 / at_ctas(HD, NT, RT) - 1) * 1024, "they fit an SM");
     auto kernel = attn_rows_tc_kernel<T, HD, NT, RT>;
     static ClusterKernel ck;
     int dev = 0;
-    cudaError_t e = cluster_prepare(ck, kernel, kSmem, &dev);
+    const cudaError_t e = cluster_prepare(ck, kernel, kSmem, &dev);
     if (e != cudaSuccess) return e;
     const long long M = (long long)p.r.max_rows * p.group;
     const long long tiles = (M + NT * RT - 1) / (NT * RT);
@@ -761,32 +772,55 @@ cudaError_t launch_tiles(RowsAttnParams p, cudaStream_t st) {
     // start and merge.  Several waves of clusters: each takes a share's blocks.
     // One wave that leaves SMs half empty: a CTA alone on an SM is faster than
     // one of two.
-    double best = 1e30;
-    p.shares = 1;
     for (int Z = 1; Z <= kMaxCluster && Z <= blocks; Z++) {
         const int at_once = cluster_active(ck, kernel, dev, at_threads(NT, RT), kSmem, Z);
         if (at_once < 1) continue;
         const double fill = (double)clusters / at_once, part = (double)blocks / Z;
         const double t = fill > 1.0 ? ceil(fill) * (part + kAtFixed) : part * std::max(fill, NT == 1 ? kAtAlone : 1.0) + kAtFixed;
-        if (t < best) {
-            best = t;
-            p.shares = Z;
+        if (t < out->cost) {
+            out->cost = t;
+            out->shares = Z;
         }
     }
+    return cudaSuccess;
+}
+
+template <typename T, int HD, int NT, int RT>
+cudaError_t launch_tiles(RowsAttnParams p, const Plan &plan, cudaStream_t st) {
+    constexpr int kKeys = at_keys(NT);
+    const long long M = (long long)p.r.max_rows * p.group;
+    const long long tiles = (M + NT * RT - 1) / (NT * RT);
+    p.shares = plan.shares;
     cudaLaunchAttribute attr;
     const cudaLaunchConfig_t cfg = cluster_config(dim3((unsigned)(p.shares * tiles), p.c.n_kv_heads, p.c.n_streams),
-                                                  at_threads(NT, RT), kSmem, p.shares, &attr, st);
+                                                  at_threads(NT, RT), at_smem<HD, NT, RT>(), p.shares, &attr, st);
     CUtensorMap mk = {}, mv = {};
     p.maps = cache_map(&mk, p.c.k + p.layer_off * 2, p.c, kKeys) && cache_map(&mv, p.c.v + p.layer_off * 2, p.c, kKeys);
-    return cudaLaunchKernelEx(&cfg, kernel, mk, mv, p);
+    return cudaLaunchKernelEx(&cfg, attn_rows_tc_kernel<T, HD, NT, RT>, mk, mv, p);
 }
+
+// A block of 128 keys of <2, 128>, of one of 64 of <1, 128>: measured, <1, 128>
+// against <2, 128> with 32 / 8 heads of 128: 256 packed rows of 8 streams over
+// 512 keys 17 / 27 us, over 4096 keys 66 / 64, of one stream 25 / 29; 1024 rows
+// of 8 streams over 4096 keys 195 / 186.
+constexpr double kAtTwoTiles = 1.55;
 
 template <typename T, int HD>
 cudaError_t launch_typed(const RowsAttnParams &p, cudaStream_t st) {
     const long long M = (long long)p.r.max_rows * p.group;
-    if (M <= 32) return launch_tiles<T, HD, 1, 32>(p, st);
-    if constexpr (HD == 64) return launch_tiles<T, HD, 1, 128>(p, st);
-    else return M <= kAtRows ? launch_tiles<T, HD, 1, 128>(p, st) : launch_tiles<T, HD, 2, 128>(p, st);
+    Plan one, two;
+    cudaError_t e;
+    if (M <= 32) {
+        if ((e = plan_tiles<T, HD, 1, 32>(p, &one)) != cudaSuccess) return e;
+        return launch_tiles<T, HD, 1, 32>(p, one, st);
+    }
+    if ((e = plan_tiles<T, HD, 1, 128>(p, &one)) != cudaSuccess) return e;
+    if constexpr (HD == 128)
+        if (M > kAtRows) {
+            if ((e = plan_tiles<T, HD, 2, 128>(p, &two)) != cudaSuccess) return e;
+            if (two.cost * kAtTwoTiles < one.cost) return launch_tiles<T, HD, 2, 128>(p, two, st);
+        }
+    return launch_tiles<T, HD, 1, 128>(p, one, st);
 }
 template <typename T>
 cudaError_t launch_dim(const RowsAttnParams &p, cudaStream_t st) {
