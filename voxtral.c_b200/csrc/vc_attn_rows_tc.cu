@@ -59,7 +59,7 @@ constexpr int kAtRows = 128;            // packed rows per MMA tile = TMEM lanes
 //             (<2, 128> took 72: 192 CTAs in two waves)
 //   <1, 32>   up to 32 rows, a token's or a few tokens' heads, bound by HBM: Q
 //             is small, 96 KB of keys in flight per CTA, two CTAs per SM.  24
-//             tokens of 32 / 8 heads over 4100 keys: 56 us, 4.8 TB/s, 0.75 of
+//             tokens of 32 / 8 heads over 4100 keys: 57 us, 4.7 TB/s, 0.73 of
 //             the copy rate (<1, 128> for them: 68)
 constexpr int at_keys(int nt) { return nt == 1 ? 64 : 128; }
 constexpr bool at_three(int hd, int nt, int rt) { return hd == 64 && nt == 1 && rt == 128; }
@@ -70,7 +70,8 @@ constexpr int at_threads(int nt, int rt) { return (nt * rt / 32 + 4) * 32; }
 constexpr uint64_t kAtWaitNs = 2000000000ull, kAtBlockNs = 10000ull;   // a CTA's waits end after this, per block as well
 constexpr float kAtRescale = 8.0f;      // log2 of the largest P before the maximum moves
 constexpr int kAtOneCta = 120 * 1024;   // more than half an SM's shared memory: one CTA per SM
-constexpr double kAtFixed = 4;          // block times of a CTA's start and merge (6 to 8 us)
+constexpr double kAtFixed = 8;          // block times of a CTA's start and merge (6 to 8 us)
+constexpr double kAtMerge = 4;          // more for the merge of 128 rows' shares (64 KB of sums to a CTA)
 constexpr double kAtAlone = 0.6;        // a block's time on an SM of its own, of that beside another CTA
 
 template <int HD, int NT, int RT>
@@ -758,6 +759,7 @@ constexpr size_t at_smem() {
 template <typename T, int HD, int NT, int RT>
 cudaError_t plan_tiles(const RowsAttnParams &p, Plan *out) {
     constexpr int kKeys = at_keys(NT);
+    constexpr int kPer = at_ctas(HD, NT, RT);
     constexpr size_t kSmem = at_smem<HD, NT, RT>();
     static_assert(kSmem <= (228 / at_ctas(HD, NT, RT) - 1) * 1024, "they fit an SM");
     auto kernel = attn_rows_tc_kernel<T, HD, NT, RT>;
@@ -768,15 +770,18 @@ cudaError_t plan_tiles(const RowsAttnParams &p, Plan *out) {
     const long long M = (long long)p.r.max_rows * p.group;
     const long long tiles = (M + NT * RT - 1) / (NT * RT);
     const long long clusters = tiles * p.c.n_kv_heads * p.c.n_streams, blocks = (most_keys(p, NT * RT) + kKeys - 1) / kKeys;
-    // Shares: the least time in units of a block, with kAtFixed for a CTA's
-    // start and merge.  Several waves of clusters: each takes a share's blocks.
-    // One wave that leaves SMs half empty: a CTA alone on an SM is faster than
-    // one of two.
+    // Shares: the least time in units of a block, with kAtFixed for each wave's
+    // starts and merges.  Several waves run into each other, so their blocks
+    // count in proportion; in one wave a CTA alone on its SM is faster than one
+    // beside others.  (The device counts these clusters for one CTA to an SM.)
+    // 24 x 8 tiles of 65 blocks: 1 share 70 us, 2 58, 4 66; 8 x 8 tiles: 2
+    // shares 39, 4 33; 128 tiles of 128 rows, 9 blocks: 1 share 17, 2 25.
     for (int Z = 1; Z <= kMaxCluster && Z <= blocks; Z++) {
-        const int at_once = cluster_active(ck, kernel, dev, at_threads(NT, RT), kSmem, Z);
+        const int at_once = cluster_active(ck, kernel, dev, at_threads(NT, RT), kSmem, Z) * kPer;
         if (at_once < 1) continue;
         const double fill = (double)clusters / at_once, part = (double)blocks / Z;
-        const double t = fill > 1.0 ? ceil(fill) * (part + kAtFixed) : part * std::max(fill, NT == 1 ? kAtAlone : 1.0) + kAtFixed;
+        const double t = part * (fill > 1.0 ? fill : kPer > 1 && fill * kPer <= 1.0 ? kAtAlone : 1.0) + std::max(1.0, ceil(fill)) * kAtFixed +
+                         (Z > 1 && RT == kAtRows ? kAtMerge : 0.0);
         if (t < out->cost) {
             out->cost = t;
             out->shares = Z;
