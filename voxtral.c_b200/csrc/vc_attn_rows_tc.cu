@@ -44,13 +44,13 @@ namespace {
 
 constexpr int kAtHalf = 64;             // keys per softmax step
 constexpr int kAtRows = 128;            // packed rows per MMA tile = TMEM lanes
-// Shapes: NT tiles of RT rows that exist (the MMA's other rows are
-// whatever lies behind Q in shared memory; nobody reads their lanes).
-//   <2, 128>  heads of 128, many rows over long contexts: bound by the MMAs' reads of
-//             shared memory and the exponentials.  128-key blocks (an MMA of N
+// Shapes: NT tiles of RT rows that exist (the MMA's other rows are whatever
+// lies behind Q in shared memory; nobody reads their lanes).
+//   <2, 128>  heads of 128, many rows over long contexts: bound by the MMAs'
+//             reads of shared memory and the exponentials.  128-key blocks (an MMA of N
 //             64 takes as long as one of N 128, reading its A tile), one CTA
-//             per SM.  2021 rows of 32 heads over 4100 keys, bf16: 195 us, 0.42
-//             of the bf16 rate (two S ranges of 64 keys: 229)
+//             per SM.  2021 rows of 32 heads over 4100 keys, bf16: 195 to
+//             200 us, 0.41 of the bf16 rate (two S ranges of 64 keys: 229)
 //   <1, 128>  heads of 128: 64-key blocks with two S ranges, so that S(b + 1)
 //             is ready when the softmax is done with S(b); two CTAs per SM.
 //             Heads of 64, any number of rows (at_three): one S range, 128 TMEM
@@ -60,7 +60,8 @@ constexpr int kAtRows = 128;            // packed rows per MMA tile = TMEM lanes
 //   <1, 32>   up to 32 rows, a token's or a few tokens' heads, bound by HBM: Q
 //             is small, 96 KB of keys in flight per CTA, two CTAs per SM.  24
 //             tokens of 32 / 8 heads over 4100 keys: 57 us, 4.7 TB/s, 0.73 of
-//             the copy rate (<1, 128> for them: 68)
+//             the copy rate (<1, 128> as long); 4 tokens of 8 streams over 512
+//             keys 13.0 us (<1, 128>: 14.5), of one over 4096 15.7 (16.6)
 constexpr int at_keys(int nt) { return nt == 1 ? 64 : 128; }
 constexpr bool at_three(int hd, int nt, int rt) { return hd == 64 && nt == 1 && rt == 128; }
 constexpr int at_stages(int hd, int nt, int rt) { return at_three(hd, nt, rt) ? 3 : nt == 2 ? 2 : (rt == 32 ? 3 : 2) * (128 / hd); }
