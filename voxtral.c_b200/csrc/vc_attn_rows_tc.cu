@@ -463,7 +463,7 @@ __global__ void __launch_bounds__(at_threads(NT, RT), at_ctas(HD, NT, RT)) attn_
                 for (int k = 0; k < kAtHalf / 16; k++)   // 16 keys: 8 columns of P, 2048 bytes of V
                     warp_mma_ta(tm + kOCol + t * HD, tm + r * kKeys + h * kAtHalf + 8 * k, v0 + (h * 8192 + k * 2048) / 16,
                                 id_o, (b | h | k) != 0 ? 1u : 0u, lead);
-                if (kTwoS || h == 0) warp_commit(&sh.o_part[t], lead);
+                if (kTwoS || h + 1 < kSteps) warp_commit(&sh.o_part[t], lead);
             };
             ok = warp_wait(&sh.q_full, 0u, deadline) && warp_wait(&sh.k_full[0], 0u, deadline);
             if (ok) {
@@ -487,7 +487,10 @@ __global__ void __launch_bounds__(at_threads(NT, RT), at_ctas(HD, NT, RT)) attn_
                     issue_o(0, b, 0);
                     warp_commit(&sh.v_empty[b % kStages], lead);
                 } else {
-                    ok = warp_wait(&sh.v_full[b % kStages], (b / kStages) & 1u, deadline);
+                    // K(b + 1) too, before P is there: a poll takes ~300 cycles once
+                    // MMAs read shared memory (8 trees of 64 rows 107.8 -> 106.2 us)
+                    ok = warp_wait(&sh.v_full[b % kStages], (b / kStages) & 1u, deadline) &&
+                         (b + 1 == nb || warp_wait(&sh.k_full[(b + 1) % kStages], ((b + 1) / kStages) & 1u, deadline));
                     for (int t = 0; t < tiles && ok; t++) {
 #pragma unroll
                         for (int h = 0; h < kSteps; h++) {
@@ -497,15 +500,10 @@ __global__ void __launch_bounds__(at_threads(NT, RT), at_ctas(HD, NT, RT)) attn_
                             issue_o(t, b, h);
                         }
                         if (!ok) break;
-                        if (t == tiles - 1) warp_commit(&sh.v_empty[b % kStages], lead);
-                        if (b + 1 < nb) {
-                            if (t == 0) {
-                                ok = warp_wait(&sh.k_full[(b + 1) % kStages], ((b + 1) / kStages) & 1u, deadline);
-                                if (!ok) break;
-                                tc_fence_after();
-                            }
-                            issue_s(t, b + 1);   // over P(b), behind the MMAs that read it
-                            if (t == tiles - 1) warp_commit(&sh.k_empty[(b + 1) % kStages], lead);
+                        if (b + 1 < nb) issue_s(t, b + 1);   // over P(b), behind the MMAs that read it
+                        if (t == tiles - 1) {
+                            warp_commit(&sh.v_empty[b % kStages], lead);
+                            if (b + 1 < nb) warp_commit(&sh.k_empty[(b + 1) % kStages], lead);
                         }
                     }
                 }
