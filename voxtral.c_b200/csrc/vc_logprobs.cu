@@ -345,7 +345,10 @@ __global__ void __launch_bounds__(NTH, NTH == kLpMany ? kLpCtas : 1024 / NTH) to
             top = 0.f;
             m = wm;
         }
-        const uint64_t l2 = pair(kLog2e, kLog2e), ml = pair(-m * kLog2e, -m * kLog2e);
+        // x - m first, then log2(e): in one multiply-add -m log2(e) would be
+        // rounded to m's size, and every weight off by as much (fp32 logits
+        // near 30000: ln Z by 1e-3)
+        const uint64_t l2 = pair(kLog2e, kLog2e), nm = pair(-m, -m);
         uint64_t s2[2] = {0, 0}, t2[2] = {0, 0};
         if (wm < m) {   // (the maximum is in another batch)
 #pragma unroll
@@ -353,7 +356,7 @@ __global__ void __launch_bounds__(NTH, NTH == kLpMany ? kLpCtas : 1024 / NTH) to
 #pragma unroll
                 for (int j = 0; j < V / 2; j++) {
                     const float2 f = Raw<T>::pair_of(u[i], j);
-                    const uint64_t t = fma2(pair(f.x, f.y), l2, ml);
+                    const uint64_t t = mul2(add2(pair(f.x, f.y), nm), l2);
                     float ta, tb;
                     unpair(t, ta, tb);
                     const uint64_t e = pair(exp2_approx(ta), exp2_approx(tb));
@@ -366,7 +369,7 @@ __global__ void __launch_bounds__(NTH, NTH == kLpMany ? kLpCtas : 1024 / NTH) to
 #pragma unroll
                 for (int j = 0; j < V / 2; j++) {
                     const float2 f = Raw<T>::pair_of(u[i], j);
-                    const uint64_t t = fma2(pair(f.x, f.y), l2, ml);
+                    const uint64_t t = mul2(add2(pair(f.x, f.y), nm), l2);
                     float ta, tb;
                     unpair(t, ta, tb);
                     const bool a = f.x == m, c = f.y == m;
