@@ -18,10 +18,14 @@
 // read it; the tiles alternate - one's softmax runs under the other's MMAs -
 // and share each K and V block.
 //
-// The running maximum moves only when a step exceeds it by more than 2^8
-// (P <= 256 in either type), and only then O is rescaled.  Rounding P to 16
-// bits is one half step of the type per weight, as the output's own rounding;
-// the sums l take the unrounded weights.
+// The running maximum m moves only when a step exceeds it by more than 2^8,
+// and only then O is rescaled.  Rounding P to 16 bits is one half step of the
+// type per weight, as the output's own rounding; the sums l take the unrounded
+// weights.  In fp16 the steps below 2^-14 are fixed ones of 2^-24: P = 2^(s - m)
+// would lose a key whose weight is 2^-25 of the largest, and a hundred thousand
+// of them are a visible part of l.  There m is the maximum less 7, so that P
+// fills the type up to 2^15 and what is lost is 2^-32 of the largest weight per
+// key: half a step of the output only from 2^21 keys on.
 //
 // Zero times a masked key's NaN or infinity would be NaN: in blocks that some
 // row does not see whole, the loading threads look for non-finite V values,
@@ -69,7 +73,9 @@ constexpr int at_ctas(int hd, int nt, int rt) { return at_three(hd, nt, rt) ? 3 
 // RT / 32 softmax warps per tile, a K and two V loaders, an MMA warp
 constexpr int at_threads(int nt, int rt) { return (nt * rt / 32 + 4) * 32; }
 constexpr uint64_t kAtWaitNs = 2000000000ull, kAtBlockNs = 10000ull;   // a CTA's waits end after this, per block as well
-constexpr float kAtRescale = 8.0f;      // log2 of the largest P before the maximum moves
+constexpr float kAtRescale = 8.0f;      // log2 of what a step may exceed the maximum by before it moves
+template <typename T>
+constexpr float kAtAbove = std::is_same<T, __half>::value ? 7.0f : 0.0f;   // the maximum less m
 constexpr int kAtOneCta = 120 * 1024;   // more than half an SM's shared memory: one CTA per SM
 constexpr double kAtFixed = 8;          // block times of a CTA's start and merge (6 to 8 us)
 constexpr double kAtMerge = 4;          // more for the merge of 128 rows' shares (64 KB of sums to a CTA)
@@ -565,7 +571,7 @@ __global__ void __launch_bounds__(at_threads(NT, RT), at_ctas(HD, NT, RT)) attn_
                 for (int h = 0; h < kSteps; h++) {
                     const uint32_t ts = tl + r * kKeys + h * kAtHalf;
                     const int c0 = (b0 + b) * kKeys + h * kAtHalf;
-                    // P against the maximum so far; a row whose keys exceed it
+                    // P against m so far; a row whose keys exceed the maximum
                     // by more than 2^8 takes theirs, and the warp goes over
                     // them again (S is intact until P is stored)
                     uint32_t w[kAtHalf / 2];
@@ -575,11 +581,11 @@ __global__ void __launch_bounds__(at_threads(NT, RT), at_ctas(HD, NT, RT)) attn_
 #pragma unroll 1
                     for (;;) {    // (one copy of its code)
                         over = weigh<T>(ts, sl2, base, full, keys, c0, anc, w, ls);
-                        const bool move = mr == -INFINITY ? over > -INFINITY : over > kAtRescale;
+                        const bool move = mr == -INFINITY ? over > -INFINITY : over > kAtRescale + kAtAbove<T>;
                         if (moved || !__any_sync(0xffffffffu, move)) break;
                         moved = true;
                         if (move) {
-                            const float mn = base + over;
+                            const float mn = base + over - kAtAbove<T>;
                             factor = mr == -INFINITY ? 0.f : exp2_approx(mr - mn);
                             mr = base = mn;
                             l *= factor;
