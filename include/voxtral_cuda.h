@@ -541,9 +541,11 @@ int vox_cuda_rope_dev(float *x, int n_heads, int head_dim, int pos, const float 
  * each other, and a call may be captured into a CUDA graph and replayed (the
  * positions, row ranges and trees are read on the device).  They run on the
  * calling thread's device (vox_cuda_set_device), whichever device is current;
- * all pointers belong to it.  Results do not depend on timing.  The kernels'
- * waits are bounded: if one runs out, the call's outputs are void, and the
- * next attention call that is made says so (VOX_CUDA_ERR_CUDA), once.
+ * all pointers belong to it.  Results do not depend on timing.  The waits of
+ * the 16-bit attention are bounded: if one runs out, the rows that it held up
+ * get NaN in out and lse (a replayed graph's too), and the next attention call
+ * of the thread that made or captured the call says so (VOX_CUDA_ERR_CUDA)
+ * once, without being enqueued; other threads' calls are not affected.
  * ------------------------------------------------------------------------ */
 
 #define VOX_CUDA_F32  0
@@ -662,6 +664,13 @@ int vox_cuda_token_logprobs_dev(const void *logits, int type, int n_rows, int vo
  * not fault and the context stays usable.  No counterpart in the reference
  * (it has no device-side waits). */
 int vox_cuda_selftest_wait_timeout(int wait_ms);
+
+/* The same for the row attention (16-bit caches): vox_cuda_attention_window_dev
+ * without a window, whose kernel, its work done, waits wait_ms for what never
+ * comes.  The call itself returns 0; its rows get NaN, and the calling
+ * thread's next attention call returns VOX_CUDA_ERR_CUDA. */
+int vox_cuda_selftest_attention_timeout(const vox_cuda_kv_cache *cache, int layer, const vox_cuda_rows *rows,
+                                        const void *q, int n_heads, void *out, float *lse, int wait_ms, void *stream);
 
 /* ------------------------------------------------------------------------
  * Synthetic weights (benchmarks and tests): fill a device bf16 buffer with

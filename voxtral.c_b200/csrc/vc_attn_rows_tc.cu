@@ -98,6 +98,8 @@ struct AtSmem {
     uint64_t q_full, v_land[kStages], k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages], s_full[2], p_full[NT][2], o_part[NT], o_done;   // s_full: by tile, or (one tile) by S range
     uint32_t tmem;
     int bad;      // a masked block holds non-finite V values
+    int failed;   // some warp's wait ran out: the CTA's rows are void
+    uint64_t stall;   // nothing arrives here
 };
 
 template <typename T>
@@ -340,7 +342,8 @@ __global__ void __launch_bounds__(at_threads(NT, RT), at_ctas(HD, NT, RT)) attn_
         mbar_init(&sh.s_full[0], 1);
         mbar_init(&sh.s_full[1], 1);
         mbar_init(&sh.o_done, 1);
-        sh.bad = 0;
+        mbar_init(&sh.stall, 1);
+        sh.bad = sh.failed = 0;
         prefetch_tensormap(&tm_k);
         prefetch_tensormap(&tm_v);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -673,7 +676,9 @@ __global__ void __launch_bounds__(at_threads(NT, RT), at_ctas(HD, NT, RT)) attn_
             }
         }
     }
+    if (p.stall_ns && warp == kWarpMma) ok = warp_wait(&sh.stall, 0u, globaltimer() + p.stall_ns) && ok;
     if (!ok) {
+        sh.failed = 1;
         if (p.err) atomicExch_system(p.err, 1u);
         const uint64_t grace = globaltimer() + 10000000ull;   // let copies and MMAs in flight land
         while (globaltimer() < grace) {
@@ -686,6 +691,19 @@ __global__ void __launch_bounds__(at_threads(NT, RT), at_ctas(HD, NT, RT)) attn_
     if (warp == kWarpMma) {
         tc_fence_after();
         tmem_dealloc(tmem, kTmemCols);
+    }
+    if (sh.failed) {   // whatever was written or is to be merged: NaN, so that no void row passes for a result
+        const int rows = min(NT * RT, M - m0);
+        for (int ml = threadIdx.x; ml < rows; ml += kThreads) {
+            const int m = m0 + ml;
+            const long long row = (long long)(s.r0 + m / p.group) * p.n_heads + head0 + m % p.group;
+            sh.mx[ml] = sh.sum[ml] = NAN;
+            if (Z > 1) continue;
+            for (int d = 0; d < HD; d += 8)
+                *reinterpret_cast<uint4 *>(static_cast<T *>(p.out) + row * HD + d) =
+                    make_uint4(0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu);   // NaN in either type
+            if (p.lse) p.lse[row] = NAN;
+        }
     }
     if (Z > 1) {
         cluster_sync_all();

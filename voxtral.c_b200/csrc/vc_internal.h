@@ -186,7 +186,8 @@ struct RowsAttnParams {
     int window;               // 0: everything that the ring holds
     float scale_log2;         // scale * log2(e)
     int shares;               // key shares of a row tile (set by the launch)
-    unsigned *err;            // raised when a bounded wait expires (mapped host memory)
+    unsigned *err;            // raised when a bounded wait expires (mapped host memory); the rows then get NaN
+    unsigned long long stall_ns;   // self-test: a wait of this length that nothing ends, after the work (0: none)
     int maps;                 // tensor maps of K and V came with the launch (set by it)
 };
 cudaError_t launch_attn_rows(const RowsAttnParams &p, cudaStream_t st);

@@ -145,10 +145,11 @@ int check_heads(const char *who, int n_heads, const CacheView &c) {
     return VOX_CUDA_ERR_ARG;
 }
 
-// A wait that ran out in an earlier call's kernel is reported once.
+// A wait that ran out in the kernel of an earlier call of this thread is
+// reported once; that call's rows are NaN.
 int check_waits(const char *who, DevCtx *c) {
-    if (!__atomic_exchange_n(c->op_err, 0u, __ATOMIC_RELAXED)) return VOX_CUDA_OK;
-    set_error("%s: a device-side wait of an earlier call timed out (its results are void)", who);
+    if (!__atomic_exchange_n(c->op_err + op_slot(), 0u, __ATOMIC_RELAXED)) return VOX_CUDA_OK;
+    set_error("%s: a device-side wait of an earlier call of this thread timed out (its rows are void: NaN)", who);
     return VOX_CUDA_ERR_CUDA;
 }
 
@@ -160,7 +161,7 @@ int launched(const char *who, cudaError_t e) {
 }
 
 int attention(const char *who, bool tree, const vox_cuda_kv_cache *cache, int layer, const vox_cuda_rows *rows, const void *q,
-              int n_heads, int window, float scale, void *out, float *lse, void *stream) {
+              int n_heads, int window, float scale, void *out, float *lse, void *stream, int stall_ms = 0) {
     RowsAttnParams p = {};
     int rc = check_cache(who, cache, &p.c);
     if (rc || (rc = check_rows(who, rows, p.c, tree ? 2 : 0, &p.r)) || (rc = check_layer(who, layer, p.c)) ||
@@ -184,7 +185,8 @@ int attention(const char *who, bool tree, const vox_cuda_kv_cache *cache, int la
     DeviceGuard guard(c->device);
     if (!guard.ok()) return launched(who, cudaGetLastError());
     if ((rc = check_waits(who, c))) return rc;
-    p.err = c->op_err;
+    p.err = c->op_err + op_slot();
+    p.stall_ns = stall_ms * 1000000ull;
     p.layer_off = (long long)layer * p.c.layer_stride;
     p.q = q;
     p.out = out;
@@ -208,6 +210,17 @@ extern "C" int vox_cuda_attention_tree_dev(const vox_cuda_kv_cache *cache, int l
                                            const void *q, int n_heads, int window, float scale, void *out, float *lse,
                                            void *stream) {
     return attention("attention_tree", true, cache, layer, rows, q, n_heads, window, scale, out, lse, stream);
+}
+
+extern "C" int vox_cuda_selftest_attention_timeout(const vox_cuda_kv_cache *cache, int layer, const vox_cuda_rows *rows,
+                                                   const void *q, int n_heads, void *out, float *lse, int wait_ms,
+                                                   void *stream) {
+    const char *who = "selftest_attention_timeout";
+    if (wait_ms < 1 || wait_ms > 10000 || (cache && cache->dtype == ELEM_F32)) {
+        set_error("%s: wait_ms must be 1..10000, the cache of 16 bits (the fp32 kernels have no waits)", who);
+        return VOX_CUDA_ERR_ARG;
+    }
+    return attention(who, false, cache, layer, rows, q, n_heads, 0, 0.f, out, lse, stream, wait_ms);
 }
 
 extern "C" int vox_cuda_rope_append_dev(const vox_cuda_kv_cache *cache, int layer, const vox_cuda_rows *rows,

@@ -8,6 +8,7 @@
 #include <stdarg.h>
 
 #include <array>
+#include <atomic>
 
 using namespace vc;
 using namespace vc::rt;
@@ -96,6 +97,12 @@ void host_rope_table(int pos, int head_dim, float *cs) {
     }
 }
 
+int op_slot() {
+    static std::atomic<unsigned> threads{0};
+    static thread_local const unsigned mine = threads.fetch_add(1) % kOpSlots;
+    return (int)mine;
+}
+
 }  // namespace rt
 }  // namespace vc
 
@@ -144,12 +151,16 @@ extern "C" int vox_cuda_init(void) {
         set_error("vox_cuda_init: stream creation failed");
         return 0;
     }
-    if (cudaHostAlloc((void **)&c->op_err, sizeof(unsigned), cudaHostAllocMapped | cudaHostAllocPortable) != cudaSuccess) {
-        cudaStreamDestroy(c->stream);
-        set_error("vox_cuda_init: allocation failed");
-        return 0;
+    if (!c->op_err) {
+        if (cudaHostAlloc((void **)&c->op_err, kOpSlots * sizeof(unsigned), cudaHostAllocMapped | cudaHostAllocPortable) !=
+            cudaSuccess) {
+            c->op_err = nullptr;
+            cudaStreamDestroy(c->stream);
+            set_error("vox_cuda_init: allocation failed");
+            return 0;
+        }
+        memset(c->op_err, 0, kOpSlots * sizeof(unsigned));
     }
-    *c->op_err = 0;
     c->device = dev;
     c->sms = prop.multiProcessorCount;
     c->ready = true;
@@ -218,8 +229,6 @@ extern "C" void vox_cuda_shutdown(void) {
         release_scratch(c);
         cudaStreamDestroy(c->stream);
         c->stream = nullptr;
-        cudaFreeHost(c->op_err);
-        c->op_err = nullptr;
         c->bytes = 0;
         c->ready = false;
     }

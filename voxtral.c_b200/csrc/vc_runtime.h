@@ -67,10 +67,15 @@ struct DevCtx {
     float *attn_part_o = nullptr, *attn_part_ml = nullptr, *rope_tab = nullptr;
     unsigned *attn_counters = nullptr;
     cudaEvent_t attn_done = nullptr;   // orders the attention scratch across caller streams
-    unsigned *op_err = nullptr;        // mapped host word: a row operator's bounded wait ran out
+    // mapped host words, one for each calling thread (op_slot): a row
+    // operator's bounded wait ran out.  Kept for the process: a captured call
+    // holds its word's address.
+    unsigned *op_err = nullptr;
     float *lp_buf = nullptr;           // results of vox_cuda_decoder_token_logprobs
 };
 
+constexpr int kOpSlots = 1024;
+int op_slot();   // the calling thread's word (threads beyond kOpSlots share)
 int current_device();
 DevCtx *ctx_for(int dev);
 // The calling thread's device context, or NULL (error set) before vox_cuda_init.
