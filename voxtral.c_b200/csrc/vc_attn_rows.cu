@@ -755,7 +755,8 @@ cudaError_t plan(ClusterKernel &ck, K kernel, size_t smem, int threads, int rb, 
     const long long clusters = tiles * p.c.n_kv_heads * p.c.n_streams;
     const double rounds = (double)most_keys(p, rb) / round;
     for (int Z = 1; Z <= most_shares && (Z == 1 || Z < rounds + 1); Z++) {
-        const int at_once = cluster_active(ck, kernel, dev, threads, smem, Z);
+        int at_once = 0;
+        if ((e = cluster_active(ck, kernel, dev, threads, smem, Z, &at_once)) != cudaSuccess) return e;
         if (at_once < 1) continue;
         const double t = (double)((clusters + at_once - 1) / at_once) * (std::max(1.0, rounds / Z) * each + kArFixed);
         if (t < out->cost) {

@@ -771,7 +771,7 @@ bool cache_map(CUtensorMap *m, char *base, const CacheView &c, int keys) {
 // A shape's launch: its cluster size and what that costs.
 struct Plan {
     double cost = 1e30;
-    int shares = 1;
+    int shares = 0;
 };
 
 template <int HD, int NT, int RT>
@@ -788,7 +788,7 @@ cudaError_t plan_tiles(const RowsAttnParams &p, Plan *out) {
     auto kernel = attn_rows_tc_kernel<T, HD, NT, RT>;
     static ClusterKernel ck;
     int dev = 0;
-    const cudaError_t e = cluster_prepare(ck, kernel, kSmem, &dev);
+    cudaError_t e = cluster_prepare(ck, kernel, kSmem, &dev);
     if (e != cudaSuccess) return e;
     const long long M = (long long)p.r.max_rows * p.group;
     const long long tiles = (M + NT * RT - 1) / (NT * RT);
@@ -800,8 +800,10 @@ cudaError_t plan_tiles(const RowsAttnParams &p, Plan *out) {
     // 24 x 8 tiles of 65 blocks: 1 share 70 us, 2 58, 4 66; 8 x 8 tiles: 2
     // shares 39, 4 33; 128 tiles of 128 rows, 9 blocks: 1 share 17, 2 25.
     for (int Z = 1; Z <= kMaxCluster && Z <= blocks; Z++) {
-        const int at_once = cluster_active(ck, kernel, dev, at_threads(NT, RT), kSmem, Z) * kPer;
+        int at_once = 0;
+        if ((e = cluster_active(ck, kernel, dev, at_threads(NT, RT), kSmem, Z, &at_once)) != cudaSuccess) return e;
         if (at_once < 1) continue;
+        at_once *= kPer;
         const double fill = (double)clusters / at_once, part = (double)blocks / Z;
         const double t = part * (fill > 1.0 ? fill : kPer > 1 && fill * kPer <= 1.0 ? kAtAlone : 1.0) + std::max(1.0, ceil(fill)) * kAtFixed +
                          (Z > 1 && RT == kAtRows ? kAtMerge : 0.0);
@@ -810,7 +812,7 @@ cudaError_t plan_tiles(const RowsAttnParams &p, Plan *out) {
             out->shares = Z;
         }
     }
-    return cudaSuccess;
+    return out->shares ? cudaSuccess : cudaErrorInvalidConfiguration;
 }
 
 template <typename T, int HD, int NT, int RT>
