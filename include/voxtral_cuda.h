@@ -672,6 +672,13 @@ int vox_cuda_selftest_wait_timeout(int wait_ms);
 int vox_cuda_selftest_attention_timeout(const vox_cuda_kv_cache *cache, int layer, const vox_cuda_rows *rows,
                                         const void *q, int n_heads, void *out, float *lse, int wait_ms, void *stream);
 
+/* Which form a row attention call takes on this device (a tree's where rows
+ * have parents): plan[0] packed rows (row x query head of a group) of a CTA,
+ * plan[1] CTAs on an SM, plan[2] key shares of a tile of rows.  Nothing is
+ * launched.  For tests that mean to reach a form. */
+int vox_cuda_selftest_attention_plan(const vox_cuda_kv_cache *cache, const vox_cuda_rows *rows, int n_heads, int window,
+                                     int *plan);
+
 /* ------------------------------------------------------------------------
  * Synthetic weights (benchmarks and tests): fill a device bf16 buffer with
  * seeded N(0, std) values, rounded to nearest even.

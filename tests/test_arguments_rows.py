@@ -9,3 +9,11 @@ from test_arguments import A, cache, rows
 def test_the_wait_that_never_ends_has_a_limit(kw, wait):
     f = V.lib().vox_cuda_selftest_attention_timeout
     assert f(cache(**kw), 0, rows(), A, 8, A, None, wait, None) == V.ERR_ARG and V.last_error()
+
+
+def test_a_form_is_asked_for_rows():
+    plan = (V.C.c_int * 3)()
+    f = V.lib().vox_cuda_selftest_attention_plan
+    assert f(cache(), rows(), 8, 0, None) == V.ERR_ARG and f(None, rows(), 8, 0, plan) == V.ERR_ARG
+    assert f(cache(), rows(n_rows=0, max_rows=0), 8, 0, plan) == V.ERR_ARG and f(cache(), None, 8, 0, plan) == V.ERR_ARG
+    assert f(cache(), rows(), 7, 0, plan) == V.ERR_ARG and f(cache(), rows(), 8, -1, plan) == V.ERR_ARG

@@ -768,7 +768,12 @@ cudaError_t plan(ClusterKernel &ck, K kernel, size_t smem, int threads, int rb, 
 }
 
 template <typename K>
-cudaError_t launch(K kernel, size_t smem, int threads, int rb, int shares, RowsAttnParams p, cudaStream_t st) {
+cudaError_t launch(K kernel, size_t smem, int threads, int rb, int ctas, int shares, RowsAttnParams p, cudaStream_t st,
+                   RowsPlan *only) {
+    if (only) {
+        *only = {rb, ctas, shares};
+        return cudaSuccess;
+    }
     const long long M = (long long)p.r.max_rows * p.group, tiles = (M + rb - 1) / rb;
     p.shares = shares;
     cudaLaunchAttribute a;
@@ -789,12 +794,12 @@ cudaError_t plan_few(const RowsAttnParams &p, Plan *large, Plan *small) {
                 kMaxCluster, p, small);
 }
 template <int HD, int RB>
-cudaError_t launch_few(const Plan &large, const Plan &small, const RowsAttnParams &p, cudaStream_t st) {
+cudaError_t launch_few(const Plan &large, const Plan &small, const RowsAttnParams &p, cudaStream_t st, RowsPlan *only) {
     using Large = AfSmem<HD, RB, false>;
     using Small = AfSmem<HD, RB, true>;
     return small.cost < large.cost
-               ? launch(attn_rows_few_kernel<HD, RB, true>, sizeof(Small), Small::kThreads, RB, small.shares, p, st)
-               : launch(attn_rows_few_kernel<HD, RB, false>, sizeof(Large), Large::kThreads, RB, large.shares, p, st);
+               ? launch(attn_rows_few_kernel<HD, RB, true>, sizeof(Small), Small::kThreads, RB, 4, small.shares, p, st, only)
+               : launch(attn_rows_few_kernel<HD, RB, false>, sizeof(Large), Large::kThreads, RB, 1, large.shares, p, st, only);
 }
 
 // Microseconds of a round, heads of 128: of the few-row kernels (HBM and the
@@ -807,12 +812,12 @@ cudaError_t launch_few(const Plan &large, const Plan &small, const RowsAttnParam
 constexpr double kArFewRound = 4.2, kArManyRound4 = 4.9, kArManyRound8 = 7.8;
 
 template <int HD>
-cudaError_t launch_dim(const RowsAttnParams &p, cudaStream_t st) {
+cudaError_t launch_dim(const RowsAttnParams &p, cudaStream_t st, RowsPlan *only) {
     const long long M = (long long)p.r.max_rows * p.group;
     Plan large, small, many, two;
     cudaError_t e = M <= 4 ? plan_few<HD, 4>(p, &large, &small) : plan_few<HD, 8>(p, &large, &small);
     if (e != cudaSuccess) return e;
-    if (M <= 4) return launch_few<HD, 4>(large, small, p, st);
+    if (M <= 4) return launch_few<HD, 4>(large, small, p, st, only);
     constexpr size_t kSmem = many_smem(HD, 1);
     static ClusterKernel ck;
     e = plan(ck, attn_rows_many_kernel<HD, 1>, kSmem, kArManyThreads, kArManyRows, kArManyKeys, 1.0, kMaxCluster, p, &many);
@@ -824,18 +829,18 @@ cudaError_t launch_dim(const RowsAttnParams &p, cudaStream_t st) {
     }
     const double round = (M <= 4 * kArWarpRows ? kArManyRound4 : kArManyRound8) * HD / 128;
     if (std::min(large.cost, small.cost) * kArFewRound < std::min(many.cost, two.cost) * round)
-        return launch_few<HD, 8>(large, small, p, st);
+        return launch_few<HD, 8>(large, small, p, st, only);
     if constexpr (HD == 64)
         if (two.cost < many.cost)
-            return launch(attn_rows_many_kernel<HD, 2>, many_smem(HD, 2), kArManyThreads, kArManyRows, 1, p, st);
-    return launch(attn_rows_many_kernel<HD, 1>, kSmem, kArManyThreads, kArManyRows, many.shares, p, st);
+            return launch(attn_rows_many_kernel<HD, 2>, many_smem(HD, 2), kArManyThreads, kArManyRows, 2, 1, p, st, only);
+    return launch(attn_rows_many_kernel<HD, 1>, kSmem, kArManyThreads, kArManyRows, 1, many.shares, p, st, only);
 }
 
 }  // namespace
 
-cudaError_t launch_attn_rows(const RowsAttnParams &p, cudaStream_t st) {
-    if (p.c.dtype != ELEM_F32) return launch_attn_rows_tc(p, st);
-    return p.c.head_dim == 64 ? launch_dim<64>(p, st) : launch_dim<128>(p, st);
+cudaError_t launch_attn_rows(const RowsAttnParams &p, cudaStream_t st, RowsPlan *only) {
+    if (p.c.dtype != ELEM_F32) return launch_attn_rows_tc(p, st, only);
+    return p.c.head_dim == 64 ? launch_dim<64>(p, st, only) : launch_dim<128>(p, st, only);
 }
 
 }  // namespace vc

@@ -816,7 +816,11 @@ cudaError_t plan_tiles(const RowsAttnParams &p, Plan *out) {
 }
 
 template <typename T, int HD, int NT, int RT>
-cudaError_t launch_tiles(RowsAttnParams p, const Plan &plan, cudaStream_t st) {
+cudaError_t launch_tiles(RowsAttnParams p, const Plan &plan, cudaStream_t st, RowsPlan *only) {
+    if (only) {
+        *only = {NT * RT, at_ctas(HD, NT, RT), plan.shares};
+        return cudaSuccess;
+    }
     constexpr int kKeys = at_keys(NT);
     const long long M = (long long)p.r.max_rows * p.group;
     const long long tiles = (M + NT * RT - 1) / (NT * RT);
@@ -836,31 +840,31 @@ cudaError_t launch_tiles(RowsAttnParams p, const Plan &plan, cudaStream_t st) {
 constexpr double kAtTwoTiles = 1.55;
 
 template <typename T, int HD>
-cudaError_t launch_typed(const RowsAttnParams &p, cudaStream_t st) {
+cudaError_t launch_typed(const RowsAttnParams &p, cudaStream_t st, RowsPlan *only) {
     const long long M = (long long)p.r.max_rows * p.group;
     Plan one, two;
     cudaError_t e;
     if (M <= 32) {
         if ((e = plan_tiles<T, HD, 1, 32>(p, &one)) != cudaSuccess) return e;
-        return launch_tiles<T, HD, 1, 32>(p, one, st);
+        return launch_tiles<T, HD, 1, 32>(p, one, st, only);
     }
     if ((e = plan_tiles<T, HD, 1, 128>(p, &one)) != cudaSuccess) return e;
     if constexpr (HD == 128)
         if (M > kAtRows) {
             if ((e = plan_tiles<T, HD, 2, 128>(p, &two)) != cudaSuccess) return e;
-            if (two.cost * kAtTwoTiles < one.cost) return launch_tiles<T, HD, 2, 128>(p, two, st);
+            if (two.cost * kAtTwoTiles < one.cost) return launch_tiles<T, HD, 2, 128>(p, two, st, only);
         }
-    return launch_tiles<T, HD, 1, 128>(p, one, st);
+    return launch_tiles<T, HD, 1, 128>(p, one, st, only);
 }
 template <typename T>
-cudaError_t launch_dim(const RowsAttnParams &p, cudaStream_t st) {
-    return p.c.head_dim == 64 ? launch_typed<T, 64>(p, st) : launch_typed<T, 128>(p, st);
+cudaError_t launch_dim(const RowsAttnParams &p, cudaStream_t st, RowsPlan *only) {
+    return p.c.head_dim == 64 ? launch_typed<T, 64>(p, st, only) : launch_typed<T, 128>(p, st, only);
 }
 
 }  // namespace
 
-cudaError_t launch_attn_rows_tc(const RowsAttnParams &p, cudaStream_t st) {
-    return p.c.dtype == ELEM_BF16 ? launch_dim<__nv_bfloat16>(p, st) : launch_dim<__half>(p, st);
+cudaError_t launch_attn_rows_tc(const RowsAttnParams &p, cudaStream_t st, RowsPlan *only) {
+    return p.c.dtype == ELEM_BF16 ? launch_dim<__nv_bfloat16>(p, st, only) : launch_dim<__half>(p, st, only);
 }
 
 }  // namespace vc

@@ -190,9 +190,15 @@ struct RowsAttnParams {
     unsigned long long stall_ns;   // self-test: a wait of this length that nothing ends, after the work (0: none)
     int maps;                 // tensor maps of K and V came with the launch (set by it)
 };
-cudaError_t launch_attn_rows(const RowsAttnParams &p, cudaStream_t st);
+struct RowsPlan {             // the form that a call takes
+    int rows;                 // packed rows of a CTA
+    int ctas;                 // CTAs on an SM
+    int shares;               // key shares of a row tile
+};
+// only: nothing is launched, the form is told
+cudaError_t launch_attn_rows(const RowsAttnParams &p, cudaStream_t st, RowsPlan *only = nullptr);
 // the tensor-core kernel of the 16-bit types (vc_attn_rows_tc.cu)
-cudaError_t launch_attn_rows_tc(const RowsAttnParams &p, cudaStream_t st);
+cudaError_t launch_attn_rows_tc(const RowsAttnParams &p, cudaStream_t st, RowsPlan *only = nullptr);
 
 struct AppendParams {
     CacheView c;

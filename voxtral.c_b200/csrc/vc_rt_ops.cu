@@ -161,7 +161,8 @@ int launched(const char *who, cudaError_t e) {
 }
 
 int attention(const char *who, bool tree, const vox_cuda_kv_cache *cache, int layer, const vox_cuda_rows *rows, const void *q,
-              int n_heads, int window, float scale, void *out, float *lse, void *stream, int stall_ms = 0) {
+              int n_heads, int window, float scale, void *out, float *lse, void *stream, int stall_ms = 0,
+              RowsPlan *only = nullptr) {
     RowsAttnParams p = {};
     int rc = check_cache(who, cache, &p.c);
     if (rc || (rc = check_rows(who, rows, p.c, tree ? 2 : 0, &p.r)) || (rc = check_layer(who, layer, p.c)) ||
@@ -184,7 +185,7 @@ int attention(const char *who, bool tree, const vox_cuda_kv_cache *cache, int la
     if (!c) return VOX_CUDA_ERR_UNAVAILABLE;
     DeviceGuard guard(c->device);
     if (!guard.ok()) return launched(who, cudaGetLastError());
-    if ((rc = check_waits(who, c))) return rc;
+    if (!only && (rc = check_waits(who, c))) return rc;
     p.err = c->op_err + op_slot();
     p.stall_ns = stall_ms * 1000000ull;
     p.layer_off = (long long)layer * p.c.layer_stride;
@@ -195,7 +196,7 @@ int attention(const char *who, bool tree, const vox_cuda_kv_cache *cache, int la
     p.group = n_heads / p.c.n_kv_heads;
     p.window = window < p.c.ring ? window : 0;   // the ring holds no more: no limit (and no sum overflows)
     p.scale_log2 = (scale == 0.f ? 1.0f / sqrtf((float)p.c.head_dim) : scale) * 1.4426950408889634f;
-    return launched(who, launch_attn_rows(p, stream ? (cudaStream_t)stream : c->stream));
+    return launched(who, launch_attn_rows(p, stream ? (cudaStream_t)stream : c->stream, only));
 }
 
 }  // namespace
@@ -221,6 +222,24 @@ extern "C" int vox_cuda_selftest_attention_timeout(const vox_cuda_kv_cache *cach
         return VOX_CUDA_ERR_ARG;
     }
     return attention(who, false, cache, layer, rows, q, n_heads, 0, 0.f, out, lse, stream, wait_ms);
+}
+
+extern "C" int vox_cuda_selftest_attention_plan(const vox_cuda_kv_cache *cache, const vox_cuda_rows *rows, int n_heads,
+                                                int window, int *plan) {
+    const char *who = "selftest_attention_plan";
+    if (!plan || !rows || rows->n_rows < 1) {
+        set_error("%s: no rows, or no place for the answer", who);
+        return VOX_CUDA_ERR_ARG;
+    }
+    RowsPlan form = {};
+    void *some = cache ? cache->k : nullptr;   // (an aligned address; nothing is launched)
+    const int rc = attention(who, rows->parent != nullptr, cache, 0, rows, some, n_heads, window, 0.f, some, nullptr, nullptr, 0,
+                             &form);
+    if (rc) return rc;
+    plan[0] = form.rows;
+    plan[1] = form.ctas;
+    plan[2] = form.shares;
+    return VOX_CUDA_OK;
 }
 
 extern "C" int vox_cuda_rope_append_dev(const vox_cuda_kv_cache *cache, int layer, const vox_cuda_rows *rows,

@@ -165,6 +165,7 @@ def lib():
         "vox_cuda_selftest_wait_timeout": ([C.c_int], C.c_int),
         "vox_cuda_selftest_attention_timeout": ([C.POINTER(KvCache), C.c_int, C.POINTER(Rows), C.c_void_p, C.c_int, C.c_void_p,
                                                  C.c_void_p, C.c_int, C.c_void_p], C.c_int),
+        "vox_cuda_selftest_attention_plan": ([C.POINTER(KvCache), C.POINTER(Rows), C.c_int, C.c_int, _ip], C.c_int),
         "vox_cuda_mel_create": ([C.c_int, C.c_int], C.c_void_p),
         "vox_cuda_mel_free": ([C.c_void_p], None),
         "vox_cuda_mel_frames": ([C.c_void_p], C.c_int),
@@ -406,6 +407,13 @@ def attention_tree_dev(cache, layer, rows, q, n_heads, window, scale, out, lse=N
     """Attention of trees of drafted rows over the cache."""
     check(lib().vox_cuda_attention_tree_dev(cache, layer, rows, q, n_heads, window, scale, out, lse, stream),
           "attention_tree_dev")
+
+
+def attention_plan(cache, rows, n_heads, window):
+    """(packed rows of a CTA, CTAs on an SM, key shares) that an attention call takes."""
+    plan = (C.c_int * 3)()
+    check(lib().vox_cuda_selftest_attention_plan(cache, rows, n_heads, window, plan), "selftest_attention_plan")
+    return tuple(plan)
 
 
 def kv_commit_dev(cache, pos, path, path_stride, n_accept, max_accept, new_pos=None, stream=None):
