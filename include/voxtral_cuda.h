@@ -188,9 +188,11 @@ int vox_cuda_decoder_full_step(vox_cuda_dec_state *s, const float *embed,
  * alt_ids[0] = best and returns the number of ids written (1..n_alt). */
 int vox_cuda_decoder_fill_alts(vox_cuda_dec_state *s, int n_alt, float cutoff, int *alt_ids);
 
-/* Confidence of a token under the last step's logits: its natural log
- * probability, the distribution's entropy (nats), and the n_top (0..32) most
- * likely ids with their log probabilities, best first, ties to the lowest id.
+/* Confidence of a token under the logits of vox_cuda_decoder_full_step's last
+ * step of this state (after a reset, a prefill or a batched step there are
+ * none: VOX_CUDA_ERR_ARG): its natural log probability, the distribution's
+ * entropy (nats), and the n_top (0..32) most likely ids with their log
+ * probabilities, best first, ties to the lowest id.
  * logprob, entropy: host, one value each; top_ids, top_logprob: host [n_top].
  * Returns n_top.  The device form for rows of logits is
  * vox_cuda_token_logprobs_dev.  Additive: the reference keeps no

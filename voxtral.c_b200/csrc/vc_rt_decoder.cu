@@ -1144,6 +1144,7 @@ extern "C" int vox_cuda_decoder_full_step(vox_cuda_dec_state *s, const float *em
     if (rope_freqs) memcpy(h_rope(w), rope_freqs, kHeadDim * sizeof(float));
     else host_rope_table(s->pos, kHeadDim, h_rope(w));
     memcpy(h_x(w), embed, kDecDim * sizeof(float));
+    s->have_logits = false;   // a step that fails leaves none
     rc = run_step(d, c, w, true, c->stream, logits == nullptr);
     if (rc) return rc;
     if (logits) {
@@ -1164,7 +1165,7 @@ extern "C" int vox_cuda_decoder_fill_alts(vox_cuda_dec_state *s, int n_alt, floa
         return VOX_CUDA_ERR_ARG;
     }
     if (!s->have_logits) {
-        set_error("decoder_fill_alts: no decode step since the last reset");
+        set_error("decoder_fill_alts: no decode step of this state alone since its last reset, prefill or batched step");
         return VOX_CUDA_ERR_ARG;
     }
     DevCtx *c = ctx_for(s->dec->device);
@@ -1191,7 +1192,8 @@ extern "C" int vox_cuda_decoder_token_logprobs(vox_cuda_dec_state *s, int token,
         return VOX_CUDA_ERR_ARG;
     }
     if (!s->have_logits) {
-        set_error("decoder_token_logprobs: no decode step since the last reset");
+        set_error("decoder_token_logprobs: no decode step of this state alone since its last reset, prefill or batched step "
+                  "(vox_cuda_decoder_step_batch_ex hands out a batched step's logits)");
         return VOX_CUDA_ERR_ARG;
     }
     DevCtx *c = ctx_for(s->dec->device);
