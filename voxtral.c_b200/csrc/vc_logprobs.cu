@@ -42,7 +42,9 @@ constexpr int kLpFew = 256, kLpMany = 128;
 constexpr int kLpCtas = 7;       // CTAs of kLpMany threads on an SM
 constexpr int kLpLoads = 4;      // 16-byte loads of a thread's batch
 constexpr int kLpAhead = 1;      // batches that a thread has on their way (many rows)
-constexpr int kLpKept = 4096;    // batch maxima kept: NTH threads x 4096 / NTH slots, batch b in slot b % slots
+constexpr int kLpKept = 8192;    // bytes of batch maxima kept, batch b of a thread in slot b % slots.  As many bytes in
+                                 // either size of type: with 16 KB of fp32 maxima only five CTAs fit an SM (1001
+                                 // rows of 131072 fp32 logits, 20 alternatives 138 -> 119 us, 4000 rows 363 -> 353)
 constexpr int kLpFound = 256;    // candidates, and batches with some, kept
 constexpr int kLpShares = 16;    // CTAs of a row at most
 constexpr int kLpGroups = 64;    // groups of threads whose maxima give the floor
@@ -64,7 +66,7 @@ __device__ __forceinline__ int key_id(Key k) { return 0x7fffffff - (int)(uint32_
 
 template <typename T, int NTH>
 struct LpSmem {
-    static constexpr int kWarps = NTH / 32, kSlots = kLpKept / NTH;
+    static constexpr int kWarps = NTH / 32, kSlots = kLpKept / (int)sizeof(T) / NTH;
     static constexpr bool kAhead = NTH == kLpMany;
     uint4 ahead[kAhead ? kLpAhead + 1 : 1][kAhead ? kLpLoads : 1][kAhead ? NTH : 1];   // batches on their way, each thread's own
     T batch_max[kSlots][NTH];
@@ -298,6 +300,7 @@ __global__ void __launch_bounds__(NTH, NTH == kLpMany ? kLpCtas : 1024 / NTH) to
     __shared__ LpCluster cl;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     constexpr bool kAhead = LpSmem<T, NTH>::kAhead;
+    static_assert(!kAhead || kLpCtas * (sizeof(sh) + 1024) <= 228 * 1024, "they fit an SM");
     if (kAhead) Z = 1;   // (no code for shares)
     const int row = blockIdx.x / Z, z = blockIdx.x % Z;
     const RowView<T> x(static_cast<const T *>(p.logits) + (long long)row * p.ld, p.vocab);
