@@ -16,6 +16,25 @@ def pytest_configure(config):
     config.addinivalue_line("markers", "gpu: needs a CUDA GPU (B200, sm_100a)")
 
 
+def reference_sources():
+    """Whether the reference's tree is on this machine (the condition under
+    which __graft_entry__.build() builds its host; an empty folder is none)."""
+    return os.path.isfile(os.path.join(os.environ.get("VOX_REFERENCE_DIR", "/root/reference"), "voxtral.c"))
+
+
+def pytest_collection_modifyitems(items):
+    """What needs the reference's sources, or its host built from them, is
+    skipped where there are none."""
+    if reference_sources():
+        return
+    host = os.path.exists(os.path.join(ROOT, "integration", "_build", "libvoxhost_cuda.so"))
+    skip = pytest.mark.skip(reason="the reference's sources are not on this machine")
+    for item in items:
+        name = os.path.basename(str(item.fspath))
+        if item.name in ("test_hooks_land_once_each", "test_a_moved_anchor_stops_the_build") or (name == "test_gpu_host_cuda.py" and not host):
+            item.add_marker(skip)
+
+
 def load_golden(name):
     return np.load(os.path.join(ROOT, "tests", "golden", name + ".npz"))
 
