@@ -611,7 +611,7 @@ int vox_cuda_rope_append_dev(const vox_cuda_kv_cache *cache, int layer, const vo
  * p = pos + i, sees the positions j <= p that the cache holds and that are
  * among the n_sink first or the `window` last (j > p - window; window 0: no
  * limit).  q, out: [n_rows][n_heads][head_dim] of the cache's type (out may
- * be q); lse: fp32 [n_rows][n_heads] log of the sum of e^score (natural), or
+ * be q, but not overlap it otherwise); lse: fp32 [n_rows][n_heads] log of the sum of e^score (natural), or
  * NULL.  n_heads: a multiple of n_kv_heads, at most 64 times as many; scale 0:
  * 1 / sqrt(head_dim).  What a masked key holds, NaN included, does not
  * matter; a row all of whose scores are -inf gets zeros and lse -inf. */

@@ -177,6 +177,12 @@ int attention(const char *who, bool tree, const vox_cuda_kv_cache *cache, int la
         set_error("%s: q and out must be 16-byte aligned device pointers", who);
         return VOX_CUDA_ERR_ARG;
     }
+    const double lines = (double)p.r.n_rows * n_heads, bytes = lines * p.c.head_dim * elem_size(p.c.dtype);
+    if ((q != out && overlap(q, bytes, out, bytes)) || overlap(lse, lines * sizeof(float), q, bytes) ||
+        overlap(lse, lines * sizeof(float), out, bytes)) {   // CTAs would read what others have written
+        set_error("%s: out is q itself or apart from it, lse apart from both", who);
+        return VOX_CUDA_ERR_ARG;
+    }
     if ((long long)p.r.max_rows * (n_heads / p.c.n_kv_heads) > (1 << 28)) {
         set_error("%s: too many rows of a stream (%d)", who, p.r.max_rows);
         return VOX_CUDA_ERR_ARG;
