@@ -344,8 +344,10 @@ __global__ void __launch_bounds__(at_threads(NT, RT), at_ctas(HD, NT, RT)) attn_
         mbar_init(&sh.o_done, 1);
         mbar_init(&sh.stall, 1);
         sh.bad = sh.failed = 0;
-        prefetch_tensormap(&tm_k);
-        prefetch_tensormap(&tm_v);
+        if (p.maps) {
+            prefetch_tensormap(&tm_k);
+            prefetch_tensormap(&tm_v);
+        }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == kWarpMma) {
