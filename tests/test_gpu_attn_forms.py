@@ -34,6 +34,7 @@ TENSOR = [
     ((8, 2, 128, 5200, 8, 1, None), (32, 2, 6), 64), ((8, 2, 64, 5200, 8, 1, None), (32, 2, 6), 64),
     ((32, 32, 64, 600, 16, 8, 3), (32, 2, 1), 64),
     ((32, 8, 128, 1600, 8, 30, None), (128, 2, 4), 64), ((32, 8, 128, 600, 8, 61, 3), (128, 2, 1), 64),
+    ((32, 8, 128, 4100, 4, 400, None), (128, 2, 1), 256),   # (200 two-tile CTAs would be two whole waves)
     ((8, 2, 64, 1600, 8, 256, None), (128, 3, 3), 64), ((32, 32, 64, 1600, 8, 61, 4), (128, 3, 1), 128),
     ((32, 8, 128, 5200, 2, 520, None), (256, 1, 1), 320), ((32, 8, 128, 5200, 2, 256, 5), (256, 1, 2), 128),
     ((32, 8, 128, 1600, 16, 61, 3), (256, 1, 1), 128), ((8, 2, 128, 1600, 16, 256, None), (256, 1, 1), 128)]

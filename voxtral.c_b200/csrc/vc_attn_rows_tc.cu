@@ -796,9 +796,13 @@ cudaError_t plan_tiles(const RowsAttnParams &p, Plan *out) {
     const long long tiles = (M + NT * RT - 1) / (NT * RT);
     const long long clusters = tiles * p.c.n_kv_heads * p.c.n_streams, blocks = (most_keys(p, NT * RT) + kKeys - 1) / kKeys;
     // Shares: the least time in units of a block, with kAtFixed for each wave's
-    // starts and merges.  Several waves run into each other, so their blocks
-    // count in proportion; in one wave a CTA alone on its SM is faster than one
-    // beside others.  (The device counts these clusters for one CTA to an SM.)
+    // starts and merges.  With several CTAs to an SM waves run into each other,
+    // so their blocks count in proportion; with one, equal CTAs end together and
+    // a started wave is a whole one (4 streams of 400 rows of 32 / 8 heads over
+    // 4100 keys, 200 two-tile CTAs: 177 us, 400 of one tile 150; 12 / 12 heads, 16 streams of
+    // 800 rows over 5200 keys 598 / 499).  In one wave a CTA
+    // alone on its SM is faster than one beside others.  (The device counts
+    // these clusters for one CTA to an SM.)
     // 24 x 8 tiles of 65 blocks: 1 share 70 us, 2 58, 4 66; 8 x 8 tiles: 2
     // shares 39, 4 33; 128 tiles of 128 rows, 9 blocks: 1 share 17, 2 25.
     for (int Z = 1; Z <= kMaxCluster && Z <= blocks; Z++) {
@@ -807,8 +811,8 @@ cudaError_t plan_tiles(const RowsAttnParams &p, Plan *out) {
         if (at_once < 1) continue;
         at_once *= kPer;
         const double fill = (double)clusters / at_once, part = (double)blocks / Z;
-        const double t = part * (fill > 1.0 ? fill : kPer > 1 && fill * kPer <= 1.0 ? kAtAlone : 1.0) + std::max(1.0, ceil(fill)) * kAtFixed +
-                         (Z > 1 && RT == kAtRows ? kAtMerge : 0.0);
+        const double waves = kPer == 1 ? std::max(1.0, ceil(fill)) : fill > 1.0 ? fill : fill * kPer <= 1.0 ? kAtAlone : 1.0;
+        const double t = part * waves + std::max(1.0, ceil(fill)) * kAtFixed + (Z > 1 && RT == kAtRows ? kAtMerge : 0.0);
         if (t < out->cost) {
             out->cost = t;
             out->shares = Z;
