@@ -521,6 +521,7 @@ __global__ void __launch_bounds__(at_threads(NT, RT), at_ctas(HD, NT, RT)) attn_
             }
             warp_commit(&sh.o_done, lead);
         }
+        if (p.stall_ns) ok = warp_wait(&sh.stall, 0u, globaltimer() + p.stall_ns) && ok;
     } else {
         // ---- softmax: thread = packed row ----
         const int t = warp / kSoft, q = warp % kSoft, ml = t * RT + 32 * q + lane, m = m0 + ml;
@@ -678,7 +679,6 @@ __global__ void __launch_bounds__(at_threads(NT, RT), at_ctas(HD, NT, RT)) attn_
             }
         }
     }
-    if (p.stall_ns && warp == kWarpMma) ok = warp_wait(&sh.stall, 0u, globaltimer() + p.stall_ns) && ok;
     if (!ok) {
         sh.failed = 1;
         if (p.err) atomicExch_system(p.err, 1u);
