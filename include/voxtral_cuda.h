@@ -614,7 +614,12 @@ int vox_cuda_rope_append_dev(const vox_cuda_kv_cache *cache, int layer, const vo
  * be q, but not overlap it otherwise); lse: fp32 [n_rows][n_heads] log of the sum of e^score (natural), or
  * NULL.  n_heads: a multiple of n_kv_heads, at most 64 times as many; scale 0:
  * 1 / sqrt(head_dim).  What a masked key holds, NaN included, does not
- * matter; a row all of whose scores are -inf gets zeros and lse -inf. */
+ * matter; a row all of whose scores are -inf gets zeros and lse -inf.
+ * Scores, sums and lse are fp32.  With a 16-bit cache the softmax weights are
+ * rounded to the cache's type before their product with V (each is off by half
+ * a step of it, or in fp16 by 2^-32 of the row's largest where that is more),
+ * and part of the 2^x are a polynomial good to 2.6e-6.  fp32 caches keep fp32
+ * weights. */
 int vox_cuda_attention_window_dev(const vox_cuda_kv_cache *cache, int layer, const vox_cuda_rows *rows,
                                   const void *q, int n_heads, int window, float scale, void *out, float *lse,
                                   void *stream);
@@ -653,7 +658,9 @@ int vox_cuda_kv_fork_dev(const vox_cuda_kv_cache *cache, const int *src, const i
  * [n_rows][n_top], best first, ties to the lowest id (top_logprob may be
  * NULL).  A logit of -inf has probability 0; a row with a NaN or +inf, or
  * without a finite logit, gives NaN, and NaN logits are no alternatives
- * (places left over get id -1).  Enqueued on `stream` as the row operators. */
+ * (places left over get id -1).  An offset common to a row's logits changes
+ * nothing; the sums are fp32, good to about 1e-6 of ln Z and of the entropy for
+ * 131072 logits.  Enqueued on `stream` as the row operators. */
 int vox_cuda_token_logprobs_dev(const void *logits, int type, int n_rows, int vocab, long long row_stride,
                                 const int *tokens, int n_top, float *logprob, float *entropy, int *top_ids,
                                 float *top_logprob, void *stream);

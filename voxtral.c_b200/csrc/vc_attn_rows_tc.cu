@@ -50,8 +50,10 @@ constexpr int kAtHalf = 64;             // keys per softmax step
 constexpr int kAtRows = 128;            // packed rows per MMA tile = TMEM lanes
 // Shapes: NT tiles of RT rows that exist (the MMA's other rows are whatever
 // lies behind Q in shared memory; nobody reads their lanes).
-//   <2, 128>  heads of 128, many rows over long contexts: bound by the MMAs'
-//             reads of shared memory and the exponentials.  128-key blocks (an MMA of N
+//   <2, 128>  heads of 128, many rows over long contexts: bound by the
+//             latency of the softmax chain (~5450 cycles a block; the MMAs'
+//             reads of shared memory are ~1540, the exponentials ~1280).
+//             128-key blocks (an MMA of N
 //             64 takes as long as one of N 128, reading its A tile), one CTA
 //             per SM.  2021 rows of 32 heads over 4100 keys, bf16: 195 to
 //             200 us, 0.41 of the bf16 rate (two S ranges of 64 keys: 229)
@@ -59,8 +61,10 @@ constexpr int kAtRows = 128;            // packed rows per MMA tile = TMEM lanes
 //             is ready when the softmax is done with S(b); two CTAs per SM.
 //             Heads of 64, any number of rows (at_three): one S range, 128 TMEM
 //             columns, three CTAs per SM, whose chains S - softmax - P - P.V
-//             fill each other's gaps.  1500 rows of 32 heads, window 750: 52 us
-//             (<2, 128> took 72: 192 CTAs in two waves)
+//             fill each other's gaps.  1500 rows of 32 heads, window 750: 51 us
+//             (<2, 128> took 72: 192 CTAs in two waves; vc_enc_attn_tc.cu, whose
+//             P goes through shared memory, so that S(b + 1) need not wait for
+//             it, takes 31 over its own ring)
 //   <1, 32>   up to 32 rows, a token's or a few tokens' heads, bound by HBM: Q
 //             is small, 96 KB of keys in flight per CTA, two CTAs per SM.  24
 //             tokens of 32 / 8 heads over 4100 keys: 57 us, 4.7 TB/s, 0.73 of
