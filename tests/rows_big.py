@@ -41,7 +41,7 @@ class Big:
         hide = torch.ones(streams, cap, dtype=torch.bool)
         for s, (p, n) in enumerate(zip(positions, counts)):
             end, ring = p + n, cap - n_sink
-            j = torch.tensor([] if p < 0 else list(range(min(end, n_sink))) + list(range(max(n_sink, end - ring), end)), dtype=torch.long)
+            j = torch.tensor([] if p < 0 or n == 0 else list(range(min(end, n_sink))) + list(range(max(n_sink, end - ring), end)), dtype=torch.long)
             self.key_pos.append(j)
             i = torch.arange(n)
             if tree:
@@ -104,6 +104,8 @@ class Big:
         keep = [d for d in range(self.dim) if d not in skip]
         for s, (p, n) in enumerate(zip(self.positions, self.counts)):
             a, b = self.start[s], self.start[s] + n
+            if n == 0:
+                continue
             if p < 0:
                 assert bool((out[a:b] == 7.0).all()) and bool((lse[a:b] == 7.0).all())
                 continue
