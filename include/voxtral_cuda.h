@@ -650,6 +650,77 @@ int vox_cuda_kv_commit_dev(const vox_cuda_kv_cache *cache, const int *pos, const
 int vox_cuda_kv_fork_dev(const vox_cuda_kv_cache *cache, const int *src, const int *dst, int n, const int *pos,
                          void *stream);
 
+/* ------------------------------------------------------------------------
+ * The same over a paged cache in 8 bits, for servers of many or long streams:
+ * a position costs half of what it does in 16 bits, and a stream owns only the
+ * pages that it has filled.  Rotary append, attention (one token, drafted
+ * tokens, chunks, whole prompts), copies of pages.  What is said of the row
+ * operators above - streams, devices, captures, waits - holds for these too.
+ * ------------------------------------------------------------------------ */
+
+/* A pool of pages.  Page g of a layer holds page_size positions of every KV
+ * head: element (layer, page, head, slot, dim) of k and v lies at layer *
+ * layer_stride + page * page_stride + head * head_stride + slot * slot_stride +
+ * dim, e4m3, one byte each.  A stride of 0 is the contiguous one for
+ * [layer][page][head][slot][dim]; others are multiples of 16 bytes, and k and v
+ * are 16-byte aligned.  A number of the cache is its e4m3 value times the scale
+ * of its page and head, k_scale / v_scale [n_layers][n_pages][n_kv_heads]: powers
+ * of two, as vox_cuda_rope_append_paged_dev writes them (K and V apart).
+ * Position j of stream s is slot j mod page_size of page table[s * table_stride +
+ * j / page_size].  An entry outside [0, n_pages) is a page that is not there:
+ * no row sees its positions, and what is appended to it is dropped.  A stream
+ * has table_stride * page_size positions at most (rows->max_rows is no more
+ * than that); rows beyond are left out.
+ * Streams may share pages that they only read. */
+typedef struct {
+    void *k, *v;                 /* device */
+    float *k_scale, *v_scale;    /* device */
+    const int *table;            /* device [n_streams][table_stride] */
+    int table_stride;
+    int n_layers, n_pages, page_size;        /* page_size 16, 32, 64 or 128 */
+    int n_streams, n_kv_heads, head_dim;     /* head_dim 64 or 128 */
+    long long layer_stride, page_stride, head_stride, slot_stride;   /* bytes */
+} vox_cuda_paged_cache;
+
+/* One pass over rows of fused q|k|v projections, as vox_cuda_rope_append_dev
+ * (norm, rotation, arguments), into a paged cache: q goes to q_out
+ * [n_rows][n_heads][head_dim] of type q_type (bf16 or fp16), k and v to the
+ * rows' slots.  qkv_type: fp32 or q_type.  rows->parent is NULL.
+ * Scales: with a = the largest finite |x| of a page's new values of a head, the
+ * scale becomes s = 2^e, e the smallest whole number >= -100 with a <= 448 * 2^e,
+ * when the page's slot 0 is among the new rows; else the larger of s and what it
+ * was, and where it grows, the earlier slots are rounded again under the new
+ * scale (exact but for values below 2^-6 of it).  Values are rounded to nearest
+ * even; what is not finite becomes NaN.  Slots behind the new rows stay as they
+ * were.  The pages that a call writes belong to one stream each. */
+int vox_cuda_rope_append_paged_dev(const vox_cuda_paged_cache *cache, int layer, const vox_cuda_rows *rows,
+                                   const void *qkv, int qkv_type, int n_heads, long long qkv_stride,
+                                   const float *q_norm, const float *k_norm, float eps, float theta, void *q_out,
+                                   int q_type, void *stream);
+
+/* Attention of rows whose keys are in the paged cache already: row i, at
+ * position p = pos + i, sees the positions j <= p whose pages are there and that
+ * are among the n_sink first or the `window` last (j > p - window; window 0: no
+ * limit).  q, out: [n_rows][n_heads][head_dim] of type q_type, bf16 or fp16 (out
+ * may be q, but not overlap it otherwise); lse: fp32 [n_rows][n_heads] log of
+ * the sum of e^score (natural), or NULL.  n_heads: a multiple of n_kv_heads, at
+ * most 64 times as many; scale 0: 1 / sqrt(head_dim).  What a masked key holds,
+ * NaN included, does not matter; a row that sees no key, or all of whose scores
+ * are -inf, gets zeros and lse -inf.  Entries of the table whose positions no
+ * row sees are not followed: their pages may be given to others.
+ * Scores, sums and lse are fp32; the softmax weights are rounded to 16 bits
+ * (fp16, relative to the largest) before their product with V. */
+int vox_cuda_attention_paged_dev(const vox_cuda_paged_cache *cache, int layer, const vox_cuda_rows *rows,
+                                 const void *q, int q_type, int n_heads, int window, int n_sink, float scale,
+                                 void *out, float *lse, void *stream);
+
+/* Copy pages src[i] to pages dst[i] with their scales, in every layer, for
+ * i < n.  src, dst: device [n]; a pair with an entry outside [0, n_pages) is
+ * left out.  No page is written twice, or both read and written.  A fork of a
+ * stream shares its full pages through the table and copies the one that both
+ * would append to. */
+int vox_cuda_kv_copy_pages_dev(const vox_cuda_paged_cache *cache, const int *src, const int *dst, int n, void *stream);
+
 /* Natural log probability of a given token, entropy (nats) and the n_top
  * (0..32) most likely ids of each row of logits [n_rows][vocab], row_stride
  * elements apart (0: vocab), fp32, bf16 or fp16.  tokens: device [n_rows] with

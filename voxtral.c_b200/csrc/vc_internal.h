@@ -200,6 +200,51 @@ cudaError_t launch_attn_rows(const RowsAttnParams &p, cudaStream_t st, RowsPlan 
 // the tensor-core kernel of the 16-bit types (vc_attn_rows_tc.cu)
 cudaError_t launch_attn_rows_tc(const RowsAttnParams &p, cudaStream_t st, RowsPlan *only = nullptr);
 
+// ---- the same over a paged cache in 8 bits (vc_rt_paged.cu and its kernels) ----
+struct PagedView {            // vox_cuda_paged_cache, checked
+    unsigned char *k, *v;     // layer 0, page 0, head 0, slot 0
+    float *k_scale, *v_scale; // [layer][page][head]
+    const int *table;         // [stream][table_stride]
+    long long layer_stride, page_stride, head_stride, slot_stride;   // bytes
+    int table_stride, n_layers, n_pages, page, page_shift;           // page = 1 << page_shift
+    int n_streams, n_kv_heads, head_dim;
+};
+struct PagedAppendParams {
+    PagedView c;
+    RowsView r;
+    int layer;
+    const void *qkv;          // [n_rows] rows of (n_heads + 2 n_kv_heads) heads
+    int src_type;             // ElemType of qkv
+    long long ld;             // elements between its rows
+    int n_heads, group;
+    const float *q_norm, *k_norm;   // [head_dim] or NULL
+    float eps;
+    int rotate;               // 0: q and k keep their angles
+    double log2_theta;
+    void *q_out;              // [n_rows][n_heads][head_dim]
+    int q_type;
+};
+cudaError_t launch_paged_append(const PagedAppendParams &p, cudaStream_t st);
+struct PagedAttnParams {
+    PagedView c;
+    RowsView r;
+    int layer;
+    const void *q;            // [n_rows][n_heads][head_dim]
+    void *out;                // the same shape and type
+    int q_type;
+    float *lse;               // [n_rows][n_heads] or NULL
+    int n_heads, group;
+    int window, n_sink;       // window 0: no limit
+    float scale_log2;         // scale * log2(e)
+};
+cudaError_t launch_paged_attn(const PagedAttnParams &p, cudaStream_t st);
+struct PagedCopyParams {
+    PagedView c;
+    const int *src, *dst;     // [n]
+    int n;
+};
+cudaError_t launch_paged_copy(const PagedCopyParams &p, int sms, cudaStream_t st);
+
 struct AppendParams {
     CacheView c;
     RowsView r;

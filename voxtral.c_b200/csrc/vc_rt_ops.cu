@@ -3,41 +3,12 @@
 // log probabilities: argument checks and launches.  None of them allocates,
 // waits for the host or keeps a workspace, so calls on different streams are
 // independent and a call may be captured into a CUDA graph.
-#include "vc_runtime.h"
+#include "vc_rt_check.h"
 
 using namespace vc;
 using namespace vc::rt;
 
 namespace {
-
-bool aligned16(const void *p) { return ((uintptr_t)p & 15u) == 0; }
-int elem_size(int dtype) { return dtype == ELEM_F32 ? 4 : 2; }
-bool known_type(int dtype) { return dtype == ELEM_F32 || dtype == ELEM_BF16 || dtype == ELEM_F16; }
-
-// Launches go to the library's device of the calling thread, whichever device
-// the caller's other code made current.
-class DeviceGuard {
-  public:
-    explicit DeviceGuard(int device) {
-        if (cudaGetDevice(&before_) != cudaSuccess) before_ = -1;
-        if (before_ != device) ok_ = cudaSetDevice(device) == cudaSuccess;
-        else before_ = -1;
-    }
-    ~DeviceGuard() {
-        if (before_ >= 0) cudaSetDevice(before_);
-    }
-    bool ok() const { return ok_; }
-
-  private:
-    int before_ = -1;
-    bool ok_ = true;
-};
-
-// [a, a + an) and [b, b + bn) share a byte
-bool overlap(const void *a, double an, const void *b, double bn) {
-    const double x = (double)(uintptr_t)a, y = (double)(uintptr_t)b;
-    return a && b && x < y + bn && y < x + an;
-}
 
 int check_cache(const char *who, const vox_cuda_kv_cache *c, CacheView *out) {
     if (!c || !c->k || !c->v) {
@@ -98,75 +69,13 @@ int check_cache(const char *who, const vox_cuda_kv_cache *c, CacheView *out) {
     return VOX_CUDA_OK;
 }
 
-// parents: 0 refused, 1 optional, 2 required
-int check_rows(const char *who, const vox_cuda_rows *r, const CacheView &c, int parents, RowsView *out) {
-    if (!r || !r->pos) {
-        set_error("%s: no rows or positions", who);
-        return VOX_CUDA_ERR_ARG;
-    }
-    if (r->n_rows < 0 || r->max_rows < 0 || r->max_rows > r->n_rows || (r->n_rows > 0 && r->max_rows < 1)) {
-        set_error("%s: bad row counts (%d rows, at most %d of a stream)", who, r->n_rows, r->max_rows);
-        return VOX_CUDA_ERR_ARG;
-    }
-    if (!r->row_start && r->n_rows > 0 && (r->n_rows != c.n_streams || r->max_rows != 1)) {
-        set_error("%s: without row_start there is one row for each of the %d streams, not %d", who, c.n_streams, r->n_rows);
-        return VOX_CUDA_ERR_ARG;
-    }
-    if ((parents == 2 && !r->parent) || (parents == 0 && r->parent)) {
-        set_error(parents ? "%s: a tree needs the rows' parents" : "%s: the rows of a window have no parents", who);
-        return VOX_CUDA_ERR_ARG;
-    }
-    if (r->parent && r->max_rows > kTreeMax) {
-        set_error("%s: a tree holds at most %d rows of a stream, not %d", who, kTreeMax, r->max_rows);
-        return VOX_CUDA_ERR_ARG;
-    }
-    if (r->max_rows > c.ring) {
-        set_error("%s: a ring of %d positions cannot hold %d rows", who, c.ring, r->max_rows);
-        return VOX_CUDA_ERR_CAPACITY;
-    }
-    out->pos = r->pos;
-    out->start = r->row_start;
-    out->parent = r->parent;
-    out->n_rows = r->n_rows;
-    out->max_rows = r->max_rows;
-    return VOX_CUDA_OK;
-}
-
-int check_layer(const char *who, int layer, const CacheView &c) {
-    if (layer >= 0 && layer < c.n_layers) return VOX_CUDA_OK;
-    set_error("%s: layer %d of %d", who, layer, c.n_layers);
-    return VOX_CUDA_ERR_ARG;
-}
-
-int check_heads(const char *who, int n_heads, const CacheView &c) {
-    if (n_heads >= 1 && n_heads % c.n_kv_heads == 0 && n_heads / c.n_kv_heads <= kMaxGroup) return VOX_CUDA_OK;
-    set_error("%s: %d heads over %d KV heads (a multiple of them, at most %d times as many)", who, n_heads, c.n_kv_heads,
-              kMaxGroup);
-    return VOX_CUDA_ERR_ARG;
-}
-
-// A wait that ran out in the kernel of an earlier call of this thread is
-// reported once; that call's rows are NaN.
-int check_waits(const char *who, DevCtx *c) {
-    if (!__atomic_exchange_n(c->op_err + op_slot(), 0u, __ATOMIC_RELAXED)) return VOX_CUDA_OK;
-    set_error("%s: a device-side wait of an earlier call of this thread timed out (its rows are void: NaN)", who);
-    return VOX_CUDA_ERR_CUDA;
-}
-
-int launched(const char *who, cudaError_t e) {
-    if (e == cudaSuccess) return VOX_CUDA_OK;
-    cudaGetLastError();   // reported here, not by whoever asks next
-    set_error("%s: %s", who, cudaGetErrorString(e));
-    return VOX_CUDA_ERR_CUDA;
-}
-
 int attention(const char *who, bool tree, const vox_cuda_kv_cache *cache, int layer, const vox_cuda_rows *rows, const void *q,
               int n_heads, int window, float scale, void *out, float *lse, void *stream, int stall_ms = 0,
               RowsPlan *only = nullptr) {
     RowsAttnParams p = {};
     int rc = check_cache(who, cache, &p.c);
-    if (rc || (rc = check_rows(who, rows, p.c, tree ? 2 : 0, &p.r)) || (rc = check_layer(who, layer, p.c)) ||
-        (rc = check_heads(who, n_heads, p.c)))
+    if (rc || (rc = check_rows(who, rows, p.c.n_streams, p.c.ring, tree ? 2 : 0, &p.r)) ||
+        (rc = check_layer(who, layer, p.c.n_layers)) || (rc = check_heads(who, n_heads, p.c.n_kv_heads)))
         return rc;
     if (window < 0 || !(fabsf(scale) <= 2.0e38f)) {
         set_error("%s: bad window or scale", who);
@@ -255,8 +164,8 @@ extern "C" int vox_cuda_rope_append_dev(const vox_cuda_kv_cache *cache, int laye
     const char *who = "rope_append";
     AppendParams p = {};
     int rc = check_cache(who, cache, &p.c);
-    if (rc || (rc = check_rows(who, rows, p.c, 1, &p.r)) || (rc = check_layer(who, layer, p.c)) ||
-        (rc = check_heads(who, n_heads, p.c)))
+    if (rc || (rc = check_rows(who, rows, p.c.n_streams, p.c.ring, 1, &p.r)) ||
+        (rc = check_layer(who, layer, p.c.n_layers)) || (rc = check_heads(who, n_heads, p.c.n_kv_heads)))
         return rc;
     if (qkv_type != ELEM_F32 && qkv_type != p.c.dtype) {
         set_error("%s: q|k|v must be fp32 or of the cache's type", who);

@@ -82,6 +82,21 @@ class KvCache(C.Structure):
                          stream_stride, slot_stride, head_stride)
 
 
+class PagedCache(C.Structure):
+    """A pool of pages of K and V in e4m3 with a scale per page and head
+    (vox_cuda_paged_cache); device addresses, strides in bytes (0: contiguous
+    [layer][page][head][slot][dim])."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p), ("table", C.c_void_p),
+                ("table_stride", C.c_int), ("n_layers", C.c_int), ("n_pages", C.c_int), ("page_size", C.c_int),
+                ("n_streams", C.c_int), ("n_kv_heads", C.c_int), ("head_dim", C.c_int), ("layer_stride", C.c_longlong),
+                ("page_stride", C.c_longlong), ("head_stride", C.c_longlong), ("slot_stride", C.c_longlong)]
+
+    def __init__(self, k=None, v=None, k_scale=None, v_scale=None, table=None, table_stride=0, n_layers=1, n_pages=0, page_size=64,
+                 n_streams=1, n_kv_heads=8, head_dim=128, layer_stride=0, page_stride=0, head_stride=0, slot_stride=0):
+        super().__init__(k, v, k_scale, v_scale, table, table_stride, n_layers, n_pages, page_size, n_streams, n_kv_heads,
+                         head_dim, layer_stride, page_stride, head_stride, slot_stride)
+
+
 class Rows(C.Structure):
     """The rows of a call (vox_cuda_rows): device addresses of the streams'
     positions, their row ranges (None: one row each) and the rows' parents
@@ -194,6 +209,12 @@ def lib():
         "vox_cuda_kv_commit_dev": ([C.POINTER(KvCache), C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, C.c_int,
                                     C.c_void_p, C.c_void_p], C.c_int),
         "vox_cuda_kv_fork_dev": ([C.POINTER(KvCache), _ip, _ip, C.c_int, C.c_void_p, C.c_void_p], C.c_int),
+        "vox_cuda_rope_append_paged_dev": ([C.POINTER(PagedCache), C.c_int, C.POINTER(Rows), C.c_void_p, C.c_int, C.c_int,
+                                            C.c_longlong, C.c_void_p, C.c_void_p, C.c_float, C.c_float, C.c_void_p, C.c_int,
+                                            C.c_void_p], C.c_int),
+        "vox_cuda_attention_paged_dev": ([C.POINTER(PagedCache), C.c_int, C.POINTER(Rows), C.c_void_p, C.c_int, C.c_int,
+                                          C.c_int, C.c_int, C.c_float, C.c_void_p, C.c_void_p, C.c_void_p], C.c_int),
+        "vox_cuda_kv_copy_pages_dev": ([C.POINTER(PagedCache), C.c_void_p, C.c_void_p, C.c_int, C.c_void_p], C.c_int),
         "vox_cuda_token_logprobs_dev": ([C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_longlong, C.c_void_p, C.c_int,
                                          C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p], C.c_int),
         "vox_cuda_fill_normal_bf16_dev": ([C.c_void_p, C.c_size_t, C.c_uint64, C.c_float,
@@ -428,6 +449,24 @@ def kv_fork_dev(cache, src, dst, pos, stream=None):
         raise ValueError("kv_fork_dev: as many sources as destinations")
     arr = C.c_int * len(src)
     check(lib().vox_cuda_kv_fork_dev(cache, arr(*src), arr(*dst), len(src), pos, stream), "kv_fork_dev")
+
+
+def rope_append_paged_dev(cache, layer, rows, qkv, qkv_type, n_heads, qkv_stride, q_norm, k_norm, eps, theta, q_out, q_type,
+                          stream=None):
+    """Norm (optional), rotation and write of fused q|k|v rows to a paged 8-bit cache."""
+    check(lib().vox_cuda_rope_append_paged_dev(cache, layer, rows, qkv, TYPES[qkv_type], n_heads, qkv_stride, q_norm, k_norm, eps,
+                                               theta, q_out, TYPES[q_type], stream), "rope_append_paged_dev")
+
+
+def attention_paged_dev(cache, layer, rows, q, q_type, n_heads, window, n_sink, scale, out, lse=None, stream=None):
+    """Attention of rows over a paged 8-bit cache, with a sliding window and sinks."""
+    check(lib().vox_cuda_attention_paged_dev(cache, layer, rows, q, TYPES[q_type], n_heads, window, n_sink, scale, out, lse,
+                                             stream), "attention_paged_dev")
+
+
+def kv_copy_pages_dev(cache, src, dst, n, stream=None):
+    """Copy pages with their scales, in every layer (src, dst: device addresses of n page numbers)."""
+    check(lib().vox_cuda_kv_copy_pages_dev(cache, src, dst, n, stream), "kv_copy_pages_dev")
 
 
 def token_logprobs_dev(logits, dtype, n_rows, vocab, row_stride, tokens, n_top, logprob, entropy, top_ids, top_logprob,
