@@ -236,8 +236,9 @@ struct PagedAttnParams {
     int n_heads, group;
     int window, n_sink;       // window 0: no limit
     float scale_log2;         // scale * log2(e)
+    int shares;               // key shares of a row tile (set by the launch)
 };
-cudaError_t launch_paged_attn(const PagedAttnParams &p, cudaStream_t st);
+cudaError_t launch_paged_attn(const PagedAttnParams &p, int sms, cudaStream_t st);
 struct PagedCopyParams {
     PagedView c;
     const int *src, *dst;     // [n]

@@ -1,87 +1,502 @@
-// vc_paged_attn.cu - attention of a call's rows over a paged cache in 8 bits.
+// vc_paged_attn.cu - attention of a few rows per stream over a paged cache in
+// 8 bits: one token, a few drafted ones.
+//
+// Bound by HBM: every key is read once, 2 HD bytes, and 4 HD operations per
+// query head of its group follow, on the tensor cores (mma.sync m16n8k16, fp16
+// operands, fp32 sums), which leaves them mostly idle at these row counts.
+// Nothing goes through shared memory on its way: e4m3 is exact in fp16, and the
+// orders of dims and keys within an MMA are free as long as both operands have
+// the same, so that each lane takes 16 consecutive bytes of a key at a time:
+//   S^T = K Q^T    A = 16 keys, lane (g, t) has dims 16 t .. 16 t + 15 (and 64
+//                  more on) of keys g and g + 8; B = packed rows (row x head of
+//                  the group), 8 to a column tile
+//   O^T += V^T P^T A = V^T, lane (g, t) has dims g HD / 8 .. of keys 2 t, 2 t + 1,
+//                  2 t + 8, 2 t + 9, which a byte permutation pairs; B = P^T,
+//                  which is S^T transposed in 8 x 8 tiles (movmatrix)
+// A lane's S and O columns are the same two packed rows, so that their maximum
+// and sum are its own.
+//
+// A warp takes 32 keys at a time, by itself, and holds the next 32 keys' K while
+// it works on P and V, the next V while it works on S: 8 KB in flight per warp,
+// 12 warps to an SM.  Its CTA's warps and then the CTAs of a cluster, which
+// share the keys of a tile of rows, join their sums at the end, in order.
+//
+// q: bf16 rows are scaled by a power of two into fp16's range (exact but for
+// values 2^-29 of the row's largest).  The weights P = 2^(s - m) are rounded to
+// fp16, half a step of 2^-11; m is the running maximum less 7, and moves only when
+// a score exceeds it by 15, so that P fills the type up to 2^15 and what is lost
+// is 2^-32 of the largest weight per key.  V's scales go into P relative to the
+// largest of them so far.  Sums, maxima and O are fp32.
+#include "vc_cluster.h"
 #include "vc_paged.cuh"
+#include "vc_tc.cuh"
+
+#include <math.h>
 
 namespace vc {
 
+using namespace tc;
+
 namespace {
 
-// A CTA has one row and the query heads of a KV head, a warp every fourth key:
-// a lane holds HD / 32 dims of q, K and V, and the running maximum, sum and
-// output of its warp's keys, which the CTA joins at the end.
-constexpr int kPtWarps = 4;
+constexpr int kFwWarps = 4, kFwThreads = kFwWarps * 32;
+constexpr int kFwKeys = 32;              // keys of a warp's step
+constexpr float kFwBelow = 7.f;          // the maximum less m
+constexpr float kFwAbove = 15.f;         // log2 of what a weight may reach before m moves
+
+__device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose8(uint32_t v) {
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
+}
+__device__ __forceinline__ uint32_t half2_bits(uint32_t e4m3x2) {
+    const __half2 h = from_e4m3x2(e4m3x2);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+// 4 N bytes of the cache, read once: no place in L1
+template <int N>
+__device__ __forceinline__ void load_words(uint32_t *w, const unsigned char *p) {
+    if constexpr (N == 4)
+        asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "l"(p));
+    else
+        asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "l"(p));
+}
+
+template <int HD, int NR>
+struct FwSmem {
+    float o[kFwWarps][8 * NR][HD];
+    float mx[kFwWarps][8 * NR], sum[kFwWarps][8 * NR];
+};
+
+// NR: column tiles of 8 packed rows
+template <typename T, int HD, int NR>
+__global__ void __launch_bounds__(kFwThreads, NR == 1 ? 3 : 2) paged_few_kernel(const PagedAttnParams p) {
+    constexpr int KC = HD / 64;       // 64-dim parts of a key
+    constexpr int MT = HD / 16;       // 16-dim tiles of O
+    constexpr int VW = HD / 32;       // words that a lane has of a V row
+    constexpr int kRows = 8 * NR;
+    __shared__ FwSmem<HD, NR> sh;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int z = blockIdx.x % p.shares, Z = p.shares;
+    const int m0 = blockIdx.x / p.shares * kRows, kvh = blockIdx.y, stream = blockIdx.z;
+    const RowSpan s = paged_span(p.r, p.c, stream);
+    const int M = s.n * p.group;
+    if (m0 >= M) return;   // the whole cluster leaves
+    const int i0 = m0 / p.group, i1 = (min(m0 + kRows, M) - 1) / p.group;
+    // positions that some row sees: [0, ns) and [lo, hi), in units of 32
+    const int p_min = s.pos + i0, p_max = s.pos + i1, hi = p_max + 1, ns = min(p.n_sink, hi);
+    const int lo = p.window > 0 ? max(0, p_min - p.window + 1) : 0;
+    const int sink_units = (ns + kFwKeys - 1) / kFwKeys, first = max(lo / kFwKeys, sink_units);
+    const int units = sink_units + max(0, (hi + kFwKeys - 1) / kFwKeys - first);
+    const int u0 = (int)((long long)z * units / Z), u1 = (int)((long long)(z + 1) * units / Z);
+    auto key_of = [&](int u) { return (u < sink_units ? u : first + u - sink_units) * kFwKeys; };
+
+    // q as B operands: lane (g, t) has row g's dims in the order of K's
+    uint32_t qf[NR][KC * 4][2];
+    float cf[NR][2];          // score factor of the lane's rows 2 t, 2 t + 1, in log2
+    int at[NR][2];            // their positions; -1: no row
+#pragma unroll
+    for (int n = 0; n < NR; n++) {
+        const int m = m0 + n * 8 + g;
+        float x[KC][16], big = 0.f;
+        if (m < M) {
+            const T *q = static_cast<const T *>(p.q) + ((long long)(s.r0 + m / p.group) * p.n_heads + kvh * p.group + m % p.group) * HD;
+#pragma unroll
+            for (int c = 0; c < KC; c++)
+#pragma unroll
+                for (int e = 0; e < 16; e += 4) {
+                    const float4 v = load4<T>(q + c * 64 + t * 16 + e);
+                    x[c][e] = v.x, x[c][e + 1] = v.y, x[c][e + 2] = v.z, x[c][e + 3] = v.w;
+                }
+        } else {
+#pragma unroll
+            for (int c = 0; c < KC; c++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) x[c][e] = 0.f;
+        }
+        float up = 1.f;       // a power of two that takes the row's largest to [2^14, 2^15)
+        if constexpr (sizeof(T) == 2 && !std::is_same<T, __half>::value) {
+#pragma unroll
+            for (int c = 0; c < KC; c++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) big = fmaxf(big, fabsf(x[c][e]) < INFINITY ? fabsf(x[c][e]) : 0.f);
+            big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
+            big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
+            const int e = (int)(__float_as_uint(big) >> 23) - 127;
+            up = big > 0.f ? __uint_as_float((uint32_t)(min(14 - e, 126) + 127) << 23) : 1.f;
+        }
+#pragma unroll
+        for (int c = 0; c < KC; c++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                qf[n][c * 4 + e][0] = pack2<__half>(x[c][4 * e] * up, x[c][4 * e + 1] * up);
+                qf[n][c * 4 + e][1] = pack2<__half>(x[c][4 * e + 2] * up, x[c][4 * e + 3] * up);
+            }
+        const float f = p.scale_log2 / up;
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+            const int mm = m0 + n * 8 + 2 * t + e;
+            cf[n][e] = __shfl_sync(0xffffffffu, f, (2 * t + e) * 4);
+            at[n][e] = mm < M ? s.pos + mm / p.group : -1;
+        }
+    }
+
+    float o[NR][MT][4], mb[NR][2], l[NR][2];
+#pragma unroll
+    for (int n = 0; n < NR; n++) {
+#pragma unroll
+        for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) o[n][mt][e] = 0.f;
+        mb[n][0] = mb[n][1] = -INFINITY;
+        l[n][0] = l[n][1] = 0.f;
+    }
+    float vref = 0.f, inv_vref = 0.f;   // V's largest scale so far: O is in units of it
+
+    const long long k_lane = g * p.c.slot_stride + t * 16, v_lane = 2 * t * p.c.slot_stride + g * (HD / 8);
+    const long long row8 = 8 * p.c.slot_stride, row16 = 16 * p.c.slot_stride;
+    // a unit's pages, of its two groups of 16 keys
+    auto pages_of = [&](int u, int (&pg)[2]) {
+        pg[0] = pg[1] = -1;
+        if (u >= u1) return;
+        const int key = key_of(u);
+#pragma unroll
+        for (int a = 0; a < 2; a++) {
+            const int k = key + 16 * a;
+            if (k < hi && (k + 16 > lo || k < ns)) pg[a] = page_at(p.c, stream, k >> p.c.page_shift);
+        }
+    };
+    auto offset_of = [&](int pg, int key) {
+        return page_base(p.c, p.layer, pg, kvh) + (key & (p.c.page - 1)) * p.c.slot_stride;
+    };
+    uint32_t kw[2][2][KC][4], vw[2][4][VW];
+    float ks[2], vs[2];
+    auto load_k = [&](int u, const int (&pg)[2]) {
+        const int key = key_of(u);
+#pragma unroll
+        for (int a = 0; a < 2; a++) {
+            if (pg[a] >= 0) {
+                const unsigned char *const k = p.c.k + offset_of(pg[a], key + 16 * a) + k_lane;
+#pragma unroll
+                for (int c = 0; c < KC; c++) {
+                    load_words<4>(kw[a][0][c], k + c * 64);
+                    load_words<4>(kw[a][1][c], k + row8 + c * 64);
+                }
+                const long long sc = scale_at(p.c, p.layer, pg[a], kvh);
+                ks[a] = __ldg(p.c.k_scale + sc);
+                vs[a] = __ldg(p.c.v_scale + sc);
+            } else {
+#pragma unroll
+                for (int c = 0; c < KC; c++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) kw[a][0][c][e] = kw[a][1][c][e] = 0u;
+                ks[a] = vs[a] = 0.f;
+            }
+        }
+    };
+    auto load_v = [&](int u, const int (&pg)[2]) {
+        const int key = key_of(u);
+#pragma unroll
+        for (int a = 0; a < 2; a++) {
+            if (pg[a] >= 0) {
+                const unsigned char *const v = p.c.v + offset_of(pg[a], key + 16 * a) + v_lane;
+                load_words<VW>(vw[a][0], v);
+                load_words<VW>(vw[a][1], v + p.c.slot_stride);
+                load_words<VW>(vw[a][2], v + row8);
+                load_words<VW>(vw[a][3], v + row8 + p.c.slot_stride);
+            } else {
+#pragma unroll
+                for (int r = 0; r < 4; r++)
+#pragma unroll
+                    for (int e = 0; e < VW; e++) vw[a][r][e] = 0u;
+            }
+        }
+    };
+    (void)row16;
+    // 16 dims x 16 keys of V^T as an A operand
+    auto v_tile = [&](const uint32_t (&w)[4][VW], int mt, uint32_t (&a)[4]) {
+        const uint32_t sel = (mt & 1) ? 0x7362u : 0x5140u;
+        const uint32_t x = __byte_perm(w[0][mt / 2], w[1][mt / 2], sel), y = __byte_perm(w[2][mt / 2], w[3][mt / 2], sel);
+        a[0] = half2_bits(x & 0xffffu);
+        a[1] = half2_bits(x >> 16);
+        a[2] = half2_bits(y & 0xffffu);
+        a[3] = half2_bits(y >> 16);
+    };
+
+    int pg[2], pg_next[2];
+    pages_of(u0 + warp, pg);
+    pages_of(u0 + warp + kFwWarps, pg_next);
+    if (u0 + warp < u1) {
+        load_k(u0 + warp, pg);
+        load_v(u0 + warp, pg);
+    }
+    for (int u = u0 + warp; u < u1; u += kFwWarps) {
+        const int key = key_of(u);
+        const bool there = pg[0] >= 0 && pg[1] >= 0;
+        const bool whole = there && key + kFwKeys - 1 <= p_min &&
+                           (p.window <= 0 || key > p_max - p.window || key + kFwKeys <= p.n_sink);
+        // scores
+        float x[NR][2][4];
+#pragma unroll
+        for (int n = 0; n < NR; n++)
+#pragma unroll
+            for (int a = 0; a < 2; a++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) x[n][a][e] = 0.f;
+#pragma unroll
+        for (int a = 0; a < 2; a++)
+#pragma unroll
+            for (int c = 0; c < KC; c++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    uint32_t f[4];
+                    f[0] = half2_bits(kw[a][0][c][e] & 0xffffu);
+                    f[1] = half2_bits(kw[a][1][c][e] & 0xffffu);
+                    f[2] = half2_bits(kw[a][0][c][e] >> 16);
+                    f[3] = half2_bits(kw[a][1][c][e] >> 16);
+#pragma unroll
+                    for (int n = 0; n < NR; n++) mma_f16(x[n][a], f, qf[n][c * 4 + e][0], qf[n][c * 4 + e][1]);
+                }
+        const float k_now[2] = {ks[0], ks[1]}, v_now[2] = {vs[0], vs[1]};
+        if (u + kFwWarps < u1) load_k(u + kFwWarps, pg_next);
+        bool over = false;
+        uint32_t vis = 0xffffffffu;   // bit 4 (2 n + a) + e: the lane's row sees its key
+#pragma unroll
+        for (int n = 0; n < NR; n++)
+#pragma unroll
+            for (int a = 0; a < 2; a++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    float &v = x[n][a][e];
+                    v *= cf[n][e & 1] * k_now[a];
+                    if (!whole) {
+                        const int j = key + 16 * a + g + (e >> 1) * 8, i = at[n][e & 1];
+                        const bool see = pg[a] >= 0 && j <= i && (p.window <= 0 || j > i - p.window || j < p.n_sink);
+                        v = see ? v : -INFINITY;
+                        if (!see) vis &= ~(1u << (8 * n + 4 * a + e));
+                    }
+                    over |= v > mb[n][e & 1] + kFwAbove;
+                }
+        if (__any_sync(0xffffffffu, over)) {
+#pragma unroll
+            for (int n = 0; n < NR; n++)
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    float top = fmaxf(fmaxf(x[n][0][e], x[n][0][e + 2]), fmaxf(x[n][1][e], x[n][1][e + 2]));
+#pragma unroll
+                    for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+                    if (top > mb[n][e] + kFwAbove) {
+                        const float f = exp2f(mb[n][e] - (top - kFwBelow));
+                        mb[n][e] = top - kFwBelow;
+                        l[n][e] *= f;
+#pragma unroll
+                        for (int mt = 0; mt < MT; mt++) {
+                            o[n][mt][e] *= f;
+                            o[n][mt][e + 2] *= f;
+                        }
+                    }
+                }
+        }
+        const float v_top = fmaxf(v_now[0], v_now[1]);
+        if (v_top > vref) {
+            const float f = vref / v_top;
+            vref = v_top;
+            inv_vref = 1.0f / v_top;
+#pragma unroll
+            for (int n = 0; n < NR; n++)
+#pragma unroll
+                for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) o[n][mt][e] *= f;
+        }
+        uint32_t pb[NR][2][2];
+#pragma unroll
+        for (int n = 0; n < NR; n++) {
+            const float base[2] = {mb[n][0] == -INFINITY ? 0.f : mb[n][0], mb[n][1] == -INFINITY ? 0.f : mb[n][1]};
+#pragma unroll
+            for (int a = 0; a < 2; a++) {
+                const float rel = v_now[a] * inv_vref;
+                float w[4];
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    w[e] = exp2_approx(x[n][a][e] - base[e & 1]);
+                    l[n][e & 1] += w[e];
+                    w[e] *= rel;
+                }
+                pb[n][a][0] = transpose8(pack2<__half>(w[0], w[1]));
+                pb[n][a][1] = transpose8(pack2<__half>(w[2], w[3]));
+            }
+        }
+        bool nan = false;
+        if (!whole) {
+            // zero times a masked key's NaN would be NaN: zeros in its place, and
+            // NaN for the rows that do see it
+            uint32_t bad[2][4][VW];
+#pragma unroll
+            for (int a = 0; a < 2; a++)
+#pragma unroll
+                for (int r = 0; r < 4; r++)
+#pragma unroll
+                    for (int e = 0; e < VW; e++) {
+                        bad[a][r][e] = __vcmpeq4(vw[a][r][e] & 0x7f7f7f7fu, 0x7f7f7f7fu);
+                        vw[a][r][e] &= ~bad[a][r][e];
+                        nan |= bad[a][r][e] != 0u;
+                    }
+            if (__any_sync(0xffffffffu, nan)) {
+#pragma unroll
+                for (int n = 0; n < NR; n++)
+#pragma unroll
+                    for (int a = 0; a < 2; a++) {
+                        const uint32_t b = vis >> (8 * n + 4 * a);
+                        const uint32_t s0 = transpose8(pack2<__half>(b & 1u ? 1.f : 0.f, b & 2u ? 1.f : 0.f));
+                        const uint32_t s1 = transpose8(pack2<__half>(b & 4u ? 1.f : 0.f, b & 8u ? 1.f : 0.f));
+                        uint32_t one[4][VW];
+#pragma unroll
+                        for (int r = 0; r < 4; r++)
+#pragma unroll
+                            for (int e = 0; e < VW; e++) one[r][e] = bad[a][r][e] & 0x38383838u;   // 1.0
+#pragma unroll
+                        for (int mt = 0; mt < MT; mt++) {
+                            uint32_t f[4];
+                            float d[4] = {0.f, 0.f, 0.f, 0.f};
+                            v_tile(one, mt, f);
+                            mma_f16(d, f, s0, s1);
+#pragma unroll
+                            for (int e = 0; e < 4; e++)
+                                if (d[e] > 0.f) o[n][mt][e] = NAN;
+                        }
+                    }
+            }
+        }
+#pragma unroll
+        for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+            for (int a = 0; a < 2; a++) {
+                uint32_t f[4];
+                v_tile(vw[a], mt, f);
+#pragma unroll
+                for (int n = 0; n < NR; n++) mma_f16(o[n][mt], f, pb[n][a][0], pb[n][a][1]);
+            }
+        if (u + kFwWarps < u1) load_v(u + kFwWarps, pg_next);
+        pg[0] = pg_next[0];
+        pg[1] = pg_next[1];
+        pages_of(u + 2 * kFwWarps, pg_next);
+    }
+
+    // the warp's share: O in V's units, base, sum over its lanes
+#pragma unroll
+    for (int n = 0; n < NR; n++)
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+            float sum = l[n][e];
+#pragma unroll
+            for (int d = 4; d < 32; d <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+            const int r = n * 8 + 2 * t + e;
+            if (g == 0) {
+                sh.mx[warp][r] = mb[n][e];
+                sh.sum[warp][r] = sum;
+            }
+            float *const to = sh.o[warp][r] + g * (HD / 8);
+#pragma unroll
+            for (int mt = 0; mt < MT; mt += 2)
+                *reinterpret_cast<float4 *>(to + 2 * mt) = make_float4(o[n][mt][e] * vref, o[n][mt][e + 2] * vref,
+                                                                       o[n][mt + 1][e] * vref, o[n][mt + 1][e + 2] * vref);
+        }
+    __syncthreads();
+    // the CTA's: into its first warp's place
+    const int rows = min(kRows, M - m0);
+    for (int e = threadIdx.x; e < kRows * (HD / 4); e += kFwThreads) {
+        const int r = e / (HD / 4), d = e % (HD / 4) * 4;
+        float top = sh.mx[0][r];
+#pragma unroll
+        for (int w = 1; w < kFwWarps; w++) top = fmaxf(top, sh.mx[w][r]);
+        const float base = top == -INFINITY ? 0.f : top;
+        float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < kFwWarps; w++) {
+            const float f = exp2_approx(sh.mx[w][r] - base);
+            const float4 v = *reinterpret_cast<const float4 *>(sh.o[w][r] + d);
+            a.x = fmaf(f, v.x, a.x), a.y = fmaf(f, v.y, a.y), a.z = fmaf(f, v.z, a.z), a.w = fmaf(f, v.w, a.w);
+        }
+        *reinterpret_cast<float4 *>(sh.o[0][r] + d) = a;
+    }
+    __syncthreads();
+    if (threadIdx.x < kRows) {
+        const int r = threadIdx.x;
+        float top = sh.mx[0][r], sum = 0.f;
+#pragma unroll
+        for (int w = 1; w < kFwWarps; w++) top = fmaxf(top, sh.mx[w][r]);
+        const float base = top == -INFINITY ? 0.f : top;
+#pragma unroll
+        for (int w = 0; w < kFwWarps; w++) sum = fmaf(exp2_approx(sh.mx[w][r] - base), sh.sum[w][r], sum);
+        sh.mx[0][r] = top;
+        sh.sum[0][r] = sum;
+    }
+    if (Z > 1) cluster_sync_all();
+    else __syncthreads();
+    const uint32_t o_s = smem_u32(sh.o[0]), m_s = smem_u32(sh.mx[0]), l_s = smem_u32(sh.sum[0]);
+    for (int e = z * kFwThreads + threadIdx.x; e < rows * (HD / 4); e += Z * kFwThreads) {
+        const int r = e / (HD / 4), d = e % (HD / 4) * 4, m = m0 + r;
+        float top = -INFINITY, sum = 0.f;
+        for (int c = 0; c < Z; c++) top = fmaxf(top, ld_dsmem_f1(mapa_shared(m_s + 4 * r, c)));
+        const float base = top == -INFINITY ? 0.f : top;
+        float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int c = 0; c < Z; c++) {
+            const float f = exp2_approx(ld_dsmem_f1(mapa_shared(m_s + 4 * r, c)) - base);
+            const float4 v = ld_dsmem_f4(mapa_shared(o_s + 4 * (r * HD + d), c));
+            sum = fmaf(f, ld_dsmem_f1(mapa_shared(l_s + 4 * r, c)), sum);
+            a.x = fmaf(f, v.x, a.x), a.y = fmaf(f, v.y, a.y), a.z = fmaf(f, v.z, a.z), a.w = fmaf(f, v.w, a.w);
+        }
+        const float il = sum == 0.f ? 0.f : 1.0f / sum;
+        const long long line = (long long)(s.r0 + m / p.group) * p.n_heads + kvh * p.group + m % p.group;
+        store4<T>(static_cast<T *>(p.out) + line * HD + d, make_float4(a.x * il, a.y * il, a.z * il, a.w * il));
+        if (p.lse && d == 0) p.lse[line] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * 0.69314718055994531f;
+    }
+    if (Z > 1) cluster_sync_all();   // no CTA leaves while a peer still reads its share
+}
+
+template <typename T, int HD, int NR>
+cudaError_t launch_few(PagedAttnParams p, int sms, cudaStream_t st) {
+    auto kernel = paged_few_kernel<T, HD, NR>;
+    static ClusterKernel ck;
+    int dev = 0;
+    cudaError_t e = cluster_prepare(ck, kernel, 0, &dev);
+    if (e != cudaSuccess) return e;
+    const long long M = (long long)p.r.max_rows * p.group, tiles = (M + 8 * NR - 1) / (8 * NR);
+    const long long all = tiles * p.c.n_kv_heads * p.c.n_streams;
+    long long keys = (long long)p.c.table_stride * p.c.page;
+    if (p.window > 0) keys = min(keys, (long long)p.window + p.n_sink + p.r.max_rows);
+    const long long units = (keys + kFwKeys - 1) / kFwKeys;
+    int Z = 1;
+    while (Z < 8 && all * (Z + 1) <= 3ll * sms && units / (Z + 1) >= 2 * kFwWarps) Z++;
+    p.shares = Z;
+    cudaLaunchAttribute attr;
+    const cudaLaunchConfig_t cfg =
+        cluster_config(dim3((unsigned)(Z * tiles), p.c.n_kv_heads, p.c.n_streams), kFwThreads, 0, Z, &attr, st);
+    return cudaLaunchKernelEx(&cfg, kernel, p);
+}
 
 template <typename T, int HD>
-__global__ void __launch_bounds__(kPtWarps * 32) paged_attn_kernel(const PagedAttnParams p) {
-    constexpr int D = HD / 32;
-    __shared__ float o_s[kPtWarps][HD], m_s[kPtWarps], l_s[kPtWarps];
-    const int i = blockIdx.x, kvh = blockIdx.y, stream = blockIdx.z, warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-    const RowSpan s = paged_span(p.r, p.c, stream);
-    if (i >= s.n) return;
-    const int at = s.pos + i, low = p.window > 0 ? max(0, at - p.window + 1) : 0;
-    for (int h = kvh * p.group; h < (kvh + 1) * p.group; h++) {
-        const long long line = (long long)(s.r0 + i) * p.n_heads + h;
-        float q[D], o[D], m = -INFINITY, l = 0.f;
-#pragma unroll
-        for (int d = 0; d < D; d++) {
-            q[d] = (float)static_cast<const T *>(p.q)[line * HD + lane * D + d] * p.scale_log2;
-            o[d] = 0.f;
-        }
-        for (int j = warp; j <= at; j += kPtWarps) {
-            if (j >= p.n_sink && j < low) continue;
-            const int page = page_at(p.c, stream, j >> p.c.page_shift);
-            if (page < 0) continue;
-            const long long sc = scale_at(p.c, p.layer, page, kvh);
-            const long long off = page_base(p.c, p.layer, page, kvh) + (j & (p.c.page - 1)) * p.c.slot_stride + lane * D;
-            float x = 0.f, v[D];
-#pragma unroll
-            for (int d = 0; d < D; d += 2) {
-                const float2 kk = __half22float2(from_e4m3x2(*reinterpret_cast<const uint16_t *>(p.c.k + off + d)));
-                const float2 vv = __half22float2(from_e4m3x2(*reinterpret_cast<const uint16_t *>(p.c.v + off + d)));
-                x += q[d] * kk.x + q[d + 1] * kk.y;
-                v[d] = vv.x;
-                v[d + 1] = vv.y;
-            }
-            x = warp_sum(x) * p.c.k_scale[sc];
-            const float mn = fmaxf(m, x), base = mn == -INFINITY ? 0.f : mn;
-            const float f = exp2f(m - base), w = exp2f(x - base), vs = p.c.v_scale[sc];
-            m = mn;
-            l = l * f + w;
-#pragma unroll
-            for (int d = 0; d < D; d++) o[d] = o[d] * f + w * vs * v[d];
-        }
-        __syncthreads();
-#pragma unroll
-        for (int d = 0; d < D; d++) o_s[warp][lane * D + d] = o[d];
-        if (lane == 0) {
-            m_s[warp] = m;
-            l_s[warp] = l;
-        }
-        __syncthreads();
-        float gm = -INFINITY, gl = 0.f;
-        for (int w = 0; w < kPtWarps; w++) gm = fmaxf(gm, m_s[w]);
-        const float base = gm == -INFINITY ? 0.f : gm;
-        for (int w = 0; w < kPtWarps; w++) gl += l_s[w] * exp2f(m_s[w] - base);
-        for (int d = threadIdx.x; d < HD; d += kPtWarps * 32) {
-            float a = 0.f;
-            for (int w = 0; w < kPtWarps; w++) a += o_s[w][d] * exp2f(m_s[w] - base);
-            static_cast<T *>(p.out)[line * HD + d] = (T)(gl == 0.f ? 0.f : a / gl);
-        }
-        if (p.lse && threadIdx.x == 0) p.lse[line] = gl == 0.f ? -INFINITY : (gm + log2f(gl)) * 0.69314718055994531f;
-    }
+cudaError_t launch_dim(const PagedAttnParams &p, int sms, cudaStream_t st) {
+    const long long M = (long long)p.r.max_rows * p.group;
+    return M <= 8 ? launch_few<T, HD, 1>(p, sms, st) : launch_few<T, HD, 2>(p, sms, st);
 }
 
 template <typename T>
-cudaError_t attn_typed(const PagedAttnParams &p, cudaStream_t st) {
-    const dim3 grid(p.r.max_rows, p.c.n_kv_heads, p.c.n_streams);
-    if (p.c.head_dim == 64) paged_attn_kernel<T, 64><<<grid, kPtWarps * 32, 0, st>>>(p);
-    else paged_attn_kernel<T, 128><<<grid, kPtWarps * 32, 0, st>>>(p);
-    return cudaGetLastError();
+cudaError_t attn_typed(const PagedAttnParams &p, int sms, cudaStream_t st) {
+    return p.c.head_dim == 64 ? launch_dim<T, 64>(p, sms, st) : launch_dim<T, 128>(p, sms, st);
 }
 
 }  // namespace
 
-cudaError_t launch_paged_attn(const PagedAttnParams &p, cudaStream_t st) {
-    return p.q_type == ELEM_BF16 ? attn_typed<__nv_bfloat16>(p, st) : attn_typed<__half>(p, st);
+cudaError_t launch_paged_attn(const PagedAttnParams &p, int sms, cudaStream_t st) {
+    return p.q_type == ELEM_BF16 ? attn_typed<__nv_bfloat16>(p, sms, st) : attn_typed<__half>(p, sms, st);
 }
 
 }  // namespace vc

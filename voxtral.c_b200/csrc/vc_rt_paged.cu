@@ -186,7 +186,7 @@ extern "C" int vox_cuda_attention_paged_dev(const vox_cuda_paged_cache *cache, i
     p.window = window < room ? window : 0;   // a stream has no more positions: no limit (and no sum overflows)
     p.n_sink = p.window > 0 ? min(n_sink, room) : 0;
     p.scale_log2 = (scale == 0.f ? 1.0f / sqrtf((float)p.c.head_dim) : scale) * 1.4426950408889634f;
-    return launched(who, launch_paged_attn(p, stream ? (cudaStream_t)stream : c->stream));
+    return launched(who, launch_paged_attn(p, c->sms, stream ? (cudaStream_t)stream : c->stream));
 }
 
 extern "C" int vox_cuda_kv_copy_pages_dev(const vox_cuda_paged_cache *cache, const int *src, const int *dst, int n, void *stream) {
