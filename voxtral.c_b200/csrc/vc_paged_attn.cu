@@ -41,6 +41,7 @@ namespace {
 
 constexpr int kFwWarps = 4, kFwThreads = kFwWarps * 32;
 constexpr int kFwKeys = 32;              // keys of a warp's step
+constexpr int kFwStages = 3;             // of a warp's ring
 constexpr float kFwBelow = 7.f;          // the maximum less m
 constexpr float kFwAbove = 15.f;         // log2 of what a weight may reach before m moves
 
@@ -59,29 +60,53 @@ __device__ __forceinline__ uint32_t half2_bits(uint32_t e4m3x2) {
     const __half2 h = from_e4m3x2(e4m3x2);
     return *reinterpret_cast<const uint32_t *>(&h);
 }
-// 4 N bytes of the cache, read once: no place in L1
-template <int N>
-__device__ __forceinline__ void load_words(uint32_t *w, const unsigned char *p) {
+template <int N>   // 4 N bytes of shared memory
+__device__ __forceinline__ void lds_words(uint32_t (&w)[N], uint32_t addr) {
     if constexpr (N == 4)
-        asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "l"(p));
+        asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(addr));
     else
-        asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "l"(p));
+        asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(addr));
+}
+__device__ __forceinline__ void cp_async4(uint32_t dst_smem, const void *src, bool ok) {
+    const int n = ok ? 4 : 0;
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst_smem), "l"(src), "r"(n) : "memory");
+}
+
+// A stage: 32 keys' K, then V, as lines of 128 bytes (HD = 64: two keys a line)
+// whose 16-byte chunks are permuted so that the lanes of a load meet no bank
+// twice.
+template <int HD>
+__device__ __forceinline__ int k_chunk(int r, int ch) {
+    return HD == 128 ? r * 128 + ((ch ^ ((r & 1) << 2)) << 4) : r * 64 + (ch << 4);
+}
+template <int HD>
+__device__ __forceinline__ int v_chunk(int r, int ch) {
+    const int sw = ((r >> 1) & 3) << 1;
+    return HD == 128 ? r * 128 + ((ch ^ sw) << 4) : (r >> 1) * 128 + ((((r & 1) * 4 + ch) ^ sw) << 4);
 }
 
 template <int HD, int NR>
 struct FwSmem {
-    float o[kFwWarps][8 * NR][HD];
+    static constexpr int kTile = kFwKeys * HD;
+    static constexpr int kStages = kFwStages;
+    union {
+        unsigned char kv[kFwWarps][kStages][2][kTile];
+        float o[kFwWarps][8 * NR][HD];
+    };
+    float scale[kFwWarps][kStages][4];   // K's of the two groups of 16 keys, V's
     float mx[kFwWarps][8 * NR], sum[kFwWarps][8 * NR];
 };
 
 // NR: column tiles of 8 packed rows
 template <typename T, int HD, int NR>
-__global__ void __launch_bounds__(kFwThreads, NR == 1 ? 3 : 2) paged_few_kernel(const PagedAttnParams p) {
+__global__ void __launch_bounds__(kFwThreads, 2) paged_few_kernel(const PagedAttnParams p) {
     constexpr int KC = HD / 64;       // 64-dim parts of a key
     constexpr int MT = HD / 16;       // 16-dim tiles of O
     constexpr int VW = HD / 32;       // words that a lane has of a V row
     constexpr int kRows = 8 * NR;
-    __shared__ FwSmem<HD, NR> sh;
+    constexpr int kStages = FwSmem<HD, NR>::kStages, kTile = FwSmem<HD, NR>::kTile;
+    extern __shared__ __align__(128) unsigned char fw_smem_raw[];
+    FwSmem<HD, NR> &sh = *reinterpret_cast<FwSmem<HD, NR> *>(fw_smem_raw);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int z = blockIdx.x % p.shares, Z = p.shares;
     const int m0 = blockIdx.x / p.shares * kRows, kvh = blockIdx.y, stream = blockIdx.z;
@@ -159,8 +184,6 @@ __global__ void __launch_bounds__(kFwThreads, NR == 1 ? 3 : 2) paged_few_kernel(
     }
     float vref = 0.f, inv_vref = 0.f;   // V's largest scale so far: O is in units of it
 
-    const long long k_lane = g * p.c.slot_stride + t * 16, v_lane = 2 * t * p.c.slot_stride + g * (HD / 8);
-    const long long row8 = 8 * p.c.slot_stride, row16 = 16 * p.c.slot_stride;
     // a unit's pages, of its two groups of 16 keys
     auto pages_of = [&](int u, int (&pg)[2]) {
         pg[0] = pg[1] = -1;
@@ -172,53 +195,34 @@ __global__ void __launch_bounds__(kFwThreads, NR == 1 ? 3 : 2) paged_few_kernel(
             if (k < hi && (k + 16 > lo || k < ns)) pg[a] = page_at(p.c, stream, k >> p.c.page_shift);
         }
     };
-    auto offset_of = [&](int pg, int key) {
-        return page_base(p.c, p.layer, pg, kvh) + (key & (p.c.page - 1)) * p.c.slot_stride;
-    };
-    uint32_t kw[2][2][KC][4], vw[2][4][VW];
-    float ks[2], vs[2];
-    auto load_k = [&](int u, const int (&pg)[2]) {
-        const int key = key_of(u);
+    // a unit's keys and scales on their way to a stage (zeros where there is no page)
+    const uint32_t ring = smem_u32(sh.kv[warp]), scales = smem_u32(sh.scale[warp]);
+    auto fetch = [&](int u, int stage, const int (&pg)[2]) {
+        if (u < u1) {
+            constexpr int kCh = HD / 16, kAtOnce = 32 / kCh;   // chunks of a row, rows of a step
+            const int key = key_of(u), r0 = lane / kCh, ch = lane % kCh;
+            const uint32_t k_to = ring + stage * (2 * kTile), v_to = k_to + kTile;
 #pragma unroll
-        for (int a = 0; a < 2; a++) {
-            if (pg[a] >= 0) {
-                const unsigned char *const k = p.c.k + offset_of(pg[a], key + 16 * a) + k_lane;
+            for (int a = 0; a < 2; a++) {
+                const bool ok = pg[a] >= 0;
+                const long long from = ok ? page_base(p.c, p.layer, pg[a], kvh) + ((key + 16 * a) & (p.c.page - 1)) * p.c.slot_stride +
+                                                r0 * p.c.slot_stride + ch * 16
+                                          : 0;
 #pragma unroll
-                for (int c = 0; c < KC; c++) {
-                    load_words<4>(kw[a][0][c], k + c * 64);
-                    load_words<4>(kw[a][1][c], k + row8 + c * 64);
+                for (int i = 0; i < 16; i += kAtOnce) {
+                    const long long off = from + (ok ? i * p.c.slot_stride : 0);
+                    cp_async16(k_to + k_chunk<HD>(16 * a + i + r0, ch), p.c.k + off, ok);
+                    cp_async16(v_to + v_chunk<HD>(16 * a + i + r0, ch), p.c.v + off, ok);
                 }
-                const long long sc = scale_at(p.c, p.layer, pg[a], kvh);
-                ks[a] = __ldg(p.c.k_scale + sc);
-                vs[a] = __ldg(p.c.v_scale + sc);
-            } else {
-#pragma unroll
-                for (int c = 0; c < KC; c++)
-#pragma unroll
-                    for (int e = 0; e < 4; e++) kw[a][0][c][e] = kw[a][1][c][e] = 0u;
-                ks[a] = vs[a] = 0.f;
+            }
+            if (lane < 4) {
+                const int of = lane & 1 ? pg[1] : pg[0];
+                const float *const from = lane < 2 ? p.c.k_scale : p.c.v_scale;
+                cp_async4(scales + stage * 16 + lane * 4, from + (of >= 0 ? scale_at(p.c, p.layer, of, kvh) : 0), of >= 0);
             }
         }
+        cp_async_commit();
     };
-    auto load_v = [&](int u, const int (&pg)[2]) {
-        const int key = key_of(u);
-#pragma unroll
-        for (int a = 0; a < 2; a++) {
-            if (pg[a] >= 0) {
-                const unsigned char *const v = p.c.v + offset_of(pg[a], key + 16 * a) + v_lane;
-                load_words<VW>(vw[a][0], v);
-                load_words<VW>(vw[a][1], v + p.c.slot_stride);
-                load_words<VW>(vw[a][2], v + row8);
-                load_words<VW>(vw[a][3], v + row8 + p.c.slot_stride);
-            } else {
-#pragma unroll
-                for (int r = 0; r < 4; r++)
-#pragma unroll
-                    for (int e = 0; e < VW; e++) vw[a][r][e] = 0u;
-            }
-        }
-    };
-    (void)row16;
     // 16 dims x 16 keys of V^T as an A operand
     auto v_tile = [&](const uint32_t (&w)[4][VW], int mt, uint32_t (&a)[4]) {
         const uint32_t sel = (mt & 1) ? 0x7362u : 0x5140u;
@@ -229,17 +233,30 @@ __global__ void __launch_bounds__(kFwThreads, NR == 1 ? 3 : 2) paged_few_kernel(
         a[3] = half2_bits(y >> 16);
     };
 
-    int pg[2], pg_next[2];
-    pages_of(u0 + warp, pg);
-    pages_of(u0 + warp + kFwWarps, pg_next);
-    if (u0 + warp < u1) {
-        load_k(u0 + warp, pg);
-        load_v(u0 + warp, pg);
+    int pg[2] = {-1, -1};
+    uint32_t have = 0u;   // two bits a unit, the newest lowest: its groups' pages are there
+    auto note = [&]() { have = have << 2 | (pg[1] >= 0 ? 2u : 0u) | (pg[0] >= 0 ? 1u : 0u); };
+#pragma unroll
+    for (int i = 0; i < kStages - 1; i++) {
+        pages_of(u0 + warp + i * kFwWarps, pg);
+        fetch(u0 + warp + i * kFwWarps, i, pg);
+        note();
     }
+    pages_of(u0 + warp + (kStages - 1) * kFwWarps, pg);
+    int stage = 0;
     for (int u = u0 + warp; u < u1; u += kFwWarps) {
+        cp_async_wait<kStages - 2>();
+        __syncwarp();   // this unit is there for all lanes, and all have done with the one before
+        fetch(u + (kStages - 1) * kFwWarps, stage == 0 ? kStages - 1 : stage - 1, pg);
+        note();
+        pages_of(u + kStages * kFwWarps, pg);
+        const uint32_t k_at = ring + stage * (2 * kTile), v_at = k_at + kTile;
+        const uint32_t there = have >> (2 * (kStages - 1));
+        const float4 sc = *reinterpret_cast<const float4 *>(sh.scale[warp][stage]);
+        const float k_now[2] = {sc.x, sc.y}, v_now[2] = {sc.z, sc.w};
+        stage = stage + 1 == kStages ? 0 : stage + 1;
         const int key = key_of(u);
-        const bool there = pg[0] >= 0 && pg[1] >= 0;
-        const bool whole = there && key + kFwKeys - 1 <= p_min &&
+        const bool whole = (there & 3u) == 3u && key + kFwKeys - 1 <= p_min &&
                            (p.window <= 0 || key > p_max - p.window || key + kFwKeys <= p.n_sink);
         // scores
         float x[NR][2][4];
@@ -252,19 +269,21 @@ __global__ void __launch_bounds__(kFwThreads, NR == 1 ? 3 : 2) paged_few_kernel(
 #pragma unroll
         for (int a = 0; a < 2; a++)
 #pragma unroll
-            for (int c = 0; c < KC; c++)
+            for (int c = 0; c < KC; c++) {
+                uint32_t w0[4], w1[4];
+                lds_words<4>(w0, k_at + k_chunk<HD>(16 * a + g, c * 4 + t));
+                lds_words<4>(w1, k_at + k_chunk<HD>(16 * a + g + 8, c * 4 + t));
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
                     uint32_t f[4];
-                    f[0] = half2_bits(kw[a][0][c][e] & 0xffffu);
-                    f[1] = half2_bits(kw[a][1][c][e] & 0xffffu);
-                    f[2] = half2_bits(kw[a][0][c][e] >> 16);
-                    f[3] = half2_bits(kw[a][1][c][e] >> 16);
+                    f[0] = half2_bits(w0[e] & 0xffffu);
+                    f[1] = half2_bits(w1[e] & 0xffffu);
+                    f[2] = half2_bits(w0[e] >> 16);
+                    f[3] = half2_bits(w1[e] >> 16);
 #pragma unroll
                     for (int n = 0; n < NR; n++) mma_f16(x[n][a], f, qf[n][c * 4 + e][0], qf[n][c * 4 + e][1]);
                 }
-        const float k_now[2] = {ks[0], ks[1]}, v_now[2] = {vs[0], vs[1]};
-        if (u + kFwWarps < u1) load_k(u + kFwWarps, pg_next);
+            }
         bool over = false;
         uint32_t vis = 0xffffffffu;   // bit 4 (2 n + a) + e: the lane's row sees its key
 #pragma unroll
@@ -277,7 +296,7 @@ __global__ void __launch_bounds__(kFwThreads, NR == 1 ? 3 : 2) paged_few_kernel(
                     v *= cf[n][e & 1] * k_now[a];
                     if (!whole) {
                         const int j = key + 16 * a + g + (e >> 1) * 8, i = at[n][e & 1];
-                        const bool see = pg[a] >= 0 && j <= i && (p.window <= 0 || j > i - p.window || j < p.n_sink);
+                        const bool see = ((there >> a) & 1u) && j <= i && (p.window <= 0 || j > i - p.window || j < p.n_sink);
                         v = see ? v : -INFINITY;
                         if (!see) vis &= ~(1u << (8 * n + 4 * a + e));
                     }
@@ -333,6 +352,14 @@ __global__ void __launch_bounds__(kFwThreads, NR == 1 ? 3 : 2) paged_few_kernel(
                 pb[n][a][1] = transpose8(pack2<__half>(w[2], w[3]));
             }
         }
+        uint32_t vw[2][4][VW];
+#pragma unroll
+        for (int a = 0; a < 2; a++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                const int row = 16 * a + 2 * t + (r & 1) + (r >> 1) * 8;
+                lds_words<VW>(vw[a][r], v_at + (HD == 128 ? v_chunk<HD>(row, g) : v_chunk<HD>(row, g >> 1) + (g & 1) * 8));
+            }
         bool nan = false;
         if (!whole) {
             // zero times a masked key's NaN would be NaN: zeros in its place, and
@@ -383,11 +410,9 @@ __global__ void __launch_bounds__(kFwThreads, NR == 1 ? 3 : 2) paged_few_kernel(
 #pragma unroll
                 for (int n = 0; n < NR; n++) mma_f16(o[n][mt], f, pb[n][a][0], pb[n][a][1]);
             }
-        if (u + kFwWarps < u1) load_v(u + kFwWarps, pg_next);
-        pg[0] = pg_next[0];
-        pg[1] = pg_next[1];
-        pages_of(u + 2 * kFwWarps, pg_next);
     }
+    cp_async_wait<0>();
+    __syncthreads();   // the ring becomes the warps' sums
 
     // the warp's share: O in V's units, base, sum over its lanes
 #pragma unroll
@@ -466,7 +491,8 @@ cudaError_t launch_few(PagedAttnParams p, int sms, cudaStream_t st) {
     auto kernel = paged_few_kernel<T, HD, NR>;
     static ClusterKernel ck;
     int dev = 0;
-    cudaError_t e = cluster_prepare(ck, kernel, 0, &dev);
+    constexpr size_t kSmem = sizeof(FwSmem<HD, NR>);
+    cudaError_t e = cluster_prepare(ck, kernel, kSmem, &dev);
     if (e != cudaSuccess) return e;
     const long long M = (long long)p.r.max_rows * p.group, tiles = (M + 8 * NR - 1) / (8 * NR);
     const long long all = tiles * p.c.n_kv_heads * p.c.n_streams;
@@ -474,11 +500,11 @@ cudaError_t launch_few(PagedAttnParams p, int sms, cudaStream_t st) {
     if (p.window > 0) keys = min(keys, (long long)p.window + p.n_sink + p.r.max_rows);
     const long long units = (keys + kFwKeys - 1) / kFwKeys;
     int Z = 1;
-    while (Z < 8 && all * (Z + 1) <= 3ll * sms && units / (Z + 1) >= 2 * kFwWarps) Z++;
+    while (Z < 8 && all * (Z + 1) <= 2ll * sms && units / (Z + 1) >= 2 * kFwWarps) Z++;
     p.shares = Z;
     cudaLaunchAttribute attr;
     const cudaLaunchConfig_t cfg =
-        cluster_config(dim3((unsigned)(Z * tiles), p.c.n_kv_heads, p.c.n_streams), kFwThreads, 0, Z, &attr, st);
+        cluster_config(dim3((unsigned)(Z * tiles), p.c.n_kv_heads, p.c.n_streams), kFwThreads, kSmem, Z, &attr, st);
     return cudaLaunchKernelEx(&cfg, kernel, p);
 }
 
