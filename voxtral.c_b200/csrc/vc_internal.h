@@ -237,8 +237,12 @@ struct PagedAttnParams {
     int window, n_sink;       // window 0: no limit
     float scale_log2;         // scale * log2(e)
     int shares;               // key shares of a row tile (set by the launch)
+    unsigned *err;            // raised when a bounded wait expires (mapped host memory); the rows then get NaN
+    unsigned long long stall_ns;   // self-test: a wait of this length that nothing ends, after the work (0: none)
 };
 cudaError_t launch_paged_attn(const PagedAttnParams &p, int sms, cudaStream_t st);
+// the tensor-core kernel of many rows (vc_paged_attn_tc.cu)
+cudaError_t launch_paged_attn_tc(const PagedAttnParams &p, cudaStream_t st);
 struct PagedCopyParams {
     PagedView c;
     const int *src, *dst;     // [n]

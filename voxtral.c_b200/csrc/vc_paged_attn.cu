@@ -122,6 +122,55 @@ __global__ void __launch_bounds__(kFwThreads, 2) paged_few_kernel(const PagedAtt
     const int u0 = (int)((long long)z * units / Z), u1 = (int)((long long)(z + 1) * units / Z);
     auto key_of = [&](int u) { return (u < sink_units ? u : first + u - sink_units) * kFwKeys; };
 
+    // a unit's pages, of its two groups of 16 keys
+    auto pages_of = [&](int u, int (&pg)[2]) {
+        pg[0] = pg[1] = -1;
+        if (u >= u1) return;
+        const int key = key_of(u);
+#pragma unroll
+        for (int a = 0; a < 2; a++) {
+            const int k = key + 16 * a;
+            if (k < hi && (k + 16 > lo || k < ns)) pg[a] = page_at(p.c, stream, k >> p.c.page_shift);
+        }
+    };
+    // a unit's keys and scales on their way to a stage (zeros where there is no page)
+    const uint32_t ring = smem_u32(sh.kv[warp]), scales = smem_u32(sh.scale[warp]);
+    auto fetch = [&](int u, int stage, const int (&pg)[2]) {
+        if (u < u1) {
+            constexpr int kCh = HD / 16, kAtOnce = 32 / kCh;   // chunks of a row, rows of a step
+            const int key = key_of(u), r0 = lane / kCh, ch = lane % kCh;
+            const uint32_t k_to = ring + stage * (2 * kTile), v_to = k_to + kTile;
+#pragma unroll
+            for (int a = 0; a < 2; a++) {
+                const bool ok = pg[a] >= 0;
+                const long long from = ok ? page_base(p.c, p.layer, pg[a], kvh) + ((key + 16 * a) & (p.c.page - 1)) * p.c.slot_stride +
+                                                r0 * p.c.slot_stride + ch * 16
+                                          : 0;
+#pragma unroll
+                for (int i = 0; i < 16; i += kAtOnce) {
+                    const long long off = from + (ok ? i * p.c.slot_stride : 0);
+                    cp_async16(k_to + k_chunk<HD>(16 * a + i + r0, ch), p.c.k + off, ok);
+                    cp_async16(v_to + v_chunk<HD>(16 * a + i + r0, ch), p.c.v + off, ok);
+                }
+            }
+            if (lane < 4) {
+                const int of = lane & 1 ? pg[1] : pg[0];
+                const float *const from = lane < 2 ? p.c.k_scale : p.c.v_scale;
+                cp_async4(scales + stage * 16 + lane * 4, from + (of >= 0 ? scale_at(p.c, p.layer, of, kvh) : 0), of >= 0);
+            }
+        }
+        cp_async_commit();
+    };
+    int pg[2] = {-1, -1};
+    uint32_t have = 0u;   // two bits a unit, the newest lowest: its groups' pages are there
+    auto note = [&]() { have = have << 2 | (pg[1] >= 0 ? 2u : 0u) | (pg[0] >= 0 ? 1u : 0u); };
+#pragma unroll
+    for (int i = 0; i < kStages - 1; i++) {
+        pages_of(u0 + warp + i * kFwWarps, pg);
+        fetch(u0 + warp + i * kFwWarps, i, pg);
+        note();
+    }
+    pages_of(u0 + warp + (kStages - 1) * kFwWarps, pg);
     // q as B operands: lane (g, t) has row g's dims in the order of K's
     uint32_t qf[NR][KC * 4][2];
     float cf[NR][2];          // score factor of the lane's rows 2 t, 2 t + 1, in log2
@@ -184,45 +233,6 @@ __global__ void __launch_bounds__(kFwThreads, 2) paged_few_kernel(const PagedAtt
     }
     float vref = 0.f, inv_vref = 0.f;   // V's largest scale so far: O is in units of it
 
-    // a unit's pages, of its two groups of 16 keys
-    auto pages_of = [&](int u, int (&pg)[2]) {
-        pg[0] = pg[1] = -1;
-        if (u >= u1) return;
-        const int key = key_of(u);
-#pragma unroll
-        for (int a = 0; a < 2; a++) {
-            const int k = key + 16 * a;
-            if (k < hi && (k + 16 > lo || k < ns)) pg[a] = page_at(p.c, stream, k >> p.c.page_shift);
-        }
-    };
-    // a unit's keys and scales on their way to a stage (zeros where there is no page)
-    const uint32_t ring = smem_u32(sh.kv[warp]), scales = smem_u32(sh.scale[warp]);
-    auto fetch = [&](int u, int stage, const int (&pg)[2]) {
-        if (u < u1) {
-            constexpr int kCh = HD / 16, kAtOnce = 32 / kCh;   // chunks of a row, rows of a step
-            const int key = key_of(u), r0 = lane / kCh, ch = lane % kCh;
-            const uint32_t k_to = ring + stage * (2 * kTile), v_to = k_to + kTile;
-#pragma unroll
-            for (int a = 0; a < 2; a++) {
-                const bool ok = pg[a] >= 0;
-                const long long from = ok ? page_base(p.c, p.layer, pg[a], kvh) + ((key + 16 * a) & (p.c.page - 1)) * p.c.slot_stride +
-                                                r0 * p.c.slot_stride + ch * 16
-                                          : 0;
-#pragma unroll
-                for (int i = 0; i < 16; i += kAtOnce) {
-                    const long long off = from + (ok ? i * p.c.slot_stride : 0);
-                    cp_async16(k_to + k_chunk<HD>(16 * a + i + r0, ch), p.c.k + off, ok);
-                    cp_async16(v_to + v_chunk<HD>(16 * a + i + r0, ch), p.c.v + off, ok);
-                }
-            }
-            if (lane < 4) {
-                const int of = lane & 1 ? pg[1] : pg[0];
-                const float *const from = lane < 2 ? p.c.k_scale : p.c.v_scale;
-                cp_async4(scales + stage * 16 + lane * 4, from + (of >= 0 ? scale_at(p.c, p.layer, of, kvh) : 0), of >= 0);
-            }
-        }
-        cp_async_commit();
-    };
     // 16 dims x 16 keys of V^T as an A operand
     auto v_tile = [&](const uint32_t (&w)[4][VW], int mt, uint32_t (&a)[4]) {
         const uint32_t sel = (mt & 1) ? 0x7362u : 0x5140u;
@@ -233,16 +243,6 @@ __global__ void __launch_bounds__(kFwThreads, 2) paged_few_kernel(const PagedAtt
         a[3] = half2_bits(y >> 16);
     };
 
-    int pg[2] = {-1, -1};
-    uint32_t have = 0u;   // two bits a unit, the newest lowest: its groups' pages are there
-    auto note = [&]() { have = have << 2 | (pg[1] >= 0 ? 2u : 0u) | (pg[0] >= 0 ? 1u : 0u); };
-#pragma unroll
-    for (int i = 0; i < kStages - 1; i++) {
-        pages_of(u0 + warp + i * kFwWarps, pg);
-        fetch(u0 + warp + i * kFwWarps, i, pg);
-        note();
-    }
-    pages_of(u0 + warp + (kStages - 1) * kFwWarps, pg);
     int stage = 0;
     for (int u = u0 + warp; u < u1; u += kFwWarps) {
         cp_async_wait<kStages - 2>();
@@ -522,6 +522,7 @@ cudaError_t attn_typed(const PagedAttnParams &p, int sms, cudaStream_t st) {
 }  // namespace
 
 cudaError_t launch_paged_attn(const PagedAttnParams &p, int sms, cudaStream_t st) {
+    if ((long long)p.r.max_rows * p.group > 32) return launch_paged_attn_tc(p, st);
     return p.q_type == ELEM_BF16 ? attn_typed<__nv_bfloat16>(p, sms, st) : attn_typed<__half>(p, sms, st);
 }
 

@@ -1,0 +1,637 @@
+// vc_paged_attn_tc.cu - attention of many rows per stream over a paged cache in
+// 8 bits, on the tcgen05 tensor cores: chunks and whole prompts.
+//
+// A CTA takes NT (1 or 2) tiles of 128 packed query rows (m = row * group +
+// head, TMEM lane = packed row) of one (stream, KV head) and a share of the
+// blocks of 64 or 128 keys that they see; the shares are a cluster.
+//   4 warps per tile softmax, thread = packed row, 64 keys a step: P = 2^(s - m)
+//                    of S (TMEM), rounded to fp16, over the S columns it came
+//                    from; before that they load their rows of Q
+//   4 warps          K and V: 16 bytes of a key to a thread, e4m3 to fp16 (exact),
+//                    into the MMAs' swizzled layout, the next block's loads under
+//                    way meanwhile
+//   1 warp per tile  issues its MMAs, M 128: S_t = Q_t K^T (K HD) and, by steps
+//                    of 64 keys, O_t += P_t V (N HD; A from TMEM, V an MN-major
+//                    operand)
+// Two tiles share each K and V block, so that its conversion (about a quarter
+// of the CTA's instructions) is paid once per 256 rows.
+//
+// All operands are fp16, whatever q's type: bf16 rows of Q are scaled by a power
+// of two into its range (exact but for values 2^-29 of the row's largest), K's
+// scales multiply the scores, V's the values, relative to the largest that the
+// CTA sees.  The weights are rounded to fp16, half a step of 2^-11; m is the
+// running maximum less 7 and moves only when a score exceeds it by 15, so that P
+// fills the type up to 2^15 and what is lost is 2^-32 of the largest weight per
+// key.  Sums, maxima and O are fp32.
+//
+// Zero times a masked key's NaN would be NaN: in blocks that some row does not
+// see whole, the converting threads put zeros in the place of NaN in V and set a
+// flag, and the rows that do see them get NaN at the end.
+#include "vc_attn_tc.cuh"
+#include "vc_cluster.h"
+#include "vc_paged.cuh"
+
+#include <algorithm>
+
+namespace vc {
+
+using namespace tc;
+
+namespace {
+
+constexpr int kPtHalf = 64;             // keys per softmax step
+constexpr int kPtConv = 128;            // threads that convert K and V
+constexpr int kPtStages = 2;
+constexpr int pt_keys(int nt) { return nt == 1 ? 64 : 128; }
+constexpr int pt_ctas(int nt) { return nt == 1 ? 2 : 1; }
+constexpr int pt_threads(int nt) { return nt * kAtRows + kPtConv + nt * 32; }
+constexpr uint64_t kPtWaitNs = 2000000000ull, kPtBlockNs = 10000ull;   // a CTA's waits end after this, per block as well
+constexpr float kPtBelow = 7.f;         // the maximum less m
+constexpr float kPtAbove = 15.f;        // log2 of what a weight may reach before m moves
+constexpr int kPtOneCta = 120 * 1024;   // more than half an SM's shared memory: one CTA per SM
+
+template <int HD, int NT>
+struct PtSmem {
+    static constexpr int kKeys = pt_keys(NT);
+    // Q, K and V tiles are HD / 64 sub-tiles of [rows or keys][128 bytes]
+    static constexpr int kTile = kKeys * HD * 2, kSubTile = kKeys * 128, kQTile = kAtRows * HD * 2, kQSub = kAtRows * 128;
+    static constexpr int kO = NT * kAtRows * HD * 4;   // bytes of O in fp32, over K and V at the end
+    unsigned char q[NT][kQTile];
+    union {
+        unsigned char kv[2][kPtStages][kTile];         // K, V
+        unsigned char o[kO];
+    };
+    float mx[NT * kAtRows], sum[NT * kAtRows], factor[NT * kAtRows];
+    uint64_t q_full[NT], k_full[kPtStages], k_empty[kPtStages], v_full[kPtStages], v_empty[kPtStages], s_full[2], p_full[NT][2],
+        o_part[NT], o_done[NT];   // s_full: by tile, or (one tile) by S range
+    uint32_t tmem;
+    int v_top;    // V's largest scale, as the bits of a float >= 0
+    int bad;      // a masked block holds NaN in V
+    int failed;   // some warp's wait ran out: the CTA's rows are void
+    uint64_t stall;   // nothing arrives here
+};
+
+// The weights of 64 keys of a row: w = 2^(s f - base) as pairs of fp16, ls their
+// sum before rounding; the largest s f - base as the result.  f: the row's factor
+// times K's scale, by groups of 16 keys in the warp's lanes.  The next 16 scores
+// are on their way from TMEM while 16 are worked on.  In blocks without a mask
+// kPtPoly of 8 pairs take 2^x on the FMA pipe, since the exponential unit takes 8
+// cycles per warp.
+constexpr int kPtPoly = 3;
+template <bool MASKED>
+__device__ __forceinline__ float weigh64(uint32_t ts, float sl2, float ks, int g0, float base, uint64_t vis, uint32_t (&w)[32], float &ls) {
+    float mx[2] = {-INFINITY, -INFINITY};
+    uint64_t rs[2] = {0, 0};
+    const uint64_t nb = pair(-base, -base);
+    uint32_t ra[16], rb[16];
+    tmem_ld16_async(ts, ra);
+#pragma unroll
+    for (int c = 0; c < 64; c += 16) {
+        uint32_t(&cur)[16] = (c & 16) ? rb : ra;
+        const float f = sl2 * __shfl_sync(0xffffffffu, ks, g0 + c / 16);
+        const uint64_t sl = pair(f, f);
+        tmem_ld_wait(cur);
+        if (c + 16 < 64) tmem_ld16_async(ts + c + 16, (c & 16) ? ra : rb);
+#pragma unroll
+        for (int j = 0; j < 16; j += 2) {
+            float xa, xb;
+            unpair(fma2(pair(__uint_as_float(cur[j]), __uint_as_float(cur[j + 1])), sl, nb), xa, xb);
+            if (MASKED) {
+                xa = (vis >> (c + j)) & 1u ? xa : -INFINITY;
+                xb = (vis >> (c + j + 1)) & 1u ? xb : -INFINITY;
+            }
+            mx[0] = fmaxf(mx[0], xa);
+            mx[1] = fmaxf(mx[1], xb);
+            if (!MASKED && (j >> 1) % 8 < kPtPoly) {
+                exp2_poly2(xa, xb);
+            } else {
+                xa = exp2_approx(xa);
+                xb = exp2_approx(xb);
+            }
+            rs[(j >> 1) & 1] = add2(rs[(j >> 1) & 1], pair(xa, xb));
+            w[(c + j) >> 1] = pack2<__half>(xa, xb);
+        }
+    }
+    float a, b;
+    unpair(add2(rs[0], rs[1]), a, b);
+    ls = a + b;
+    return fmaxf(mx[0], mx[1]);
+}
+
+template <typename T, int HD, int NT>
+__global__ void __launch_bounds__(pt_threads(NT), pt_ctas(NT)) paged_many_kernel(const PagedAttnParams p) {
+    using Sm = PtSmem<HD, NT>;
+    constexpr int kSub = HD / 64;            // 64-dim sub-tiles of a tile
+    constexpr int kWarpConv = NT * 4, kWarpMma = kWarpConv + kPtConv / 32;
+    constexpr int kThreads = pt_threads(NT), kKeys = Sm::kKeys, kSteps = kKeys / kPtHalf, kGroups = kKeys / 16;
+    constexpr bool kTwoS = NT == 1;          // two S ranges: S(b + 1) is ready when the softmax is done with S(b)
+    constexpr uint32_t kTmemCols = NT == 2 ? 512 : 256;
+    constexpr uint32_t kOCol = kTwoS ? 2 * kKeys : NT * kKeys;   // S ranges first, then O tiles
+    extern __shared__ __align__(1024) unsigned char pt_smem_raw[];
+    Sm &sh = *reinterpret_cast<Sm *>(pt_smem_raw);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int z = blockIdx.x % p.shares, Z = p.shares;
+    const int m0 = blockIdx.x / p.shares * (NT * kAtRows), kvh = blockIdx.y, stream = blockIdx.z;
+    const RowSpan s = paged_span(p.r, p.c, stream);
+    const int M = s.n * p.group;
+    if (m0 >= M) return;   // the whole cluster leaves
+    const int i0 = m0 / p.group, i1 = (min(m0 + NT * kAtRows, M) - 1) / p.group;
+    // positions that some row sees: [0, ns) and [lo, hi)
+    const int p_min = s.pos + i0, p_max = s.pos + i1, hi = p_max + 1, ns = min(p.n_sink, hi);
+    const int lo = p.window > 0 ? max(0, p_min - p.window + 1) : 0;
+    const int sink_blocks = (ns + kKeys - 1) / kKeys, first = max(lo / kKeys, sink_blocks);
+    const int blocks = sink_blocks + max(0, (hi + kKeys - 1) / kKeys - first);
+    const int b0 = (int)((long long)z * blocks / Z), nb = (int)((long long)(z + 1) * blocks / Z) - b0;
+    const int tiles = M - m0 > kAtRows ? NT : 1;   // tiles with rows
+    const int head0 = kvh * p.group;
+    auto key_of = [&](int b) { return (b0 + b < sink_blocks ? b0 + b : first + b0 + b - sink_blocks) * kKeys; };
+    // every row sees the block's positions
+    auto whole = [&](int key) {
+        return key + kKeys - 1 <= p_min && (p.window <= 0 || key > p_max - p.window || key + kKeys <= p.n_sink);
+    };
+    // the page of 16 positions, -1: none, or no row sees them
+    auto page_of = [&](int key) {
+        return key < hi && (key + 16 > lo || key < ns) ? page_at(p.c, stream, key >> p.c.page_shift) : -1;
+    };
+    bool ok = true;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < kPtStages; i++) {
+            mbar_init(&sh.k_full[i], kPtConv / 32);
+            mbar_init(&sh.v_full[i], kPtConv / 32);
+            mbar_init(&sh.k_empty[i], tiles);
+            mbar_init(&sh.v_empty[i], tiles);
+        }
+        for (int t = 0; t < NT; t++) {
+            const int warps = max(1, min(4, (M - m0 - t * kAtRows + 31) / 32));   // of the tile, with rows
+            mbar_init(&sh.q_full[t], warps);
+            mbar_init(&sh.p_full[t][0], warps);
+            mbar_init(&sh.p_full[t][1], warps);
+            mbar_init(&sh.o_part[t], 1);
+            mbar_init(&sh.o_done[t], 1);
+        }
+        mbar_init(&sh.s_full[0], 1);
+        mbar_init(&sh.s_full[1], 1);
+        mbar_init(&sh.stall, 1);
+        sh.v_top = sh.bad = sh.failed = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == kWarpMma) {
+        tmem_alloc(&sh.tmem, kTmemCols);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = sh.tmem;
+    const uint64_t deadline = globaltimer() + kPtWaitNs + (uint64_t)nb * kPtBlockNs;   // (TMEM may have been another kernel's)
+
+    if (warp >= kWarpConv && warp < kWarpMma) {
+        // ---- K and V ----
+        constexpr int kRowsAtOnce = kPtConv * 16 / HD, kLoads = kKeys / kRowsAtOnce;
+        // a thread's 16 dims of a row, so that the lanes of a store meet no bank twice
+        const int tid = threadIdx.x - kWarpConv * 32;
+        const int r0 = HD == 128 ? ((tid >> 4) << 1 | ((tid >> 2) & 1)) : tid >> 2, sub = HD == 128 ? (tid >> 3) & 1 : 0, ch = tid & 3;
+        const long long mine = sub * 64 + ch * 16;
+        int pg[kLoads], pg_next[kLoads];
+        uint4 k_raw[kLoads], v_raw[kLoads];
+        float vs[kLoads];
+        auto pages = [&](int b, int (&g)[kLoads]) {
+            const int key = b < nb ? key_of(b) : 0;
+#pragma unroll
+            for (int i = 0; i < kLoads; i++) g[i] = b < nb ? page_of((key + i * kRowsAtOnce + r0) & ~15) : -1;
+        };
+        auto load = [&](int b, const unsigned char *pool, const int (&g)[kLoads], uint4 (&raw)[kLoads]) {
+            const int key = b < nb ? key_of(b) : 0;
+#pragma unroll
+            for (int i = 0; i < kLoads; i++) {
+                raw[i] = make_uint4(0u, 0u, 0u, 0u);
+                const int slot = (key + i * kRowsAtOnce + r0) & (p.c.page - 1);
+                if (g[i] >= 0)
+                    raw[i] = __ldg(reinterpret_cast<const uint4 *>(pool + page_base(p.c, p.layer, g[i], kvh) + slot * p.c.slot_stride + mine));
+            }
+        };
+        auto scales = [&](const int (&g)[kLoads]) {
+#pragma unroll
+            for (int i = 0; i < kLoads; i++) vs[i] = g[i] >= 0 ? __ldg(p.c.v_scale + scale_at(p.c, p.layer, g[i], kvh)) : 0.f;
+        };
+        auto put = [&](unsigned char *tile, int r, const uint4 &u, __half2 by, bool scaled) {
+            const uint32_t in[4] = {u.x, u.y, u.z, u.w};
+            uint32_t out[8];
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                __half2 a = from_e4m3x2(in[e] & 0xffffu), b = from_e4m3x2(in[e] >> 16);
+                if (scaled) {
+                    a = __hmul2(a, by);
+                    b = __hmul2(b, by);
+                }
+                out[2 * e] = *reinterpret_cast<const uint32_t *>(&a);
+                out[2 * e + 1] = *reinterpret_cast<const uint32_t *>(&b);
+            }
+            unsigned char *const row = tile + sub * Sm::kSubTile + r * 128;
+            *reinterpret_cast<uint4 *>(row + (((2 * ch) ^ (r & 7)) << 4)) = make_uint4(out[0], out[1], out[2], out[3]);
+            *reinterpret_cast<uint4 *>(row + (((2 * ch + 1) ^ (r & 7)) << 4)) = make_uint4(out[4], out[5], out[6], out[7]);
+        };
+        pages(0, pg);
+        load(0, p.c.k, pg, k_raw);
+        load(0, p.c.v, pg, v_raw);
+        scales(pg);
+        pages(1, pg_next);
+        {   // the largest scale of V
+            const int step = min(p.c.page, kKeys), n = nb * (kKeys / step);
+            float top = 0.f;
+            for (int i = tid; i < n; i += kPtConv) {
+                int key = key_of(i / (kKeys / step)) + i % (kKeys / step) * step;
+                // a page's first positions may be among those that nobody sees
+                const bool seen = key < hi && (key + step > lo || key < ns);
+                const int g = seen ? page_at(p.c, stream, key >> p.c.page_shift) : -1;
+                if (g >= 0) top = fmaxf(top, __ldg(p.c.v_scale + scale_at(p.c, p.layer, g, kvh)));
+            }
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            if (lane == 0) atomicMax(&sh.v_top, __float_as_int(top));
+            asm volatile("bar.sync 1, %0;" ::"n"(kPtConv) : "memory");
+        }
+        const float v_top = __int_as_float(*(volatile int *)&sh.v_top), inv_top = v_top > 0.f ? 1.0f / v_top : 0.f;
+        for (int b = 0; b < nb; b++) {
+            const int st = b % kPtStages;
+            const uint32_t back = (b / kPtStages + 1) & 1u;
+            const int key = key_of(b);
+            if (b >= kPtStages && !warp_wait(&sh.k_empty[st], back, deadline)) {
+                ok = false;
+                break;
+            }
+#pragma unroll
+            for (int i = 0; i < kLoads; i++) put(sh.kv[0][st], i * kRowsAtOnce + r0, k_raw[i], __half2(), false);
+            fence_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh.k_full[st]);
+            load(b + 1, p.c.k, pg_next, k_raw);
+            if (b >= kPtStages && !warp_wait(&sh.v_empty[st], back, deadline)) {
+                ok = false;
+                break;
+            }
+            if (!whole(key)) {
+                bool found = false;
+#pragma unroll
+                for (int i = 0; i < kLoads; i++) {
+                    uint4 &u = v_raw[i];
+                    const uint4 n = make_uint4(__vcmpeq4(u.x & 0x7f7f7f7fu, 0x7f7f7f7fu), __vcmpeq4(u.y & 0x7f7f7f7fu, 0x7f7f7f7fu),
+                                               __vcmpeq4(u.z & 0x7f7f7f7fu, 0x7f7f7f7fu), __vcmpeq4(u.w & 0x7f7f7f7fu, 0x7f7f7f7fu));
+                    found |= (n.x | n.y | n.z | n.w) != 0u;
+                    u = make_uint4(u.x & ~n.x, u.y & ~n.y, u.z & ~n.z, u.w & ~n.w);
+                }
+                if (found) atomicExch(&sh.bad, 1);
+            }
+#pragma unroll
+            for (int i = 0; i < kLoads; i++)
+                put(sh.kv[1][st], i * kRowsAtOnce + r0, v_raw[i], __float2half2_rn(vs[i] * inv_top), true);
+            fence_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh.v_full[st]);
+            load(b + 1, p.c.v, pg_next, v_raw);
+            scales(pg_next);
+            pages(b + 2, pg_next);
+        }
+    } else if (warp >= kWarpMma) {
+        // ---- the MMAs of tile t ----
+        const int t = warp - kWarpMma;
+        if (nb > 0 && t < tiles) {
+            const uint32_t lead = lane == 0, tm = __shfl_sync(0xffffffffu, tmem, 0);
+            constexpr uint32_t id_s = at_idesc<__half>(kKeys, false), id_o = at_idesc<__half>(HD, true);
+            auto issue_s = [&](int b) {   // S range t of two tiles, b % 2 of one
+                const uint64_t a0 = smem_desc_sw128(sh.q[t]), k0 = smem_desc_sw128(sh.kv[0][b % kPtStages]);
+                const int r = kTwoS ? b & 1 : t;
+#pragma unroll
+                for (int h = 0; h < kSub; h++)
+#pragma unroll
+                    for (int k = 0; k < 4; k++)   // 16 dims: +32 bytes
+                        warp_mma(tm + r * kKeys, a0 + h * (Sm::kQSub / 16) + 2 * k, k0 + h * (Sm::kSubTile / 16) + 2 * k, id_s,
+                                 (h | k) != 0 ? 1u : 0u, lead);
+                warp_commit(&sh.s_full[r], lead);
+                warp_commit(&sh.k_empty[b % kPtStages], lead);
+            };
+            auto issue_o = [&](int b, int h) {   // 64 keys of O += P V
+                const uint64_t v0 = at_desc_mn(sh.kv[1][b % kPtStages], Sm::kSubTile);
+                const int r = kTwoS ? b & 1 : t;
+#pragma unroll
+                for (int k = 0; k < kPtHalf / 16; k++)   // 16 keys: 8 columns of P, 2048 bytes of V
+                    warp_mma_ta(tm + kOCol + t * HD, tm + r * kKeys + h * kPtHalf + 8 * k, v0 + (h * 8192 + k * 2048) / 16, id_o,
+                                (b | h | k) != 0 ? 1u : 0u, lead);
+                if (kTwoS || h + 1 < kSteps) warp_commit(&sh.o_part[t], lead);
+            };
+            auto wait_k = [&](int b) { return warp_wait(&sh.k_full[b % kPtStages], (b / kPtStages) & 1u, deadline); };
+            ok = warp_wait(&sh.q_full[t], 0u, deadline) && wait_k(0);
+            if (ok) {
+                tc_fence_after();
+                issue_s(0);
+            }
+            for (int b = 0; b < nb && ok; b++) {
+                if constexpr (kTwoS) {
+                    if (b + 1 < nb) {   // over P(b - 1), behind the MMAs that read it
+                        ok = wait_k(b + 1);
+                        if (!ok) break;
+                        tc_fence_after();
+                        issue_s(b + 1);
+                    }
+                }
+                ok = warp_wait(&sh.v_full[b % kPtStages], (b / kPtStages) & 1u, deadline);
+#pragma unroll
+                for (int h = 0; h < kSteps; h++) {
+                    if (ok) ok = warp_wait(&sh.p_full[t][kTwoS ? b & 1 : h], (kTwoS ? b >> 1 : b) & 1u, deadline);
+                    if (!ok) break;
+                    tc_fence_after();
+                    issue_o(b, h);
+                }
+                if (!ok) break;
+                if constexpr (!kTwoS) {
+                    if (b + 1 < nb) {   // over P(b), behind the MMAs that read it
+                        ok = wait_k(b + 1);
+                        if (!ok) break;
+                        tc_fence_after();
+                        issue_s(b + 1);
+                    }
+                }
+                warp_commit(&sh.v_empty[b % kPtStages], lead);
+            }
+            warp_commit(&sh.o_done[t], lead);
+        }
+        if (p.stall_ns && t == 0) ok = warp_wait(&sh.stall, 0u, globaltimer() + p.stall_ns) && ok;
+    } else {
+        // ---- softmax: thread = packed row ----
+        const int t = warp / 4, q = warp % 4, ml = t * kAtRows + 32 * q + lane, m = m0 + ml;
+        const bool here = m0 + t * kAtRows + 32 * q < M;   // the warp has rows
+        if (here) {
+            {   // the warp's 32 rows of Q as fp16: HD / 8 lanes a row, zeros past M
+                constexpr int kCh = HD / 8, kAtOnce = 32 / kCh;
+                const int ch = lane % kCh;
+                unsigned char *const to = sh.q[t] + (ch >> 3) * Sm::kQSub;
+#pragma unroll 4
+                for (int it = 0; it < 32 / kAtOnce; it++) {
+                    const int rt = 32 * q + it * kAtOnce + lane / kCh, mm = m0 + t * kAtRows + rt;
+                    float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
+                    if (mm < M) {
+                        const T *src = static_cast<const T *>(p.q) + ((long long)(s.r0 + mm / p.group) * p.n_heads + head0 + mm % p.group) * HD + ch * 8;
+                        a = load4<T>(src);
+                        b = load4<T>(src + 4);
+                    }
+                    float up = 1.f;   // a power of two that takes the row's largest to [2^14, 2^15)
+                    if constexpr (!std::is_same<T, __half>::value) {
+                        const float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+                        float big = 0.f;
+#pragma unroll
+                        for (int e = 0; e < 8; e++) big = fmaxf(big, fabsf(v[e]) < INFINITY ? fabsf(v[e]) : 0.f);
+#pragma unroll
+                        for (int o = kCh / 2; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
+                        const int e = (int)(__float_as_uint(big) >> 23) - 127;
+                        up = big > 0.f ? __uint_as_float((uint32_t)(min(14 - e, 126) + 127) << 23) : 1.f;
+                    }
+                    *reinterpret_cast<uint4 *>(to + rt * 128 + (((ch & 7) ^ (rt & 7)) << 4)) =
+                        make_uint4(pack2<__half>(a.x * up, a.y * up), pack2<__half>(a.z * up, a.w * up),
+                                   pack2<__half>(b.x * up, b.y * up), pack2<__half>(b.z * up, b.w * up));
+                    if (ch == 0) sh.factor[t * kAtRows + rt] = p.scale_log2 / up;
+                }
+            }
+            const int i = min(m, M - 1) / p.group, at = s.pos + i;
+            // positions that the row sees: [0, e1) and [s2, at]
+            const int e1 = min(ns, at + 1), s2 = p.window > 0 ? max(0, at - p.window + 1) : 0;
+            const uint32_t tl = tmem + ((uint32_t)(32 * q) << 16);
+            const uint32_t to = tl + kOCol + t * HD;
+            float mr = -INFINITY, l = 0.f;
+            float sv[32];
+            fence_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh.q_full[t]);
+            const float sl2 = sh.factor[ml];
+            // lane g: page and K's scale of a block's positions 16 g ..
+            auto group_page = [&](int b) { return b < nb && lane < kGroups ? page_of(key_of(b) + 16 * lane) : -1; };
+            int page = group_page(0), page_next = group_page(1);
+            float ks = page >= 0 ? __ldg(p.c.k_scale + scale_at(p.c, p.layer, page, kvh)) : 0.f;
+            for (int b = 0; b < nb; b++) {
+                const int r = kTwoS ? b & 1 : t;   // the S range
+                const int key = key_of(b);
+                const uint32_t there = __ballot_sync(0xffffffffu, page >= 0);
+                const bool full = whole(key) && there == (1u << kGroups) - 1;
+                page = page_next;
+                const float ks_now = ks;
+                ks = page >= 0 ? __ldg(p.c.k_scale + scale_at(p.c, p.layer, page, kvh)) : 0.f;
+                page_next = group_page(b + 2);
+                if (!warp_wait(&sh.s_full[r], (kTwoS ? b >> 1 : b) & 1u, deadline)) ok = false;
+                tc_fence_after();
+#pragma unroll 1
+                for (int h = 0; h < kSteps; h++) {
+                    const uint32_t ts = tl + r * kKeys + h * kPtHalf;
+                    const int c0 = key + h * kPtHalf;
+                    uint64_t vis = 0;
+                    if (!full) {
+                        uint32_t word[2];
+#pragma unroll
+                        for (int e = 0; e < 2; e++) {
+                            const uint32_t two = there >> (4 * h + 2 * e);
+                            word[e] = (range_bits(c0 + 32 * e, 0, e1) | range_bits(c0 + 32 * e, s2, at + 1)) &
+                                      ((two & 1u ? 0xffffu : 0u) | (two & 2u ? 0xffff0000u : 0u));
+                        }
+                        vis = (uint64_t)word[1] << 32 | word[0];
+                    }
+                    // P against m so far; a row whose keys exceed it by 2^15 takes
+                    // theirs, and the warp goes over them again (S is intact until P
+                    // is stored)
+                    uint32_t w[32];
+                    float base = mr == -INFINITY ? 0.f : mr, factor = 1.f, ls = 0.f;
+                    float over;   // the largest less base
+                    bool moved = false;
+#pragma unroll 1
+                    for (;;) {    // (one copy of its code)
+                        over = full ? weigh64<false>(ts, sl2, ks_now, 4 * h, base, vis, w, ls)
+                                    : weigh64<true>(ts, sl2, ks_now, 4 * h, base, vis, w, ls);
+                        const bool move = mr == -INFINITY ? over > -INFINITY : over > kPtAbove;
+                        if (moved || !__any_sync(0xffffffffu, move)) break;
+                        moved = true;
+                        if (move) {
+                            const float mn = base + over - kPtBelow;
+                            factor = mr == -INFINITY ? 0.f : exp2_approx(mr - mn);
+                            mr = base = mn;
+                            l *= factor;
+                        }
+                    }
+                    if (mr > -INFINITY || ls != ls) l += ls;   // (without a finite score: 0 or NaN, not the polynomial's 2^-126)
+                    tmem_st32_async(ts, w);       // over S
+                    if (moved && b + h > 0) {
+                        // O must hold the weights before these.  Two S ranges: S(b)
+                        // is behind the MMAs of block b - 2, those of b - 1 may be
+                        // under way; else S(b) is behind block b - 1's, and the
+                        // second step waits for the first's.
+                        if (kTwoS || h == 1)
+                            if (!warp_wait(&sh.o_part[t], (kTwoS ? b - 1 : b) & 1u, deadline)) ok = false;
+                        tc_fence_after();
+#pragma unroll
+                        for (int c = 0; c < HD; c += 32) {
+                            tmem_ld32(to + c, sv);
+#pragma unroll
+                            for (int j = 0; j < 32; j++) sv[j] *= factor;
+                            tmem_st32(to + c, sv);
+                        }
+                    }
+                    tmem_wait_st();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&sh.p_full[t][kTwoS ? r : h]);
+                }
+            }
+            // shares go over K and V, which the other tile's MMAs may still read
+            for (int e = Z > 1 ? 0 : t; e < (Z > 1 ? tiles : t + 1); e++)
+                if (nb > 0 && !warp_wait(&sh.o_done[e], 0u, deadline)) ok = false;
+            tc_fence_after();
+            const float v_top = __int_as_float(*(volatile int *)&sh.v_top);
+            const float il = l == 0.f ? 0.f : v_top / l;   // no weight at all: zeros (O is tiny, not NaN)
+            const bool bad = *(volatile int *)&sh.bad != 0;
+            const long long row = (long long)(s.r0 + i) * p.n_heads + head0 + min(m, M - 1) % p.group;
+#pragma unroll
+            for (int c = 0; c < HD; c += 32) {
+                if (nb > 0) tmem_ld32(to + c, sv);
+                else {
+#pragma unroll
+                    for (int j = 0; j < 32; j++) sv[j] = 0.f;
+                }
+                if (bad)   // the NaN of V that this row sees in masked blocks
+                    for (int b = 0; b < nb; b++) {
+                        const int key = key_of(b);
+                        if (whole(key)) continue;
+                        for (int j = key; j < key + kKeys; j++) {
+                            if (j >= at + 1 || (j >= e1 && j < s2)) continue;
+                            const int pg = page_at(p.c, stream, j >> p.c.page_shift);
+                            if (pg < 0) continue;
+                            const unsigned char *v = p.c.v + page_base(p.c, p.layer, pg, kvh) + (j & (p.c.page - 1)) * p.c.slot_stride + c;
+                            for (int d = 0; d < 32; d++)
+                                if ((v[d] & 0x7fu) == 0x7fu)
+#pragma unroll
+                                    for (int e = 0; e < 32; e++) sv[e] = e == d ? NAN : sv[e];
+                        }
+                    }
+                if (Z > 1) {
+                    // this share's sums, 16-byte chunks swizzled by the row
+                    float *o = reinterpret_cast<float *>(sh.o) + ml * HD;
+#pragma unroll
+                    for (int j = 0; j < 32; j += 4)
+                        *reinterpret_cast<float4 *>(o + ((((c + j) >> 2) ^ (ml & 7)) << 2)) =
+                            make_float4(sv[j] * v_top, sv[j + 1] * v_top, sv[j + 2] * v_top, sv[j + 3] * v_top);
+                } else if (ok && m < M) {
+                    T *dst = static_cast<T *>(p.out) + row * HD + c;
+#pragma unroll
+                    for (int j = 0; j < 32; j += 8)
+                        *reinterpret_cast<uint4 *>(dst + j) =
+                            make_uint4(pack2<T>(sv[j] * il, sv[j + 1] * il), pack2<T>(sv[j + 2] * il, sv[j + 3] * il),
+                                       pack2<T>(sv[j + 4] * il, sv[j + 5] * il), pack2<T>(sv[j + 6] * il, sv[j + 7] * il));
+                }
+            }
+            if (Z > 1) {
+                sh.mx[ml] = mr;
+                sh.sum[ml] = l;
+            } else if (ok && m < M && p.lse) {
+                p.lse[row] = l == 0.f ? -INFINITY : (mr + log2f(l)) * 0.69314718055994531f;
+            }
+        }
+    }
+    if (!ok) {
+        sh.failed = 1;
+        if (p.err) atomicExch_system(p.err, 1u);
+        const uint64_t grace = globaltimer() + 10000000ull;   // let copies and MMAs in flight land
+        while (globaltimer() < grace) {
+        }
+    }
+    // TMEM goes back before the cluster meets: no CTA holds it while it waits
+    // for a peer that may itself wait for TMEM
+    tc_fence_before();
+    __syncthreads();
+    if (warp == kWarpMma) {
+        tc_fence_after();
+        tmem_dealloc(tmem, kTmemCols);
+    }
+    if (sh.failed) {   // whatever was written or is to be merged: NaN, so that no void row passes for a result
+        const int rows = min(NT * kAtRows, M - m0);
+        for (int ml = threadIdx.x; ml < rows; ml += kThreads) {
+            const int m = m0 + ml;
+            const long long row = (long long)(s.r0 + m / p.group) * p.n_heads + head0 + m % p.group;
+            sh.mx[ml] = sh.sum[ml] = NAN;
+            if (Z > 1) continue;
+            for (int d = 0; d < HD; d += 8)
+                *reinterpret_cast<uint4 *>(static_cast<T *>(p.out) + row * HD + d) =
+                    make_uint4(0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu);   // NaN in either type
+            if (p.lse) p.lse[row] = NAN;
+        }
+    }
+    if (Z > 1) {
+        cluster_sync_all();
+        const uint32_t o_s = smem_u32(sh.o), m_s = smem_u32(sh.mx), l_s = smem_u32(sh.sum);
+        const int rows = min(NT * kAtRows, M - m0);
+        for (int e = z * kThreads + threadIdx.x; e < rows * (HD / 4); e += Z * kThreads) {
+            const int ml = e / (HD / 4), d4 = e % (HD / 4), m = m0 + ml;
+            float gm = -INFINITY;
+            for (int r = 0; r < Z; r++) gm = fmaxf(gm, ld_dsmem_f1(mapa_shared(m_s + 4 * ml, r)));
+            float gl = 0.f;
+            float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int r = 0; r < Z; r++) {
+                const float mr = ld_dsmem_f1(mapa_shared(m_s + 4 * ml, r));
+                const float w = mr == -INFINITY ? 0.f : exp2_approx(mr - gm);
+                const float l = ld_dsmem_f1(mapa_shared(l_s + 4 * ml, r));
+                const float4 v = ld_dsmem_f4(mapa_shared(o_s + 4 * (ml * HD + ((d4 ^ (ml & 7)) << 2)), r));
+                if (mr == -INFINITY && l == 0.f) continue;   // this share saw no key of the row
+                gl = fmaf(w, l, gl);
+                a.x = fmaf(w, v.x, a.x);
+                a.y = fmaf(w, v.y, a.y);
+                a.z = fmaf(w, v.z, a.z);
+                a.w = fmaf(w, v.w, a.w);
+            }
+            const float il = gl == 0.f ? 0.f : 1.0f / gl;
+            const long long row = (long long)(s.r0 + m / p.group) * p.n_heads + head0 + m % p.group;
+            store4<T>(static_cast<T *>(p.out) + row * HD + 4 * d4, make_float4(a.x * il, a.y * il, a.z * il, a.w * il));
+            if (p.lse && d4 == 0) p.lse[row] = gl == 0.f ? -INFINITY : (gm + log2f(gl)) * 0.69314718055994531f;
+        }
+        cluster_sync_all();   // no CTA leaves while a peer still reads its share
+    }
+}
+
+template <int HD, int NT>
+constexpr size_t pt_smem() {
+    return std::max<size_t>(sizeof(PtSmem<HD, NT>), NT == 2 ? kPtOneCta : 0);
+}
+
+template <typename T, int HD, int NT>
+cudaError_t launch_many(PagedAttnParams p, cudaStream_t st) {
+    auto kernel = paged_many_kernel<T, HD, NT>;
+    constexpr size_t kSmem = pt_smem<HD, NT>();
+    static_assert(kSmem <= (228 / pt_ctas(NT) - 1) * 1024, "they fit an SM");
+    static ClusterKernel ck;
+    int dev = 0;
+    cudaError_t e = cluster_prepare(ck, kernel, kSmem, &dev);
+    if (e != cudaSuccess) return e;
+    const long long M = (long long)p.r.max_rows * p.group, tiles = (M + NT * kAtRows - 1) / (NT * kAtRows);
+    long long keys = (long long)p.c.table_stride * p.c.page;
+    if (p.window > 0) keys = std::min(keys, (long long)p.window + p.n_sink + (NT * kAtRows - 1) / p.group + 2);
+    const long long blocks = (keys + pt_keys(NT) - 1) / pt_keys(NT), all = tiles * p.c.n_kv_heads * p.c.n_streams;
+    int Z = 1;
+    while (Z < 8 && all * (Z + 1) <= 148ll * pt_ctas(NT) && blocks / (Z + 1) >= 4) Z++;
+    p.shares = Z;
+    cudaLaunchAttribute attr;
+    const cudaLaunchConfig_t cfg = cluster_config(dim3((unsigned)(Z * tiles), p.c.n_kv_heads, p.c.n_streams), pt_threads(NT), kSmem, Z,
+                                                  &attr, st);
+    return cudaLaunchKernelEx(&cfg, kernel, p);
+}
+
+template <typename T, int HD>
+cudaError_t launch_dim(const PagedAttnParams &p, cudaStream_t st) {
+    const long long M = (long long)p.r.max_rows * p.group;
+    return M <= kAtRows ? launch_many<T, HD, 1>(p, st) : launch_many<T, HD, 2>(p, st);
+}
+template <typename T>
+cudaError_t launch_typed(const PagedAttnParams &p, cudaStream_t st) {
+    return p.c.head_dim == 64 ? launch_dim<T, 64>(p, st) : launch_dim<T, 128>(p, st);
+}
+
+}  // namespace
+
+cudaError_t launch_paged_attn_tc(const PagedAttnParams &p, cudaStream_t st) {
+    return p.q_type == ELEM_BF16 ? launch_typed<__nv_bfloat16>(p, st) : launch_typed<__half>(p, st);
+}
+
+}  // namespace vc

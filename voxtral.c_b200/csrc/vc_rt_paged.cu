@@ -175,6 +175,8 @@ extern "C" int vox_cuda_attention_paged_dev(const vox_cuda_paged_cache *cache, i
     if (!c) return VOX_CUDA_ERR_UNAVAILABLE;
     DeviceGuard guard(c->device);
     if (!guard.ok()) return launched(who, cudaGetLastError());
+    if ((rc = check_waits(who, c))) return rc;
+    p.err = c->op_err + op_slot();
     p.layer = layer;
     p.q = q;
     p.out = out;
