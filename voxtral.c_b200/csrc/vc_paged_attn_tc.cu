@@ -71,16 +71,22 @@ struct PtSmem {
     uint64_t stall;   // nothing arrives here
 };
 
+__device__ __forceinline__ float max3(float a, float b, float c) {   // a NaN is passed over
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+
 // The weights of 64 keys of a row: w = 2^(s f - base) as pairs of fp16, ls their
 // sum before rounding; the largest s f - base as the result.  f: the row's factor
 // times K's scale, by groups of 16 keys in the warp's lanes.  The next 16 scores
-// are on their way from TMEM while 16 are worked on.  In blocks without a mask
-// kPtPoly of 8 pairs take 2^x on the FMA pipe, since the exponential unit takes 8
-// cycles per warp.
-constexpr int kPtPoly = 3;
+// are on their way from TMEM while 16 are worked on.  (2^x on the FMA pipe for
+// some of the pairs, which the exponential unit's 8 cycles a warp suggest, costs
+// more issue slots than it saves: 3 of 8 pairs 601 against 531 us for the prompt
+// chunks of 15035 and 8008 keys.)
 template <bool MASKED>
 __device__ __forceinline__ float weigh64(uint32_t ts, float sl2, float ks, int g0, float base, uint64_t vis, uint32_t (&w)[32], float &ls) {
-    float mx[2] = {-INFINITY, -INFINITY};
+    float mx = -INFINITY;
     uint64_t rs[2] = {0, 0};
     const uint64_t nb = pair(-base, -base);
     uint32_t ra[16], rb[16];
@@ -100,14 +106,9 @@ __device__ __forceinline__ float weigh64(uint32_t ts, float sl2, float ks, int g
                 xa = (vis >> (c + j)) & 1u ? xa : -INFINITY;
                 xb = (vis >> (c + j + 1)) & 1u ? xb : -INFINITY;
             }
-            mx[0] = fmaxf(mx[0], xa);
-            mx[1] = fmaxf(mx[1], xb);
-            if (!MASKED && (j >> 1) % 8 < kPtPoly) {
-                exp2_poly2(xa, xb);
-            } else {
-                xa = exp2_approx(xa);
-                xb = exp2_approx(xb);
-            }
+            mx = max3(mx, xa, xb);
+            xa = exp2_approx(xa);
+            xb = exp2_approx(xb);
             rs[(j >> 1) & 1] = add2(rs[(j >> 1) & 1], pair(xa, xb));
             w[(c + j) >> 1] = pack2<__half>(xa, xb);
         }
@@ -115,7 +116,7 @@ __device__ __forceinline__ float weigh64(uint32_t ts, float sl2, float ks, int g
     float a, b;
     unpair(add2(rs[0], rs[1]), a, b);
     ls = a + b;
-    return fmaxf(mx[0], mx[1]);
+    return mx;
 }
 
 template <typename T, int HD, int NT>
@@ -149,10 +150,11 @@ __global__ void __launch_bounds__(pt_threads(NT), pt_ctas(NT)) paged_many_kernel
     auto whole = [&](int key) {
         return key + kKeys - 1 <= p_min && (p.window <= 0 || key > p_max - p.window || key + kKeys <= p.n_sink);
     };
-    // the page of 16 positions, -1: none, or no row sees them
-    auto page_of = [&](int key) {
-        return key < hi && (key + 16 > lo || key < ns) ? page_at(p.c, stream, key >> p.c.page_shift) : -1;
-    };
+    // the table's entry for 16 positions, -1: no row sees them; whether it is a
+    // page is asked where it is used, blocks later, so that nothing waits for it here
+    const int *const table = p.c.table + (long long)stream * p.c.table_stride;
+    auto entry_of = [&](int key) { return key < hi && (key + 16 > lo || key < ns) ? __ldg(table + (key >> p.c.page_shift)) : -1; };
+    auto is_page = [&](int g) { return g >= 0 && g < p.c.n_pages; };
     bool ok = true;
 
     if (threadIdx.x == 0) {
@@ -192,28 +194,32 @@ __global__ void __launch_bounds__(pt_threads(NT), pt_ctas(NT)) paged_many_kernel
         // a thread's 16 dims of a row, so that the lanes of a store meet no bank twice
         const int tid = threadIdx.x - kWarpConv * 32;
         const int r0 = HD == 128 ? ((tid >> 4) << 1 | ((tid >> 2) & 1)) : tid >> 2, sub = HD == 128 ? (tid >> 3) & 1 : 0, ch = tid & 3;
-        const long long mine = sub * 64 + ch * 16;
-        int pg[kLoads], pg_next[kLoads];
+        const long long mine = (r0 & 15) * p.c.slot_stride + sub * 64 + ch * 16;
         uint4 k_raw[kLoads], v_raw[kLoads];
-        float vs[kLoads];
-        auto pages = [&](int b, int (&g)[kLoads]) {
-            const int key = b < nb ? key_of(b) : 0;
-#pragma unroll
-            for (int i = 0; i < kLoads; i++) g[i] = b < nb ? page_of((key + i * kRowsAtOnce + r0) & ~15) : -1;
+        // lane g has the place of a block's positions 16 g .. and V's scale of
+        // their page; the threads that load them ask for it
+        struct Place {
+            long long off;   // -1: no page
+            float vs;
         };
-        auto load = [&](int b, const unsigned char *pool, const int (&g)[kLoads], uint4 (&raw)[kLoads]) {
-            const int key = b < nb ? key_of(b) : 0;
+        const long long base = page_base(p.c, p.layer, 0, kvh), scale0 = scale_at(p.c, p.layer, 0, kvh);
+        auto entry = [&](int b) { return b < nb && lane < kGroups ? entry_of(key_of(b) + 16 * lane) : -1; };
+        auto place = [&](int b, int g) {
+            Place at = {-1, 0.f};
+            if (is_page(g)) {
+                at.off = base + (long long)g * p.c.page_stride + ((key_of(b) + 16 * lane) & (p.c.page - 1)) * p.c.slot_stride;
+                at.vs = __ldg(p.c.v_scale + scale0 + (long long)g * p.c.n_kv_heads);
+            }
+            return at;
+        };
+        auto group = [&](int i) { return HD == 128 ? i : 2 * i + (r0 >> 4); };   // of the thread's load i
+        auto load = [&](const unsigned char *pool, const Place &at, uint4 (&raw)[kLoads]) {
 #pragma unroll
             for (int i = 0; i < kLoads; i++) {
                 raw[i] = make_uint4(0u, 0u, 0u, 0u);
-                const int slot = (key + i * kRowsAtOnce + r0) & (p.c.page - 1);
-                if (g[i] >= 0)
-                    raw[i] = __ldg(reinterpret_cast<const uint4 *>(pool + page_base(p.c, p.layer, g[i], kvh) + slot * p.c.slot_stride + mine));
+                const long long off = __shfl_sync(0xffffffffu, at.off, group(i));
+                if (off >= 0) raw[i] = __ldg(reinterpret_cast<const uint4 *>(pool + off + mine));
             }
-        };
-        auto scales = [&](const int (&g)[kLoads]) {
-#pragma unroll
-            for (int i = 0; i < kLoads; i++) vs[i] = g[i] >= 0 ? __ldg(p.c.v_scale + scale_at(p.c, p.layer, g[i], kvh)) : 0.f;
         };
         auto put = [&](unsigned char *tile, int r, const uint4 &u, __half2 by, bool scaled) {
             const uint32_t in[4] = {u.x, u.y, u.z, u.w};
@@ -232,11 +238,10 @@ __global__ void __launch_bounds__(pt_threads(NT), pt_ctas(NT)) paged_many_kernel
             *reinterpret_cast<uint4 *>(row + (((2 * ch) ^ (r & 7)) << 4)) = make_uint4(out[0], out[1], out[2], out[3]);
             *reinterpret_cast<uint4 *>(row + (((2 * ch + 1) ^ (r & 7)) << 4)) = make_uint4(out[4], out[5], out[6], out[7]);
         };
-        pages(0, pg);
-        load(0, p.c.k, pg, k_raw);
-        load(0, p.c.v, pg, v_raw);
-        scales(pg);
-        pages(1, pg_next);
+        Place here = place(0, entry(0));
+        load(p.c.k, here, k_raw);
+        load(p.c.v, here, v_raw);
+        int next = entry(1);
         {   // the largest scale of V
             const int step = min(p.c.page, kKeys), n = nb * (kKeys / step);
             float top = 0.f;
@@ -266,7 +271,8 @@ __global__ void __launch_bounds__(pt_threads(NT), pt_ctas(NT)) paged_many_kernel
             fence_async_smem();
             __syncwarp();
             if (lane == 0) mbar_arrive(&sh.k_full[st]);
-            load(b + 1, p.c.k, pg_next, k_raw);
+            const Place then = place(b + 1, next);
+            load(p.c.k, then, k_raw);
             if (b >= kPtStages && !warp_wait(&sh.v_empty[st], back, deadline)) {
                 ok = false;
                 break;
@@ -285,13 +291,14 @@ __global__ void __launch_bounds__(pt_threads(NT), pt_ctas(NT)) paged_many_kernel
             }
 #pragma unroll
             for (int i = 0; i < kLoads; i++)
-                put(sh.kv[1][st], i * kRowsAtOnce + r0, v_raw[i], __float2half2_rn(vs[i] * inv_top), true);
+                put(sh.kv[1][st], i * kRowsAtOnce + r0, v_raw[i],
+                    __float2half2_rn(__shfl_sync(0xffffffffu, here.vs, group(i)) * inv_top), true);
             fence_async_smem();
             __syncwarp();
             if (lane == 0) mbar_arrive(&sh.v_full[st]);
-            load(b + 1, p.c.v, pg_next, v_raw);
-            scales(pg_next);
-            pages(b + 2, pg_next);
+            load(p.c.v, then, v_raw);
+            here = then;
+            next = entry(b + 2);
         }
     } else if (warp >= kWarpMma) {
         // ---- the MMAs of tile t ----
@@ -403,19 +410,20 @@ __global__ void __launch_bounds__(pt_threads(NT), pt_ctas(NT)) paged_many_kernel
             __syncwarp();
             if (lane == 0) mbar_arrive(&sh.q_full[t]);
             const float sl2 = sh.factor[ml];
-            // lane g: page and K's scale of a block's positions 16 g ..
-            auto group_page = [&](int b) { return b < nb && lane < kGroups ? page_of(key_of(b) + 16 * lane) : -1; };
-            int page = group_page(0), page_next = group_page(1);
-            float ks = page >= 0 ? __ldg(p.c.k_scale + scale_at(p.c, p.layer, page, kvh)) : 0.f;
+            // lane g: table entry and K's scale of a block's positions 16 g ..
+            auto entry = [&](int b) { return b < nb && lane < kGroups ? entry_of(key_of(b) + 16 * lane) : -1; };
+            auto scale = [&](int g) { return is_page(g) ? __ldg(p.c.k_scale + scale_at(p.c, p.layer, g, kvh)) : 0.f; };
+            int page = entry(0), page_next = entry(1);
+            float ks = scale(page);
             for (int b = 0; b < nb; b++) {
                 const int r = kTwoS ? b & 1 : t;   // the S range
                 const int key = key_of(b);
-                const uint32_t there = __ballot_sync(0xffffffffu, page >= 0);
+                const uint32_t there = __ballot_sync(0xffffffffu, is_page(page));
                 const bool full = whole(key) && there == (1u << kGroups) - 1;
-                page = page_next;
                 const float ks_now = ks;
-                ks = page >= 0 ? __ldg(p.c.k_scale + scale_at(p.c, p.layer, page, kvh)) : 0.f;
-                page_next = group_page(b + 2);
+                page = page_next;
+                ks = scale(page);
+                page_next = entry(b + 2);
                 if (!warp_wait(&sh.s_full[r], (kTwoS ? b >> 1 : b) & 1u, deadline)) ok = false;
                 tc_fence_after();
 #pragma unroll 1
@@ -454,7 +462,7 @@ __global__ void __launch_bounds__(pt_threads(NT), pt_ctas(NT)) paged_many_kernel
                             l *= factor;
                         }
                     }
-                    if (mr > -INFINITY || ls != ls) l += ls;   // (without a finite score: 0 or NaN, not the polynomial's 2^-126)
+                    l += ls;
                     tmem_st32_async(ts, w);       // over S
                     if (moved && b + h > 0) {
                         // O must hold the weights before these.  Two S ranges: S(b)
