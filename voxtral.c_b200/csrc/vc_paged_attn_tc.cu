@@ -10,11 +10,13 @@
 //   4 warps          K and V: 16 bytes of a key to a thread, e4m3 to fp16 (exact),
 //                    into the MMAs' swizzled layout, the next block's loads under
 //                    way meanwhile
-//   1 warp per tile  issues its MMAs, M 128: S_t = Q_t K^T (K HD) and, by steps
-//                    of 64 keys, O_t += P_t V (N HD; A from TMEM, V an MN-major
-//                    operand)
+//   1 warp per tile  issues its MMAs by steps of 64 keys, M 128: S_t = Q_t K^T (K
+//                    HD) and O_t += P_t V (N HD; A from TMEM, V an MN-major operand)
 // Two tiles share each K and V block, so that its conversion (about a quarter
-// of the CTA's instructions) is paid once per 256 rows.
+// of the CTA's instructions) is paid once per 256 rows.  A tile has two S ranges
+// in turn: S(u + 2) goes over P(u) as soon as O has it, so that S(u + 1) waits for
+// the softmax and not the softmax for it (one range of 128 keys, whose MMAs read
+// Q half as often, took 527 us for the prompt chunks).
 //
 // All operands are fp16, whatever q's type: bf16 rows of Q are scaled by a power
 // of two into its range (exact but for values 2^-29 of the row's largest), K's
@@ -62,8 +64,8 @@ struct PtSmem {
         unsigned char o[kO];
     };
     float mx[NT * kAtRows], sum[NT * kAtRows], factor[NT * kAtRows];
-    uint64_t q_full[NT], k_full[kPtStages], k_empty[kPtStages], v_full[kPtStages], v_empty[kPtStages], s_full[2], p_full[NT][2],
-        o_part[NT], o_done[NT];   // s_full: by tile, or (one tile) by S range
+    uint64_t q_full[NT], k_full[kPtStages], k_empty[kPtStages], v_full[kPtStages], v_empty[kPtStages];
+    uint64_t s_full[NT][2], p_full[NT][2], o_part[NT], o_done[NT];   // [2]: by S range
     uint32_t tmem;
     int v_top;    // V's largest scale, as the bits of a float >= 0
     int bad;      // a masked block holds NaN in V
@@ -125,9 +127,8 @@ __global__ void __launch_bounds__(pt_threads(NT), pt_ctas(NT)) paged_many_kernel
     constexpr int kSub = HD / 64;            // 64-dim sub-tiles of a tile
     constexpr int kWarpConv = NT * 4, kWarpMma = kWarpConv + kPtConv / 32;
     constexpr int kThreads = pt_threads(NT), kKeys = Sm::kKeys, kSteps = kKeys / kPtHalf, kGroups = kKeys / 16;
-    constexpr bool kTwoS = NT == 1;          // two S ranges: S(b + 1) is ready when the softmax is done with S(b)
     constexpr uint32_t kTmemCols = NT == 2 ? 512 : 256;
-    constexpr uint32_t kOCol = kTwoS ? 2 * kKeys : NT * kKeys;   // S ranges first, then O tiles
+    constexpr uint32_t kOCol = NT * 2 * kPtHalf;   // S ranges first, two a tile, then O tiles
     extern __shared__ __align__(1024) unsigned char pt_smem_raw[];
     Sm &sh = *reinterpret_cast<Sm *>(pt_smem_raw);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -169,11 +170,11 @@ __global__ void __launch_bounds__(pt_threads(NT), pt_ctas(NT)) paged_many_kernel
             mbar_init(&sh.q_full[t], warps);
             mbar_init(&sh.p_full[t][0], warps);
             mbar_init(&sh.p_full[t][1], warps);
+            mbar_init(&sh.s_full[t][0], 1);
+            mbar_init(&sh.s_full[t][1], 1);
             mbar_init(&sh.o_part[t], 1);
             mbar_init(&sh.o_done[t], 1);
         }
-        mbar_init(&sh.s_full[0], 1);
-        mbar_init(&sh.s_full[1], 1);
         mbar_init(&sh.stall, 1);
         sh.v_top = sh.bad = sh.failed = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -305,61 +306,48 @@ __global__ void __launch_bounds__(pt_threads(NT), pt_ctas(NT)) paged_many_kernel
         const int t = warp - kWarpMma;
         if (nb > 0 && t < tiles) {
             const uint32_t lead = lane == 0, tm = __shfl_sync(0xffffffffu, tmem, 0);
-            constexpr uint32_t id_s = at_idesc<__half>(kKeys, false), id_o = at_idesc<__half>(HD, true);
-            auto issue_s = [&](int b) {   // S range t of two tiles, b % 2 of one
-                const uint64_t a0 = smem_desc_sw128(sh.q[t]), k0 = smem_desc_sw128(sh.kv[0][b % kPtStages]);
-                const int r = kTwoS ? b & 1 : t;
+            constexpr uint32_t id_s = at_idesc<__half>(kPtHalf, false), id_o = at_idesc<__half>(HD, true);
+            // step u: 64 keys, half u % kSteps of block u / kSteps, S range u % 2
+            const int steps = nb * kSteps;
+            auto issue_s = [&](int u) {
+                const int b = u / kSteps, h = u % kSteps;
+                const uint64_t a0 = smem_desc_sw128(sh.q[t]), k0 = smem_desc_sw128(sh.kv[0][b % kPtStages]) + h * (kPtHalf * 128 / 16);
 #pragma unroll
-                for (int h = 0; h < kSub; h++)
+                for (int d = 0; d < kSub; d++)
 #pragma unroll
                     for (int k = 0; k < 4; k++)   // 16 dims: +32 bytes
-                        warp_mma(tm + r * kKeys, a0 + h * (Sm::kQSub / 16) + 2 * k, k0 + h * (Sm::kSubTile / 16) + 2 * k, id_s,
-                                 (h | k) != 0 ? 1u : 0u, lead);
-                warp_commit(&sh.s_full[r], lead);
-                warp_commit(&sh.k_empty[b % kPtStages], lead);
+                        warp_mma(tm + (t * 2 + (u & 1)) * kPtHalf, a0 + d * (Sm::kQSub / 16) + 2 * k, k0 + d * (Sm::kSubTile / 16) + 2 * k,
+                                 id_s, (d | k) != 0 ? 1u : 0u, lead);
+                warp_commit(&sh.s_full[t][u & 1], lead);
+                if (h == kSteps - 1) warp_commit(&sh.k_empty[b % kPtStages], lead);
             };
-            auto issue_o = [&](int b, int h) {   // 64 keys of O += P V
-                const uint64_t v0 = at_desc_mn(sh.kv[1][b % kPtStages], Sm::kSubTile);
-                const int r = kTwoS ? b & 1 : t;
+            auto issue_o = [&](int u) {   // O += P V
+                const int b = u / kSteps, h = u % kSteps;
+                const uint64_t v0 = at_desc_mn(sh.kv[1][b % kPtStages], Sm::kSubTile) + h * (kPtHalf * 128 / 16);
 #pragma unroll
                 for (int k = 0; k < kPtHalf / 16; k++)   // 16 keys: 8 columns of P, 2048 bytes of V
-                    warp_mma_ta(tm + kOCol + t * HD, tm + r * kKeys + h * kPtHalf + 8 * k, v0 + (h * 8192 + k * 2048) / 16, id_o,
-                                (b | h | k) != 0 ? 1u : 0u, lead);
-                if (kTwoS || h + 1 < kSteps) warp_commit(&sh.o_part[t], lead);
+                    warp_mma_ta(tm + kOCol + t * HD, tm + (t * 2 + (u & 1)) * kPtHalf + 8 * k, v0 + k * (2048 / 16), id_o,
+                                (u | k) != 0 ? 1u : 0u, lead);
+                warp_commit(&sh.o_part[t], lead);
+                if (h == kSteps - 1) warp_commit(&sh.v_empty[b % kPtStages], lead);
             };
-            auto wait_k = [&](int b) { return warp_wait(&sh.k_full[b % kPtStages], (b / kPtStages) & 1u, deadline); };
-            ok = warp_wait(&sh.q_full[t], 0u, deadline) && wait_k(0);
-            if (ok) {
+            auto next_s = [&](int u) {   // S(u), once its keys are there
+                if (u >= steps) return true;
+                const int b = u / kSteps;
+                if (u % kSteps == 0 && !warp_wait(&sh.k_full[b % kPtStages], (b / kPtStages) & 1u, deadline)) return false;
                 tc_fence_after();
-                issue_s(0);
-            }
-            for (int b = 0; b < nb && ok; b++) {
-                if constexpr (kTwoS) {
-                    if (b + 1 < nb) {   // over P(b - 1), behind the MMAs that read it
-                        ok = wait_k(b + 1);
-                        if (!ok) break;
-                        tc_fence_after();
-                        issue_s(b + 1);
-                    }
-                }
-                ok = warp_wait(&sh.v_full[b % kPtStages], (b / kPtStages) & 1u, deadline);
-#pragma unroll
-                for (int h = 0; h < kSteps; h++) {
-                    if (ok) ok = warp_wait(&sh.p_full[t][kTwoS ? b & 1 : h], (kTwoS ? b >> 1 : b) & 1u, deadline);
-                    if (!ok) break;
-                    tc_fence_after();
-                    issue_o(b, h);
-                }
+                issue_s(u);
+                return true;
+            };
+            ok = warp_wait(&sh.q_full[t], 0u, deadline) && next_s(0) && next_s(1);
+            for (int u = 0; u < steps && ok; u++) {
+                const int b = u / kSteps;
+                ok = (u % kSteps != 0 || warp_wait(&sh.v_full[b % kPtStages], (b / kPtStages) & 1u, deadline)) &&
+                     warp_wait(&sh.p_full[t][u & 1], (u >> 1) & 1u, deadline);
                 if (!ok) break;
-                if constexpr (!kTwoS) {
-                    if (b + 1 < nb) {   // over P(b), behind the MMAs that read it
-                        ok = wait_k(b + 1);
-                        if (!ok) break;
-                        tc_fence_after();
-                        issue_s(b + 1);
-                    }
-                }
-                warp_commit(&sh.v_empty[b % kPtStages], lead);
+                tc_fence_after();
+                issue_o(u);
+                ok = next_s(u + 2);   // over P(u), behind the MMAs that read it
             }
             warp_commit(&sh.o_done[t], lead);
         }
@@ -416,7 +404,6 @@ __global__ void __launch_bounds__(pt_threads(NT), pt_ctas(NT)) paged_many_kernel
             int page = entry(0), page_next = entry(1);
             float ks = scale(page);
             for (int b = 0; b < nb; b++) {
-                const int r = kTwoS ? b & 1 : t;   // the S range
                 const int key = key_of(b);
                 const uint32_t there = __ballot_sync(0xffffffffu, is_page(page));
                 const bool full = whole(key) && there == (1u << kGroups) - 1;
@@ -424,11 +411,12 @@ __global__ void __launch_bounds__(pt_threads(NT), pt_ctas(NT)) paged_many_kernel
                 page = page_next;
                 ks = scale(page);
                 page_next = entry(b + 2);
-                if (!warp_wait(&sh.s_full[r], (kTwoS ? b >> 1 : b) & 1u, deadline)) ok = false;
-                tc_fence_after();
 #pragma unroll 1
                 for (int h = 0; h < kSteps; h++) {
-                    const uint32_t ts = tl + r * kKeys + h * kPtHalf;
+                    const int u = b * kSteps + h;
+                    if (!warp_wait(&sh.s_full[t][u & 1], (u >> 1) & 1u, deadline)) ok = false;
+                    tc_fence_after();
+                    const uint32_t ts = tl + (t * 2 + (u & 1)) * kPtHalf;
                     const int c0 = key + h * kPtHalf;
                     uint64_t vis = 0;
                     if (!full) {
@@ -464,13 +452,10 @@ __global__ void __launch_bounds__(pt_threads(NT), pt_ctas(NT)) paged_many_kernel
                     }
                     l += ls;
                     tmem_st32_async(ts, w);       // over S
-                    if (moved && b + h > 0) {
-                        // O must hold the weights before these.  Two S ranges: S(b)
-                        // is behind the MMAs of block b - 2, those of b - 1 may be
-                        // under way; else S(b) is behind block b - 1's, and the
-                        // second step waits for the first's.
-                        if (kTwoS || h == 1)
-                            if (!warp_wait(&sh.o_part[t], (kTwoS ? b - 1 : b) & 1u, deadline)) ok = false;
+                    if (moved && u > 0) {
+                        // O must hold the weights before these: S(u) is behind the
+                        // MMAs of step u - 2, those of u - 1 may be under way
+                        if (!warp_wait(&sh.o_part[t], (u - 1) & 1u, deadline)) ok = false;
                         tc_fence_after();
 #pragma unroll
                         for (int c = 0; c < HD; c += 32) {
@@ -483,7 +468,7 @@ __global__ void __launch_bounds__(pt_threads(NT), pt_ctas(NT)) paged_many_kernel
                     tmem_wait_st();
                     tc_fence_before();
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(&sh.p_full[t][kTwoS ? r : h]);
+                    if (lane == 0) mbar_arrive(&sh.p_full[t][u & 1]);
                 }
             }
             // shares go over K and V, which the other tile's MMAs may still read
