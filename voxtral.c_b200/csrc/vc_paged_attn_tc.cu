@@ -87,7 +87,8 @@ __device__ __forceinline__ float max3(float a, float b, float c) {   // a NaN is
 // more issue slots than it saves: 3 of 8 pairs 601 against 531 us for the prompt
 // chunks of 15035 and 8008 keys.)
 template <bool MASKED>
-__device__ __forceinline__ float weigh64(uint32_t ts, float sl2, float ks, int g0, float base, uint64_t vis, uint32_t (&w)[32], float &ls) {
+__device__ __forceinline__ float weigh64(uint32_t ts, float sl2, float ks, int g0, float base, const uint32_t (&vis)[2], uint32_t (&w)[32],
+                                          float &ls) {
     float mx = -INFINITY;
     uint64_t rs[2] = {0, 0};
     const uint64_t nb = pair(-base, -base);
@@ -105,8 +106,8 @@ __device__ __forceinline__ float weigh64(uint32_t ts, float sl2, float ks, int g
             float xa, xb;
             unpair(fma2(pair(__uint_as_float(cur[j]), __uint_as_float(cur[j + 1])), sl, nb), xa, xb);
             if (MASKED) {
-                xa = (vis >> (c + j)) & 1u ? xa : -INFINITY;
-                xb = (vis >> (c + j + 1)) & 1u ? xb : -INFINITY;
+                xa = vis[c / 32] & (1u << ((c & 16) + j)) ? xa : -INFINITY;
+                xb = vis[c / 32] & (2u << ((c & 16) + j)) ? xb : -INFINITY;
             }
             mx = max3(mx, xa, xb);
             xa = exp2_approx(xa);
@@ -127,6 +128,12 @@ __global__ void __launch_bounds__(pt_threads(NT), pt_ctas(NT)) paged_many_kernel
     constexpr int kSub = HD / 64;            // 64-dim sub-tiles of a tile
     constexpr int kWarpConv = NT * 4, kWarpMma = kWarpConv + kPtConv / 32;
     constexpr int kThreads = pt_threads(NT), kKeys = Sm::kKeys, kSteps = kKeys / kPtHalf, kGroups = kKeys / 16;
+    // Steps that a tile's rows do not see are left out, and masks are applied by
+    // warp: for heads of 64, an encoder's, whose tiles are long (a row per
+    // position) and windows short: its chunk 69 -> 62 us.  The registers that this
+    // takes cost heads of 128, where a group's heads share positions, more than it
+    // gives (prompt chunks 454 -> 490 us).
+    constexpr bool kSkip = HD == 64;
     constexpr uint32_t kTmemCols = NT == 2 ? 512 : 256;
     constexpr uint32_t kOCol = NT * 2 * kPtHalf;   // S ranges first, two a tile, then O tiles
     extern __shared__ __align__(1024) unsigned char pt_smem_raw[];
@@ -156,6 +163,28 @@ __global__ void __launch_bounds__(pt_threads(NT), pt_ctas(NT)) paged_many_kernel
     const int *const table = p.c.table + (long long)stream * p.c.table_stride;
     auto entry_of = [&](int key) { return key < hi && (key + 16 > lo || key < ns) ? __ldg(table + (key >> p.c.page_shift)) : -1; };
     auto is_page = [&](int g) { return g >= 0 && g < p.c.n_pages; };
+    // Steps of 64 keys: half u % kSteps of block u / kSteps.  A tile leaves out
+    // those that none of its rows sees: [gap, on) between the sinks and the window,
+    // and from `end` on.
+    const int steps = nb * kSteps;
+    struct Steps {
+        int gap, on, end;
+        __device__ bool left_out(int u) const { return (u >= gap && u < on) || u >= end; }
+    };
+    auto steps_below = [&](int key) {   // steps whose first key is less
+        const int c = (max(key, 0) + kPtHalf - 1) / kPtHalf;
+        const int all = min(c, sink_blocks * kSteps) + max(0, min(c, first * kSteps + (blocks - sink_blocks) * kSteps) - first * kSteps);
+        return min(max(all - b0 * kSteps, 0), steps);
+    };
+    auto steps_of = [&](int t) {
+        const int a = s.pos + (m0 + t * kAtRows) / p.group, b = s.pos + (min(m0 + (t + 1) * kAtRows, M) - 1) / p.group;
+        Steps st = {0, 0, steps_below(b + 1)};
+        if (p.window > 0) {
+            st.gap = steps_below(p.n_sink);
+            st.on = max(st.gap, steps_below(a - p.window + 1 - (kPtHalf - 1)));
+        }
+        return st;
+    };
     bool ok = true;
 
     if (threadIdx.x == 0) {
@@ -307,9 +336,12 @@ __global__ void __launch_bounds__(pt_threads(NT), pt_ctas(NT)) paged_many_kernel
         if (nb > 0 && t < tiles) {
             const uint32_t lead = lane == 0, tm = __shfl_sync(0xffffffffu, tmem, 0);
             constexpr uint32_t id_s = at_idesc<__half>(kPtHalf, false), id_o = at_idesc<__half>(HD, true);
-            // step u: 64 keys, half u % kSteps of block u / kSteps, S range u % 2
-            const int steps = nb * kSteps;
-            auto issue_s = [&](int u) {
+            // Step u has S range u % 2.  Operands depend on u alone, which counts,
+            // and what is left out is issued by no lane, not branched around: where
+            // the compiler cannot see that all lanes have the same, each MMA costs
+            // moves to uniform registers (60 us of 450 for the prompt chunks).
+            const Steps st = steps_of(t);
+            auto issue_s = [&](int u, uint32_t lead) {
                 const int b = u / kSteps, h = u % kSteps;
                 const uint64_t a0 = smem_desc_sw128(sh.q[t]), k0 = smem_desc_sw128(sh.kv[0][b % kPtStages]) + h * (kPtHalf * 128 / 16);
 #pragma unroll
@@ -319,35 +351,41 @@ __global__ void __launch_bounds__(pt_threads(NT), pt_ctas(NT)) paged_many_kernel
                         warp_mma(tm + (t * 2 + (u & 1)) * kPtHalf, a0 + d * (Sm::kQSub / 16) + 2 * k, k0 + d * (Sm::kSubTile / 16) + 2 * k,
                                  id_s, (d | k) != 0 ? 1u : 0u, lead);
                 warp_commit(&sh.s_full[t][u & 1], lead);
-                if (h == kSteps - 1) warp_commit(&sh.k_empty[b % kPtStages], lead);
             };
-            auto issue_o = [&](int u) {   // O += P V
+            auto issue_o = [&](int u, bool more, uint32_t lead) {   // O += P V
                 const int b = u / kSteps, h = u % kSteps;
                 const uint64_t v0 = at_desc_mn(sh.kv[1][b % kPtStages], Sm::kSubTile) + h * (kPtHalf * 128 / 16);
 #pragma unroll
                 for (int k = 0; k < kPtHalf / 16; k++)   // 16 keys: 8 columns of P, 2048 bytes of V
                     warp_mma_ta(tm + kOCol + t * HD, tm + (t * 2 + (u & 1)) * kPtHalf + 8 * k, v0 + k * (2048 / 16), id_o,
-                                (u | k) != 0 ? 1u : 0u, lead);
+                                more || k != 0 ? 1u : 0u, lead);
                 warp_commit(&sh.o_part[t], lead);
-                if (h == kSteps - 1) warp_commit(&sh.v_empty[b % kPtStages], lead);
             };
-            auto next_s = [&](int u) {   // S(u), once its keys are there
-                if (u >= steps) return true;
-                const int b = u / kSteps;
-                if (u % kSteps == 0 && !warp_wait(&sh.k_full[b % kPtStages], (b / kPtStages) & 1u, deadline)) return false;
-                tc_fence_after();
-                issue_s(u);
-                return true;
-            };
-            ok = warp_wait(&sh.q_full[t], 0u, deadline) && next_s(0) && next_s(1);
-            for (int u = 0; u < steps && ok; u++) {
-                const int b = u / kSteps;
-                ok = (u % kSteps != 0 || warp_wait(&sh.v_full[b % kPtStages], (b / kPtStages) & 1u, deadline)) &&
-                     warp_wait(&sh.p_full[t][u & 1], (u >> 1) & 1u, deadline);
-                if (!ok) break;
-                tc_fence_after();
-                issue_o(u);
-                ok = next_s(u + 2);   // over P(u), behind the MMAs that read it
+            uint32_t phase = 0u;   // bit r: of p_full[t][r]
+            bool more = false;     // O holds something
+            ok = warp_wait(&sh.q_full[t], 0u, deadline);
+            for (int u = -2; u < steps && ok; u++) {
+                const int b = u / kSteps, s2 = u + 2, bs = s2 / kSteps;
+                if (u >= 0) {
+                    if (u % kSteps == 0) ok = warp_wait(&sh.v_full[b % kPtStages], (b / kPtStages) & 1u, deadline);
+                    const bool take = !kSkip || !st.left_out(u);
+                    if (take) {
+                        ok = ok && warp_wait(&sh.p_full[t][u & 1], kSkip ? (phase >> (u & 1)) & 1u : (u >> 1) & 1u, deadline);
+                        phase ^= 1u << (u & 1);
+                    }
+                    if (!ok) break;
+                    tc_fence_after();
+                    issue_o(u, kSkip ? more : u > 0, take ? lead : 0u);
+                    more |= take;
+                    if (u % kSteps == kSteps - 1) warp_commit(&sh.v_empty[b % kPtStages], lead);
+                }
+                if (ok && s2 < steps) {   // S of the second step on, over P(u) and behind the MMAs that read it
+                    if (s2 % kSteps == 0) ok = warp_wait(&sh.k_full[bs % kPtStages], (bs / kPtStages) & 1u, deadline);
+                    if (!ok) break;
+                    tc_fence_after();
+                    issue_s(s2, kSkip && st.left_out(s2) ? 0u : lead);
+                    if (s2 % kSteps == kSteps - 1) warp_commit(&sh.k_empty[bs % kPtStages], lead);
+                }
             }
             warp_commit(&sh.o_done[t], lead);
         }
@@ -357,37 +395,48 @@ __global__ void __launch_bounds__(pt_threads(NT), pt_ctas(NT)) paged_many_kernel
         const int t = warp / 4, q = warp % 4, ml = t * kAtRows + 32 * q + lane, m = m0 + ml;
         const bool here = m0 + t * kAtRows + 32 * q < M;   // the warp has rows
         if (here) {
-            {   // the warp's 32 rows of Q as fp16: HD / 8 lanes a row, zeros past M
-                constexpr int kCh = HD / 8, kAtOnce = 32 / kCh;
+            const int i = min(m, M - 1) / p.group, at = s.pos + i;
+            const long long row = (long long)(s.r0 + i) * p.n_heads + head0 + min(m, M - 1) % p.group;
+            {   // the warp's 32 rows of Q as fp16: HD / 8 lanes a row, zeros past M; all on their way at once
+                constexpr int kCh = HD / 8, kAtOnce = 32 / kCh, kIts = 32 / kAtOnce;
                 const int ch = lane % kCh;
                 unsigned char *const to = sh.q[t] + (ch >> 3) * Sm::kQSub;
-#pragma unroll 4
-                for (int it = 0; it < 32 / kAtOnce; it++) {
-                    const int rt = 32 * q + it * kAtOnce + lane / kCh, mm = m0 + t * kAtRows + rt;
-                    float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
-                    if (mm < M) {
-                        const T *src = static_cast<const T *>(p.q) + ((long long)(s.r0 + mm / p.group) * p.n_heads + head0 + mm % p.group) * HD + ch * 8;
-                        a = load4<T>(src);
-                        b = load4<T>(src + 4);
-                    }
+                uint4 raw[kIts];
+#pragma unroll
+                for (int it = 0; it < kIts; it++) {
+                    const int r = it * kAtOnce + lane / kCh;
+                    const long long from = __shfl_sync(0xffffffffu, row, r);
+                    raw[it] = make_uint4(0u, 0u, 0u, 0u);
+                    if (m0 + t * kAtRows + 32 * q + r < M)
+                        raw[it] = *reinterpret_cast<const uint4 *>(static_cast<const T *>(p.q) + from * HD + ch * 8);
+                }
+#pragma unroll
+                for (int it = 0; it < kIts; it++) {
+                    const int rt = 32 * q + it * kAtOnce + lane / kCh;
+                    uint4 u = raw[it];
                     float up = 1.f;   // a power of two that takes the row's largest to [2^14, 2^15)
                     if constexpr (!std::is_same<T, __half>::value) {
-                        const float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-                        float big = 0.f;
+                        const uint32_t in[4] = {u.x, u.y, u.z, u.w};
+                        float v[8], big = 0.f;
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            const float2 f = unpack2<T>(in[e]);
+                            v[2 * e] = f.x;
+                            v[2 * e + 1] = f.y;
+                        }
 #pragma unroll
                         for (int e = 0; e < 8; e++) big = fmaxf(big, fabsf(v[e]) < INFINITY ? fabsf(v[e]) : 0.f);
 #pragma unroll
                         for (int o = kCh / 2; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
                         const int e = (int)(__float_as_uint(big) >> 23) - 127;
                         up = big > 0.f ? __uint_as_float((uint32_t)(min(14 - e, 126) + 127) << 23) : 1.f;
+                        u = make_uint4(pack2<__half>(v[0] * up, v[1] * up), pack2<__half>(v[2] * up, v[3] * up),
+                                       pack2<__half>(v[4] * up, v[5] * up), pack2<__half>(v[6] * up, v[7] * up));
                     }
-                    *reinterpret_cast<uint4 *>(to + rt * 128 + (((ch & 7) ^ (rt & 7)) << 4)) =
-                        make_uint4(pack2<__half>(a.x * up, a.y * up), pack2<__half>(a.z * up, a.w * up),
-                                   pack2<__half>(b.x * up, b.y * up), pack2<__half>(b.z * up, b.w * up));
+                    *reinterpret_cast<uint4 *>(to + rt * 128 + (((ch & 7) ^ (rt & 7)) << 4)) = u;
                     if (ch == 0) sh.factor[t * kAtRows + rt] = p.scale_log2 / up;
                 }
             }
-            const int i = min(m, M - 1) / p.group, at = s.pos + i;
             // positions that the row sees: [0, e1) and [s2, at]
             const int e1 = min(ns, at + 1), s2 = p.window > 0 ? max(0, at - p.window + 1) : 0;
             const uint32_t tl = tmem + ((uint32_t)(32 * q) << 16);
@@ -403,32 +452,35 @@ __global__ void __launch_bounds__(pt_threads(NT), pt_ctas(NT)) paged_many_kernel
             auto scale = [&](int g) { return is_page(g) ? __ldg(p.c.k_scale + scale_at(p.c, p.layer, g, kvh)) : 0.f; };
             int page = entry(0), page_next = entry(1);
             float ks = scale(page);
+            const Steps st = kSkip ? steps_of(t) : Steps{};
+            const int w_min = __shfl_sync(0xffffffffu, at, 0), w_max = __shfl_sync(0xffffffffu, at, 31);
+            uint32_t phase = 0u, turns = 0u;   // bit r: of s_full[t][r]; steps taken
             for (int b = 0; b < nb; b++) {
                 const int key = key_of(b);
                 const uint32_t there = __ballot_sync(0xffffffffu, is_page(page));
-                const bool full = whole(key) && there == (1u << kGroups) - 1;
+                const bool all = !kSkip && whole(key) && there == (1u << kGroups) - 1;   // the CTA's rows see the whole block
                 const float ks_now = ks;
                 page = page_next;
                 ks = scale(page);
                 page_next = entry(b + 2);
 #pragma unroll 1
                 for (int h = 0; h < kSteps; h++) {
-                    const int u = b * kSteps + h;
-                    if (!warp_wait(&sh.s_full[t][u & 1], (u >> 1) & 1u, deadline)) ok = false;
-                    tc_fence_after();
-                    const uint32_t ts = tl + (t * 2 + (u & 1)) * kPtHalf;
                     const int c0 = key + h * kPtHalf;
-                    uint64_t vis = 0;
-                    if (!full) {
-                        uint32_t word[2];
+                    const int u = b * kSteps + h;
+                    if (kSkip && st.left_out(u)) continue;
+                    const uint32_t ts = tl + (t * 2 + (u & 1)) * kPtHalf, pages = (there >> (4 * h)) & 15u;
+                    const bool full = !kSkip ? all
+                                             : c0 + kPtHalf - 1 <= w_min && pages == 15u &&
+                                                   (p.window <= 0 || c0 > w_max - p.window || c0 + kPtHalf <= p.n_sink);
+                    if (!warp_wait(&sh.s_full[t][u & 1], kSkip ? (phase >> (u & 1)) & 1u : (u >> 1) & 1u, deadline)) ok = false;
+                    phase ^= 1u << (u & 1);
+                    tc_fence_after();
+                    uint32_t vis[2] = {0u, 0u};
+                    if (!full)
 #pragma unroll
-                        for (int e = 0; e < 2; e++) {
-                            const uint32_t two = there >> (4 * h + 2 * e);
-                            word[e] = (range_bits(c0 + 32 * e, 0, e1) | range_bits(c0 + 32 * e, s2, at + 1)) &
-                                      ((two & 1u ? 0xffffu : 0u) | (two & 2u ? 0xffff0000u : 0u));
-                        }
-                        vis = (uint64_t)word[1] << 32 | word[0];
-                    }
+                        for (int e = 0; e < 2; e++)
+                            vis[e] = (range_bits(c0 + 32 * e, 0, e1) | range_bits(c0 + 32 * e, s2, at + 1)) &
+                                     ((pages >> (2 * e) & 1u ? 0xffffu : 0u) | (pages >> (2 * e) & 2u ? 0xffff0000u : 0u));
                     // P against m so far; a row whose keys exceed it by 2^15 takes
                     // theirs, and the warp goes over them again (S is intact until P
                     // is stored)
@@ -452,10 +504,10 @@ __global__ void __launch_bounds__(pt_threads(NT), pt_ctas(NT)) paged_many_kernel
                     }
                     l += ls;
                     tmem_st32_async(ts, w);       // over S
-                    if (moved && u > 0) {
-                        // O must hold the weights before these: S(u) is behind the
-                        // MMAs of step u - 2, those of u - 1 may be under way
-                        if (!warp_wait(&sh.o_part[t], (u - 1) & 1u, deadline)) ok = false;
+                    if (moved && (kSkip ? turns : u) > 0) {
+                        // O must hold the weights before these: the step before
+                        // this one may be under way
+                        if (!warp_wait(&sh.o_part[t], ((kSkip ? turns : u) - 1) & 1u, deadline)) ok = false;
                         tc_fence_after();
 #pragma unroll
                         for (int c = 0; c < HD; c += 32) {
@@ -469,6 +521,7 @@ __global__ void __launch_bounds__(pt_threads(NT), pt_ctas(NT)) paged_many_kernel
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&sh.p_full[t][u & 1]);
+                    turns++;
                 }
             }
             // shares go over K and V, which the other tile's MMAs may still read
@@ -478,10 +531,9 @@ __global__ void __launch_bounds__(pt_threads(NT), pt_ctas(NT)) paged_many_kernel
             const float v_top = __int_as_float(*(volatile int *)&sh.v_top);
             const float il = l == 0.f ? 0.f : v_top / l;   // no weight at all: zeros (O is tiny, not NaN)
             const bool bad = *(volatile int *)&sh.bad != 0;
-            const long long row = (long long)(s.r0 + i) * p.n_heads + head0 + min(m, M - 1) % p.group;
 #pragma unroll
             for (int c = 0; c < HD; c += 32) {
-                if (nb > 0) tmem_ld32(to + c, sv);
+                if ((kSkip ? turns : steps) > 0) tmem_ld32(to + c, sv);
                 else {
 #pragma unroll
                     for (int j = 0; j < 32; j++) sv[j] = 0.f;
