@@ -641,8 +641,26 @@ constexpr size_t pt_smem() {
     return std::max<size_t>(sizeof(PtSmem<HD, NT>), NT == 2 ? kPtOneCta : 0);
 }
 
+// A shape's launch: its cluster size and what that costs.
+struct PtPlan {
+    double cost = 1e30;
+    int shares = 0;
+};
+
+// Microseconds, measured: a CTA's start and end; the merge of shares; a block of
+// keys, of 128 for two tiles, of 64 for a tile alone on its SM and beside another.
+constexpr double kPtFixed = 11, kPtMerge = 6, kPtTwo = 2.5, kPtAlone = 1.15, kPtBeside = 1.75;
+
+// Shares by the least time.  With one CTA to an SM equal CTAs end together, so a
+// started wave is a whole one; with two, waves run into each other and their blocks
+// count in proportion.  The keys are those that the table has room for: the
+// lengths are on the device.
+// 8 streams of 64 packed rows over 3016 keys: 1 share 72 us, 2 48, 4 39, 8 53; of 256
+// over 2064: two tiles, 1 share 64, 2 51, 4 68, one tile 56, 54, 67.  Encoder chunk
+// (192 two-tile CTAs): 64, one tile 58.  300 rows of 12 heads, 2 streams, 3300 keys:
+// one tile, 2 shares 52, 3 51, 4 62.
 template <typename T, int HD, int NT>
-cudaError_t launch_many(PagedAttnParams p, cudaStream_t st) {
+cudaError_t plan_many(const PagedAttnParams &p, PtPlan *out) {
     auto kernel = paged_many_kernel<T, HD, NT>;
     constexpr size_t kSmem = pt_smem<HD, NT>();
     static_assert(kSmem <= (228 / pt_ctas(NT) - 1) * 1024, "they fit an SM");
@@ -653,20 +671,43 @@ cudaError_t launch_many(PagedAttnParams p, cudaStream_t st) {
     const long long M = (long long)p.r.max_rows * p.group, tiles = (M + NT * kAtRows - 1) / (NT * kAtRows);
     long long keys = (long long)p.c.table_stride * p.c.page;
     if (p.window > 0) keys = std::min(keys, (long long)p.window + p.n_sink + (NT * kAtRows - 1) / p.group + 2);
-    const long long blocks = (keys + pt_keys(NT) - 1) / pt_keys(NT), all = tiles * p.c.n_kv_heads * p.c.n_streams;
-    int Z = 1;
-    while (Z < 8 && all * (Z + 1) <= 148ll * pt_ctas(NT) && blocks / (Z + 1) >= 4) Z++;
-    p.shares = Z;
+    const long long blocks = (keys + pt_keys(NT) - 1) / pt_keys(NT), clusters = tiles * p.c.n_kv_heads * p.c.n_streams;
+    for (int Z = 1; Z <= kMaxCluster && Z <= blocks; Z++) {
+        int at_once = 0;   // (the device counts for one CTA to an SM)
+        if ((e = cluster_active(ck, kernel, dev, pt_threads(NT), kSmem, Z, &at_once)) != cudaSuccess) return e;
+        if (at_once < 1) continue;
+        const double fill = (double)clusters / (at_once * pt_ctas(NT)), waves = std::max(1.0, ceil(fill));
+        const double part = (double)((blocks + Z - 1) / Z);
+        const double work = NT == 2 ? part * waves * kPtTwo : part * (fill <= 0.5 ? kPtAlone : std::max(1.0, fill) * kPtBeside);
+        const double t = work + waves * kPtFixed + (Z > 1 ? kPtMerge : 0.0);
+        if (t < out->cost) {
+            out->cost = t;
+            out->shares = Z;
+        }
+    }
+    return out->shares ? cudaSuccess : cudaErrorInvalidConfiguration;
+}
+
+template <typename T, int HD, int NT>
+cudaError_t launch_many(PagedAttnParams p, const PtPlan &plan, cudaStream_t st) {
+    const long long M = (long long)p.r.max_rows * p.group, tiles = (M + NT * kAtRows - 1) / (NT * kAtRows);
+    p.shares = plan.shares;
     cudaLaunchAttribute attr;
-    const cudaLaunchConfig_t cfg = cluster_config(dim3((unsigned)(Z * tiles), p.c.n_kv_heads, p.c.n_streams), pt_threads(NT), kSmem, Z,
-                                                  &attr, st);
-    return cudaLaunchKernelEx(&cfg, kernel, p);
+    const cudaLaunchConfig_t cfg = cluster_config(dim3((unsigned)(p.shares * tiles), p.c.n_kv_heads, p.c.n_streams), pt_threads(NT),
+                                                  pt_smem<HD, NT>(), p.shares, &attr, st);
+    return cudaLaunchKernelEx(&cfg, paged_many_kernel<T, HD, NT>, p);
 }
 
 template <typename T, int HD>
 cudaError_t launch_dim(const PagedAttnParams &p, cudaStream_t st) {
-    const long long M = (long long)p.r.max_rows * p.group;
-    return M <= kAtRows ? launch_many<T, HD, 1>(p, st) : launch_many<T, HD, 2>(p, st);
+    PtPlan one, two;
+    cudaError_t e = plan_many<T, HD, 1>(p, &one);
+    if (e != cudaSuccess) return e;
+    if ((long long)p.r.max_rows * p.group > kAtRows) {
+        if ((e = plan_many<T, HD, 2>(p, &two)) != cudaSuccess) return e;
+        if (two.cost < one.cost) return launch_many<T, HD, 2>(p, two, st);
+    }
+    return launch_many<T, HD, 1>(p, one, st);
 }
 template <typename T>
 cudaError_t launch_typed(const PagedAttnParams &p, cudaStream_t st) {
