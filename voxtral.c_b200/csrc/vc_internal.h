@@ -240,9 +240,10 @@ struct PagedAttnParams {
     unsigned *err;            // raised when a bounded wait expires (mapped host memory); the rows then get NaN
     unsigned long long stall_ns;   // self-test: a wait of this length that nothing ends, after the work (0: none)
 };
-cudaError_t launch_paged_attn(const PagedAttnParams &p, int sms, cudaStream_t st);
-// the tensor-core kernel of many rows (vc_paged_attn_tc.cu)
-cudaError_t launch_paged_attn_tc(const PagedAttnParams &p, cudaStream_t st);
+// only: nothing is launched, the form is told
+cudaError_t launch_paged_attn(const PagedAttnParams &p, int sms, cudaStream_t st, RowsPlan *only = nullptr);
+// the kernel of many rows (vc_paged_attn_tc.cu); cost: nothing is launched, its modelled microseconds are told
+cudaError_t launch_paged_attn_tc(const PagedAttnParams &p, cudaStream_t st, RowsPlan *only, double *cost);
 struct PagedCopyParams {
     PagedView c;
     const int *src, *dst;     // [n]

@@ -31,6 +31,7 @@
 #include "vc_paged.cuh"
 #include "vc_tc.cuh"
 
+#include <algorithm>
 #include <math.h>
 
 namespace vc {
@@ -39,9 +40,8 @@ using namespace tc;
 
 namespace {
 
-constexpr int kFwWarps = 4, kFwThreads = kFwWarps * 32;
 constexpr int kFwKeys = 32;              // keys of a warp's step
-constexpr int kFwStages = 3;             // of a warp's ring
+constexpr int fw_ctas(int w, int s) { return w == 8 ? 1 : s == 2 ? 3 : 2; }
 constexpr float kFwBelow = 7.f;          // the maximum less m
 constexpr float kFwAbove = 15.f;         // log2 of what a weight may reach before m moves
 
@@ -85,28 +85,27 @@ __device__ __forceinline__ int v_chunk(int r, int ch) {
     return HD == 128 ? r * 128 + ((ch ^ sw) << 4) : (r >> 1) * 128 + ((((r & 1) * 4 + ch) ^ sw) << 4);
 }
 
-template <int HD, int NR>
+template <int HD, int NR, int W, int S>
 struct FwSmem {
     static constexpr int kTile = kFwKeys * HD;
-    static constexpr int kStages = kFwStages;
     union {
-        unsigned char kv[kFwWarps][kStages][2][kTile];
-        float o[kFwWarps][8 * NR][HD];
+        unsigned char kv[W][S][2][kTile];
+        float o[W][8 * NR][HD];
     };
-    float scale[kFwWarps][kStages][4];   // K's of the two groups of 16 keys, V's
-    float mx[kFwWarps][8 * NR], sum[kFwWarps][8 * NR];
+    float scale[W][S][4];   // K's of the two groups of 16 keys, V's
+    float mx[W][8 * NR], sum[W][8 * NR];
 };
 
-// NR: column tiles of 8 packed rows
-template <typename T, int HD, int NR>
-__global__ void __launch_bounds__(kFwThreads, 2) paged_few_kernel(const PagedAttnParams p) {
+// NR: column tiles of 8 packed rows; W warps, rings of S stages
+template <typename T, int HD, int NR, int W, int S>
+__global__ void __launch_bounds__(W * 32, fw_ctas(W, S)) paged_few_kernel(const PagedAttnParams p) {
     constexpr int KC = HD / 64;       // 64-dim parts of a key
     constexpr int MT = HD / 16;       // 16-dim tiles of O
     constexpr int VW = HD / 32;       // words that a lane has of a V row
     constexpr int kRows = 8 * NR;
-    constexpr int kStages = FwSmem<HD, NR>::kStages, kTile = FwSmem<HD, NR>::kTile;
+    constexpr int kWarps = W, kThreads = W * 32, kStages = S, kTile = FwSmem<HD, NR, W, S>::kTile;
     extern __shared__ __align__(128) unsigned char fw_smem_raw[];
-    FwSmem<HD, NR> &sh = *reinterpret_cast<FwSmem<HD, NR> *>(fw_smem_raw);
+    FwSmem<HD, NR, W, S> &sh = *reinterpret_cast<FwSmem<HD, NR, W, S> *>(fw_smem_raw);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int z = blockIdx.x % p.shares, Z = p.shares;
     const int m0 = blockIdx.x / p.shares * kRows, kvh = blockIdx.y, stream = blockIdx.z;
@@ -166,11 +165,11 @@ __global__ void __launch_bounds__(kFwThreads, 2) paged_few_kernel(const PagedAtt
     auto note = [&]() { have = have << 2 | (pg[1] >= 0 ? 2u : 0u) | (pg[0] >= 0 ? 1u : 0u); };
 #pragma unroll
     for (int i = 0; i < kStages - 1; i++) {
-        pages_of(u0 + warp + i * kFwWarps, pg);
-        fetch(u0 + warp + i * kFwWarps, i, pg);
+        pages_of(u0 + warp + i * kWarps, pg);
+        fetch(u0 + warp + i * kWarps, i, pg);
         note();
     }
-    pages_of(u0 + warp + (kStages - 1) * kFwWarps, pg);
+    pages_of(u0 + warp + (kStages - 1) * kWarps, pg);
     // q as B operands: lane (g, t) has row g's dims in the order of K's
     uint32_t qf[NR][KC * 4][2];
     float cf[NR][2];          // score factor of the lane's rows 2 t, 2 t + 1, in log2
@@ -244,12 +243,12 @@ __global__ void __launch_bounds__(kFwThreads, 2) paged_few_kernel(const PagedAtt
     };
 
     int stage = 0;
-    for (int u = u0 + warp; u < u1; u += kFwWarps) {
+    for (int u = u0 + warp; u < u1; u += kWarps) {
         cp_async_wait<kStages - 2>();
         __syncwarp();   // this unit is there for all lanes, and all have done with the one before
-        fetch(u + (kStages - 1) * kFwWarps, stage == 0 ? kStages - 1 : stage - 1, pg);
+        fetch(u + (kStages - 1) * kWarps, stage == 0 ? kStages - 1 : stage - 1, pg);
         note();
-        pages_of(u + kStages * kFwWarps, pg);
+        pages_of(u + kStages * kWarps, pg);
         const uint32_t k_at = ring + stage * (2 * kTile), v_at = k_at + kTile;
         const uint32_t there = have >> (2 * (kStages - 1));
         const float4 sc = *reinterpret_cast<const float4 *>(sh.scale[warp][stage]);
@@ -436,15 +435,15 @@ __global__ void __launch_bounds__(kFwThreads, 2) paged_few_kernel(const PagedAtt
     __syncthreads();
     // the CTA's: into its first warp's place
     const int rows = min(kRows, M - m0);
-    for (int e = threadIdx.x; e < kRows * (HD / 4); e += kFwThreads) {
+    for (int e = threadIdx.x; e < kRows * (HD / 4); e += kThreads) {
         const int r = e / (HD / 4), d = e % (HD / 4) * 4;
         float top = sh.mx[0][r];
 #pragma unroll
-        for (int w = 1; w < kFwWarps; w++) top = fmaxf(top, sh.mx[w][r]);
+        for (int w = 1; w < kWarps; w++) top = fmaxf(top, sh.mx[w][r]);
         const float base = top == -INFINITY ? 0.f : top;
         float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-        for (int w = 0; w < kFwWarps; w++) {
+        for (int w = 0; w < kWarps; w++) {
             const float f = exp2_approx(sh.mx[w][r] - base);
             const float4 v = *reinterpret_cast<const float4 *>(sh.o[w][r] + d);
             a.x = fmaf(f, v.x, a.x), a.y = fmaf(f, v.y, a.y), a.z = fmaf(f, v.z, a.z), a.w = fmaf(f, v.w, a.w);
@@ -456,17 +455,17 @@ __global__ void __launch_bounds__(kFwThreads, 2) paged_few_kernel(const PagedAtt
         const int r = threadIdx.x;
         float top = sh.mx[0][r], sum = 0.f;
 #pragma unroll
-        for (int w = 1; w < kFwWarps; w++) top = fmaxf(top, sh.mx[w][r]);
+        for (int w = 1; w < kWarps; w++) top = fmaxf(top, sh.mx[w][r]);
         const float base = top == -INFINITY ? 0.f : top;
 #pragma unroll
-        for (int w = 0; w < kFwWarps; w++) sum = fmaf(exp2_approx(sh.mx[w][r] - base), sh.sum[w][r], sum);
+        for (int w = 0; w < kWarps; w++) sum = fmaf(exp2_approx(sh.mx[w][r] - base), sh.sum[w][r], sum);
         sh.mx[0][r] = top;
         sh.sum[0][r] = sum;
     }
     if (Z > 1) cluster_sync_all();
     else __syncthreads();
     const uint32_t o_s = smem_u32(sh.o[0]), m_s = smem_u32(sh.mx[0]), l_s = smem_u32(sh.sum[0]);
-    for (int e = z * kFwThreads + threadIdx.x; e < rows * (HD / 4); e += Z * kFwThreads) {
+    for (int e = z * kThreads + threadIdx.x; e < rows * (HD / 4); e += Z * kThreads) {
         const int r = e / (HD / 4), d = e % (HD / 4) * 4, m = m0 + r;
         float top = -INFINITY, sum = 0.f;
         for (int c = 0; c < Z; c++) top = fmaxf(top, ld_dsmem_f1(mapa_shared(m_s + 4 * r, c)));
@@ -486,44 +485,110 @@ __global__ void __launch_bounds__(kFwThreads, 2) paged_few_kernel(const PagedAtt
     if (Z > 1) cluster_sync_all();   // no CTA leaves while a peer still reads its share
 }
 
-template <typename T, int HD, int NR>
-cudaError_t launch_few(PagedAttnParams p, int sms, cudaStream_t st) {
-    auto kernel = paged_few_kernel<T, HD, NR>;
+// A shape's launch: its cluster size and what that costs.
+struct FwPlan {
+    double cost = 1e30;
+    int shares = 0;
+};
+
+// Microseconds: fitted to the times of 40 calls (1 to 64 streams, 1 to 16 rows, 100
+// to 16000 positions, 5 head layouts) in every shape and with 1 to 8 shares; the
+// least by the model is within 2% of the least measured on the average, 15% at most.
+//   a CTA's start and end, the merge of shares, and per share; a further wave of CTAs
+constexpr double kFwFixed = 3.9, kFwMerge = 0.9, kFwShare = 0.23, kFwWave = 4.4, kFwWide = 1.1;   // kFwWide: of 8 warps
+//   a step of 32 keys: what a warp by itself takes, and what the SM does for each,
+//   for heads of 128 and 8 packed rows; and of 64, 16 rows, rings of two stages
+constexpr double kFwStep = 1.07, kFwStepSm = 0.155;
+constexpr double kFwStep64 = 1.5, kFwStepSm64 = 0.32, kFwStep16 = 2.1, kFwStepSm16 = 1.85, kFwStepTwo = 1.9;
+constexpr double kFwRagged = 0.7;   // how far a started wave counts whole
+
+template <typename T, int HD, int NR, int W, int S>
+cudaError_t plan_few(const PagedAttnParams &p, int sms, FwPlan *out) {
+    auto kernel = paged_few_kernel<T, HD, NR, W, S>;
     static ClusterKernel ck;
     int dev = 0;
-    constexpr size_t kSmem = sizeof(FwSmem<HD, NR>);
+    constexpr size_t kSmem = sizeof(FwSmem<HD, NR, W, S>);
+    static_assert(kSmem <= (228 / fw_ctas(W, S) - 1) * 1024, "they fit an SM");
     cudaError_t e = cluster_prepare(ck, kernel, kSmem, &dev);
     if (e != cudaSuccess) return e;
     const long long M = (long long)p.r.max_rows * p.group, tiles = (M + 8 * NR - 1) / (8 * NR);
-    const long long all = tiles * p.c.n_kv_heads * p.c.n_streams;
-    long long keys = (long long)p.c.table_stride * p.c.page;
-    if (p.window > 0) keys = min(keys, (long long)p.window + p.n_sink + p.r.max_rows);
-    const long long units = (keys + kFwKeys - 1) / kFwKeys;
-    int Z = 1;
-    while (Z < 8 && all * (Z + 1) <= 2ll * sms && units / (Z + 1) >= 2 * kFwWarps) Z++;
-    p.shares = Z;
-    cudaLaunchAttribute attr;
-    const cudaLaunchConfig_t cfg =
-        cluster_config(dim3((unsigned)(Z * tiles), p.c.n_kv_heads, p.c.n_streams), kFwThreads, kSmem, Z, &attr, st);
-    return cudaLaunchKernelEx(&cfg, kernel, p);
+    long long keys = (long long)p.c.table_stride * p.c.page;   // that the table has room for: the lengths are on the device
+    if (p.window > 0) keys = std::min(keys, (long long)p.window + p.n_sink + (8 * NR - 1) / p.group + 2);
+    const long long units = (keys + kFwKeys - 1) / kFwKeys, clusters = tiles * p.c.n_kv_heads * p.c.n_streams;
+    const double alone = kFwStep * (HD == 64 ? kFwStep64 : 1.0) * (NR == 2 ? kFwStep16 : 1.0) * (S == 2 ? kFwStepTwo : 1.0);
+    const double each = kFwStepSm * (HD == 64 ? kFwStepSm64 : 1.0) * (NR == 2 ? kFwStepSm16 : 1.0);
+    for (int Z = 1; Z <= 8 && Z <= units; Z++) {
+        int at_once = 0;
+        if ((e = cluster_active(ck, kernel, dev, W * 32, kSmem, Z, &at_once)) != cudaSuccess) return e;
+        if (at_once < 1) continue;
+        const double fill = (double)clusters / at_once, most = (double)at_once * Z / sms;   // CTAs on an SM
+        const double ctas = fill < 1.0 ? std::min(most, ceil((double)clusters * Z / sms)) : most;
+        const double steps = (double)((units + (long long)Z * W - 1) / ((long long)Z * W)), waves = std::max(1.0, fill);
+        const double t = kFwFixed + (W == 8 ? kFwWide : 0.0) + (Z > 1 ? kFwMerge : 0.0) + kFwShare * Z + kFwWave * (ceil(waves) - 1.0) +
+                         steps * std::max(alone, ctas * W * each) * ((1.0 - kFwRagged) * waves + kFwRagged * ceil(waves));
+        if (t < out->cost) {
+            out->cost = t;
+            out->shares = Z;
+        }
+    }
+    return out->shares ? cudaSuccess : cudaErrorInvalidConfiguration;
 }
 
+template <typename T, int HD, int NR, int W, int S>
+cudaError_t launch_few(PagedAttnParams p, const FwPlan &plan, cudaStream_t st, RowsPlan *only) {
+    if (only) {
+        *only = {8 * NR, fw_ctas(W, S), plan.shares};
+        return cudaSuccess;
+    }
+    const long long M = (long long)p.r.max_rows * p.group, tiles = (M + 8 * NR - 1) / (8 * NR);
+    p.shares = plan.shares;
+    cudaLaunchAttribute attr;
+    const cudaLaunchConfig_t cfg = cluster_config(dim3((unsigned)(p.shares * tiles), p.c.n_kv_heads, p.c.n_streams), W * 32,
+                                                  sizeof(FwSmem<HD, NR, W, S>), p.shares, &attr, st);
+    return cudaLaunchKernelEx(&cfg, paged_few_kernel<T, HD, NR, W, S>, p);
+}
+
+// Up to this many packed rows of a stream the few-rows kernel may be faster
+// (2 streams of 64 over 3016 keys 21 us; 24), beyond it tiles of 8 and 16 read the
+// keys too often.
+constexpr long long kFwMost = 128;
+
+// The shapes, by their modelled times: 4 warps, two CTAs to an SM; 8 warps, one,
+// where there are few CTAs (one token over 8192 keys 14.6 -> 12.7 us); rings of two
+// stages, three, where there are many short ones (48 streams of 1000 keys 33 -> 22);
+// tiles of 16 rows, which read the keys once for more than 8; or the many-rows
+// kernel.
 template <typename T, int HD>
-cudaError_t launch_dim(const PagedAttnParams &p, int sms, cudaStream_t st) {
+cudaError_t launch_dim(const PagedAttnParams &p, int sms, cudaStream_t st, RowsPlan *only) {
     const long long M = (long long)p.r.max_rows * p.group;
-    return M <= 8 ? launch_few<T, HD, 1>(p, sms, st) : launch_few<T, HD, 2>(p, sms, st);
+    if (M > kFwMost) return launch_paged_attn_tc(p, st, only, nullptr);
+    FwPlan two, one, three, wide;
+    cudaError_t e;
+    if ((e = plan_few<T, HD, 1, 4, 3>(p, sms, &two)) != cudaSuccess || (e = plan_few<T, HD, 1, 8, 3>(p, sms, &one)) != cudaSuccess ||
+        (e = plan_few<T, HD, 1, 4, 2>(p, sms, &three)) != cudaSuccess)
+        return e;
+    const double best = std::min(two.cost, std::min(one.cost, three.cost));
+    if (M > 8) {
+        double many = 0;
+        if ((e = plan_few<T, HD, 2, 4, 3>(p, sms, &wide)) != cudaSuccess || (e = launch_paged_attn_tc(p, st, nullptr, &many)) != cudaSuccess)
+            return e;
+        if (many < std::min(best, wide.cost)) return launch_paged_attn_tc(p, st, only, nullptr);
+        if (wide.cost < best) return launch_few<T, HD, 2, 4, 3>(p, wide, st, only);
+    }
+    if (one.cost == best) return launch_few<T, HD, 1, 8, 3>(p, one, st, only);
+    if (three.cost == best) return launch_few<T, HD, 1, 4, 2>(p, three, st, only);
+    return launch_few<T, HD, 1, 4, 3>(p, two, st, only);
 }
 
 template <typename T>
-cudaError_t attn_typed(const PagedAttnParams &p, int sms, cudaStream_t st) {
-    return p.c.head_dim == 64 ? launch_dim<T, 64>(p, sms, st) : launch_dim<T, 128>(p, sms, st);
+cudaError_t attn_typed(const PagedAttnParams &p, int sms, cudaStream_t st, RowsPlan *only) {
+    return p.c.head_dim == 64 ? launch_dim<T, 64>(p, sms, st, only) : launch_dim<T, 128>(p, sms, st, only);
 }
 
 }  // namespace
 
-cudaError_t launch_paged_attn(const PagedAttnParams &p, int sms, cudaStream_t st) {
-    if ((long long)p.r.max_rows * p.group > 32) return launch_paged_attn_tc(p, st);
-    return p.q_type == ELEM_BF16 ? attn_typed<__nv_bfloat16>(p, sms, st) : attn_typed<__half>(p, sms, st);
+cudaError_t launch_paged_attn(const PagedAttnParams &p, int sms, cudaStream_t st, RowsPlan *only) {
+    return p.q_type == ELEM_BF16 ? attn_typed<__nv_bfloat16>(p, sms, st, only) : attn_typed<__half>(p, sms, st, only);
 }
 
 }  // namespace vc

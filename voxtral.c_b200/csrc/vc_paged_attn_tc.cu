@@ -689,7 +689,11 @@ cudaError_t plan_many(const PagedAttnParams &p, PtPlan *out) {
 }
 
 template <typename T, int HD, int NT>
-cudaError_t launch_many(PagedAttnParams p, const PtPlan &plan, cudaStream_t st) {
+cudaError_t launch_many(PagedAttnParams p, const PtPlan &plan, cudaStream_t st, RowsPlan *only) {
+    if (only) {
+        *only = {NT * kAtRows, pt_ctas(NT), plan.shares};
+        return cudaSuccess;
+    }
     const long long M = (long long)p.r.max_rows * p.group, tiles = (M + NT * kAtRows - 1) / (NT * kAtRows);
     p.shares = plan.shares;
     cudaLaunchAttribute attr;
@@ -699,25 +703,26 @@ cudaError_t launch_many(PagedAttnParams p, const PtPlan &plan, cudaStream_t st) 
 }
 
 template <typename T, int HD>
-cudaError_t launch_dim(const PagedAttnParams &p, cudaStream_t st) {
+cudaError_t launch_dim(const PagedAttnParams &p, cudaStream_t st, RowsPlan *only, double *cost) {
     PtPlan one, two;
     cudaError_t e = plan_many<T, HD, 1>(p, &one);
     if (e != cudaSuccess) return e;
-    if ((long long)p.r.max_rows * p.group > kAtRows) {
-        if ((e = plan_many<T, HD, 2>(p, &two)) != cudaSuccess) return e;
-        if (two.cost < one.cost) return launch_many<T, HD, 2>(p, two, st);
+    if ((long long)p.r.max_rows * p.group > kAtRows && (e = plan_many<T, HD, 2>(p, &two)) != cudaSuccess) return e;
+    if (cost) {
+        *cost = std::min(one.cost, two.cost);
+        return cudaSuccess;
     }
-    return launch_many<T, HD, 1>(p, one, st);
+    return two.cost < one.cost ? launch_many<T, HD, 2>(p, two, st, only) : launch_many<T, HD, 1>(p, one, st, only);
 }
 template <typename T>
-cudaError_t launch_typed(const PagedAttnParams &p, cudaStream_t st) {
-    return p.c.head_dim == 64 ? launch_dim<T, 64>(p, st) : launch_dim<T, 128>(p, st);
+cudaError_t launch_typed(const PagedAttnParams &p, cudaStream_t st, RowsPlan *only, double *cost) {
+    return p.c.head_dim == 64 ? launch_dim<T, 64>(p, st, only, cost) : launch_dim<T, 128>(p, st, only, cost);
 }
 
 }  // namespace
 
-cudaError_t launch_paged_attn_tc(const PagedAttnParams &p, cudaStream_t st) {
-    return p.q_type == ELEM_BF16 ? launch_typed<__nv_bfloat16>(p, st) : launch_typed<__half>(p, st);
+cudaError_t launch_paged_attn_tc(const PagedAttnParams &p, cudaStream_t st, RowsPlan *only, double *cost) {
+    return p.q_type == ELEM_BF16 ? launch_typed<__nv_bfloat16>(p, st, only, cost) : launch_typed<__half>(p, st, only, cost);
 }
 
 }  // namespace vc
