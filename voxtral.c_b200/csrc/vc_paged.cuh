@@ -11,8 +11,6 @@
 
 namespace vc {
 
-constexpr float kE4m3Max = 448.f;
-
 // The stream's page at index i, or -1: none, or a number that is no page.
 __device__ __forceinline__ int page_at(const PagedView &c, int stream, int i) {
     const int g = __ldg(c.table + (long long)stream * c.table_stride + i);
@@ -33,14 +31,9 @@ __device__ __forceinline__ RowSpan paged_span(const RowsView &r, const PagedView
     return s;
 }
 
-// Four fp32 values as e4m3, rounded to nearest even; what is not finite
-// becomes NaN.  Finite values are at most 448.
+// Four fp32 values as e4m3, rounded to nearest even; NaN stays NaN, larger ones
+// than 448 become 448.
 __device__ __forceinline__ uint32_t to_e4m3x4(float4 v) {
-    const float nan = __int_as_float(0x7fffffff);
-    v.x = fabsf(v.x) < INFINITY ? v.x : nan;
-    v.y = fabsf(v.y) < INFINITY ? v.y : nan;
-    v.z = fabsf(v.z) < INFINITY ? v.z : nan;
-    v.w = fabsf(v.w) < INFINITY ? v.w : nan;
     const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(v.x, v.y), __NV_SATFINITE, __NV_E4M3);
     const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(v.z, v.w), __NV_SATFINITE, __NV_E4M3);
     return lo | hi << 16;
