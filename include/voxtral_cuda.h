@@ -708,8 +708,9 @@ int vox_cuda_rope_append_paged_dev(const vox_cuda_paged_cache *cache, int layer,
  * NaN included, does not matter; a row that sees no key, or all of whose scores
  * are -inf, gets zeros and lse -inf.  Entries of the table whose positions no
  * row sees are not followed: their pages may be given to others.
- * Scores, sums and lse are fp32; the softmax weights are rounded to 16 bits
- * (fp16, relative to the largest) before their product with V. */
+ * Scores, sums and lse are fp32; the softmax weights are rounded to fp16 (each is
+ * off by half a step of it, 2^-11, or by 2^-32 of the row's largest where that is
+ * more) before their product with V. */
 int vox_cuda_attention_paged_dev(const vox_cuda_paged_cache *cache, int layer, const vox_cuda_rows *rows,
                                  const void *q, int q_type, int n_heads, int window, int n_sink, float scale,
                                  void *out, float *lse, void *stream);
@@ -758,6 +759,15 @@ int vox_cuda_selftest_attention_timeout(const vox_cuda_kv_cache *cache, int laye
  * launched.  For tests that mean to reach a form. */
 int vox_cuda_selftest_attention_plan(const vox_cuda_kv_cache *cache, const vox_cuda_rows *rows, int n_heads, int window,
                                      int *plan);
+
+/* The same two for the attention over a paged cache: plan[0] 8 or 16 packed rows
+ * are the few-rows kernel's, 128 or 256 the many-rows kernel's, which alone has
+ * waits (else the timeout's call is refused). */
+int vox_cuda_selftest_attention_paged_plan(const vox_cuda_paged_cache *cache, const vox_cuda_rows *rows, int q_type,
+                                           int n_heads, int window, int n_sink, int *plan);
+int vox_cuda_selftest_attention_paged_timeout(const vox_cuda_paged_cache *cache, int layer, const vox_cuda_rows *rows,
+                                              const void *q, int q_type, int n_heads, void *out, float *lse, int wait_ms,
+                                              void *stream);
 
 /* ------------------------------------------------------------------------
  * Synthetic weights (benchmarks and tests): fill a device bf16 buffer with

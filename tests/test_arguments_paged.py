@@ -87,3 +87,12 @@ def test_append(bad):
 @pytest.mark.parametrize("bad", [dict(n=-1), dict(n=21), dict(src=None), dict(dst=None)])
 def test_copies(bad):
     assert copy(**bad) == V.ERR_ARG and V.last_error(), bad
+
+
+def test_a_form_is_asked_for_rows():
+    plan = (V.C.c_int * 3)()
+    f = V.lib().vox_cuda_selftest_attention_paged_plan
+    assert f(pool(), rows(), 1, 8, 0, 0, None) == V.ERR_ARG and f(pool(), None, 1, 8, 0, 0, plan) == V.ERR_ARG
+    assert f(None, rows(), 1, 8, 0, 0, plan) == V.ERR_ARG and f(pool(), rows(n_rows=0, max_rows=0), 1, 8, 0, 0, plan) == V.ERR_ARG
+    assert f(pool(), rows(), 0, 8, 0, 0, plan) == V.ERR_ARG and f(pool(), rows(), 1, 7, 0, 0, plan) == V.ERR_ARG
+    assert f(pool(), rows(), 1, 8, -1, 0, plan) == V.ERR_ARG and f(pool(), rows(), 1, 8, 0, -1, plan) == V.ERR_ARG

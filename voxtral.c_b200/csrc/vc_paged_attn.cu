@@ -553,30 +553,32 @@ cudaError_t launch_few(PagedAttnParams p, const FwPlan &plan, cudaStream_t st, R
 // keys too often.
 constexpr long long kFwMost = 128;
 
-// The shapes, by their modelled times: 4 warps, two CTAs to an SM; 8 warps, one,
-// where there are few CTAs (one token over 8192 keys 14.6 -> 12.7 us); rings of two
-// stages, three, where there are many short ones (48 streams of 1000 keys 33 -> 22);
-// tiles of 16 rows, which read the keys once for more than 8; or the many-rows
-// kernel.
+// The shapes, by their modelled times: 4 warps, two CTAs to an SM (three with heads
+// of 64); 8 warps, one, where there are few CTAs (one token over 8192 keys 14.6 ->
+// 12.7 us); for heads of 128 also rings of two stages, three CTAs, where there are
+// many short ones (48 streams of 1000 keys 33 -> 22), and tiles of 16 rows, which
+// read the keys once for more than 8 (8 streams of 32 rows over 3008 keys 32); or
+// the many-rows kernel.
 template <typename T, int HD>
 cudaError_t launch_dim(const PagedAttnParams &p, int sms, cudaStream_t st, RowsPlan *only) {
     const long long M = (long long)p.r.max_rows * p.group;
     if (M > kFwMost) return launch_paged_attn_tc(p, st, only, nullptr);
     FwPlan two, one, three, wide;
+    double many = 1e30;
     cudaError_t e;
-    if ((e = plan_few<T, HD, 1, 4, 3>(p, sms, &two)) != cudaSuccess || (e = plan_few<T, HD, 1, 8, 3>(p, sms, &one)) != cudaSuccess ||
-        (e = plan_few<T, HD, 1, 4, 2>(p, sms, &three)) != cudaSuccess)
-        return e;
-    const double best = std::min(two.cost, std::min(one.cost, three.cost));
-    if (M > 8) {
-        double many = 0;
-        if ((e = plan_few<T, HD, 2, 4, 3>(p, sms, &wide)) != cudaSuccess || (e = launch_paged_attn_tc(p, st, nullptr, &many)) != cudaSuccess)
-            return e;
-        if (many < std::min(best, wide.cost)) return launch_paged_attn_tc(p, st, only, nullptr);
-        if (wide.cost < best) return launch_few<T, HD, 2, 4, 3>(p, wide, st, only);
+    if ((e = plan_few<T, HD, 1, 4, 3>(p, sms, &two)) != cudaSuccess || (e = plan_few<T, HD, 1, 8, 3>(p, sms, &one)) != cudaSuccess) return e;
+    if constexpr (HD == 128) {
+        if ((e = plan_few<T, HD, 1, 4, 2>(p, sms, &three)) != cudaSuccess) return e;
+        if (M > 8 && (e = plan_few<T, HD, 2, 4, 3>(p, sms, &wide)) != cudaSuccess) return e;
+    }
+    if (M > 8 && (e = launch_paged_attn_tc(p, st, nullptr, &many)) != cudaSuccess) return e;
+    const double best = std::min({two.cost, one.cost, three.cost, wide.cost, many});
+    if (many == best) return launch_paged_attn_tc(p, st, only, nullptr);
+    if constexpr (HD == 128) {
+        if (three.cost == best) return launch_few<T, HD, 1, 4, 2>(p, three, st, only);
+        if (wide.cost == best) return launch_few<T, HD, 2, 4, 3>(p, wide, st, only);
     }
     if (one.cost == best) return launch_few<T, HD, 1, 8, 3>(p, one, st, only);
-    if (three.cost == best) return launch_few<T, HD, 1, 4, 2>(p, three, st, only);
     return launch_few<T, HD, 1, 4, 3>(p, two, st, only);
 }
 

@@ -308,7 +308,7 @@ constexpr int kPcThreads = 256;
 constexpr int kPcLoads = 4;
 
 __global__ void __launch_bounds__(kPcThreads) paged_copy_kernel(const PagedCopyParams p) {
-    const int layer = blockIdx.y >> 1, per_row = p.c.head_dim / 16;
+    const int layer = blockIdx.y >> 1, row_shift = p.c.head_dim == 64 ? 2 : 3;   // 16-byte chunks of a row
     const bool is_v = blockIdx.y & 1;
     for (int i = blockIdx.z; i < p.n; i += gridDim.z) {
         const int src = __ldg(p.src + i), dst = __ldg(p.dst + i);
@@ -317,14 +317,14 @@ __global__ void __launch_bounds__(kPcThreads) paged_copy_kernel(const PagedCopyP
         float *const scales = is_v ? p.c.v_scale : p.c.k_scale;
         const unsigned char *const from = base + page_base(p.c, layer, src, 0);
         unsigned char *const to = base + page_base(p.c, layer, dst, 0);
-        const int n = p.c.n_kv_heads * p.c.page * per_row, step = gridDim.x * kPcThreads;
+        const int n = p.c.n_kv_heads * p.c.page << row_shift, step = gridDim.x * kPcThreads;
         for (int e0 = blockIdx.x * kPcThreads + threadIdx.x; e0 < n; e0 += step * kPcLoads) {
             uint4 v[kPcLoads];
             long long off[kPcLoads];
 #pragma unroll
             for (int b = 0; b < kPcLoads; b++) {
-                const int e = e0 + b * step, row = e / per_row;
-                off[b] = (row >> p.c.page_shift) * p.c.head_stride + (row & (p.c.page - 1)) * p.c.slot_stride + e % per_row * 16;
+                const int e = e0 + b * step, row = e >> row_shift;
+                off[b] = (row >> p.c.page_shift) * p.c.head_stride + (row & (p.c.page - 1)) * p.c.slot_stride + (e & ((1 << row_shift) - 1)) * 16;
                 if (e < n) v[b] = *reinterpret_cast<const uint4 *>(from + off[b]);
             }
 #pragma unroll

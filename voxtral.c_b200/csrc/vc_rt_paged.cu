@@ -87,6 +87,54 @@ int check_q_type(const char *who, int type) {
     return VOX_CUDA_ERR_ARG;
 }
 
+int attention(const char *who, const vox_cuda_paged_cache *cache, int layer, const vox_cuda_rows *rows, const void *q, int q_type,
+              int n_heads, int window, int n_sink, float scale, void *out, float *lse, void *stream, int stall_ms = 0,
+              RowsPlan *only = nullptr) {
+    PagedAttnParams p = {};
+    int rc = check_pool(who, cache, true, &p.c);
+    if (rc || (rc = check_paged_rows(who, rows, p.c, &p.r)) || (rc = check_layer(who, layer, p.c.n_layers)) ||
+        (rc = check_heads(who, n_heads, p.c.n_kv_heads)) || (rc = check_q_type(who, q_type)))
+        return rc;
+    if (window < 0 || n_sink < 0 || !(fabsf(scale) <= 2.0e38f)) {
+        set_error("%s: bad window, sinks or scale", who);
+        return VOX_CUDA_ERR_ARG;
+    }
+    if (p.r.n_rows == 0) return VOX_CUDA_OK;
+    if (!q || !out || !aligned16(q) || !aligned16(out) || (uintptr_t)lse % 4) {
+        set_error("%s: q and out must be 16-byte aligned device pointers", who);
+        return VOX_CUDA_ERR_ARG;
+    }
+    const double lines = (double)p.r.n_rows * n_heads, bytes = lines * p.c.head_dim * 2;
+    if ((q != out && overlap(q, bytes, out, bytes)) || overlap(lse, lines * sizeof(float), q, bytes) ||
+        overlap(lse, lines * sizeof(float), out, bytes)) {   // CTAs would read what others have written
+        set_error("%s: out is q itself or apart from it, lse apart from both", who);
+        return VOX_CUDA_ERR_ARG;
+    }
+    if ((long long)p.r.max_rows * (n_heads / p.c.n_kv_heads) > (1 << 28)) {
+        set_error("%s: too many rows of a stream (%d)", who, p.r.max_rows);
+        return VOX_CUDA_ERR_ARG;
+    }
+    DevCtx *c = cur_ctx();
+    if (!c) return VOX_CUDA_ERR_UNAVAILABLE;
+    DeviceGuard guard(c->device);
+    if (!guard.ok()) return launched(who, cudaGetLastError());
+    if (!only && (rc = check_waits(who, c))) return rc;
+    p.err = c->op_err + op_slot();
+    p.stall_ns = stall_ms * 1000000ull;
+    p.layer = layer;
+    p.q = q;
+    p.out = out;
+    p.q_type = q_type;
+    p.lse = lse;
+    p.n_heads = n_heads;
+    p.group = n_heads / p.c.n_kv_heads;
+    const int room = p.c.table_stride * p.c.page;
+    p.window = window < room ? window : 0;   // a stream has no more positions: no limit (and no sum overflows)
+    p.n_sink = p.window > 0 ? min(n_sink, room) : 0;
+    p.scale_log2 = (scale == 0.f ? 1.0f / sqrtf((float)p.c.head_dim) : scale) * 1.4426950408889634f;
+    return launched(who, launch_paged_attn(p, c->sms, stream ? (cudaStream_t)stream : c->stream, only));
+}
+
 }  // namespace
 
 extern "C" int vox_cuda_rope_append_paged_dev(const vox_cuda_paged_cache *cache, int layer, const vox_cuda_rows *rows,
@@ -146,49 +194,38 @@ extern "C" int vox_cuda_rope_append_paged_dev(const vox_cuda_paged_cache *cache,
 extern "C" int vox_cuda_attention_paged_dev(const vox_cuda_paged_cache *cache, int layer, const vox_cuda_rows *rows,
                                             const void *q, int q_type, int n_heads, int window, int n_sink, float scale,
                                             void *out, float *lse, void *stream) {
-    const char *who = "attention_paged";
-    PagedAttnParams p = {};
-    int rc = check_pool(who, cache, true, &p.c);
-    if (rc || (rc = check_paged_rows(who, rows, p.c, &p.r)) || (rc = check_layer(who, layer, p.c.n_layers)) ||
-        (rc = check_heads(who, n_heads, p.c.n_kv_heads)) || (rc = check_q_type(who, q_type)))
-        return rc;
-    if (window < 0 || n_sink < 0 || !(fabsf(scale) <= 2.0e38f)) {
-        set_error("%s: bad window, sinks or scale", who);
+    return attention("attention_paged", cache, layer, rows, q, q_type, n_heads, window, n_sink, scale, out, lse, stream);
+}
+
+extern "C" int vox_cuda_selftest_attention_paged_plan(const vox_cuda_paged_cache *cache, const vox_cuda_rows *rows, int q_type,
+                                                      int n_heads, int window, int n_sink, int *plan) {
+    const char *who = "selftest_attention_paged_plan";
+    if (!plan || !rows || rows->n_rows < 1) {
+        set_error("%s: no rows, or no place for the answer", who);
         return VOX_CUDA_ERR_ARG;
     }
-    if (p.r.n_rows == 0) return VOX_CUDA_OK;
-    if (!q || !out || !aligned16(q) || !aligned16(out) || (uintptr_t)lse % 4) {
-        set_error("%s: q and out must be 16-byte aligned device pointers", who);
+    RowsPlan form = {};
+    void *some = cache ? cache->k : nullptr;   // (an aligned address; nothing is launched)
+    const int rc = attention(who, cache, 0, rows, some, q_type, n_heads, window, n_sink, 0.f, some, nullptr, nullptr, 0, &form);
+    if (rc) return rc;
+    plan[0] = form.rows;
+    plan[1] = form.ctas;
+    plan[2] = form.shares;
+    return VOX_CUDA_OK;
+}
+
+extern "C" int vox_cuda_selftest_attention_paged_timeout(const vox_cuda_paged_cache *cache, int layer, const vox_cuda_rows *rows,
+                                                         const void *q, int q_type, int n_heads, void *out, float *lse, int wait_ms,
+                                                         void *stream) {
+    const char *who = "selftest_attention_paged_timeout";
+    int plan[3];
+    const int rc = vox_cuda_selftest_attention_paged_plan(cache, rows, q_type, n_heads, 0, 0, plan);
+    if (rc) return rc;
+    if (wait_ms < 1 || wait_ms > 10000 || plan[0] < 128) {
+        set_error("%s: wait_ms must be 1..10000, the rows many (the few-rows kernel has no waits)", who);
         return VOX_CUDA_ERR_ARG;
     }
-    const double lines = (double)p.r.n_rows * n_heads, bytes = lines * p.c.head_dim * 2;
-    if ((q != out && overlap(q, bytes, out, bytes)) || overlap(lse, lines * sizeof(float), q, bytes) ||
-        overlap(lse, lines * sizeof(float), out, bytes)) {   // CTAs would read what others have written
-        set_error("%s: out is q itself or apart from it, lse apart from both", who);
-        return VOX_CUDA_ERR_ARG;
-    }
-    if ((long long)p.r.max_rows * (n_heads / p.c.n_kv_heads) > (1 << 28)) {
-        set_error("%s: too many rows of a stream (%d)", who, p.r.max_rows);
-        return VOX_CUDA_ERR_ARG;
-    }
-    DevCtx *c = cur_ctx();
-    if (!c) return VOX_CUDA_ERR_UNAVAILABLE;
-    DeviceGuard guard(c->device);
-    if (!guard.ok()) return launched(who, cudaGetLastError());
-    if ((rc = check_waits(who, c))) return rc;
-    p.err = c->op_err + op_slot();
-    p.layer = layer;
-    p.q = q;
-    p.out = out;
-    p.q_type = q_type;
-    p.lse = lse;
-    p.n_heads = n_heads;
-    p.group = n_heads / p.c.n_kv_heads;
-    const int room = p.c.table_stride * p.c.page;
-    p.window = window < room ? window : 0;   // a stream has no more positions: no limit (and no sum overflows)
-    p.n_sink = p.window > 0 ? min(n_sink, room) : 0;
-    p.scale_log2 = (scale == 0.f ? 1.0f / sqrtf((float)p.c.head_dim) : scale) * 1.4426950408889634f;
-    return launched(who, launch_paged_attn(p, c->sms, stream ? (cudaStream_t)stream : c->stream));
+    return attention(who, cache, layer, rows, q, q_type, n_heads, 0, 0, 0.f, out, lse, stream, wait_ms);
 }
 
 extern "C" int vox_cuda_kv_copy_pages_dev(const vox_cuda_paged_cache *cache, const int *src, const int *dst, int n, void *stream) {

@@ -214,6 +214,10 @@ def lib():
                                             C.c_void_p], C.c_int),
         "vox_cuda_attention_paged_dev": ([C.POINTER(PagedCache), C.c_int, C.POINTER(Rows), C.c_void_p, C.c_int, C.c_int,
                                           C.c_int, C.c_int, C.c_float, C.c_void_p, C.c_void_p, C.c_void_p], C.c_int),
+        "vox_cuda_selftest_attention_paged_plan": ([C.POINTER(PagedCache), C.POINTER(Rows), C.c_int, C.c_int, C.c_int, C.c_int, _ip],
+                                                   C.c_int),
+        "vox_cuda_selftest_attention_paged_timeout": ([C.POINTER(PagedCache), C.c_int, C.POINTER(Rows), C.c_void_p, C.c_int, C.c_int,
+                                                       C.c_void_p, C.c_void_p, C.c_int, C.c_void_p], C.c_int),
         "vox_cuda_kv_copy_pages_dev": ([C.POINTER(PagedCache), C.c_void_p, C.c_void_p, C.c_int, C.c_void_p], C.c_int),
         "vox_cuda_token_logprobs_dev": ([C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_longlong, C.c_void_p, C.c_int,
                                          C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p], C.c_int),
@@ -462,6 +466,14 @@ def attention_paged_dev(cache, layer, rows, q, q_type, n_heads, window, n_sink, 
     """Attention of rows over a paged 8-bit cache, with a sliding window and sinks."""
     check(lib().vox_cuda_attention_paged_dev(cache, layer, rows, q, TYPES[q_type], n_heads, window, n_sink, scale, out, lse,
                                              stream), "attention_paged_dev")
+
+
+def attention_paged_plan(cache, rows, q_type, n_heads, window, n_sink):
+    """(packed rows of a CTA, CTAs on an SM, key shares) that a paged attention call takes."""
+    plan = (C.c_int * 3)()
+    check(lib().vox_cuda_selftest_attention_paged_plan(cache, rows, TYPES[q_type], n_heads, window, n_sink, plan),
+          "selftest_attention_paged_plan")
+    return tuple(plan)
 
 
 def kv_copy_pages_dev(cache, src, dst, n, stream=None):
