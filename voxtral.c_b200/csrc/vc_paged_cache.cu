@@ -17,11 +17,16 @@ namespace {
 //            page again where it grew, and the new ones
 //   q        some rows' q heads, which need no scale and share their rows' angles
 // q and k are normalised (x / sqrt(mean(x^2) + eps) * g, if g is given) and rotated
-// in interleaved pairs, (a, b) -> (a cos - b sin, a sin + b cos): the angle in turns
-// in fp64 (a far position times a frequency keeps its fraction only there), its
-// fraction to sincospi in fp32.  A head is HD / 8 lanes with 8 values each.
+// in interleaved pairs, (a, b) -> (a cos - b sin, a sin + b cos): the angle in quarter
+// turns in fp64 (a far position times a frequency keeps its fraction only there).  A
+// head is HD / 8 lanes with 8 values each.
 //
-// Bound by HBM for long chunks, by launch latency for a step.
+// Bound by HBM for long chunks, by the launch and three dependent reads (position,
+// page, keys) for a step.  4 streams of up to 1021 rows of 32 / 8 heads of 128, fp32 to
+// bf16: 29.5 us, 0.63 of the copy rate (issue 54% busy); an encoder chunk of 1500 rows
+// of 32 / 32 heads of 64, fp16: 16 us, 0.29 (issue 65% busy); one token of 8 streams
+// 3.1 us on the device.  All heads of a page and KV head in one kind of CTA, as their
+// angles ask for, took 33 and 18 us: few loads at a time.
 // ---------------------------------------------------------------------------
 
 constexpr int kLeastExp = -100;   // of a scale
@@ -48,18 +53,27 @@ __device__ __forceinline__ float largest_finite(const float (&x)[N], float most)
     return most;
 }
 
-// Turns per position of pair d of a head, in fp64.
-__device__ __forceinline__ double turns_of(const PagedAppendParams &p, int d, int hd) {
-    return p.rotate ? exp2(-2.0 * d / hd * p.log2_theta) * 0.15915494309189535 : 0.0;
+// Quarter turns per position of pair d of a head, in fp64.
+__device__ __forceinline__ double quarters_of(const PagedAppendParams &p, int d, int hd) {
+    return p.rotate ? exp2(-2.0 * d / hd * p.log2_theta) * 0.6366197723675814 : 0.0;
 }
-// Of an angle within half a turn the hardware's sine and cosine are off by 2^-21.2
-// at most (and by the angle's rounding, 2^-23): far below half a step of q's types
-// and of e4m3.  With sincospif, six times the instructions, issue slots bound the
-// encoder chunk (20.5 us; every KV head's CTA needs its rows' angles).
-__device__ __forceinline__ float2 cos_sin(double turns) {
-    float2 v;
-    __sincosf(6.2831853f * (float)(turns - rint(turns)), &v.y, &v.x);
-    return v;
+// Cosine and sine of an angle in quarter turns, 2^-23.7 off at most over a million
+// angles: what is left of the nearest whole number, r in [-1/2, 1/2], is taken in fp64
+// and kept in two parts; sin(pi r / 2) / r and cos(pi r / 2) are minimax polynomials
+// in r^2 (own Remez fits, 2^-27 and 2^-34), pi / 2 in two parts, and what goes to a
+// leading term is added last.  An angle that is 2^-21 off (the hardware's sine; 2 us
+// faster for the encoder chunk) rounds a key in a million to the other neighbour.
+__device__ __forceinline__ float2 cos_sin(double quarters) {
+    const double whole = rint(quarters), rest = quarters - whole;
+    const int n = (int)(long long)whole;
+    const float r = (float)rest, lo = (float)(rest - (double)r), u = r * r;
+    const float q = fmaf(fmaf(fmaf(0.000903631677f, u, -0.0208600722f), u, 0.253669202f), u, -1.23370051f);
+    const float c = 1.0f + fmaf(q, u, r * lo * -2.46740110f);
+    const float t = fmaf(fmaf(fmaf(-0.00460217707f, u, 0.0796802267f), u, -0.64596349f), u, -4.37113883e-8f);
+    const float s = fmaf(r, 1.57079637f, fmaf(c * 1.57079637f, lo, r * t));
+    const float a = n & 1 ? s : c, b = n & 1 ? c : s;   // the angle's cosine and sine but for their signs
+    return make_float2(__uint_as_float(__float_as_uint(a) ^ ((uint32_t)(n + 1) << 30 & 0x80000000u)),
+                       __uint_as_float(__float_as_uint(b) ^ ((uint32_t)n << 30 & 0x80000000u)));
 }
 
 template <typename TS>
@@ -109,14 +123,14 @@ __device__ __forceinline__ void rotate8(float (&x)[8], const float2 (&c)[4]) {
 #pragma unroll
     for (int e = 0; e < 4; e++) {
         const float a = x[2 * e], b = x[2 * e + 1];
-        x[2 * e] = a * c[e].x - b * c[e].y;
-        x[2 * e + 1] = a * c[e].y + b * c[e].x;
+        x[2 * e] = __fsub_rn(__fmul_rn(a, c[e].x), __fmul_rn(b, c[e].y));   // rounded as written: a key's e4m3 does not
+        x[2 * e + 1] = __fadd_rn(__fmul_rn(a, c[e].y), __fmul_rn(b, c[e].x));   // depend on what was contracted
     }
 }
 
 template <int HD, int NT>
 struct AppendSmem {
-    double turn[HD / 2];              // turns per position
+    double turn[HD / 2];              // quarter turns per position
     float2 cs[2 * NT / HD][HD / 2];   // q: cosines and sines of its rows
     float most[2][NT / 32];
 };
@@ -142,7 +156,7 @@ __device__ __forceinline__ void append_kv(const PagedAppendParams &p, AppendSmem
     float *const at[2] = {p.c.k_scale + scale_at(p.c, p.layer, page, kvh), p.c.v_scale + scale_at(p.c, p.layer, page, kvh)};
     const int lo = j0 & (P - 1);
     const float was[2] = {lo ? *at[0] : 0.f, lo ? *at[1] : 0.f};
-    if (threadIdx.x < HD / 2) sh.turn[threadIdx.x] = turns_of(p, threadIdx.x, HD);
+    if (threadIdx.x < HD / 2) sh.turn[threadIdx.x] = quarters_of(p, threadIdx.x, HD);
     __syncthreads();
     float x[RPT][8], most[2] = {0.f, 0.f};
 #pragma unroll
@@ -260,7 +274,7 @@ __device__ __forceinline__ void append_q(const PagedAppendParams &p, AppendSmem<
     fetch(raw[0]);
     fetch(raw[1]);
     if (p.rotate) {
-        if (threadIdx.x < HD / 2) sh.turn[threadIdx.x] = turns_of(p, threadIdx.x, HD);
+        if (threadIdx.x < HD / 2) sh.turn[threadIdx.x] = quarters_of(p, threadIdx.x, HD);
         __syncthreads();
         for (int e = threadIdx.x; e < rows * (HD / 2); e += NT)
             sh.cs[e / (HD / 2)][e % (HD / 2)] = cos_sin((double)(s.pos + i0 + e / (HD / 2)) * sh.turn[e % (HD / 2)]);
@@ -300,8 +314,9 @@ __global__ void __launch_bounds__(NT, 1024 / NT) paged_append_kernel(const Paged
 }
 
 // ---------------------------------------------------------------------------
-// Copies of pages: a CTA has one pair of one layer, K or V of some heads, or
-// the scales.  Bound by HBM.
+// Copies of pages: a CTA has one pair of one layer, K or V: some of its 16-byte
+// chunks, four in flight per thread, and the scales.  Bound by HBM: 1.75 GB moved 267
+// us, 1.0 of the copy rate; 55 MB 9.9, 0.84.
 // ---------------------------------------------------------------------------
 
 constexpr int kPcThreads = 256;
