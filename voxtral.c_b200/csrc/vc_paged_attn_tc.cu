@@ -314,7 +314,8 @@ __global__ void __launch_bounds__(pt_threads(NT), pt_ctas(NT)) paged_many_kernel
                     uint4 &u = v_raw[i];
                     const uint4 n = make_uint4(__vcmpeq4(u.x & 0x7f7f7f7fu, 0x7f7f7f7fu), __vcmpeq4(u.y & 0x7f7f7f7fu, 0x7f7f7f7fu),
                                                __vcmpeq4(u.z & 0x7f7f7f7fu, 0x7f7f7f7fu), __vcmpeq4(u.w & 0x7f7f7f7fu, 0x7f7f7f7fu));
-                    found |= (n.x | n.y | n.z | n.w) != 0u;
+                    const int j = key + i * kRowsAtOnce + r0;   // (what nobody sees, a page's unwritten end, needs no flag)
+                    found |= (n.x | n.y | n.z | n.w) != 0u && j < hi && (j >= lo || j < ns);
                     u = make_uint4(u.x & ~n.x, u.y & ~n.y, u.z & ~n.z, u.w & ~n.w);
                 }
                 if (found) atomicExch(&sh.bad, 1);
