@@ -23,8 +23,8 @@
 // their sums at the end, in order.
 //
 // Measured, 32 / 8 heads of 128: 64 tokens over 5 to 16 thousand keys 217 us, 6.4
-// TB/s, 0.98 of the copy rate; 24 tokens over 4100 keys 38 us, 0.54 (384 CTAs in waves
-// of 444 and 296); 8 streams of 6 tokens over 1 to 3 thousand keys 25 us; one token
+// TB/s, 0.98 of the copy rate; 24 tokens over 4100 keys 38 us, 0.54 (384 CTAs, two or
+// three to an SM); 8 streams of 6 tokens over 1 to 3 thousand keys 25 us; one token
 // over 8192 keys 13.9 us, of which ~7 are the launch, three dependent reads before the
 // first key and the merge, the rest 4 to 5 steps of a warp at ~1.3 us each: reads from
 // shared memory, conversions, MMAs and exponentials in turn.
