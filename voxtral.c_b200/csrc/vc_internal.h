@@ -236,7 +236,7 @@ struct PagedAttnParams {
     int n_heads, group;
     int window, n_sink;       // window 0: no limit
     float scale_log2;         // scale * log2(e)
-    int shares;               // key shares of a row tile (set by the launch)
+    int shares, tiles;        // key shares of a row tile, tiles of a stream (set by the launch)
     unsigned *err;            // raised when a bounded wait expires (mapped host memory); the rows then get NaN
     unsigned long long stall_ns;   // self-test: a wait of this length that nothing ends, after the work (0: none)
 };

@@ -122,6 +122,24 @@ __device__ __forceinline__ float weigh64(uint32_t ts, float sl2, float ks, int g
     return mx;
 }
 
+// The stream that reaches n-th farthest (of up to 32; of more simply the n-th): a
+// warp's lanes each have one.  Prompt chunks over 15035 and 8008 keys: 456 us, with
+// the streams in turn 575.
+__device__ __forceinline__ int nth_longest(const PagedAttnParams &p, int n, int lane) {
+    const int streams = p.c.n_streams;
+    if (streams > 32) return n;
+    int end = -1, rank = 0;
+    if (lane < streams) {
+        const RowSpan s = paged_span(p.r, p.c, lane);
+        end = s.n > 0 ? s.pos + s.n : 0;
+    }
+    for (int i = 0; i < streams; i++) {
+        const int other = __shfl_sync(0xffffffffu, end, i);
+        rank += other > end || (other == end && i < lane);
+    }
+    return __ffs(__ballot_sync(0xffffffffu, lane < streams && rank == n)) - 1;
+}
+
 template <typename T, int HD, int NT>
 __global__ void __launch_bounds__(pt_threads(NT), pt_ctas(NT)) paged_many_kernel(const PagedAttnParams p) {
     using Sm = PtSmem<HD, NT>;
@@ -139,8 +157,12 @@ __global__ void __launch_bounds__(pt_threads(NT), pt_ctas(NT)) paged_many_kernel
     extern __shared__ __align__(1024) unsigned char pt_smem_raw[];
     Sm &sh = *reinterpret_cast<Sm *>(pt_smem_raw);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int z = blockIdx.x % p.shares, Z = p.shares;
-    const int m0 = blockIdx.x / p.shares * (NT * kAtRows), kvh = blockIdx.y, stream = blockIdx.z;
+    // CTAs in order: the streams that reach farthest, their later tiles first - in a
+    // prompt those see the most - so that what starts last ends soon
+    const int Z = p.shares, z = blockIdx.x % Z;
+    const unsigned nth = blockIdx.x / Z, of = nth / p.c.n_kv_heads;
+    const int kvh = nth % p.c.n_kv_heads, m0 = (p.tiles - 1 - (int)(of % p.tiles)) * (NT * kAtRows);
+    const int stream = nth_longest(p, of / p.tiles, lane);
     const RowSpan s = paged_span(p.r, p.c, stream);
     const int M = s.n * p.group;
     if (m0 >= M) return;   // the whole cluster leaves
@@ -698,8 +720,10 @@ cudaError_t launch_many(PagedAttnParams p, const PtPlan &plan, cudaStream_t st, 
     const long long M = (long long)p.r.max_rows * p.group, tiles = (M + NT * kAtRows - 1) / (NT * kAtRows);
     p.shares = plan.shares;
     cudaLaunchAttribute attr;
-    const cudaLaunchConfig_t cfg = cluster_config(dim3((unsigned)(p.shares * tiles), p.c.n_kv_heads, p.c.n_streams), pt_threads(NT),
-                                                  pt_smem<HD, NT>(), p.shares, &attr, st);
+    const long long ctas = p.shares * tiles * p.c.n_kv_heads * p.c.n_streams;
+    if (ctas > INT_MAX) return cudaErrorInvalidConfiguration;   // (2^31 CTAs would take hours)
+    p.tiles = (int)tiles;
+    const cudaLaunchConfig_t cfg = cluster_config(dim3((unsigned)ctas), pt_threads(NT), pt_smem<HD, NT>(), p.shares, &attr, st);
     return cudaLaunchKernelEx(&cfg, paged_many_kernel<T, HD, NT>, p);
 }
 
