@@ -83,3 +83,16 @@ def test_a_nan_outside_every_window(heads, kv, dim, rows, pos):
     for i, r in enumerate(c.keys[0]):
         want[i, :heads // kv, 7] = at in r
     assert torch.equal(hit, want) and not bool(torch.isnan(lse).any())
+
+
+@pytest.mark.parametrize("streams", [2, 31, 32, 33, 40])
+def test_every_stream_once(streams):
+    """Streams of many lengths, equal ones and ones that sit out among them, in the order of their reach or, beyond 32, in turn."""
+    pos = [(s * 37) % 5 * 40 if s % 7 != 3 else -1 for s in range(streams)]
+    counts = [(s * 13) % 50 + 1 if s % 5 else 0 for s in range(streams)]
+    counts[-1] = 50
+    c = Case("bf16", 4, 1, 64, 16, pos, counts, seed=streams, tail=1)
+    assert V.attention_paged_plan(c.cache(V), c.rows(V), "bf16", 4, 0, 0)[0] > 0
+    out, lse = c.run(V)
+    torch.cuda.synchronize()
+    c.check(out, lse)
