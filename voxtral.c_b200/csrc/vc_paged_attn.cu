@@ -30,11 +30,13 @@
 // shared memory, conversions, MMAs and exponentials in turn.
 //
 // q: bf16 rows are scaled by a power of two into fp16's range (exact but for
-// values 2^-29 of the row's largest).  The weights P = 2^(s - m) are rounded to
-// fp16, half a step of 2^-11; m is the running maximum less 7, and moves only when
-// a score exceeds it by 15, so that P fills the type up to 2^15 and what is lost
-// is 2^-32 of the largest weight per key.  V's scales go into P relative to the
-// largest of them so far.  Sums, maxima and O are fp32.
+// values 2^-29 of the row's largest).  V's scales vs go into P: P = 2^(s - m) vs is
+// rounded to fp16, half a step of 2^-11, with m the row's own maximum of s + log2 vs so
+// far, less 8, which moves only when one exceeds it by 15: P fills the type up to 2^15,
+// and what is lost is 2^-32 of the row's largest weight times scale, whatever the
+// scales of pages that it does not see.  The weights' sum has a base of its own, the
+// row's maximum of s: with one for both, a weight on a page of small V (zeros have the
+// scale 2^-100) would be lost to one or the other.  Sums, maxima and O are fp32.
 #include "vc_cluster.h"
 #include "vc_paged.cuh"
 #include "vc_tc.cuh"
@@ -50,8 +52,9 @@ namespace {
 
 constexpr int kFwKeys = 32;              // keys of a warp's step
 constexpr int fw_ctas(int w, int s) { return w == 8 ? 1 : s == 2 ? 3 : 2; }
-constexpr float kFwBelow = 7.f;          // the maximum less m
-constexpr float kFwAbove = 15.f;         // log2 of what a weight may reach before m moves
+constexpr float kFwBelow = 8.f;          // P's maximum, rounded up, less m
+constexpr float kFwAbove = 15.f;         // log2 of what P, or a weight, may reach before its base moves
+constexpr float kFwWide = 0x1p100f;      // from this factor on P is not taken from the weight, which may have left fp32
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile(
@@ -74,6 +77,11 @@ __device__ __forceinline__ void lds_words(uint32_t (&w)[N], uint32_t addr) {
         asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(addr));
     else
         asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(addr));
+}
+__device__ __forceinline__ float log2_approx(float x) {
+    float y;
+    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
 }
 __device__ __forceinline__ void cp_async4(uint32_t dst_smem, const void *src, bool ok) {
     const int n = ok ? 4 : 0;
@@ -228,17 +236,18 @@ __global__ void __launch_bounds__(W * 32, fw_ctas(W, S)) paged_few_kernel(const 
         }
     }
 
-    float o[NR][MT][4], mb[NR][2], l[NR][2];
+    float o[NR][MT][4], l[NR][2];
+    float lb[NR][2], pb[NR][2];   // bases of the sums and of P, whole numbers; -inf: nothing yet
+    float up[NR][2];              // 2^(lb - pb); 0: nothing yet
 #pragma unroll
     for (int n = 0; n < NR; n++) {
 #pragma unroll
         for (int mt = 0; mt < MT; mt++)
 #pragma unroll
             for (int e = 0; e < 4; e++) o[n][mt][e] = 0.f;
-        mb[n][0] = mb[n][1] = -INFINITY;
-        l[n][0] = l[n][1] = 0.f;
+        lb[n][0] = lb[n][1] = pb[n][0] = pb[n][1] = -INFINITY;
+        l[n][0] = l[n][1] = up[n][0] = up[n][1] = 0.f;
     }
-    float vref = 0.f, inv_vref = 0.f;   // V's largest scale so far: O is in units of it
 
     // 16 dims x 16 keys of V^T as an A operand
     auto v_tile = [&](const uint32_t (&w)[4][VW], int mt, uint32_t (&a)[4]) {
@@ -261,6 +270,7 @@ __global__ void __launch_bounds__(W * 32, fw_ctas(W, S)) paged_few_kernel(const 
         const uint32_t there = have >> (2 * (kStages - 1));
         const float4 sc = *reinterpret_cast<const float4 *>(sh.scale[warp][stage]);
         const float k_now[2] = {sc.x, sc.y}, v_now[2] = {sc.z, sc.w};
+        const float v_log[2] = {log2_approx(sc.z), log2_approx(sc.w)};
         stage = stage + 1 == kStages ? 0 : stage + 1;
         const int key = key_of(u);
         const bool whole = (there & 3u) == 3u && key + kFwKeys - 1 <= p_min &&
@@ -296,7 +306,9 @@ __global__ void __launch_bounds__(W * 32, fw_ctas(W, S)) paged_few_kernel(const 
 #pragma unroll
         for (int n = 0; n < NR; n++)
 #pragma unroll
-            for (int a = 0; a < 2; a++)
+            for (int a = 0; a < 2; a++) {
+                const float most[2] = {fminf(lb[n][0] + kFwAbove, pb[n][0] + kFwAbove - v_log[a]),
+                                       fminf(lb[n][1] + kFwAbove, pb[n][1] + kFwAbove - v_log[a])};
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
                     float &v = x[n][a][e];
@@ -307,56 +319,59 @@ __global__ void __launch_bounds__(W * 32, fw_ctas(W, S)) paged_few_kernel(const 
                         v = see ? v : -INFINITY;
                         if (!see) vis &= ~(1u << (8 * n + 4 * a + e));
                     }
-                    over |= v > mb[n][e & 1] + kFwAbove;
+                    over |= v > most[e & 1];
                 }
+            }
         if (__any_sync(0xffffffffu, over)) {
 #pragma unroll
             for (int n = 0; n < NR; n++)
 #pragma unroll
                 for (int e = 0; e < 2; e++) {
-                    float top = fmaxf(fmaxf(x[n][0][e], x[n][0][e + 2]), fmaxf(x[n][1][e], x[n][1][e + 2]));
+                    const float x0 = fmaxf(x[n][0][e], x[n][0][e + 2]), x1 = fmaxf(x[n][1][e], x[n][1][e + 2]);
+                    float top = fmaxf(x0, x1), p_top = fmaxf(x0 + v_log[0], x1 + v_log[1]);
 #pragma unroll
-                    for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-                    if (top > mb[n][e] + kFwAbove) {
-                        const float f = exp2f(mb[n][e] - (top - kFwBelow));
-                        mb[n][e] = top - kFwBelow;
-                        l[n][e] *= f;
+                    for (int d = 4; d < 32; d <<= 1) {
+                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+                        p_top = fmaxf(p_top, __shfl_xor_sync(0xffffffffu, p_top, d));
+                    }
+                    if (top > lb[n][e] + kFwAbove) {
+                        const float base = ceilf(top);
+                        l[n][e] *= exp2f(lb[n][e] - base);
+                        lb[n][e] = base;
+                    }
+                    if (p_top > pb[n][e] + kFwAbove) {
+                        const float base = ceilf(p_top) - kFwBelow, f = exp2f(pb[n][e] - base);
+                        pb[n][e] = base;
 #pragma unroll
                         for (int mt = 0; mt < MT; mt++) {
                             o[n][mt][e] *= f;
                             o[n][mt][e + 2] *= f;
                         }
                     }
+                    up[n][e] = pb[n][e] == -INFINITY ? 0.f : exp2f(lb[n][e] - pb[n][e]);
                 }
         }
-        const float v_top = fmaxf(v_now[0], v_now[1]);
-        if (v_top > vref) {
-            const float f = vref / v_top;
-            vref = v_top;
-            inv_vref = 1.0f / v_top;
-#pragma unroll
-            for (int n = 0; n < NR; n++)
-#pragma unroll
-                for (int mt = 0; mt < MT; mt++)
-#pragma unroll
-                    for (int e = 0; e < 4; e++) o[n][mt][e] *= f;
-        }
-        uint32_t pb[NR][2][2];
+        uint32_t pf[NR][2][2];
 #pragma unroll
         for (int n = 0; n < NR; n++) {
-            const float base[2] = {mb[n][0] == -INFINITY ? 0.f : mb[n][0], mb[n][1] == -INFINITY ? 0.f : mb[n][1]};
+            const float base[2] = {lb[n][0] == -INFINITY ? 0.f : lb[n][0], lb[n][1] == -INFINITY ? 0.f : lb[n][1]};
 #pragma unroll
             for (int a = 0; a < 2; a++) {
-                const float rel = v_now[a] * inv_vref;
+                const float by[2] = {v_now[a] * up[n][0], v_now[a] * up[n][1]};
                 float w[4];
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
                     w[e] = exp2_approx(x[n][a][e] - base[e & 1]);
                     l[n][e & 1] += w[e];
-                    w[e] *= rel;
+                    w[e] *= by[e & 1];
                 }
-                pb[n][a][0] = transpose8(pack2<__half>(w[0], w[1]));
-                pb[n][a][1] = transpose8(pack2<__half>(w[2], w[3]));
+                if (by[0] > kFwWide || by[1] > kFwWide) {
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        if (by[e & 1] > kFwWide) w[e] = exp2_approx(x[n][a][e] + (v_log[a] - pb[n][e & 1]));
+                }
+                pf[n][a][0] = transpose8(pack2<__half>(w[0], w[1]));
+                pf[n][a][1] = transpose8(pack2<__half>(w[2], w[3]));
             }
         }
         uint32_t vw[2][4][VW];
@@ -415,13 +430,14 @@ __global__ void __launch_bounds__(W * 32, fw_ctas(W, S)) paged_few_kernel(const 
                 uint32_t f[4];
                 v_tile(vw[a], mt, f);
 #pragma unroll
-                for (int n = 0; n < NR; n++) mma_f16(o[n][mt], f, pb[n][a][0], pb[n][a][1]);
+                for (int n = 0; n < NR; n++) mma_f16(o[n][mt], f, pf[n][a][0], pf[n][a][1]);
             }
     }
     cp_async_wait<0>();
     __syncthreads();   // the ring becomes the warps' sums
 
-    // the warp's share: O in V's units, base, sum over its lanes
+    // the warp's share: its sum over the lanes as a number of [1, 2) times a power of
+    // two, which is its base, and O in the same units, so that no merge overflows
 #pragma unroll
     for (int n = 0; n < NR; n++)
 #pragma unroll
@@ -429,16 +445,17 @@ __global__ void __launch_bounds__(W * 32, fw_ctas(W, S)) paged_few_kernel(const 
             float sum = l[n][e];
 #pragma unroll
             for (int d = 4; d < 32; d <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-            const int r = n * 8 + 2 * t + e;
+            const int r = n * 8 + 2 * t + e, bits = sum > 0.f && sum < INFINITY ? (int)(__float_as_uint(sum) >> 23) - 127 : 0;
+            const float down = __uint_as_float((uint32_t)(127 - bits) << 23), f = pb[n][e] == -INFINITY ? 0.f : exp2f(pb[n][e] - lb[n][e]);
             if (g == 0) {
-                sh.mx[warp][r] = mb[n][e];
-                sh.sum[warp][r] = sum;
+                sh.mx[warp][r] = lb[n][e] + (float)bits;
+                sh.sum[warp][r] = sum * down;
             }
             float *const to = sh.o[warp][r] + g * (HD / 8);
 #pragma unroll
             for (int mt = 0; mt < MT; mt += 2)
-                *reinterpret_cast<float4 *>(to + 2 * mt) = make_float4(o[n][mt][e] * vref, o[n][mt][e + 2] * vref,
-                                                                       o[n][mt + 1][e] * vref, o[n][mt + 1][e + 2] * vref);
+                *reinterpret_cast<float4 *>(to + 2 * mt) = make_float4(o[n][mt][e] * down * f, o[n][mt][e + 2] * down * f,
+                                                                       o[n][mt + 1][e] * down * f, o[n][mt + 1][e + 2] * down * f);
         }
     __syncthreads();
     // the CTA's: into its first warp's place
@@ -503,7 +520,7 @@ struct FwPlan {
 // to 16000 positions, 5 head layouts) in every shape and with 1 to 8 shares; the
 // least by the model is within 2% of the least measured on the average, 15% at most.
 //   a CTA's start and end, the merge of shares, and per share; a further wave of CTAs
-constexpr double kFwFixed = 3.9, kFwMerge = 0.9, kFwShare = 0.23, kFwWave = 4.4, kFwWide = 1.1;   // kFwWide: of 8 warps
+constexpr double kFwFixed = 3.9, kFwMerge = 0.9, kFwShare = 0.23, kFwWave = 4.4, kFwEight = 1.1;   // kFwEight: of 8 warps
 //   a step of 32 keys: what a warp by itself takes, and what the SM does for each,
 //   for heads of 128 and 8 packed rows; and of 64, 16 rows, rings of two stages
 constexpr double kFwStep = 1.07, kFwStepSm = 0.155;
@@ -532,7 +549,7 @@ cudaError_t plan_few(const PagedAttnParams &p, int sms, FwPlan *out) {
         const double fill = (double)clusters / at_once, most = (double)at_once * Z / sms;   // CTAs on an SM
         const double ctas = fill < 1.0 ? std::min(most, ceil((double)clusters * Z / sms)) : most;
         const double steps = (double)((units + (long long)Z * W - 1) / ((long long)Z * W)), waves = std::max(1.0, fill);
-        const double t = kFwFixed + (W == 8 ? kFwWide : 0.0) + (Z > 1 ? kFwMerge : 0.0) + kFwShare * Z + kFwWave * (ceil(waves) - 1.0) +
+        const double t = kFwFixed + (W == 8 ? kFwEight : 0.0) + (Z > 1 ? kFwMerge : 0.0) + kFwShare * Z + kFwWave * (ceil(waves) - 1.0) +
                          steps * std::max(alone, ctas * W * each) * ((1.0 - kFwRagged) * waves + kFwRagged * ceil(waves));
         if (t < out->cost) {
             out->cost = t;
