@@ -708,9 +708,12 @@ int vox_cuda_rope_append_paged_dev(const vox_cuda_paged_cache *cache, int layer,
  * NaN included, does not matter; a row that sees no key, or all of whose scores
  * are -inf, gets zeros and lse -inf.  Entries of the table whose positions no
  * row sees are not followed: their pages may be given to others.
- * Scores, sums and lse are fp32; the softmax weights are rounded to fp16 (each is
- * off by half a step of it, 2^-11, or by 2^-32 of the row's largest where that is
- * more) before their product with V. */
+ * Scores, sums and lse are fp32; the softmax weights are rounded to fp16 before
+ * their product with V: each, times its V's scale, is off by half a step, 2^-11, or
+ * where that is more by 2^-32 of the row's largest weight times the largest V scale
+ * that the row sees.  (Where a stream has many rows and V scales are more than
+ * 2^15 apart, scales that a row does not see may turn that rounding one way or the
+ * other.) */
 int vox_cuda_attention_paged_dev(const vox_cuda_paged_cache *cache, int layer, const vox_cuda_rows *rows,
                                  const void *q, int q_type, int n_heads, int window, int n_sink, float scale,
                                  void *out, float *lse, void *stream);

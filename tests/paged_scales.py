@@ -44,7 +44,10 @@ def check(c, out, lse, scale=0.0, some=None):
     with V's scale, is off by d = (dim + 10) u S + 2^-22 relative.  The product is rounded to fp16, by half a step of it
     (2^-11), or by 2^-32 of the row's largest product where that is more.  N sums of fp32, each off by 2 u at most of what has
     come together (the tensor cores cut off).  So an output is off by (2 d + 2^-11 + 3 N u) sum(w |v|) + 2^-32 max(w s) sum(|v| / s)
-    and half a step of its own type; the lse by d + N u + (4 |lse| + 16) u."""
+    and half a step of its own type; the lse by d + N u + (4 |lse| + 16) u.
+    The kernel of many rows, where V's scales are near one another, rounds the weights and has s in V, exactly: a weight is then
+    off by 2^-32 of the row's largest weight (a half step of fp16 is 2^-25 at least, and the largest P is 2^7 at least), an output
+    by 2^-32 max(w) sum(|v|) in the place of the term with s, which may be more or less: the larger one is taken."""
     out, lse = out.double().cpu(), lse.double().cpu()
     scale, group, u = scale or 1.0 / math.sqrt(c.dim), c.heads // c.kv, half_step(c.dtype)
     for s, rows in enumerate(c.keys):
@@ -67,8 +70,10 @@ def check(c, out, lse, scale=0.0, some=None):
             o, mean, n = w @ v, w @ v.abs(), mask.sum(-1)
             big = ((q.abs() @ k.abs().T) * abs(scale)).masked_fill(~mask, 0).amax(-1)
             d = (c.dim + 10) * U32 * big + 2.0 ** -22
-            lost = 2.0 ** -32 * (w * vs).amax(-1)[:, None] * (mask.double() @ (v.abs() / vs[:, None]))
-            tol = (2 * d + 2.0 ** -11 + 3 * n * U32)[:, None] * mean + lost + u * o.abs() + LEAST[c.dtype]
+            lost = (w * vs).amax(-1)[:, None] * (mask.double() @ (v.abs() / vs[:, None]))
+            if c.many:
+                lost = torch.maximum(lost, w.amax(-1)[:, None] * (mask.double() @ v.abs()))
+            tol = (2 * d + 2.0 ** -11 + 3 * n * U32)[:, None] * mean + 2.0 ** -32 * lost + u * o.abs() + LEAST[c.dtype]
             err = (out[at, h] - o).abs()
             assert bool((err <= tol).all()), (s, h, float((err / tol).max()), int((err / tol).amax(-1).argmax()))
             off = (lse[at, h] - z).abs()
@@ -77,9 +82,9 @@ def check(c, out, lse, scale=0.0, some=None):
 
 def run(c, form=None, **kw):
     """form: packed rows of a CTA and CTAs on an SM that the call has to take."""
-    if form:
-        plan = V.attention_paged_plan(c.cache(V), c.rows(V), c.dtype, c.heads, c.window, c.n_sink)
-        assert plan[:2] == form, plan
+    plan = V.attention_paged_plan(c.cache(V), c.rows(V), c.dtype, c.heads, c.window, c.n_sink)
+    assert plan[:2] == (form or plan[:2]), plan
+    c.many = plan[0] >= 128
     out, lse = c.run(V, **kw)
     torch.cuda.synchronize()
     return out, lse
@@ -127,13 +132,13 @@ def any_scales(form, heads, kv, dim, page, counts, far):
         check(c, *run(c, form))
 
 
-def others_pages_change_nothing(dtype, form, heads, kv, dim, page, counts, far):
-    """Rows give the same bits whatever stands in pages, and in their scales, that they do not see."""
+def others_pages_change_nothing(dtype, form, heads, kv, dim, page, counts, far, same_to=110):
+    """Rows give the same bits whatever stands in pages, and in their scales (up to 2^same_to), that they do not see."""
     c = Case(dtype, heads, kv, dim, page, [3] * len(counts) + far, counts + [1] * len(far), seed=7)
     spread(c, lambda s, i: -9)
     out, lse = run(c, form)
     assert min(counts) > page
-    for high in (7, 110) if dtype == "bf16" else (7,):
+    for high in (5, 7, 110) if dtype == "bf16" else (5, 7):
         for s in range(len(counts)):
             for i in range(1, len(c.table[s])):
                 g = c.table[s][i]
@@ -143,5 +148,5 @@ def others_pages_change_nothing(dtype, form, heads, kv, dim, page, counts, far):
         out2, lse2 = run(c, form)
         for s in range(len(counts)):
             a, b = c.start[s], c.start[s] + page - 3
-            assert torch.equal(out[a:b], out2[a:b]) and torch.equal(lse[a:b], lse2[a:b]), (high, s)
+            assert high > same_to or torch.equal(out[a:b], out2[a:b]) and torch.equal(lse[a:b], lse2[a:b]), (high, s)
         check(c, out2, lse2, some=range(len(counts)))

@@ -27,10 +27,19 @@
 // All operands are fp16, whatever q's type: bf16 rows of Q are scaled by a power
 // of two into its range (exact but for values 2^-29 of the row's largest), K's
 // scales multiply the scores, V's the values, relative to the largest that the
-// CTA sees.  The weights are rounded to fp16, half a step of 2^-11; m is the
-// running maximum less 7 and moves only when a score exceeds it by 15, so that P
-// fills the type up to 2^15 and what is lost is 2^-32 of the largest weight per
-// key.  Sums, maxima and O are fp32.
+// CTA sees: exact down to 2^-15 of it, where e4m3's least number is fp16's.  The
+// weights are rounded to fp16, half a step of 2^-11; m is the running maximum less 7
+// and moves only when a score exceeds it by 15, so that P fills the type up to 2^15
+// and what is lost is 2^-32 of the row's largest weight per key.  Sums, maxima and O
+// are fp32.
+//
+// Scales farther apart, or outside 2^-60 .. 2^60 (a page of zeros has 2^-100): a row
+// goes by the scales that it sees, which may be the small ones.  A CTA that meets such
+// leaves V as it is and puts its scale into the weights' exponents, with a base for P,
+// the row's largest s + log2 vs, and one for the weights' sum, its largest s.  That is
+// two 2^x for each score: the prompt chunks take 794 us so, the encoder chunk 120.  One loop for both cases, with the sums of P brought to
+// weights by groups of 16 keys, cost the ordinary case 20% (spills, and MMA operands
+// that left their uniform registers).
 //
 // Zero times a masked key's NaN would be NaN: in blocks that some row does not
 // see whole, the converting threads put zeros in the place of NaN in V and set a
@@ -73,7 +82,7 @@ struct PtSmem {
     uint64_t q_full[NT], k_full[kPtStages], k_empty[kPtStages], v_full[kPtStages], v_empty[kPtStages];
     uint64_t s_full[NT][2], p_full[NT][2], o_part[NT], o_done[NT];   // [2]: by S range
     uint32_t tmem;
-    int v_top;    // V's largest scale, as the bits of a float >= 0
+    int v_top, v_least;   // V's largest scale and its least but 0, as the bits of floats >= 0
     int bad;      // a masked block holds NaN in V
     int failed;   // some warp's wait ran out: the CTA's rows are void
     uint64_t stall;   // nothing arrives here
@@ -126,6 +135,36 @@ __device__ __forceinline__ float weigh64(uint32_t ts, float sl2, float ks, int g
     unpair(add2(rs[0], rs[1]), a, b);
     ls = a + b;
     return mx;
+}
+
+// The same where V's scales stand far apart: P 2^(s f + log2 vs - p_base), weights 2^(s f - l_base), both bases the row's
+// own.  lv: log2 vs, as ks.
+struct Tops {
+    float l, p;   // the largest s f, the largest s f + log2 vs
+};
+__device__ __forceinline__ Tops weigh64_wide(uint32_t ts, float sl2, float ks, float lv, int g0, float l_base, float p_base,
+                                             const uint32_t (&vis)[2], uint32_t (&w)[32], float &ls) {
+    Tops top = {-INFINITY, -INFINITY};
+    ls = 0.f;
+#pragma unroll
+    for (int c = 0; c < 64; c += 16) {
+        uint32_t r[16];
+        tmem_ld16_async(ts + c, r);
+        const float f = sl2 * __shfl_sync(0xffffffffu, ks, g0 + c / 16), v = __shfl_sync(0xffffffffu, lv, g0 + c / 16);
+        float most = -INFINITY;
+        tmem_ld_wait(r);
+#pragma unroll
+        for (int j = 0; j < 16; j += 2) {
+            const float xa = vis[c / 32] & (1u << ((c & 16) + j)) ? __uint_as_float(r[j]) * f : -INFINITY;
+            const float xb = vis[c / 32] & (2u << ((c & 16) + j)) ? __uint_as_float(r[j + 1]) * f : -INFINITY;
+            most = max3(most, xa, xb);
+            ls += exp2_approx(xa - l_base) + exp2_approx(xb - l_base);
+            w[(c + j) >> 1] = pack2<__half>(exp2_approx(xa + (v - p_base)), exp2_approx(xb + (v - p_base)));
+        }
+        top.l = fmaxf(top.l, most);
+        top.p = fmaxf(top.p, most + v);
+    }
+    return top;
 }
 
 // The stream that reaches n-th farthest (of up to 32; of more simply the n-th): a
@@ -214,6 +253,11 @@ __global__ void __launch_bounds__(pt_threads(NT), pt_ctas(NT)) paged_many_kernel
         return st;
     };
     bool ok = true;
+    // V's scales do not fit fp16 beside one another, or their products fp32 (once they have been looked through)
+    auto far_apart = [&] {
+        const float top = __int_as_float(*(volatile int *)&sh.v_top), least = __int_as_float(*(volatile int *)&sh.v_least);
+        return top > 0.f && (least < top * 0x1p-15f || top > 0x1p60f || top < 0x1p-60f);
+    };
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < kPtStages; i++) {
@@ -234,6 +278,7 @@ __global__ void __launch_bounds__(pt_threads(NT), pt_ctas(NT)) paged_many_kernel
         }
         mbar_init(&sh.stall, 1);
         sh.v_top = sh.bad = sh.failed = 0;
+        sh.v_least = 0x7f800000;   // infinity
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == kWarpMma) {
@@ -300,22 +345,28 @@ __global__ void __launch_bounds__(pt_threads(NT), pt_ctas(NT)) paged_many_kernel
         load(p.c.k, here, k_raw);
         load(p.c.v, here, v_raw);
         int next = entry(1);
-        {   // the largest scale of V
+        {   // the largest scale of V and the least
             const int step = min(p.c.page, kKeys), n = nb * (kKeys / step);
-            float top = 0.f;
+            float top = 0.f, least = INFINITY;
             for (int i = tid; i < n; i += kPtConv) {
                 int key = key_of(i / (kKeys / step)) + i % (kKeys / step) * step;
                 // a page's first positions may be among those that nobody sees
                 const bool seen = key < hi && (key + step > lo || key < ns);
                 const int g = seen ? page_at(p.c, stream, key >> p.c.page_shift) : -1;
-                if (g >= 0) top = fmaxf(top, __ldg(p.c.v_scale + scale_at(p.c, p.layer, g, kvh)));
+                const float v = g >= 0 ? __ldg(p.c.v_scale + scale_at(p.c, p.layer, g, kvh)) : 0.f;
+                top = fmaxf(top, v);
+                least = fminf(least, v > 0.f ? v : INFINITY);
             }
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-            if (lane == 0) atomicMax(&sh.v_top, __float_as_int(top));
+            const int most = __reduce_max_sync(0xffffffffu, __float_as_int(top)), few = __reduce_min_sync(0xffffffffu, __float_as_int(least));
+            if (lane == 0) {
+                atomicMax(&sh.v_top, most);
+                atomicMin(&sh.v_least, few);
+            }
             asm volatile("bar.sync 1, %0;" ::"n"(kPtConv) : "memory");
+            asm volatile("bar.arrive 2, %0;" ::"n"(kPtConv + NT * kAtRows) : "memory");
         }
         const float v_top = __int_as_float(*(volatile int *)&sh.v_top), inv_top = v_top > 0.f ? 1.0f / v_top : 0.f;
+        const bool apart = far_apart();
         for (int b = 0; b < nb; b++) {
             const int st = b % kPtStages;
             const uint32_t back = (b / kPtStages + 1) & 1u;
@@ -351,7 +402,7 @@ __global__ void __launch_bounds__(pt_threads(NT), pt_ctas(NT)) paged_many_kernel
 #pragma unroll
             for (int i = 0; i < kLoads; i++)
                 put(sh.kv[1][st], i * kRowsAtOnce + r0, v_raw[i],
-                    __float2half2_rn(__shfl_sync(0xffffffffu, here.vs, group(i)) * inv_top), true);
+                    __float2half2_rn(apart ? 1.0f : __shfl_sync(0xffffffffu, here.vs, group(i)) * inv_top), true);
             fence_async_smem();
             __syncwarp();
             if (lane == 0) mbar_arrive(&sh.v_full[st]);
@@ -423,6 +474,7 @@ __global__ void __launch_bounds__(pt_threads(NT), pt_ctas(NT)) paged_many_kernel
         // ---- softmax: thread = packed row ----
         const int t = warp / 4, q = warp % 4, ml = t * kAtRows + 32 * q + lane, m = m0 + ml;
         const bool here = m0 + t * kAtRows + 32 * q < M;   // the warp has rows
+        if (!here) asm volatile("bar.arrive 2, %0;" ::"n"(kPtConv + NT * kAtRows) : "memory");
         if (here) {
             const int i = min(m, M - 1) / p.group, at = s.pos + i;
             const long long row = (long long)(s.r0 + i) * p.n_heads + head0 + min(m, M - 1) % p.group;
@@ -484,81 +536,128 @@ __global__ void __launch_bounds__(pt_threads(NT), pt_ctas(NT)) paged_many_kernel
             const Steps st = kSkip ? steps_of(t) : Steps{};
             const int w_min = __shfl_sync(0xffffffffu, at, 0), w_max = __shfl_sync(0xffffffffu, at, 31);
             uint32_t phase = 0u, turns = 0u;   // bit r: of s_full[t][r]; steps taken
-            for (int b = 0; b < nb; b++) {
-                const int key = key_of(b);
-                const uint32_t there = __ballot_sync(0xffffffffu, is_page(page));
-                const bool all = !kSkip && whole(key) && there == (1u << kGroups) - 1;   // the CTA's rows see the whole block
-                const float ks_now = ks;
-                page = page_next;
-                ks = scale(page);
-                page_next = entry(b + 2);
-#pragma unroll 1
-                for (int h = 0; h < kSteps; h++) {
-                    const int c0 = key + h * kPtHalf;
-                    const int u = b * kSteps + h;
-                    if (kSkip && st.left_out(u)) continue;
-                    const uint32_t ts = tl + (t * 2 + (u & 1)) * kPtHalf, pages = (there >> (4 * h)) & 15u;
-                    const bool full = !kSkip ? all
-                                             : c0 + kPtHalf - 1 <= w_min && pages == 15u &&
-                                                   (p.window <= 0 || c0 > w_max - p.window || c0 + kPtHalf <= p.n_sink);
-                    if (!warp_wait(&sh.s_full[t][u & 1], kSkip ? (phase >> (u & 1)) & 1u : (u >> 1) & 1u, deadline)) ok = false;
-                    phase ^= 1u << (u & 1);
-                    tc_fence_after();
-                    uint32_t vis[2] = {0u, 0u};
-                    if (!full)
-#pragma unroll
-                        for (int e = 0; e < 2; e++)
-                            vis[e] = (range_bits(c0 + 32 * e, 0, e1) | range_bits(c0 + 32 * e, s2, at + 1)) &
-                                     ((pages >> (2 * e) & 1u ? 0xffffu : 0u) | (pages >> (2 * e) & 2u ? 0xffff0000u : 0u));
-                    // P against m so far; a row whose keys exceed it by 2^15 takes
-                    // theirs, and the warp goes over them again (S is intact until P
-                    // is stored)
-                    uint32_t w[32];
-                    float base = mr == -INFINITY ? 0.f : mr, factor = 1.f, ls = 0.f;
-                    float over;   // the largest less base
-                    bool moved = false;
-#pragma unroll 1
-                    for (;;) {    // (one copy of its code)
-                        over = full ? weigh64<false>(ts, sl2, ks_now, 4 * h, base, vis, w, ls)
-                                    : weigh64<true>(ts, sl2, ks_now, 4 * h, base, vis, w, ls);
-                        const bool move = mr == -INFINITY ? over > -INFINITY : over > kPtAbove;
-                        if (moved || !__any_sync(0xffffffffu, move)) break;
-                        moved = true;
-                        if (move) {
-                            const float mn = base + over - kPtBelow;
-                            factor = mr == -INFINITY ? 0.f : exp2_approx(mr - mn);
-                            mr = base = mn;
-                            l *= factor;
-                        }
+            float pb = -INFINITY;   // P's base where V's scales are far apart; mr is the sum's
+            auto weights = [&](auto wide) {
+                constexpr bool kWide = decltype(wide)::value;
+                float vs = 0.f;
+                if constexpr (kWide) vs = is_page(page) ? __ldg(p.c.v_scale + scale_at(p.c, p.layer, page, kvh)) : 0.f;
+                for (int b = 0; b < nb; b++) {
+                    const int key = key_of(b);
+                    const uint32_t there = __ballot_sync(0xffffffffu, is_page(page));
+                    const bool all = !kSkip && whole(key) && there == (1u << kGroups) - 1;   // the CTA's rows see the whole block
+                    const float ks_now = ks;
+                    float lv_now = 0.f;
+                    page = page_next;
+                    ks = scale(page);
+                    if constexpr (kWide) {
+                        lv_now = log2f(vs);   // (exact for powers of two; 0: -inf)
+                        vs = is_page(page) ? __ldg(p.c.v_scale + scale_at(p.c, p.layer, page, kvh)) : 0.f;
                     }
-                    l += ls;
-                    tmem_st32_async(ts, w);       // over S
-                    if (moved && (kSkip ? turns : u) > 0) {
-                        // O must hold the weights before these: the step before
-                        // this one may be under way
-                        if (!warp_wait(&sh.o_part[t], ((kSkip ? turns : u) - 1) & 1u, deadline)) ok = false;
+                    page_next = entry(b + 2);
+#pragma unroll 1
+                    for (int h = 0; h < kSteps; h++) {
+                        const int c0 = key + h * kPtHalf;
+                        const int u = b * kSteps + h;
+                        if (kSkip && st.left_out(u)) continue;
+                        const uint32_t ts = tl + (t * 2 + (u & 1)) * kPtHalf, pages = (there >> (4 * h)) & 15u;
+                        const bool full = !kSkip ? all
+                                                 : c0 + kPtHalf - 1 <= w_min && pages == 15u &&
+                                                       (p.window <= 0 || c0 > w_max - p.window || c0 + kPtHalf <= p.n_sink);
+                        if (!warp_wait(&sh.s_full[t][u & 1], kSkip ? (phase >> (u & 1)) & 1u : (u >> 1) & 1u, deadline)) ok = false;
+                        phase ^= 1u << (u & 1);
                         tc_fence_after();
+                        uint32_t vis[2] = {0u, 0u};
+                        if (!full)
 #pragma unroll
-                        for (int c = 0; c < HD; c += 32) {
-                            tmem_ld32(to + c, sv);
-#pragma unroll
-                            for (int j = 0; j < 32; j++) sv[j] *= factor;
-                            tmem_st32(to + c, sv);
+                            for (int e = 0; e < 2; e++)
+                                vis[e] = (range_bits(c0 + 32 * e, 0, e1) | range_bits(c0 + 32 * e, s2, at + 1)) &
+                                         ((pages >> (2 * e) & 1u ? 0xffffu : 0u) | (pages >> (2 * e) & 2u ? 0xffff0000u : 0u));
+                        // P against m so far; a row whose keys exceed it by 2^15 takes
+                        // theirs, and the warp goes over them again (S is intact until P
+                        // is stored)
+                        uint32_t w[32];
+                        if constexpr (kWide)
+                            if (full) vis[0] = vis[1] = 0xffffffffu;
+                        float base = mr == -INFINITY ? 0.f : mr, factor = 1.f, ls = 0.f;
+                        float over;   // the largest less base
+                        bool moved = false;
+#pragma unroll 1
+                        for (;;) {    // (one copy of its code)
+                            if constexpr (kWide) {
+                                const Tops top = weigh64_wide(ts, sl2, ks_now, lv_now, 4 * h, base, pb == -INFINITY ? 0.f : pb, vis, w, ls);
+                                const bool sum = top.l > mr + kPtAbove, move = top.p > pb + kPtAbove;   // (-inf: nothing yet)
+                                if (moved || !__any_sync(0xffffffffu, sum || move)) break;
+                                moved = true;
+                                if (sum) {
+                                    const float mn = ceilf(top.l);
+                                    l *= exp2f(mr - mn);
+                                    mr = base = mn;
+                                }
+                                if (move) {
+                                    const float mn = ceilf(top.p) - kPtBelow - 1.f;
+                                    factor = exp2f(pb - mn);
+                                    pb = mn;
+                                }
+                                continue;
+                            }
+                            over = full ? weigh64<false>(ts, sl2, ks_now, 4 * h, base, vis, w, ls)
+                                        : weigh64<true>(ts, sl2, ks_now, 4 * h, base, vis, w, ls);
+                            const bool move = mr == -INFINITY ? over > -INFINITY : over > kPtAbove;
+                            if (moved || !__any_sync(0xffffffffu, move)) break;
+                            moved = true;
+                            if (move) {
+                                const float mn = base + over - kPtBelow;
+                                factor = mr == -INFINITY ? 0.f : exp2_approx(mr - mn);
+                                mr = base = mn;
+                                l *= factor;
+                            }
                         }
+                        l += ls;
+                        tmem_st32_async(ts, w);       // over S
+                        if (moved && (kSkip ? turns : u) > 0) {
+                            // O must hold the weights before these: the step before
+                            // this one may be under way
+                            if (!warp_wait(&sh.o_part[t], ((kSkip ? turns : u) - 1) & 1u, deadline)) ok = false;
+                            tc_fence_after();
+#pragma unroll
+                            for (int c = 0; c < HD; c += 32) {
+                                tmem_ld32(to + c, sv);
+#pragma unroll
+                                for (int j = 0; j < 32; j++) sv[j] *= factor;
+                                tmem_st32(to + c, sv);
+                            }
+                        }
+                        tmem_wait_st();
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&sh.p_full[t][u & 1]);
+                        turns++;
                     }
-                    tmem_wait_st();
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&sh.p_full[t][u & 1]);
-                    turns++;
                 }
-            }
+            };
+            asm volatile("bar.sync 2, %0;" ::"n"(kPtConv + NT * kAtRows) : "memory");   // V's scales have been looked through
+            if (far_apart()) weights(std::true_type());
+            else weights(std::false_type());
             // shares go over K and V, which the other tile's MMAs may still read
             for (int e = Z > 1 ? 0 : t; e < (Z > 1 ? tiles : t + 1); e++)
                 if (nb > 0 && !warp_wait(&sh.o_done[e], 0u, deadline)) ok = false;
             tc_fence_after();
-            const float v_top = __int_as_float(*(volatile int *)&sh.v_top);
-            const float il = l == 0.f ? 0.f : v_top / l;   // no weight at all: zeros (O is tiny, not NaN)
+            float unit = __int_as_float(*(volatile int *)&sh.v_top);   // of O
+            if (far_apart()) {   // to a sum in [1, 2), so that no product leaves fp32
+                const int up = l > 0.f && l < INFINITY ? (int)(__float_as_uint(l) >> 23) - 127 : 0;
+                const float down = __uint_as_float((uint32_t)(127 - up) << 23);
+                unit = pb == -INFINITY ? 0.f : exp2f(pb - mr);
+#pragma unroll 1
+                for (int c = 0; c < HD && (kSkip ? turns : steps) > 0; c += 32) {
+                    tmem_ld32(to + c, sv);
+#pragma unroll
+                    for (int j = 0; j < 32; j++) sv[j] *= down;
+                    tmem_st32(to + c, sv);
+                }
+                l *= down;
+                mr += (float)up;
+            }
+            const float il = l == 0.f ? 0.f : unit / l;   // no weight at all: zeros (O is tiny, not NaN)
             const bool bad = *(volatile int *)&sh.bad != 0;
 #pragma unroll
             for (int c = 0; c < HD; c += 32) {
@@ -588,7 +687,7 @@ __global__ void __launch_bounds__(pt_threads(NT), pt_ctas(NT)) paged_many_kernel
 #pragma unroll
                     for (int j = 0; j < 32; j += 4)
                         *reinterpret_cast<float4 *>(o + ((((c + j) >> 2) ^ (ml & 7)) << 2)) =
-                            make_float4(sv[j] * v_top, sv[j + 1] * v_top, sv[j + 2] * v_top, sv[j + 3] * v_top);
+                            make_float4(sv[j] * unit, sv[j + 1] * unit, sv[j + 2] * unit, sv[j + 3] * unit);
                 } else if (ok && m < M) {
                     T *dst = static_cast<T *>(p.out) + row * HD + c;
 #pragma unroll
