@@ -8,6 +8,7 @@ namespace vc {
 namespace rt {
 
 inline bool aligned16(const void *p) { return ((uintptr_t)p & 15u) == 0; }
+inline bool aligned4(const void *p) { return ((uintptr_t)p & 3u) == 0; }   // as an int or an fp32 is
 inline int elem_size(int dtype) { return dtype == ELEM_F32 ? 4 : 2; }
 inline bool known_type(int dtype) { return dtype == ELEM_F32 || dtype == ELEM_BF16 || dtype == ELEM_F16; }
 
@@ -40,6 +41,10 @@ inline bool overlap(const void *a, double an, const void *b, double bn) {
 inline int check_rows(const char *who, const vox_cuda_rows *r, int n_streams, int ring, int parents, RowsView *out) {
     if (!r || !r->pos) {
         set_error("%s: no rows or positions", who);
+        return VOX_CUDA_ERR_ARG;
+    }
+    if (!aligned4(r->pos) || !aligned4(r->row_start) || !aligned4(r->parent)) {
+        set_error("%s: positions, row ranges and parents must be aligned as int is", who);
         return VOX_CUDA_ERR_ARG;
     }
     if (r->n_rows < 0 || r->max_rows < 0 || r->max_rows > r->n_rows || (r->n_rows > 0 && r->max_rows < 1)) {

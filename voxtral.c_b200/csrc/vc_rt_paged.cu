@@ -63,8 +63,8 @@ int check_pool(const char *who, const vox_cuda_paged_cache *c, bool table, Paged
         set_error("%s: cache strides are too large", who);
         return VOX_CUDA_ERR_ARG;
     }
-    if (!aligned16(c->k) || !aligned16(c->v) || (uintptr_t)c->k_scale % 4 || (uintptr_t)c->v_scale % 4) {
-        set_error("%s: the cache must be 16-byte aligned, its scales as fp32 is", who);
+    if (!aligned16(c->k) || !aligned16(c->v) || !aligned4(c->k_scale) || !aligned4(c->v_scale) || (table && !aligned4(c->table))) {
+        set_error("%s: the cache must be 16-byte aligned, its scales as fp32 is, its table as int is", who);
         return VOX_CUDA_ERR_ARG;
     }
     *out = v;
@@ -100,7 +100,7 @@ int attention(const char *who, const vox_cuda_paged_cache *cache, int layer, con
         return VOX_CUDA_ERR_ARG;
     }
     if (p.r.n_rows == 0) return VOX_CUDA_OK;
-    if (!q || !out || !aligned16(q) || !aligned16(out) || (uintptr_t)lse % 4) {
+    if (!q || !out || !aligned16(q) || !aligned16(out) || !aligned4(lse)) {
         set_error("%s: q and out must be 16-byte aligned device pointers", who);
         return VOX_CUDA_ERR_ARG;
     }
@@ -238,6 +238,10 @@ extern "C" int vox_cuda_kv_copy_pages_dev(const vox_cuda_paged_cache *cache, con
         return VOX_CUDA_ERR_ARG;
     }
     if (n == 0) return VOX_CUDA_OK;
+    if (!aligned4(src) || !aligned4(dst)) {
+        set_error("%s: the pages' numbers must be aligned as int is", who);
+        return VOX_CUDA_ERR_ARG;
+    }
     DevCtx *c = cur_ctx();
     if (!c) return VOX_CUDA_ERR_UNAVAILABLE;
     DeviceGuard guard(c->device);
