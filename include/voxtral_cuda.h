@@ -661,9 +661,11 @@ int vox_cuda_kv_fork_dev(const vox_cuda_kv_cache *cache, const int *src, const i
 /* A pool of pages.  Page g of a layer holds page_size positions of every KV
  * head: element (layer, page, head, slot, dim) of k and v lies at layer *
  * layer_stride + page * page_stride + head * head_stride + slot * slot_stride +
- * dim, e4m3, one byte each.  A stride of 0 is the contiguous one for
- * [layer][page][head][slot][dim]; others are multiples of 16 bytes, and k and v
- * are 16-byte aligned.  A number of the cache is its e4m3 value times the scale
+ * dim, e4m3, one byte each.  Strides are multiples of 16 bytes that keep elements
+ * apart, in any order of the axes, and k and v are 16-byte aligned.  A stride of 0:
+ * slots are head_dim apart, heads a page's slots, pages what a page's heads and slots
+ * span, layers what their pages do; with all 0 that is [layer][page][head][slot][dim].
+ * A number of the cache is its e4m3 value times the scale
  * of its page and head, k_scale / v_scale [n_layers][n_pages][n_kv_heads]: powers
  * of two, as vox_cuda_rope_append_paged_dev writes them (K and V apart).
  * Position j of stream s is slot j mod page_size of page table[s * table_stride +

@@ -5,6 +5,7 @@
 // captured into a CUDA graph.
 #include "vc_rt_check.h"
 
+#include <algorithm>
 #include <limits.h>
 
 using namespace vc;
@@ -49,8 +50,9 @@ int check_pool(const char *who, const vox_cuda_paged_cache *c, bool table, Paged
     v.head_dim = c->head_dim;
     v.slot_stride = c->slot_stride ? c->slot_stride : c->head_dim;
     v.head_stride = c->head_stride ? c->head_stride : (long long)c->page_size * v.slot_stride;
-    v.page_stride = c->page_stride ? c->page_stride : (long long)c->n_kv_heads * v.head_stride;
-    v.layer_stride = c->layer_stride ? c->layer_stride : (long long)c->n_pages * v.page_stride;
+    const double span = std::max((double)c->n_kv_heads * v.head_stride, (double)c->page_size * v.slot_stride);   // of a page, whichever is outside
+    v.page_stride = c->page_stride ? c->page_stride : (long long)std::min(span, 1e16);
+    v.layer_stride = c->layer_stride ? c->layer_stride : (long long)std::min(std::max((double)c->n_pages * v.page_stride, span), 1e16);
     const long long st[4] = {v.slot_stride, v.head_stride, v.page_stride, v.layer_stride};
     for (long long s : st)
         if (s < c->head_dim || s % 16 != 0) {
@@ -62,6 +64,20 @@ int check_pool(const char *who, const vox_cuda_paged_cache *c, bool table, Paged
     if (extent > 1e15) {
         set_error("%s: cache strides are too large", who);
         return VOX_CUDA_ERR_ARG;
+    }
+    // each axis steps over all that the ones inside it hold, whatever their order
+    struct Axis {
+        long long stride, n;
+    } axes[4] = {{v.slot_stride, v.page}, {v.head_stride, v.n_kv_heads}, {v.page_stride, v.n_pages}, {v.layer_stride, v.n_layers}};
+    std::sort(axes, axes + 4, [](const Axis &a, const Axis &b) { return a.stride < b.stride; });
+    long long inside = c->head_dim;
+    for (const Axis &a : axes) {
+        if (a.n == 1) continue;
+        if (a.stride < inside) {
+            set_error("%s: cache strides must keep slots, heads, pages and layers apart (%lld bytes over %lld)", who, a.stride, inside);
+            return VOX_CUDA_ERR_ARG;
+        }
+        inside += a.stride * (a.n - 1);
     }
     if (!aligned16(c->k) || !aligned16(c->v) || !aligned4(c->k_scale) || !aligned4(c->v_scale) || (table && !aligned4(c->table))) {
         set_error("%s: the cache must be 16-byte aligned, its scales as fp32 is, its table as int is", who);
