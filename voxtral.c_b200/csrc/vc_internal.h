@@ -216,7 +216,7 @@ struct PagedAppendParams {
     const void *qkv;          // [n_rows] rows of (n_heads + 2 n_kv_heads) heads
     int src_type;             // ElemType of qkv
     long long ld;             // elements between its rows
-    int n_heads, group;
+    int n_heads;
     const float *q_norm, *k_norm;   // [head_dim] or NULL
     float eps;
     int rotate;               // 0: q and k keep their angles

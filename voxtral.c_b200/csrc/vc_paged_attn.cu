@@ -543,7 +543,7 @@ cudaError_t plan_few(const PagedAttnParams &p, int sms, FwPlan *out) {
     const double alone = kFwStep * (HD == 64 ? kFwStep64 : 1.0) * (NR == 2 ? kFwStep16 : 1.0) * (S == 2 ? kFwStepTwo : 1.0);
     const double each = kFwStepSm * (HD == 64 ? kFwStepSm64 : 1.0) * (NR == 2 ? kFwStepSm16 : 1.0);
     for (int Z = 1; Z <= 8 && Z <= units; Z++) {
-        int at_once = 0;
+        int at_once = 0;   // of what fits an SM (444, 296 and 148 CTAs by shape, without a cluster)
         if ((e = cluster_active(ck, kernel, dev, W * 32, kSmem, Z, &at_once)) != cudaSuccess) return e;
         if (at_once < 1) continue;
         const double fill = (double)clusters / at_once, most = (double)at_once * Z / sms;   // CTAs on an SM

@@ -801,7 +801,10 @@ cudaError_t plan_many(const PagedAttnParams &p, PtPlan *out) {
     if (p.window > 0) keys = std::min(keys, (long long)p.window + p.n_sink + (NT * kAtRows - 1) / p.group + 2);
     const long long blocks = (keys + pt_keys(NT) - 1) / pt_keys(NT), clusters = tiles * p.c.n_kv_heads * p.c.n_streams;
     for (int Z = 1; Z <= kMaxCluster && Z <= blocks; Z++) {
-        int at_once = 0;   // (the device counts for one CTA to an SM)
+        // for this kernel the device's answer is one CTA to an SM (148 without a
+        // cluster), while two one-tile CTAs do run side by side: 148 of them over 2900
+        // keys take 67 us, 296 88, 368 139
+        int at_once = 0;
         if ((e = cluster_active(ck, kernel, dev, pt_threads(NT), kSmem, Z, &at_once)) != cudaSuccess) return e;
         if (at_once < 1) continue;
         const double fill = (double)clusters / (at_once * pt_ctas(NT)), waves = std::max(1.0, ceil(fill));

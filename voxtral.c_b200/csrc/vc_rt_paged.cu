@@ -196,7 +196,6 @@ extern "C" int vox_cuda_rope_append_paged_dev(const vox_cuda_paged_cache *cache,
     p.src_type = qkv_type;
     p.ld = ld;
     p.n_heads = n_heads;
-    p.group = n_heads / p.c.n_kv_heads;
     p.q_norm = q_norm;
     p.k_norm = k_norm;
     p.eps = eps;
