@@ -93,6 +93,25 @@ def test_lse_of_small_scores(dtype, heads, kv, dim, rows):
             assert bool((off <= tol).all()), (s, h, float((off / tol).max()))
 
 
+@pytest.mark.parametrize("heads,kv,dim,rows,exp", [(8, 2, 128, 1, -7), (8, 2, 64, 9, 3), (16, 16, 128, 9, -2), (8, 2, 128, 60, -7), (8, 2, 128, 60, 7),
+                                                   (8, 8, 64, 150, -3)])
+def test_a_weight_of_one_rounds_to_itself(heads, kv, dim, rows, exp):
+    """The row that sees one key gives its V: the largest weight loses nothing to fp16, 2^-20 is left for ex2, the sum and
+    their quotient.  Another page's V is 2^exp times as large as the first one's."""
+    c = Case("fp16", heads, kv, dim, 16, [0], [rows], seed=rows)
+    for i, g in enumerate(c.table[0]):
+        if 0 <= g < c.pool.pages:
+            c.pool.scale[1][0, g] = 2.0 ** (-7 + (exp if i else 0))
+    c.pool.upload()
+    out, _ = c.run(V)
+    torch.cuda.synchronize()
+    for h in range(heads):
+        v = c.values(0, [0], h // (heads // kv))[1][0]
+        low, high = ((v - 2.0 ** -20 * v.abs()).half(), (v + 2.0 ** -20 * v.abs()).half())
+        got = out[0, h].cpu()
+        assert bool((got >= low).all()) and bool((got <= high).all()), h
+
+
 @pytest.mark.parametrize("streams", [2, 31, 32, 33, 40])
 def test_streams_in_order_of_the_many_rows_kernel(streams):
     """Streams of many lengths, in the order of their reach or, beyond 32, in turn: the kernel that orders them is the one called."""

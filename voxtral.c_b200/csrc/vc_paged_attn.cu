@@ -32,11 +32,12 @@
 // q: bf16 rows are scaled by a power of two into fp16's range (exact but for
 // values 2^-29 of the row's largest).  V's scales vs go into P: P = 2^(s - m) vs is
 // rounded to fp16, half a step of 2^-11, with m the row's own maximum of s + log2 vs so
-// far, less 8, which moves only when one exceeds it by 15: P fills the type up to 2^15,
-// and what is lost is 2^-32 of the row's largest weight times scale, whatever the
-// scales of pages that it does not see.  The weights' sum has a base of its own, the
-// row's maximum of s: with one for both, a weight on a page of small V (zeros have the
-// scale 2^-100) would be lost to one or the other.  Sums, maxima and O are fp32.
+// far, less 7 (its P is 2^7, which rounds to itself), which moves only when one exceeds
+// it by 15: P fills the type up to 2^15, and what is lost is 2^-32 of the row's largest
+// weight times scale, whatever the scales of pages that it does not see.  The weights'
+// sum has a base of its own, the row's maximum of s: with one for both, a weight on a
+// page of small V (zeros have the scale 2^-100) would be lost to one or the other.
+// Sums, maxima and O are fp32.
 #include "vc_cluster.h"
 #include "vc_paged.cuh"
 #include "vc_tc.cuh"
@@ -52,7 +53,7 @@ namespace {
 
 constexpr int kFwKeys = 32;              // keys of a warp's step
 constexpr int fw_ctas(int w, int s) { return w == 8 ? 1 : s == 2 ? 3 : 2; }
-constexpr float kFwBelow = 8.f;          // P's maximum, rounded up, less m
+constexpr float kFwBelow = 7.f;          // P's maximum less m
 constexpr float kFwAbove = 15.f;         // log2 of what P, or a weight, may reach before its base moves
 constexpr float kFwWide = 0x1p100f;      // from this factor on P is not taken from the weight, which may have left fp32
 
@@ -237,7 +238,7 @@ __global__ void __launch_bounds__(W * 32, fw_ctas(W, S)) paged_few_kernel(const 
     }
 
     float o[NR][MT][4], l[NR][2];
-    float lb[NR][2], pb[NR][2];   // bases of the sums and of P, whole numbers; -inf: nothing yet
+    float lb[NR][2], pb[NR][2];   // bases of the sums (a whole number) and of P; -inf: nothing yet
     float up[NR][2];              // 2^(lb - pb); 0: nothing yet
 #pragma unroll
     for (int n = 0; n < NR; n++) {
@@ -340,7 +341,7 @@ __global__ void __launch_bounds__(W * 32, fw_ctas(W, S)) paged_few_kernel(const 
                         lb[n][e] = base;
                     }
                     if (p_top > pb[n][e] + kFwAbove) {
-                        const float base = ceilf(p_top) - kFwBelow, f = exp2f(pb[n][e] - base);
+                        const float base = p_top - kFwBelow, f = exp2f(pb[n][e] - base);
                         pb[n][e] = base;
 #pragma unroll
                         for (int mt = 0; mt < MT; mt++) {

@@ -594,7 +594,7 @@ __global__ void __launch_bounds__(pt_threads(NT), pt_ctas(NT)) paged_many_kernel
                                     mr = base = mn;
                                 }
                                 if (move) {
-                                    const float mn = ceilf(top.p) - kPtBelow - 1.f;
+                                    const float mn = top.p - kPtBelow;
                                     factor = exp2f(pb - mn);
                                     pb = mn;
                                 }
