@@ -22,10 +22,11 @@
 // warps and then the CTAs of a cluster, which share the keys of a tile of rows, join
 // their sums at the end, in order.
 //
-// Measured, 32 / 8 heads of 128: 64 tokens over 5 to 16 thousand keys 217 us, 6.4
-// TB/s, 0.98 of the copy rate; 24 tokens over 4100 keys 38 us, 0.54 (384 CTAs, two or
-// three to an SM); 8 streams of 6 tokens over 1 to 3 thousand keys 25 us; one token
-// over 8192 keys 13.9 us, of which ~7 are the launch, three dependent reads before the
+// Measured, 32 / 8 heads of 128, inputs that L2 does not hold: 64 tokens over 5 to 16
+// thousand keys 246 us, 5.7 TB/s, 0.86 of the copy rate (217 to 234 where a graph replays
+// the call over the same few caches); 24 tokens over 4100 keys 40 us, 0.53 (384 CTAs, two
+// or three to an SM); 8 streams of 6 tokens over 1 to 3 thousand keys 28 us; one token
+// over 8192 keys 14.8 us, of which ~7 are the launch, three dependent reads before the
 // first key and the merge, the rest 4 to 5 steps of a warp at ~1.3 us each: reads from
 // shared memory, conversions, MMAs and exponentials in turn.
 //
@@ -580,9 +581,9 @@ cudaError_t launch_few(PagedAttnParams p, const FwPlan &plan, cudaStream_t st, R
 constexpr long long kFwMost = 128;
 
 // The shapes, by their modelled times: 4 warps, two CTAs to an SM (three with heads
-// of 64); 8 warps, one, where there are few CTAs (one token over 8192 keys 14.6 ->
-// 12.7 us); for heads of 128 also rings of two stages, three CTAs, where there are
-// many short ones (48 streams of 1000 keys 33 -> 22), and tiles of 16 rows, which
+// of 64); 8 warps, one, where there are few CTAs (one token over 8192 keys 15.9 ->
+// 14.7 us); for heads of 128 also rings of two stages, three CTAs, where there are
+// many short ones (48 streams of 1000 keys 33 -> 26), and tiles of 16 rows, which
 // read the keys once for more than 8 (8 streams of 32 rows over 3008 keys 32); or
 // the many-rows kernel.
 template <typename T, int HD>

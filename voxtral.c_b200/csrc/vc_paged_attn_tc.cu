@@ -19,10 +19,10 @@
 // Q half as often, took 527 us for the prompt chunks, this 465).
 //
 // Measured: prompt chunks of 1024 and 997 rows of 32 / 8 heads of 128 over 15035 and
-// 8008 keys, bf16: 451 us, 0.50 of the bf16 rate - the MMA pipe is 66% busy (an S of
+// 8008 keys, bf16: 447 us, 0.50 of the bf16 rate - the MMA pipe is 66% busy (an S of
 // 64 keys takes 48 cycles per 16 dims to read Q and K where 32 are mathematics), the
 // exponential unit 46%, issue 51%, and each waits for the others; a prompt of 2000 rows
-// 68 us; an encoder chunk of 1500 rows of 32 heads of 64, window 750: 58 us.
+// 72 us; an encoder chunk of 1500 rows of 32 heads of 64, window 750: 59 us.
 //
 // All operands are fp16, whatever q's type: bf16 rows of Q are scaled by a power
 // of two into its range (exact but for values 2^-29 of the row's largest), K's
@@ -37,9 +37,10 @@
 // goes by the scales that it sees, which may be the small ones.  A CTA that meets such
 // leaves V as it is and puts its scale into the weights' exponents, with a base for P,
 // the row's largest s + log2 vs, and one for the weights' sum, its largest s.  That is
-// two 2^x for each score: the prompt chunks take 794 us so, the encoder chunk 120.  One loop for both cases, with the sums of P brought to
-// weights by groups of 16 keys, cost the ordinary case 20% (spills, and MMA operands
-// that left their uniform registers).
+// two 2^x for each score: the prompt chunks take 930 us so, the encoder chunk 131.
+// One loop for both cases, with the sums of P brought to weights by groups of 16
+// keys, cost the ordinary case 20% (spills, and MMA operands that left their uniform
+// registers).
 //
 // Zero times a masked key's NaN would be NaN: in blocks that some row does not
 // see whole, the converting threads put zeros in the place of NaN in V and set a
@@ -142,7 +143,7 @@ __device__ __forceinline__ float weigh64(uint32_t ts, float sl2, float ks, int g
 struct Tops {
     float l, p;   // the largest s f, the largest s f + log2 vs
 };
-__device__ __forceinline__ Tops weigh64_wide(uint32_t ts, float sl2, float ks, float lv, int g0, float l_base, float p_base,
+__device__ __forceinline__ Tops weigh64_far(uint32_t ts, float sl2, float ks, float lv, int g0, float l_base, float p_base,
                                              const uint32_t (&vis)[2], uint32_t (&w)[32], float &ls) {
     Tops top = {-INFINITY, -INFINITY};
     ls = 0.f;
@@ -165,6 +166,125 @@ __device__ __forceinline__ Tops weigh64_wide(uint32_t ts, float sl2, float ks, f
         top.p = fmaxf(top.p, most + v);
     }
     return top;
+}
+
+// The softmax of a warp's 32 rows over a CTA's keys where V's scales stand far apart:
+// the steps, waits and TMEM of the kernel's own loop.
+struct FarArgs {
+    const int *table;                     // the stream's
+    const float *k_scale, *v_scale;       // of page 0, by n_kv_heads
+    int n_pages, page_shift, n_kv_heads;
+    int b0, nb, sink_blocks, first;       // the CTA's blocks
+    int lo, hi, ns;                       // positions that its rows see
+    int at, e1, s2;                       // the row's, [0, e1) and [s2, at]
+    int gap, on, end;                     // steps that the tile leaves out: [gap, on), [end, ..)
+    float sl2;
+    uint32_t s_tmem, o_tmem;              // S ranges and O of the warp's lanes
+    int t;
+    uint64_t deadline;
+};
+struct FarResult {
+    float l, base, unit;   // the weights' sum, in [1, 2), and its base; O's unit for it
+    uint32_t turns;        // steps taken
+    bool ok;
+};
+template <int HD, int NT>
+__device__ __forceinline__ FarResult weigh_far(PtSmem<HD, NT> &sh, const FarArgs &a) {
+    constexpr int kKeys = pt_keys(NT), kSteps = kKeys / kPtHalf, kGroups = kKeys / 16;
+    const int lane = threadIdx.x & 31;
+    FarResult r = {0.f, -INFINITY, 0.f, 0u, true};
+    float p_base = -INFINITY;
+    uint32_t phase = 0u;
+    for (int b = 0; b < a.nb; b++) {
+        const int key = (a.b0 + b < a.sink_blocks ? a.b0 + b : a.first + a.b0 + b - a.sink_blocks) * kKeys, mine = key + 16 * lane;
+        const int g = lane < kGroups && mine < a.hi && (mine + 16 > a.lo || mine < a.ns) ? __ldg(a.table + (mine >> a.page_shift)) : -1;
+        const bool page = g >= 0 && g < a.n_pages;
+        const uint32_t there = __ballot_sync(0xffffffffu, page);
+        const float ks = page ? __ldg(a.k_scale + (long long)g * a.n_kv_heads) : 0.f;
+        const float lv = log2f(page ? __ldg(a.v_scale + (long long)g * a.n_kv_heads) : 0.f);   // (exact for powers of two; 0: -inf)
+#pragma unroll 1
+        for (int h = 0; h < kSteps; h++) {
+            const int c0 = key + h * kPtHalf, u = b * kSteps + h;
+            if ((u >= a.gap && u < a.on) || u >= a.end) continue;
+            const uint32_t ts = a.s_tmem + (u & 1) * kPtHalf, pages = (there >> (4 * h)) & 15u;
+            if (!warp_wait(&sh.s_full[a.t][u & 1], (phase >> (u & 1)) & 1u, a.deadline)) r.ok = false;
+            phase ^= 1u << (u & 1);
+            tc_fence_after();
+            uint32_t vis[2], w[32];
+#pragma unroll
+            for (int e = 0; e < 2; e++)
+                vis[e] = (range_bits(c0 + 32 * e, 0, a.e1) | range_bits(c0 + 32 * e, a.s2, a.at + 1)) &
+                         ((pages >> (2 * e) & 1u ? 0xffffu : 0u) | (pages >> (2 * e) & 2u ? 0xffff0000u : 0u));
+            float factor = 1.f, ls;
+            bool moved = false;
+#pragma unroll 1
+            for (;;) {
+                const Tops top = weigh64_far(ts, a.sl2, ks, lv, 4 * h, r.base == -INFINITY ? 0.f : r.base,
+                                             p_base == -INFINITY ? 0.f : p_base, vis, w, ls);
+                const bool sum = top.l > r.base + kPtAbove, move = top.p > p_base + kPtAbove;   // (-inf: nothing yet)
+                if (moved || !__any_sync(0xffffffffu, sum || move)) break;
+                moved = true;
+                if (sum) {
+                    const float base = ceilf(top.l);
+                    r.l *= exp2f(r.base - base);
+                    r.base = base;
+                }
+                if (move) {
+                    const float base = top.p - kPtBelow;
+                    factor = exp2f(p_base - base);
+                    p_base = base;
+                }
+            }
+            r.l += ls;
+            tmem_st32_async(ts, w);   // over S
+            if (moved && r.turns > 0) {
+                // O must hold the P before these: the step before this one may be under way
+                if (!warp_wait(&sh.o_part[a.t], (r.turns - 1) & 1u, a.deadline)) r.ok = false;
+                tc_fence_after();
+#pragma unroll 1
+                for (int c = 0; c < HD; c += 32) {
+                    float o[32];
+                    tmem_ld32(a.o_tmem + c, o);
+#pragma unroll
+                    for (int j = 0; j < 32; j++) o[j] *= factor;
+                    tmem_st32(a.o_tmem + c, o);
+                }
+            }
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh.p_full[a.t][u & 1]);
+            r.turns++;
+        }
+    }
+    // to a sum in [1, 2), and O with it, so that no product leaves fp32
+    const int up = r.l > 0.f && r.l < INFINITY ? (int)(__float_as_uint(r.l) >> 23) - 127 : 0;
+    const float down = __uint_as_float((uint32_t)(127 - up) << 23);
+    r.unit = p_base == -INFINITY ? 0.f : exp2f(p_base - r.base);
+    r.l *= down;
+    r.base += (float)up;
+    if (r.turns > 0) {
+        if (!warp_wait(&sh.o_done[a.t], 0u, a.deadline)) r.ok = false;
+        tc_fence_after();
+#pragma unroll 1
+        for (int c = 0; c < HD; c += 32) {
+            float o[32];
+            tmem_ld32(a.o_tmem + c, o);
+#pragma unroll
+            for (int j = 0; j < 32; j++) o[j] *= down;
+            tmem_st32(a.o_tmem + c, o);
+        }
+    }
+    return r;
+}
+
+// As a call, so that its registers are not the kernel's.  That suits one tile (8 streams
+// of 32 rows over 3008 keys, which never come here, 43.7 us, without the call 45.0; encoder
+// chunk 58.8, 60.0), two tiles not (whole prompts 89.7, 87.5): what lives across the call
+// weighs on a CTA's start and end.
+template <int HD, int NT>
+__device__ __noinline__ FarResult weigh_far_call(PtSmem<HD, NT> &sh, const FarArgs a) {
+    return weigh_far<HD, NT>(sh, a);
 }
 
 // The stream that reaches n-th farthest (of up to 32; of more simply the n-th): a
@@ -536,23 +656,30 @@ __global__ void __launch_bounds__(pt_threads(NT), pt_ctas(NT)) paged_many_kernel
             const Steps st = kSkip ? steps_of(t) : Steps{};
             const int w_min = __shfl_sync(0xffffffffu, at, 0), w_max = __shfl_sync(0xffffffffu, at, 31);
             uint32_t phase = 0u, turns = 0u;   // bit r: of s_full[t][r]; steps taken
-            float pb = -INFINITY;   // P's base where V's scales are far apart; mr is the sum's
-            auto weights = [&](auto wide) {
-                constexpr bool kWide = decltype(wide)::value;
-                float vs = 0.f;
-                if constexpr (kWide) vs = is_page(page) ? __ldg(p.c.v_scale + scale_at(p.c, p.layer, page, kvh)) : 0.f;
+            float unit;                        // of O
+            asm volatile("bar.sync 2, %0;" ::"n"(kPtConv + NT * kAtRows) : "memory");   // V's scales have been looked through
+            if (far_apart()) {
+                const long long scale0 = scale_at(p.c, p.layer, 0, kvh);
+                const FarArgs args = {table, p.c.k_scale + scale0, p.c.v_scale + scale0, p.c.n_pages, p.c.page_shift, p.c.n_kv_heads, b0, nb,
+                                      sink_blocks, first, lo, hi, ns, at, e1, s2, st.gap, st.on, kSkip ? st.end : INT_MAX, sl2,
+                                      tl + t * 2 * kPtHalf, to, t, deadline};
+                FarResult r;
+                if constexpr (NT == 1) r = weigh_far_call<HD, NT>(sh, args);
+                else r = weigh_far<HD, NT>(sh, args);
+                l = r.l;
+                mr = r.base;
+                unit = r.unit;
+                turns = r.turns;
+                ok = r.ok;
+            } else {
+                unit = __int_as_float(*(volatile int *)&sh.v_top);
                 for (int b = 0; b < nb; b++) {
                     const int key = key_of(b);
                     const uint32_t there = __ballot_sync(0xffffffffu, is_page(page));
                     const bool all = !kSkip && whole(key) && there == (1u << kGroups) - 1;   // the CTA's rows see the whole block
                     const float ks_now = ks;
-                    float lv_now = 0.f;
                     page = page_next;
                     ks = scale(page);
-                    if constexpr (kWide) {
-                        lv_now = log2f(vs);   // (exact for powers of two; 0: -inf)
-                        vs = is_page(page) ? __ldg(p.c.v_scale + scale_at(p.c, p.layer, page, kvh)) : 0.f;
-                    }
                     page_next = entry(b + 2);
 #pragma unroll 1
                     for (int h = 0; h < kSteps; h++) {
@@ -576,30 +703,11 @@ __global__ void __launch_bounds__(pt_threads(NT), pt_ctas(NT)) paged_many_kernel
                         // theirs, and the warp goes over them again (S is intact until P
                         // is stored)
                         uint32_t w[32];
-                        if constexpr (kWide)
-                            if (full) vis[0] = vis[1] = 0xffffffffu;
                         float base = mr == -INFINITY ? 0.f : mr, factor = 1.f, ls = 0.f;
                         float over;   // the largest less base
                         bool moved = false;
 #pragma unroll 1
                         for (;;) {    // (one copy of its code)
-                            if constexpr (kWide) {
-                                const Tops top = weigh64_wide(ts, sl2, ks_now, lv_now, 4 * h, base, pb == -INFINITY ? 0.f : pb, vis, w, ls);
-                                const bool sum = top.l > mr + kPtAbove, move = top.p > pb + kPtAbove;   // (-inf: nothing yet)
-                                if (moved || !__any_sync(0xffffffffu, sum || move)) break;
-                                moved = true;
-                                if (sum) {
-                                    const float mn = ceilf(top.l);
-                                    l *= exp2f(mr - mn);
-                                    mr = base = mn;
-                                }
-                                if (move) {
-                                    const float mn = top.p - kPtBelow;
-                                    factor = exp2f(pb - mn);
-                                    pb = mn;
-                                }
-                                continue;
-                            }
                             over = full ? weigh64<false>(ts, sl2, ks_now, 4 * h, base, vis, w, ls)
                                         : weigh64<true>(ts, sl2, ks_now, 4 * h, base, vis, w, ls);
                             const bool move = mr == -INFINITY ? over > -INFINITY : over > kPtAbove;
@@ -634,29 +742,11 @@ __global__ void __launch_bounds__(pt_threads(NT), pt_ctas(NT)) paged_many_kernel
                         turns++;
                     }
                 }
-            };
-            asm volatile("bar.sync 2, %0;" ::"n"(kPtConv + NT * kAtRows) : "memory");   // V's scales have been looked through
-            if (far_apart()) weights(std::true_type());
-            else weights(std::false_type());
+            }
             // shares go over K and V, which the other tile's MMAs may still read
             for (int e = Z > 1 ? 0 : t; e < (Z > 1 ? tiles : t + 1); e++)
                 if (nb > 0 && !warp_wait(&sh.o_done[e], 0u, deadline)) ok = false;
             tc_fence_after();
-            float unit = __int_as_float(*(volatile int *)&sh.v_top);   // of O
-            if (far_apart()) {   // to a sum in [1, 2), so that no product leaves fp32
-                const int up = l > 0.f && l < INFINITY ? (int)(__float_as_uint(l) >> 23) - 127 : 0;
-                const float down = __uint_as_float((uint32_t)(127 - up) << 23);
-                unit = pb == -INFINITY ? 0.f : exp2f(pb - mr);
-#pragma unroll 1
-                for (int c = 0; c < HD && (kSkip ? turns : steps) > 0; c += 32) {
-                    tmem_ld32(to + c, sv);
-#pragma unroll
-                    for (int j = 0; j < 32; j++) sv[j] *= down;
-                    tmem_st32(to + c, sv);
-                }
-                l *= down;
-                mr += (float)up;
-            }
             const float il = l == 0.f ? 0.f : unit / l;   // no weight at all: zeros (O is tiny, not NaN)
             const bool bad = *(volatile int *)&sh.bad != 0;
 #pragma unroll
